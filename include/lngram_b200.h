@@ -52,8 +52,9 @@ const char* lng_last_error(void);
 /* 1 when a CUDA device of compute capability 10.x is current and usable, else 0. */
 int lng_device_ok(void);
 /* The first error code a kernel recorded on the current device since the last clear (0 = none;
- * 1 = a route code >= 2^bits, 2 = a bounded wait expired, 3 = a token id out of range), or -1 when
- * it cannot be read.  Synchronises with the device.  clear != 0 resets it. */
+ * 1 = a route code >= 2^bits, 2 = a bounded wait expired, 3 = a token id out of range, 4 = a page number,
+ * length or row offset of a key/value cache out of range), or -1 when it cannot be read.  Synchronises with
+ * the device.  clear != 0 resets it. */
 int lng_device_error(int clear);
 
 /* ------------------------------------------------------------------ router (a3, a4) */
@@ -443,6 +444,80 @@ int lng_online_counts_mix(const int64_t* codes, int64_t T, int64_t R, const int3
                           int32_t bits, const int64_t* x, const int64_t* win, const uint8_t* real, int64_t N, int64_t W,
                           const int64_t* deadline, const float* p, int64_t V, float kappa, float* out,
                           lng_stream_t stream);
+
+/* ------------------------------------------------------------------ paged keys and values */
+
+/* A cache of keys and values in pages, beside the memory layer's own cache in a decode loop.  No
+ * counterpart in the reference's memory path (its DecodeState keeps dense keys and values,
+ * ffnmem/infer.py:65-112).  Slot s of head h in page p starts at k + p * k_page_stride +
+ * h * k_head_stride + s * k_slot_stride (elements; v likewise), its head_dim values contiguous.  Key j of
+ * sequence b lives in page table[b * table_stride + j / page_size], slot j % page_size.  lengths[b] counts
+ * the keys of sequence b INCLUDING the step's new tokens: a step first raises lengths, then appends, then
+ * attends.  table and lengths are device memory and are read when the kernels run, so a captured graph
+ * replays with their current values.  Page numbers outside [0, num_pages) of needed keys, lengths outside
+ * [0, max_pages * page_size] and bad row offsets record device error 4; such keys read as zeros and are not
+ * written.  dtype LNG_BF16 or LNG_F16; k, v 16-byte aligned, strides multiples of 8 elements; head_dim a
+ * multiple of 8 up to 128; page_size a power of two in [8, 4096]; max_pages * page_size < 2^30. */
+typedef struct {
+  void* k;
+  void* v;
+  int32_t dtype;
+  int32_t page_size;
+  int64_t num_pages;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int64_t k_page_stride, k_head_stride, k_slot_stride;
+  int64_t v_page_stride, v_head_stride, v_slot_stride;
+  const int32_t* table;
+  int64_t table_stride, max_pages;
+  const int32_t* lengths;
+  int64_t batch;
+} lng_kv_cache;
+
+/* Rows of a step: [tokens, heads, head_dim] in the cache's dtype with a token and a head stride
+ * (elements, multiples of 8; 16-byte aligned base).  The tokens of sequence b are rows cu[b] .. cu[b + 1] - 1
+ * (cu: i32 [batch + 1], device), or b * max_new .. (b + 1) * max_new - 1 when cu is NULL.  max_new bounds
+ * the tokens of one sequence; rows that belong to none are neither read nor written. */
+typedef struct {
+  void* ptr;
+  int64_t token_stride, head_stride;
+  int32_t heads;
+} lng_kv_rows;
+
+/* Append a step's keys and values (k, v: num_kv_heads heads) to the cache: token i of the n new ones of
+ * sequence b becomes key lengths[b] - n + i.  With rotary_dim > 0 the first rotary_dim values of every key
+ * are rotated by the token's position (positions [tokens] i64, or its key index when NULL) times inv_freq
+ * (fp32 [rotary_dim / 2], device): the angle is formed and reduced in 64 bits, pair (a, b) becomes
+ * (a cos - b sin, b cos + a sin) in fp32 and is rounded once.  Pairs are (j, j + rotary_dim / 2), or
+ * (2j, 2j + 1) when interleaved != 0.  q (optional, any heads) is rotated likewise into q_out, which is q
+ * itself or does not overlap it. */
+int lng_kv_append(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, const lng_kv_rows* k,
+                  const lng_kv_rows* v, const lng_kv_rows* q, const lng_kv_rows* q_out, const int64_t* positions,
+                  const float* inv_freq, int32_t rotary_dim, int32_t interleaved, lng_stream_t stream);
+
+/* Causal attention of a step's tokens over the cache (append first): the token at position p of its
+ * sequence sees keys j <= p, with window > 0 only j > p - window or j < sinks; out = softmax(scale q . k) v
+ * with fp32 scores and sums (weights rounded to the cache's dtype for the product with v); 0 where a
+ * token sees no key.  Query head h reads key head h / (q.heads / num_kv_heads); at most 128 query heads a key
+ * head.  Pages that hold no visible key are not touched (their table entries may be stale).  Visible
+ * keys and values must be finite.  max_len: an upper bound of lengths that only guides how the work is split
+ * (0 = max_pages * page_size).  q and out must not overlap.  workspace: 256-byte aligned,
+ * lng_kv_attend_workspace_bytes bytes, used by this call alone until it has finished. */
+size_t lng_kv_attend_workspace_bytes(const lng_kv_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
+                                     int32_t q_heads, int32_t window, int32_t sinks);
+int lng_kv_attend(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,
+                  const lng_kv_rows* q, float scale, int32_t window, int32_t sinks, const lng_kv_rows* out,
+                  void* workspace, size_t workspace_bytes, lng_stream_t stream);
+
+/* lng_kv_attend (no window) for a batch whose sequences all begin with the same prefix_len keys, kept once in
+ * the pages prefix_table[0 .. ceil(prefix_len / page_size) - 1] (i32, device): every token sees the whole
+ * prefix and, causally, its own sequence's keys (table, lengths), which come after it.  The prefix is read
+ * once for the batch. */
+size_t lng_kv_prefix_workspace_bytes(const lng_kv_cache* cache, int64_t prefix_len, int64_t tokens, int64_t max_new,
+                                     int64_t max_len, int32_t q_heads);
+int lng_kv_prefix_attend(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len, const int32_t* cu,
+                         int64_t tokens, int64_t max_new, int64_t max_len, const lng_kv_rows* q, float scale,
+                         const lng_kv_rows* out, void* workspace, size_t workspace_bytes, lng_stream_t stream);
 
 #ifdef __cplusplus
 }

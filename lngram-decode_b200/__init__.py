@@ -20,3 +20,6 @@ from . import serving, sharded  # noqa: E402
 from .sharded import RouteShardedMemory  # noqa: E402
 
 __all__ += ["RouteShardedMemory", "serving", "sharded"]
+from .kv import PagedKVCache, attention_step, kv_append, kv_attend, kv_prefix_attend  # noqa: E402
+
+__all__ += ["PagedKVCache", "attention_step", "kv_append", "kv_attend", "kv_prefix_attend"]

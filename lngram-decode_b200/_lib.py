@@ -60,9 +60,23 @@ class DrafterNumbers(C.Structure):
                 ("orders", C.c_int32 * MAX_ORDERS)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("page_size", C.c_int32),
+                ("num_pages", C.c_int64), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("k_page_stride", C.c_int64), ("k_head_stride", C.c_int64), ("k_slot_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_head_stride", C.c_int64), ("v_slot_stride", C.c_int64),
+                ("table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int64),
+                ("lengths", C.c_void_p), ("batch", C.c_int64)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32)]
+
+
 P = C.c_void_p
 i32, i64, f32, sz = C.c_int32, C.c_int64, C.c_float, C.c_size_t
 PT, PR = C.POINTER(Tables), C.POINTER(Readout)
+PK, PW = C.POINTER(KvCache), C.POINTER(KvRows)
 
 # name -> (restype, argtypes); mirrors include/lngram_b200.h
 SIGNATURES = {
@@ -119,6 +133,11 @@ SIGNATURES = {
     "lng_tree_workspace_bytes": (C.c_size_t, [PT, PR, i64, i64, i64]),
     "lng_tree_memory_block": (C.c_int, [PT, PR, i64, i64, i64, i64, i64, i64, P, P, P, P, P, P, P, P, P, P, P,
                                         C.c_size_t, P]),
+    "lng_kv_append": (C.c_int, [PK, P, i64, i64, PW, PW, PW, PW, P, P, i32, i32, P]),
+    "lng_kv_attend_workspace_bytes": (sz, [PK, i64, i64, i64, i32, i32, i32]),
+    "lng_kv_attend": (C.c_int, [PK, P, i64, i64, i64, PW, f32, i32, i32, PW, P, sz, P]),
+    "lng_kv_prefix_workspace_bytes": (sz, [PK, i64, i64, i64, i64, i32]),
+    "lng_kv_prefix_attend": (C.c_int, [PK, P, i64, P, i64, i64, i64, PW, f32, PW, P, sz, P]),
     "lng_online_counts_mix": (C.c_int, [P, i64, i64, P, i32, i32, P, P, P, i64, i64, P, P, i64, f32, P, P]),
 }
 

@@ -14,6 +14,7 @@ enum DeviceError : unsigned int {
   DEV_ERR_CODE_RANGE = 1,   // a route code >= 2^bits (treated as an invalid window)
   DEV_ERR_WAIT_TIMEOUT = 2, // a bounded mbarrier wait expired
   DEV_ERR_TOKEN_RANGE = 3,  // a token id outside [0, vocab)
+  DEV_ERR_KV_RANGE = 4,     // a page, length or row offset of a key/value cache out of range
 };
 
 struct TableSet {

@@ -22,6 +22,7 @@
 #include "drafter_ext.cuh"
 #include "surrogate.cuh"
 #include "online.cuh"
+#include "kvcache.cuh"
 
 static int scratch_alloc(void** p, size_t bytes, cudaStream_t stream);
 
@@ -1658,3 +1659,168 @@ extern "C" int lng_online_counts_mix(const int64_t* codes, int64_t T, int64_t R,
 }
 
 #include "drafter.cuh"
+
+// ====================================================================== paged keys and values
+namespace lng {
+
+static int check_kv(const lng_kv_cache* c, const int32_t* cu, int64_t tokens, int64_t max_new) {
+  LNG_REQUIRE(c != nullptr, "cache descriptor is NULL");
+  LNG_REQUIRE(c->dtype == LNG_BF16 || c->dtype == LNG_F16, "cache dtype must be bf16 or f16");
+  LNG_REQUIRE(c->page_size >= 8 && c->page_size <= 4096 && (c->page_size & (c->page_size - 1)) == 0,
+              "page_size must be a power of two in [8, 4096]");
+  LNG_REQUIRE(c->num_pages >= 1 && c->num_pages < (int64_t(1) << 31), "num_pages must be in [1, 2^31)");
+  LNG_REQUIRE(c->num_kv_heads >= 1 && c->num_kv_heads <= 65535, "num_kv_heads must be in [1, 65535]");
+  LNG_REQUIRE(c->head_dim >= 8 && c->head_dim <= 128 && c->head_dim % 8 == 0, "head_dim must be a multiple of 8 up to 128");
+  LNG_REQUIRE(c->batch >= 0 && c->max_pages >= 0, "batch and max_pages must not be negative");
+  LNG_REQUIRE(c->max_pages < (int64_t(1) << 30) / c->page_size, "max_pages * page_size must be below 2^30");
+  LNG_REQUIRE(c->table_stride >= c->max_pages, "table_stride must be at least max_pages");
+  LNG_REQUIRE(max_new >= 0 && max_new < (int64_t(1) << 30), "max_new must be in [0, 2^30)");
+  LNG_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 31), "tokens must be in [0, 2^31)");
+  LNG_REQUIRE(cu != nullptr || tokens == c->batch * max_new, "without cu, tokens must be batch * max_new");
+  if (tokens == 0 || c->batch == 0) return LNG_OK;
+  LNG_REQUIRE(max_new >= 1, "max_new must be positive");
+  LNG_REQUIRE(c->k && c->v && c->lengths && (c->table || c->max_pages == 0), "NULL pointer in the cache descriptor");
+  LNG_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) == 0,
+              "k and v must be 16-byte aligned");
+  for (int64_t s : {c->k_page_stride, c->k_head_stride, c->k_slot_stride, c->v_page_stride, c->v_head_stride, c->v_slot_stride})
+    LNG_REQUIRE(s > 0 && s % 8 == 0 && s < (int64_t(1) << 38), "cache strides must be positive multiples of 8 elements");
+  return LNG_OK;
+}
+
+static int check_kv_rows(const lng_kv_rows* r, int64_t heads, const char* what) {
+  const std::string w(what);
+  LNG_REQUIRE(r != nullptr && r->ptr != nullptr, w + " is NULL");
+  LNG_REQUIRE(heads <= 0 || r->heads == heads, w + ": wrong number of heads");
+  LNG_REQUIRE(r->heads >= 1 && r->heads <= (1 << 20), w + ": heads must be positive");
+  LNG_REQUIRE((reinterpret_cast<uintptr_t>(r->ptr) & 15) == 0, w + " must be 16-byte aligned");
+  LNG_REQUIRE(r->token_stride > 0 && r->token_stride % 8 == 0 && r->head_stride > 0 && r->head_stride % 8 == 0 &&
+                  r->token_stride < (int64_t(1) << 38) && r->head_stride < (int64_t(1) << 38),
+              w + ": strides must be positive multiples of 8 elements");
+  return LNG_OK;
+}
+
+static KvView kv_view(const lng_kv_cache* c, const int32_t* cu, int64_t tokens, int64_t max_new) {
+  KvView v{};
+  v.k = c->k;
+  v.v = c->v;
+  v.k_page = c->k_page_stride;
+  v.k_head = c->k_head_stride;
+  v.k_slot = c->k_slot_stride;
+  v.v_page = c->v_page_stride;
+  v.v_head = c->v_head_stride;
+  v.v_slot = c->v_slot_stride;
+  v.table = c->table;
+  v.table_stride = c->table_stride;
+  v.num_pages = c->num_pages;
+  v.lengths = c->lengths;
+  v.cu = cu;
+  v.batch = c->batch;
+  v.tokens = tokens;
+  v.kv_heads = c->num_kv_heads;
+  v.head_dim = c->head_dim;
+  for (v.page_shift = 0; (1 << v.page_shift) < c->page_size; ++v.page_shift) {
+  }
+  v.capacity = int32_t(c->max_pages * c->page_size);
+  v.max_new = int32_t(max_new);
+  return v;
+}
+
+static KvRows kv_rows(const lng_kv_rows* r) { return r ? KvRows{r->ptr, r->token_stride, r->head_stride} : KvRows{}; }
+
+static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len, const int32_t* cu,
+                         int64_t tokens, int64_t max_new, int64_t max_len, const lng_kv_rows* q, float scale,
+                         int32_t window, int32_t sinks, const lng_kv_rows* out, void* workspace, size_t workspace_bytes,
+                         lng_stream_t stream) {
+  int st = check_kv(cache, cu, tokens, max_new);
+  if (st) return st;
+  LNG_REQUIRE(max_len >= 0, "max_len must not be negative");
+  LNG_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  LNG_REQUIRE(scale > 0.f && scale <= 3.0e38f, "scale must be positive and finite");
+  LNG_REQUIRE(prefix_len >= 0 && prefix_len < (int64_t(1) << 30), "prefix_len must be in [0, 2^30)");
+  if (tokens == 0 || cache->batch == 0) return LNG_OK;
+  LNG_REQUIRE(prefix_len == 0 || prefix_table != nullptr, "prefix_table is NULL");
+  if ((st = check_kv_rows(q, 0, "q"))) return st;
+  LNG_REQUIRE(q->heads % cache->num_kv_heads == 0 && q->heads / cache->num_kv_heads <= 128,
+              "query heads must be a multiple of the key heads, at most 128 a key head");
+  if ((st = check_kv_rows(out, q->heads, "out"))) return st;
+  LNG_REQUIRE(out->ptr != q->ptr, "out must not overlap q");
+  const KvView v = kv_view(cache, cu, tokens, max_new);
+  const int64_t warps = tokens * q->heads;
+  const unsigned grid = unsigned(ceil_div(warps, 4));
+  if (cache->dtype == LNG_BF16)
+    kv_attend_rows_kernel<__nv_bfloat16><<<grid, 128, 0, S(stream)>>>(v, kv_rows(q), kv_rows(out), q->heads, scale, window,
+                                                                    sinks, prefix_table, int32_t(prefix_len));
+  else
+    kv_attend_rows_kernel<__half><<<grid, 128, 0, S(stream)>>>(v, kv_rows(q), kv_rows(out), q->heads, scale, window, sinks,
+                                                              prefix_table, int32_t(prefix_len));
+  LNG_LAUNCHED("kv_attend_rows_kernel");
+  return LNG_OK;
+}
+
+}  // namespace lng
+
+extern "C" int lng_kv_append(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new,
+                             const lng_kv_rows* k, const lng_kv_rows* v, const lng_kv_rows* q, const lng_kv_rows* q_out,
+                             const int64_t* positions, const float* inv_freq, int32_t rotary_dim, int32_t interleaved,
+                             lng_stream_t stream) {
+  int st = check_kv(cache, cu, tokens, max_new);
+  if (st) return st;
+  LNG_REQUIRE(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= cache->head_dim,
+              "rotary_dim must be even and at most head_dim");
+  LNG_REQUIRE((q == nullptr) == (q_out == nullptr), "q and q_out go together");
+  if (tokens == 0 || cache->batch == 0) return LNG_OK;
+  LNG_REQUIRE(rotary_dim == 0 || inv_freq != nullptr, "inv_freq is NULL");
+  if ((st = check_kv_rows(k, cache->num_kv_heads, "k")) || (st = check_kv_rows(v, cache->num_kv_heads, "v"))) return st;
+  if (q && ((st = check_kv_rows(q, 0, "q")) || (st = check_kv_rows(q_out, q->heads, "q_out")))) return st;
+  LNG_REQUIRE(!q || q->ptr != q_out->ptr || (q->token_stride == q_out->token_stride && q->head_stride == q_out->head_stride),
+              "q_out must be q itself or not overlap it");
+  const KvView c = kv_view(cache, cu, tokens, max_new);
+  const int q_heads = q ? q->heads : 0;
+  const KvRows kr = kv_rows(k), vr = kv_rows(v), qr = kv_rows(q), qo = kv_rows(q_out);
+  // four tokens a CTA give every thread several independent 16-byte vectors; steps of few tokens spread
+  // over as many SMs as they have tokens instead
+  const bool few = tokens <= int64_t(num_sms()) * 4;
+  const unsigned grid = unsigned(std::min<int64_t>(few ? tokens : ceil_div(tokens, 4), int64_t(num_sms()) * 8));
+#define LNG_KVA(T, TPC)                                                                                          \
+  kv_append_kernel<T, TPC><<<grid, 256, 0, S(stream)>>>(c, kr, vr, qr, qo, q_heads, positions, inv_freq, rotary_dim, \
+                                                        interleaved)
+  if (cache->dtype == LNG_BF16) {
+    if (few)
+      LNG_KVA(__nv_bfloat16, 1);
+    else
+      LNG_KVA(__nv_bfloat16, 4);
+  } else {
+    if (few)
+      LNG_KVA(__half, 1);
+    else
+      LNG_KVA(__half, 4);
+  }
+#undef LNG_KVA
+  LNG_LAUNCHED("kv_append_kernel");
+  return LNG_OK;
+}
+
+extern "C" size_t lng_kv_attend_workspace_bytes(const lng_kv_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
+                                                int32_t q_heads, int32_t window, int32_t sinks) {
+  return 0;
+}
+
+extern "C" int lng_kv_attend(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,
+                             const lng_kv_rows* q, float scale, int32_t window, int32_t sinks, const lng_kv_rows* out,
+                             void* workspace, size_t workspace_bytes, lng_stream_t stream) {
+  return kv_attend_run(cache, nullptr, 0, cu, tokens, max_new, max_len, q, scale, window, sinks, out, workspace,
+                       workspace_bytes, stream);
+}
+
+extern "C" size_t lng_kv_prefix_workspace_bytes(const lng_kv_cache* cache, int64_t prefix_len, int64_t tokens,
+                                                int64_t max_new, int64_t max_len, int32_t q_heads) {
+  return 0;
+}
+
+extern "C" int lng_kv_prefix_attend(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len,
+                                    const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len, const lng_kv_rows* q,
+                                    float scale, const lng_kv_rows* out, void* workspace, size_t workspace_bytes,
+                                    lng_stream_t stream) {
+  return kv_attend_run(cache, prefix_table, prefix_len, cu, tokens, max_new, max_len, q, scale, 0, 0, out, workspace,
+                       workspace_bytes, stream);
+}

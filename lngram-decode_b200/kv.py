@@ -1,0 +1,259 @@
+"""A paged cache of keys and values for the attention that runs beside the memory layer in a decode loop.
+
+The reference's ``decode_step`` keeps dense keys and values in its ``DecodeState``
+(``ffnmem/infer.py:65-112``); here they lie in pages that a server hands out as sequences grow:
+
+* ``PagedKVCache`` -- the pages, the page table and the sequences' lengths (device tensors; the lengths count
+  a step's new tokens from ``extend`` on).
+* ``kv_append`` -- a step's keys and values into their slots, keys and queries rotated by position on the way.
+* ``kv_attend`` -- causal attention of the step's tokens over the cache: grouped heads, an optional sliding
+  window with the first ``sinks`` tokens visible beside it; one token a sequence or whole prompts.
+* ``kv_prefix_attend`` -- the same for a batch whose sequences share one prefix, read once for all of them.
+* ``attention_step`` -- extend, append and attend in one call, the counterpart of ``seams.memory_step``.
+
+A step's tokens are ``[B, n, heads, head_dim]`` (n new tokens for every sequence) or, for sequences that add
+unlike numbers of tokens, ``[tokens, heads, head_dim]`` with ``cu`` (int32 ``[B + 1]`` offsets on the device)
+and ``max_new`` (a host bound of one sequence's new tokens).  The inner dimension is contiguous, the others
+may be strided (slices of a fused projection).  Everything is asynchronous on the current stream and can be
+captured into a CUDA graph: table and lengths are read when the kernels run.
+
+    cache = PagedKVCache.allocate(B, max_len, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda")
+    cache.extend(n)                                       # the lengths now count the step's tokens
+    q = kv_append(cache, k, v, q, inv_freq=inv_freq)      # rotated queries; keys and values cached
+    out = kv_attend(cache, q, window=4096, sinks=4)       # [B, n, heads, head_dim]
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._lib import check, ptr, stream_ptr
+
+_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def _require(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+class PagedKVCache:
+    """``k``, ``v``: pages ``[pages, kv_heads, page_size, head_dim]`` (bf16 or fp16; any view whose inner dimension
+    is contiguous, so pages laid out ``[pages, page_size, kv_heads, head_dim]`` are passed transposed);
+    ``table``: int32 ``[B, max_pages]``, the page of every ``page_size`` keys of a sequence; ``lengths``: int32
+    ``[B]``.  The tensors are kept, not copied: write table and lengths in place."""
+
+    def __init__(self, k: Tensor, v: Tensor, table: Tensor, lengths: Tensor):
+        _require(k.dim() == 4 and v.shape == k.shape, "k and v must be [pages, kv_heads, page_size, head_dim], alike")
+        _require(k.dtype in _DTYPES and v.dtype == k.dtype, "k and v must be bfloat16 or float16, alike")
+        pages, heads, size, dim = k.shape
+        _require(size >= 8 and size <= 4096 and size & (size - 1) == 0, "page_size must be a power of two in [8, 4096]")
+        _require(8 <= dim <= 128 and dim % 8 == 0, "head_dim must be a multiple of 8 up to 128")
+        _require(pages >= 1 and heads >= 1, "the cache needs at least one page and one head")
+        for t in (k, v):
+            _require(t.stride(3) == 1 and all(t.stride(i) > 0 and t.stride(i) % 8 == 0 for i in range(3)),
+                     "the head dimension must be contiguous and the other strides positive multiples of 8")
+            _require(t.data_ptr() % 16 == 0, "k and v must be 16-byte aligned")
+        _require(table.dim() == 2 and table.dtype == torch.int32 and (table.shape[1] <= 1 or table.stride(1) == 1),
+                 "table must be int32 [B, max_pages] with contiguous rows")
+        _require(lengths.dim() == 1 and lengths.dtype == torch.int32 and lengths.is_contiguous(),
+                 "lengths must be contiguous int32 [B]")
+        _require(lengths.shape[0] == table.shape[0], "table and lengths must have one row a sequence")
+        _require(table.shape[1] * size < 1 << 30, "max_pages * page_size must be below 2^30")
+        _require(k.device == v.device == table.device == lengths.device, "the cache's tensors must be on one device")
+        self._k, self._v, self._table, self._lengths = k, v, table, lengths
+        self._desc = _lib.KvCache(k=k.data_ptr(), v=v.data_ptr(), dtype=_lib.dtype_code(k.dtype), page_size=size,
+                                  num_pages=pages, num_kv_heads=heads, head_dim=dim, k_page_stride=k.stride(0),
+                                  k_head_stride=k.stride(1), k_slot_stride=k.stride(2), v_page_stride=v.stride(0),
+                                  v_head_stride=v.stride(1), v_slot_stride=v.stride(2), table=table.data_ptr(),
+                                  table_stride=max(table.stride(0), table.shape[1]), max_pages=table.shape[1],
+                                  lengths=lengths.data_ptr(), batch=table.shape[0])
+        self._ref = C.byref(self._desc)
+        self.device, self.dtype = k.device, k.dtype
+        self.batch, self.page_size, self.num_kv_heads, self.head_dim = table.shape[0], size, heads, dim
+        self.capacity = table.shape[1] * size
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    table = property(lambda self: self._table)
+    lengths = property(lambda self: self._lengths)
+
+    @classmethod
+    def allocate(cls, batch: int, max_len: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
+                 dtype: torch.dtype = torch.bfloat16, device=None) -> "PagedKVCache":
+        """An empty cache in which every sequence owns ceil(max_len / page_size) pages."""
+        device = device or torch.device("cuda", torch.cuda.current_device())
+        per = -(-int(max_len) // page_size)
+        shape = (max(1, batch * per), num_kv_heads, page_size, head_dim)
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                   torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per),
+                   torch.zeros(batch, dtype=torch.int32, device=device))
+
+    def extend(self, n) -> None:
+        """Count n (an int, or int32 [B] on the device) new tokens a sequence."""
+        self._lengths.add_(n)
+
+    def truncate(self, lengths) -> None:
+        """Forget the keys behind ``lengths`` (an int, or int32 [B]), e.g. rejected drafts."""
+        if isinstance(lengths, Tensor):
+            torch.minimum(self._lengths, lengths.to(self._lengths), out=self._lengths)
+        else:
+            self._lengths.clamp_(max=int(lengths))
+
+
+def _rows(t: Tensor, what: str, cache: PagedKVCache, shape=None, heads: int | None = None) -> _lib.KvRows:
+    """The descriptor of a step's rows; ``shape``: the leading shape they must have."""
+    _require(t.dtype == cache.dtype, f"{what} must have the cache's dtype {cache.dtype}")
+    _require(t.dim() in (3, 4) and t.shape[-1] == cache.head_dim,
+             f"{what} must be [B, n, heads, {cache.head_dim}] or [tokens, heads, {cache.head_dim}]")
+    if shape is not None:
+        _require(t.shape[:-2] == shape, f"{what} must have the step's leading shape {tuple(shape)}")
+    if heads is not None:
+        _require(t.shape[-2] == heads, f"{what} must have {heads} heads")
+    st = t.stride()
+    n = t.shape[-2]
+    head = st[-2] if n > 1 else cache.head_dim
+    token = st[-3] if t.shape[-3] > 1 else (st[0] if t.dim() == 4 and t.shape[0] > 1 else n * cache.head_dim)
+    if t.dim() == 4 and t.shape[0] > 1 and t.shape[1] > 1:
+        _require(st[0] == st[1] * t.shape[1], f"{what}: the tokens of all sequences must lie at one stride")
+    _require(st[-1] == 1 and head > 0 and head % 8 == 0 and token > 0 and token % 8 == 0 and t.data_ptr() % 16 == 0,
+             f"{what} must be 16-byte aligned with a contiguous head dimension and strides of positive multiples of 8")
+    _require(t.device == cache.device, f"{what} must be on the cache's device")
+    return _lib.KvRows(t.data_ptr(), token, head, n)
+
+
+def _step(cache: PagedKVCache, t: Tensor, cu: Tensor | None, max_new: int | None):
+    """(tokens, max_new) of a step whose rows are shaped like t."""
+    if cu is None:
+        _require(t.dim() == 4 and t.shape[0] == cache.batch,
+                 f"without cu the step's rows must be [B = {cache.batch}, n, heads, {cache.head_dim}]")
+        _require(max_new is None or max_new == t.shape[1], "max_new must be the step's n when there is no cu")
+        return t.shape[0] * t.shape[1], t.shape[1]
+    _require(t.dim() == 3, "with cu the step's rows must be [tokens, heads, head_dim]")
+    _require(cu.dtype == torch.int32 and cu.dim() == 1 and cu.shape[0] == cache.batch + 1 and cu.is_contiguous()
+             and cu.device == cache.device, f"cu must be contiguous int32 [{cache.batch + 1}] on the cache's device")
+    _require(max_new is not None and max_new >= 0, "a step with cu needs max_new")
+    return t.shape[0], int(max_new)
+
+
+def _on_gpu(cache: PagedKVCache) -> None:
+    if cache.device.type != "cuda":
+        raise RuntimeError("the cache must be on a CUDA device: lngram_b200 has no CPU path")
+
+
+@torch.no_grad()
+def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None, *, cu: Tensor | None = None,
+              max_new: int | None = None, positions: Tensor | None = None, inv_freq: Tensor | None = None,
+              interleaved: bool = False, q_out: Tensor | None = None) -> Tensor | None:
+    """Write a step's keys and values to the cache: token i of the n new ones of a sequence becomes key
+    ``lengths - n + i`` (``extend`` first).  With ``inv_freq`` (fp32 ``[rotary_dim / 2]``) the first rotary_dim
+    values of keys and queries are rotated by the token's position -- ``positions`` (int64, the step's leading
+    shape) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
+    Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``."""
+    tokens, max_new = _step(cache, k, cu, max_new)
+    lead = k.shape[:-2]
+    kr = _rows(k, "k", cache, lead, cache.num_kv_heads)
+    vr = _rows(v, "v", cache, lead, cache.num_kv_heads)
+    qr = qo = None
+    if q is not None:
+        qr = C.byref(_rows(q, "q", cache, lead))
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qo = C.byref(_rows(q_out, "q_out", cache, lead, q.shape[-2]))
+    else:
+        _require(q_out is None, "q_out without q")
+    rotary = 0
+    if inv_freq is not None:
+        _require(inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
+                 and inv_freq.device == cache.device, "inv_freq must be contiguous fp32 [rotary_dim / 2] on the cache's device")
+        rotary = 2 * inv_freq.shape[0]
+        _require(rotary <= cache.head_dim, "inv_freq has more pairs than the head")
+    if positions is not None:
+        _require(positions.dtype == torch.int64 and positions.shape == lead and positions.is_contiguous()
+                 and positions.device == cache.device, "positions must be contiguous int64 of the step's leading shape")
+    _on_gpu(cache)
+    with _lib.on_device(cache.device):
+        check(_lib.library().lng_kv_append(cache._ref, ptr(cu), tokens, max_new, C.byref(kr), C.byref(vr), qr, qo,
+                                           ptr(positions), ptr(inv_freq) if rotary else None, rotary, int(bool(interleaved)),
+                                           stream_ptr()), "kv_append")
+    return q_out
+
+
+def _attend_args(cache, q, cu, max_new, max_len, scale, out):
+    tokens, max_new = _step(cache, q, cu, max_new)
+    qr = _rows(q, "q", cache)
+    heads = q.shape[-2]
+    _require(heads % cache.num_kv_heads == 0 and 1 <= heads // cache.num_kv_heads <= 128,
+             "query heads must be a multiple of the key heads, at most 128 a key head")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    orow = _rows(out, "out", cache, q.shape[:-2], heads)
+    _require(tokens == 0 or out.data_ptr() != q.data_ptr(), "out must not overlap q")
+    max_len = cache.capacity if max_len is None else int(max_len)
+    _require(max_len >= 0, "max_len must not be negative")
+    scale = cache.head_dim ** -0.5 if scale is None else float(scale)
+    _require(0.0 < scale < 3e38, "scale must be positive and finite")
+    return tokens, max_new, max_len, qr, heads, scale, out, orow
+
+
+@torch.no_grad()
+def kv_attend(cache: PagedKVCache, q: Tensor, *, cu: Tensor | None = None, max_new: int | None = None,
+              max_len: int | None = None, window: int = 0, sinks: int = 0, scale: float | None = None,
+              out: Tensor | None = None) -> Tensor:
+    """Causal attention of a step's tokens over the cache, whose lengths count them (``kv_append`` first): the
+    token at position p sees keys j <= p; with ``window`` > 0 only its last ``window`` keys and the first
+    ``sinks`` of the sequence.  softmax(scale q . k) v with ``scale`` = head_dim^-1/2 by default; a token
+    that sees no key gets zeros.  ``max_len`` (a host bound of the lengths) only guides how the work is split.
+    Rows of ``q`` that belong to no sequence are skipped: their rows of ``out`` stay as they are."""
+    tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
+    window, sinks = int(window), int(sinks)
+    _require(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+    window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
+    _on_gpu(cache)
+    lib = _lib.library()
+    with _lib.on_device(cache.device):
+        need = lib.lng_kv_attend_workspace_bytes(cache._ref, tokens, max_new, max_len, heads, window, sinks)
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        check(lib.lng_kv_attend(cache._ref, ptr(cu), tokens, max_new, max_len, C.byref(qr), scale, window, sinks,
+                                C.byref(orow), ptr(ws), need, stream_ptr()), "kv_attend")
+    return out
+
+
+@torch.no_grad()
+def kv_prefix_attend(cache: PagedKVCache, q: Tensor, prefix_table: Tensor, prefix_len: int, *, cu: Tensor | None = None,
+                     max_new: int | None = None, max_len: int | None = None, scale: float | None = None,
+                     out: Tensor | None = None) -> Tensor:
+    """``kv_attend`` (without a window) for a batch whose sequences all begin with the ``prefix_len`` keys in the
+    pages ``prefix_table`` (int32 ``[>= ceil(prefix_len / page_size)]``) of the same cache; ``table`` and
+    ``lengths`` hold what each sequence adds to it.  The prefix is read once for the whole batch."""
+    tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
+    prefix_len = int(prefix_len)
+    _require(0 <= prefix_len < 1 << 30, "prefix_len must be in [0, 2^30)")
+    _require(prefix_table.dtype == torch.int32 and prefix_table.dim() == 1 and prefix_table.is_contiguous()
+             and prefix_table.device == cache.device, "prefix_table must be contiguous int32 on the cache's device")
+    _require(prefix_table.shape[0] * cache.page_size >= prefix_len, "prefix_table has too few pages for prefix_len")
+    _on_gpu(cache)
+    lib = _lib.library()
+    with _lib.on_device(cache.device):
+        need = lib.lng_kv_prefix_workspace_bytes(cache._ref, prefix_len, tokens, max_new, max_len, heads)
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        check(lib.lng_kv_prefix_attend(cache._ref, ptr(prefix_table) if prefix_len else None, prefix_len, ptr(cu), tokens,
+                                       max_new, max_len, C.byref(qr), scale, C.byref(orow), ptr(ws), need, stream_ptr()),
+              "kv_prefix_attend")
+    return out
+
+
+def attention_step(cache: PagedKVCache, q: Tensor, k: Tensor, v: Tensor, *, cu: Tensor | None = None,
+                   max_new: int | None = None, positions: Tensor | None = None, inv_freq: Tensor | None = None,
+                   interleaved: bool = False, max_len: int | None = None, window: int = 0, sinks: int = 0,
+                   scale: float | None = None, out: Tensor | None = None) -> Tensor:
+    """The attention part of a decode step, beside ``seams.memory_step``: the lengths count the step's tokens,
+    keys and values are appended, and the rotated queries attend."""
+    _step(cache, q, cu, max_new)
+    cache.extend(q.shape[1] if cu is None else cu[1:] - cu[:-1])
+    q = kv_append(cache, k, v, q, cu=cu, max_new=max_new, positions=positions, inv_freq=inv_freq, interleaved=interleaved)
+    return kv_attend(cache, q, cu=cu, max_new=max_new, max_len=max_len, window=window, sinks=sinks, scale=scale, out=out)
