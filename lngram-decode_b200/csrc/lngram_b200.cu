@@ -23,6 +23,7 @@
 #include "surrogate.cuh"
 #include "online.cuh"
 #include "kvcache.cuh"
+#include "kv_step.cuh"
 
 static int scratch_alloc(void** p, size_t bytes, cudaStream_t stream);
 
@@ -1727,6 +1728,70 @@ static KvView kv_view(const lng_kv_cache* c, const int32_t* cu, int64_t tokens, 
 
 static KvRows kv_rows(const lng_kv_rows* r) { return r ? KvRows{r->ptr, r->token_stride, r->head_stride} : KvRows{}; }
 
+// The tensor map of the cache's keys (or values): [pages][heads][slots][head_dim], one head's slots of one
+// page a copy, 64 values wide (a head beyond 64 takes two copies; columns behind head_dim fill with zeros).
+static int kv_page_map(CUtensorMap* map, const lng_kv_cache* c, void* base, int64_t page, int64_t head, int64_t slot, int box) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (driver entry point)");
+  const cuuint64_t dims[4] = {cuuint64_t(c->head_dim), cuuint64_t(c->page_size), cuuint64_t(c->num_kv_heads),
+                              cuuint64_t(c->num_pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(slot) * 2, cuuint64_t(head) * 2, cuuint64_t(page) * 2};
+  const cuuint32_t box4[4] = {64, cuuint32_t(box), 1, 1}, one[4] = {1, 1, 1, 1};
+  const auto type = c->dtype == LNG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = enc(map, type, 4, base, dims, strides, box4, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+  return LNG_OK;
+}
+static int kv_page_maps(CUtensorMap* k, CUtensorMap* v, const lng_kv_cache* c, int box) {
+  int st = kv_page_map(k, c, c->k, c->k_page_stride, c->k_head_stride, c->k_slot_stride, box);
+  return st ? st : kv_page_map(v, c, c->v, c->v_page_stride, c->v_head_stride, c->v_slot_stride, box);
+}
+
+// How an attention call is carried out, and what it needs of the workspace.
+struct KvPlan {
+  bool step;              // at most 16 rows a key head and sequence: kv_step_kernel
+  int shares;             // its CTAs
+  size_t piece_ml, piece_o, bytes;
+};
+static KvPlan kv_plan(const lng_kv_cache* c, int64_t prefix_len, int64_t tokens, int64_t max_new, int64_t max_len, int32_t q_heads,
+                      int32_t window, int32_t sinks) {
+  KvPlan p{};
+  if (!c || tokens <= 0 || c->batch <= 0 || c->num_kv_heads <= 0 || q_heads <= 0) return p;
+  const int64_t group = q_heads / c->num_kv_heads;
+  p.step = group * max_new <= KS_ROWS && prefix_len == 0;
+  if (p.step) {
+    p.shares = num_sms();
+    const size_t rows = size_t(2) * p.shares * KS_ROWS;
+    p.piece_ml = 0;
+    p.piece_o = al256(rows * 8);
+    p.bytes = p.piece_o + al256(rows * c->head_dim * 4);
+  }
+  return p;
+}
+
+template <typename T, int HDP>
+static int launch_kv_step(const CUtensorMap& tk, const CUtensorMap& tv, const KsParams& p, cudaStream_t s) {
+  using Cfg = KsCfg<HDP>;
+  auto kern = kv_step_kernel<T, HDP>;
+  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  kern<<<p.shares, Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
+  LNG_LAUNCHED("kv_step_kernel");
+  // the join is a programmatic dependent: it finds its pieces while the step kernel runs and waits for
+  // it before it reads them
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(p.c.batch * p.c.kv_heads));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  LNG_CUDA(cudaLaunchKernelEx(&cfg, kv_step_join_kernel<T>, p, int(Cfg::WARPS)));
+  return LNG_OK;
+}
+
 static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len, const int32_t* cu,
                          int64_t tokens, int64_t max_new, int64_t max_len, const lng_kv_rows* q, float scale,
                          int32_t window, int32_t sinks, const lng_kv_rows* out, void* workspace, size_t workspace_bytes,
@@ -1744,7 +1809,36 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
               "query heads must be a multiple of the key heads, at most 128 a key head");
   if ((st = check_kv_rows(out, q->heads, "out"))) return st;
   LNG_REQUIRE(out->ptr != q->ptr, "out must not overlap q");
+  LNG_REQUIRE(cache->batch * cache->num_kv_heads < (int64_t(1) << 31), "batch * num_kv_heads must be below 2^31");
+  const KvPlan plan = kv_plan(cache, prefix_len, tokens, max_new, max_len, q->heads, window, sinks);
+  LNG_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
+              "workspace must be 256-byte aligned");
+  LNG_REQUIRE(workspace_bytes >= plan.bytes, "workspace too small");
+  window = std::min(window, 1 << 30);
+  sinks = std::min(sinks, 1 << 30);
   const KvView v = kv_view(cache, cu, tokens, max_new);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (plan.step) {
+    KsParams p{};
+    p.c = v;
+    p.q = kv_rows(q);
+    p.o = kv_rows(out);
+    p.q_heads = q->heads;
+    p.group = q->heads / cache->num_kv_heads;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.window = window;
+    p.sinks = sinks;
+    p.box = std::min(cache->page_size, KS_BK);
+    p.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
+    p.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
+    p.shares = plan.shares;
+    CUtensorMap tk, tv;
+    if ((st = kv_page_maps(&tk, &tv, cache, p.box))) return st;
+    const bool wide = cache->head_dim > 64;
+    if (cache->dtype == LNG_BF16)
+      return wide ? launch_kv_step<__nv_bfloat16, 128>(tk, tv, p, S(stream)) : launch_kv_step<__nv_bfloat16, 64>(tk, tv, p, S(stream));
+    return wide ? launch_kv_step<__half, 128>(tk, tv, p, S(stream)) : launch_kv_step<__half, 64>(tk, tv, p, S(stream));
+  }
   const int64_t warps = tokens * q->heads;
   const unsigned grid = unsigned(ceil_div(warps, 4));
   if (cache->dtype == LNG_BF16)
@@ -1802,7 +1896,7 @@ extern "C" int lng_kv_append(const lng_kv_cache* cache, const int32_t* cu, int64
 
 extern "C" size_t lng_kv_attend_workspace_bytes(const lng_kv_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
                                                 int32_t q_heads, int32_t window, int32_t sinks) {
-  return 0;
+  return kv_plan(cache, 0, tokens, max_new, max_len, q_heads, window, sinks).bytes;
 }
 
 extern "C" int lng_kv_attend(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,
@@ -1814,7 +1908,7 @@ extern "C" int lng_kv_attend(const lng_kv_cache* cache, const int32_t* cu, int64
 
 extern "C" size_t lng_kv_prefix_workspace_bytes(const lng_kv_cache* cache, int64_t prefix_len, int64_t tokens,
                                                 int64_t max_new, int64_t max_len, int32_t q_heads) {
-  return 0;
+  return kv_plan(cache, prefix_len, tokens, max_new, max_len, q_heads, 0, 0).bytes;
 }
 
 extern "C" int lng_kv_prefix_attend(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len,
