@@ -1,0 +1,573 @@
+// Attention of many rows over the paged cache on the tensor cores: prompts, chunks of prompts, batches of
+// drafts, and a whole batch against the prefix that it shares.
+//
+// A CTA takes two tiles of up to 128 (token, head of the key head's group) rows -- the group's heads share
+// every key they load -- and walks the tiles of 128 keys that any of its tokens sees.  Roles:
+//   warp 8   one thread loads: queries once, then keys and values of each tile by TMA, page by page, into a ring;
+//   warps 0-3, 4-7  a row tile each, one row a thread: the first thread issues tcgen05.mma for S = Q K^T (fp32 in
+//            TMEM), all take S from TMEM, keep the running maximum and sum in fp32 and write P, rounded to the
+//            cache's type, over S's columns; the first thread issues O += P V with P read from TMEM.
+// While one row tile's softmax runs, the tensor cores work on the other's: per 128 x 128 block at head size 128
+// both take about 1024 cycles (2 x 128^3 x 2 flops at 8192 a cycle; 16384 exponentials at 16 a cycle).
+// TMEM: S of both tiles (2 x 128 columns, P in the same ones) and O of both (2 x head size) fill its 512 columns.
+// O is rescaled only when a row's maximum has grown by more than 2^8 (8 in base 2): the old reference stays
+// valid, weights reach at most 256, exact in fp32 and in range for fp16, and the quotient is the same.
+// Values are the B operand with the head dimension contiguous (MN-major), just as the pages hold them.
+#pragma once
+
+#include "kv_step.cuh"
+
+namespace lng {
+
+constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 384;
+
+template <int HDP>
+struct KtCfg {
+  static constexpr uint32_t TILE_BYTES = 128 * HDP * 2;  // 128 rows of queries, keys or values
+  static constexpr uint32_t HALF_BYTES = 128 * 128;      // 64 columns of them
+  static constexpr int SLOTS = HDP == 128 ? 5 : 8;
+  static constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;
+  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE_BYTES + 1024 + 256;
+};
+
+struct KtParams {
+  KvView c;
+  KvRows o;
+  int32_t q_heads, group, tile_tokens;  // tile_tokens = 128 / group
+  float scale_log2;
+  int32_t window, sinks;
+  int32_t box;              // keys a TMA copy: min(page size, 128)
+  int32_t splits;           // key ranges a unit's tiles are divided into (grid z)
+  const int32_t* prefix_table;  // not null: all tokens against the shared prefix, every key visible
+  int32_t prefix_len;
+  float2* row_ml;           // split or prefix: states to [slot0 + split][row], row = token * q_heads + head
+  float* row_o;
+  int32_t slot0;
+};
+
+// Base of a column range of the CTA's TMEM for the lanes of this warp's quadrant.
+__device__ __forceinline__ uint32_t tmem_at(uint32_t tmem, int quadrant, uint32_t col) {
+  return tmem + (uint32_t(quadrant * 32) << 16) + col;
+}
+
+#define LNG_I8(a, o) "r"((a)[(o)]), "r"((a)[(o) + 1]), "r"((a)[(o) + 2]), "r"((a)[(o) + 3]), "r"((a)[(o) + 4]), \
+                     "r"((a)[(o) + 5]), "r"((a)[(o) + 6]), "r"((a)[(o) + 7])
+// (tmem_ld32 loads are asynchronous: their registers are only used behind tmem_wait32, which names them, so
+// that no use of them can be moved in front of the wait.)
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::LNG_I8(r, 0),
+      LNG_I8(r, 8), LNG_I8(r, 16), LNG_I8(r, 24), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::LNG_I8(r, 0),
+      LNG_I8(r, 8), "r"(addr)
+      : "memory");
+}
+#undef LNG_I8
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// kind::f16 with A from TMEM (two 16-bit values of a row in a column).
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+// B operand with N contiguous (one block of 64 columns), 128-byte swizzle: groups of 8 rows of K 1024 bytes
+// apart.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(const void* tile) {
+  uint64_t d = (smem_addr(tile) >> 4) & 0x3FFFull;
+  d |= uint64_t(1) << 16;  // leading byte offset (unused: one block)
+  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t umma_idesc(int M, int N, bool b_mn) {
+  const uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(b_mn) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// The unit (2 * tile_tokens tokens of one sequence) of a CTA: tokens t0 .. of the span, or n = 0 when there is
+// none.  Steps of equal n: the last units of all sequences, which see the most keys, come first.  Ragged
+// steps: the sequences' units in a line, last units first within a sequence.
+struct KtUnit {
+  SeqSpan s;
+  int64_t b;
+  int32_t t0;
+};
+
+__device__ inline KtUnit kt_find(const KvView& c, const int32_t* prefix_table, int32_t prefix_len, int64_t u, int32_t span,
+                                 int nthreads, int64_t* warp_tot, KtUnit* found) {
+  KtUnit r{};
+  if (prefix_table != nullptr) {  // all tokens of the step are one sequence
+    int64_t first = 0, end = c.tokens;
+    if (c.cu != nullptr) {
+      first = c.cu[0];
+      end = c.cu[c.batch];
+      if (first < 0 || end < first || end > c.tokens) {
+        kv_range_error();
+        first = first < 0 ? 0 : first > c.tokens ? c.tokens : first;
+        end = end > c.tokens ? c.tokens : end < first ? first : end;
+      }
+    }
+    r.b = 0;
+    r.s.first = first;
+    r.s.n = int32_t(end - first);
+    r.s.len = prefix_len;
+    r.t0 = int32_t(u * span < r.s.n ? u * span : r.s.n);
+    return r;
+  }
+  if (c.cu == nullptr) {
+    const int64_t per = (c.max_new + span - 1) / span;
+    r.b = u % c.batch;
+    r.s = kv_span(c, r.b);
+    const int64_t k = u / c.batch;
+    r.t0 = k < per ? int32_t((per - 1 - k) * span) : r.s.n;
+    return r;
+  }
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t run = (c.batch + nthreads - 1) / nthreads;
+  const int64_t b0 = tid * run, b1 = b0 + run < c.batch ? b0 + run : c.batch;
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += (kv_span(c, b).n + span - 1) / span;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_tot[warp] = incl;
+  if (tid == 0) found->b = -1;
+  __syncthreads();
+  int64_t at = incl - mine;
+  for (int w = 0; w < warp; ++w) at += warp_tot[w];
+  if (u >= at && u < at + mine) {
+    for (int64_t b = b0; b < b1; ++b) {
+      const SeqSpan s = kv_span(c, b);
+      const int64_t n = (s.n + span - 1) / span;
+      if (u < at + n) {
+        found->s = s;
+        found->b = b;
+        found->t0 = int32_t((n - 1 - (u - at)) * span);
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  if (found->b < 0) return r;
+  return *found;
+}
+
+// What every role of a CTA knows about its unit: the two row tiles' tokens, positions and key tiles.
+struct KtWork {
+  SeqSpan s;
+  int64_t b;
+  int32_t t0, window, sinks;
+  int32_t tokens0, tokens1;  // tokens of the two row tiles
+  int32_t pos0, pos1, last0, last1;  // first and last position of each row tile
+  int32_t cnt0, cnt1;        // key tiles [j0, cnt) are visited for a row tile
+  int32_t j0, jend;
+  bool shared;
+  KeySpan span;
+  KeyTiles tiles;
+};
+template <int G> __device__ __forceinline__ int32_t kt_tokens(const KtWork& w) { return G ? w.tokens1 : w.tokens0; }
+template <int G> __device__ __forceinline__ int32_t kt_first(const KtWork& w) { return G ? w.pos1 : w.pos0; }
+template <int G> __device__ __forceinline__ int32_t kt_last(const KtWork& w) { return G ? w.last1 : w.last0; }
+template <int G> __device__ __forceinline__ int32_t kt_cnt(const KtWork& w) { return G ? w.cnt1 : w.cnt0; }
+
+__device__ __forceinline__ int32_t kt_count(const KeyTiles& t, int32_t last, int32_t tokens, int32_t j0, int32_t j1) {
+  const int32_t end = last >= 0 && tokens > 0 ? last / KT_BK + 1 : 0;  // tiles of the keys up to `last`
+  int32_t n = end <= t.first ? (end < t.sink_tiles ? end : t.sink_tiles) : t.sink_tiles + end - t.first;
+  n = n < j1 ? n : j1;
+  return n > j0 ? n : j0;
+}
+
+// Shared memory behind the tiles.
+template <int HDP>
+struct KtBars {
+  uint64_t kv_full[KtCfg<HDP>::SLOTS], kv_empty[KtCfg<HDP>::SLOTS];  // empty: one arrival a row tile
+  uint64_t q_full;
+  uint64_t s_full[2];   // a row tile's scores are in TMEM
+  uint64_t pv_done[2];  // its O += P V is done: O may be read, P overwritten
+  uint32_t tmem, abort;
+};
+
+template <int HDP>
+__device__ __forceinline__ bool kt_wait(KtBars<HDP>* bars, uint64_t* bar, uint32_t parity) {
+  if (*reinterpret_cast<volatile uint32_t*>(&bars->abort)) return false;
+  if (mbar_wait_bounded(bar, parity, &g_error_word, DEV_ERR_WAIT_TIMEOUT)) return true;
+  *reinterpret_cast<volatile uint32_t*>(&bars->abort) = 1u;
+  return false;
+}
+
+// One thread: queries once, then keys and values of every tile, page by page, into the ring.
+template <int HDP>
+__device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv, const KtParams& p,
+                                        const KtWork& w, KtBars<HDP>* bars, uint8_t* qs, uint8_t* ring, int hk) {
+  using Cfg = KtCfg<HDP>;
+  constexpr uint32_t NS = Cfg::SLOTS;
+  const KvView& c = p.c;
+  const int tiles_q = w.tokens1 > 0 ? 2 : 1;
+  mbar_arrive_expect_tx(&bars->q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
+  for (int g = 0; g < tiles_q; ++g)
+#pragma unroll
+    for (int hh = 0; hh < HDP / 64; ++hh)
+      tma_load_3d(qs + g * Cfg::TILE_BYTES + hh * Cfg::HALF_BYTES, tmq, hh * 64, hk * p.group,
+                  int32_t(w.s.first + w.t0 + g * p.tile_tokens), &bars->q_full);
+  const int32_t* row = w.shared ? p.prefix_table : c.table + w.b * c.table_stride;
+  uint32_t it = 0;
+  bool ok = true;
+  for (int32_t j = w.j0; j < w.jend && ok; ++j) {
+    const int32_t key0 = tile_index(w.tiles, j) * KT_BK;
+    uint32_t bytes = 0;
+    for (int32_t r = 0; r < KT_BK; r += p.box)
+      if (any_needed(w.span, key0 + r, key0 + r + p.box)) bytes += uint32_t(p.box) * 128u * (HDP / 64);
+    auto fill = [&](const CUtensorMap* map) -> bool {
+      const uint32_t s = it % NS;
+      if (it >= NS && !kt_wait(bars, &bars->kv_empty[s], (it / NS - 1) & 1)) return false;
+      ++it;
+      mbar_arrive_expect_tx(&bars->kv_full[s], bytes);
+      uint8_t* dst = ring + s * Cfg::TILE_BYTES;
+      for (int32_t r = 0; r < KT_BK; r += p.box) {
+        const int32_t key = key0 + r;
+        if (!any_needed(w.span, key, key + p.box)) continue;
+        int32_t page = page_of(row, key, c.page_shift, c.num_pages);
+        if (page < 0) {
+          kv_range_error();
+          page = int32_t(c.num_pages);  // behind the last page: the copy fills zeros
+        }
+        const int32_t slot = key & ((1 << c.page_shift) - 1);
+#pragma unroll
+        for (int hh = 0; hh < HDP / 64; ++hh)
+          tma_load_4d(dst + hh * Cfg::HALF_BYTES + r * 128, map, hh * 64, slot, hk, page, &bars->kv_full[s]);
+      }
+      return true;
+    };
+    ok = fill(tmk) && fill(tmv);
+  }
+  // the last uses of the ring's slots: behind them no copy and no product is in flight
+  for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait(bars, &bars->kv_empty[k % NS], (k / NS) & 1);
+}
+
+// The 128 threads of row tile G.  Thread 0 of them issues the tile's products; per key tile
+//   S = Q K^T -> softmax in registers, P over S -> O += P V,
+// each committed to an mbarrier and waited for before its operands are touched again (the ISA orders products
+// of unlike operands only through their completion).  The other row tile's products run meanwhile.
+template <typename T, int HDP, int G>
+__device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBars<HDP>* bars, uint32_t tmem, const uint8_t* qs,
+                                        uint8_t* ring, int hk, int split) {
+  using Cfg = KtCfg<HDP>;
+  constexpr uint32_t NS = Cfg::SLOTS;
+  const KvView& c = p.c;
+  const int quad = (threadIdx.x >> 5) & 3, r = quad * 32 + (threadIdx.x & 31);
+  const bool leader = r == 0;
+  const int32_t tok = r / p.group, head = hk * p.group + (r - tok * p.group);
+  const bool mine = tok < kt_tokens<G>(w);
+  const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
+  const int32_t first = kt_first<G>(w), last = kt_last<G>(w), cnt = kt_cnt<G>(w);
+  const int32_t pos = w.shared ? last : first + tok;
+  const int ksteps = (c.head_dim + 15) >> 4;
+  const uint32_t t_s = tmem + Cfg::TMEM_S + G * 128, t_o = tmem + Cfg::TMEM_O + G * HDP;
+  const uint32_t ts = tmem_at(t_s, quad, 0), to = tmem_at(t_o, quad, 0);
+  float m = -INFINITY, l = 0.f;
+  bool ok = true;
+  for (int32_t j = w.j0; j < w.jend; ++j) {
+    const uint32_t i = uint32_t(j - w.j0), ik = 2 * i, iv = 2 * i + 1;
+    const uint32_t sk = ik % NS, sv = iv % NS;
+    if (j >= cnt) {  // none of this row tile's tokens sees a key of the tile
+      if (leader) {
+        mbar_arrive(&bars->kv_empty[sk]);
+        mbar_arrive(&bars->kv_empty[sv]);
+      }
+      continue;
+    }
+    const int32_t key0 = tile_index(w.tiles, j) * KT_BK;
+    if (leader) {
+      if (i == 0) ok = ok && kt_wait(bars, &bars->q_full, 0);
+      ok = ok && kt_wait(bars, &bars->kv_full[sk], (ik / NS) & 1);
+      if (i > 0) ok = ok && kt_wait(bars, &bars->pv_done[G], (i - 1) & 1);
+      if (ok) {
+        tc_fence_after();
+        const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
+        const uint64_t dq = umma_desc_sw128(qs + G * Cfg::TILE_BYTES), dk = umma_desc_sw128(ring + sk * Cfg::TILE_BYTES);
+#pragma unroll
+        for (int k = 0; k < HDP / 16; ++k)
+          if (k < ksteps) {
+            const uint64_t off = uint64_t((k >> 2) * int(Cfg::HALF_BYTES >> 4) + (k & 3) * 2);
+            umma_bf16(t_s, dq + off, dk + off, idesc, k > 0 ? 1u : 0u);
+          }
+        umma_commit(&bars->s_full[G]);
+        umma_commit(&bars->kv_empty[sk]);
+      }
+    }
+    __syncwarp();
+    if (!all_needed(w.span, key0, key0 + KT_BK)) {
+      // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
+      // tiles clear them, each before its own product)
+      ok = ok && kt_wait(bars, &bars->kv_full[sv], (iv / NS) & 1);
+      if (ok && !key_needed(w.span, key0 + r)) {
+        uint8_t* v = ring + sv * Cfg::TILE_BYTES + r * 128;
+#pragma unroll
+        for (int hh = 0; hh < HDP / 64; ++hh)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(v + hh * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    ok = ok && kt_wait(bars, &bars->s_full[G], i & 1);
+    __syncwarp();
+    tc_fence_after();
+    uint32_t s[4][32];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tmem_ld32(ts + x * 32, s[x]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tmem_wait32(s[x]);
+    if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
+      // visible columns of this row: x <= hi and (x > lo or x < sink)
+      const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
+#pragma unroll
+      for (int x = 0; x < 128; ++x)
+        if (x > hi || (x <= lo && x >= sink)) s[x >> 5][x & 31] = 0xff800000u;
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int x = 0; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x >> 5][x & 31]));
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+    const bool grow = top > m + 8.f || (i == 0 && top > m);
+    if (i > 0 && __any_sync(0xffffffffu, grow)) {
+      const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
+      l *= f;
+#pragma unroll 1
+      for (int x = 0; x < HDP; x += 32) {
+        uint32_t o[32];
+        tmem_ld32(to + x, o);
+        tmem_wait32(o);
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+        tmem_store32(to + x, o);
+      }
+    }
+    if (grow) m = top;
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      uint32_t w16[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const float a = exp2_fast(fmaf(__uint_as_float(s[x][2 * y]), p.scale_log2, -ref));
+        const float b = exp2_fast(fmaf(__uint_as_float(s[x][2 * y + 1]), p.scale_log2, -ref));
+        sum[(2 * y) & 3] += a;
+        sum[(2 * y + 1) & 3] += b;
+        w16[y] = pack2<T>(a, b);  // rounded for the matrix unit; the sum keeps the unrounded weights
+      }
+      tmem_store16(ts + x * 16, w16);
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    tmem_wait_st();
+    tc_fence_before();
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
+    if (leader) {
+      ok = ok && kt_wait(bars, &bars->kv_full[sv], (iv / NS) & 1);
+      if (ok) {
+        tc_fence_after();
+        const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
+        const uint64_t dv = umma_desc_mn_sw128(ring + sv * Cfg::TILE_BYTES);
+#pragma unroll
+        for (int k = 0; k < KT_BK / 16; ++k)  // 16 keys: 16 rows of 128 bytes
+#pragma unroll
+          for (int hh = 0; hh < HDP / 64; ++hh)  // one product per block of 64 columns
+            umma_f16_ts(t_o + hh * 64, t_s + k * 8, dv + uint64_t(k * 128 + hh * int(Cfg::HALF_BYTES >> 4)), idesc,
+                        i > 0 || k > 0 ? 1u : 0u);
+        umma_commit(&bars->pv_done[G]);
+        umma_commit(&bars->kv_empty[sv]);
+      }
+    }
+    __syncwarp();
+  }
+  const bool any = cnt > w.j0;
+  if (any) ok = ok && kt_wait(bars, &bars->pv_done[G], uint32_t(cnt - w.j0 - 1) & 1);
+  __syncwarp();
+  tc_fence_after();
+  const int64_t row = int64_t(p.slot0 + split) * c.tokens * p.q_heads + token * p.q_heads + head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const bool state = p.row_ml != nullptr;
+  if (state && mine && ok) p.row_ml[row] = make_float2(any ? m : -INFINITY, l);
+#pragma unroll 1
+  for (int x = 0; x < HDP; x += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    if (any) {
+      tmem_ld32(to + x, o);
+      tmem_wait32(o);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 32; ++y) o[y] = 0u;
+    }
+    if (!mine || !ok) continue;
+    if (state) {
+      if (any) {  // (a state of sum 0 is not read)
+        float* dst = p.row_o + row * c.head_dim + x;
+#pragma unroll
+        for (int y = 0; y < 32; y += 4)
+          if (x + y < c.head_dim)
+            *reinterpret_cast<float4*>(dst + y) = make_float4(__uint_as_float(o[y]), __uint_as_float(o[y + 1]),
+                                                              __uint_as_float(o[y + 2]), __uint_as_float(o[y + 3]));
+      }
+    } else {
+      T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + x;
+#pragma unroll
+      for (int y = 0; y < 32; y += 8) {
+        if (x + y < c.head_dim) {
+          uint32_t w4[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+            w4[z] = pack2<T>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
+          *reinterpret_cast<uint4*>(dst + y) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(KT_THREADS, 1)
+    kv_tile_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                   const __grid_constant__ CUtensorMap tmv, const __grid_constant__ KtParams p) {
+  using Cfg = KtCfg<HDP>;
+  extern __shared__ uint8_t kt_smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kt_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* qs = base;
+  uint8_t* ring = base + 2 * Cfg::TILE_BYTES;
+  auto* bars = reinterpret_cast<KtBars<HDP>*>(ring + Cfg::SLOTS * Cfg::TILE_BYTES);
+  __shared__ int64_t warp_tot[KT_THREADS / 32];
+  __shared__ KtUnit found;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t unit = blockIdx.x / p.c.kv_heads;
+  const int hk = int(blockIdx.x - unit * p.c.kv_heads), split = blockIdx.y;
+  const int32_t tt = p.tile_tokens;
+
+  const KtUnit un = kt_find(p.c, p.prefix_table, p.prefix_len, unit, 2 * tt, KT_THREADS, warp_tot, &found);
+  if (un.t0 >= un.s.n) return;  // (the same for all threads: no unit here)
+  KtWork w;
+  w.s = un.s;
+  w.b = un.b;
+  w.t0 = un.t0;
+  w.shared = p.prefix_table != nullptr;
+  w.window = w.shared ? 0 : p.window;
+  w.sinks = w.shared ? 0 : p.sinks;
+  const int32_t left = un.s.n - un.t0;
+  w.tokens0 = left < tt ? left : tt;
+  w.tokens1 = left <= tt ? 0 : (left < 2 * tt ? left - tt : tt);
+  // against a prefix all rows stand behind its last key
+  const int32_t at = un.s.len - un.s.n + un.t0;
+  w.pos0 = w.shared ? un.s.len - 1 : at;
+  w.last0 = w.shared ? un.s.len - 1 : at + w.tokens0 - 1;
+  w.pos1 = w.shared ? un.s.len - 1 : at + tt;
+  w.last1 = w.shared ? un.s.len - 1 : at + tt + w.tokens1 - 1;
+  w.span = key_span(w.pos0, w.tokens1 > 0 ? w.last1 : w.last0, w.window, w.sinks);
+  w.tiles = key_tiles(w.span, KT_BK);
+  w.j0 = int32_t(int64_t(w.tiles.count) * split / p.splits);
+  const int32_t j1 = int32_t(int64_t(w.tiles.count) * (split + 1) / p.splits);
+  w.cnt0 = kt_count(w.tiles, w.last0, w.tokens0, w.j0, j1);
+  w.cnt1 = kt_count(w.tiles, w.last1, w.tokens1, w.j0, j1);
+  w.jend = w.cnt0 > w.cnt1 ? w.cnt0 : w.cnt1;
+
+  if (tid == 0) {
+    const uint32_t row_tiles = w.tokens1 > 0 ? 2 : 1;
+    for (int s = 0; s < Cfg::SLOTS; ++s) {
+      mbar_init(&bars->kv_full[s], 1);
+      mbar_init(&bars->kv_empty[s], row_tiles);
+    }
+    mbar_init(&bars->q_full, 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&bars->s_full[g], 1);
+      mbar_init(&bars->pv_done[g], 1);
+    }
+    bars->abort = 0u;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem)),
+                 "r"(Cfg::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem);
+
+  // registers: 384 threads x 168 at launch; the row tiles' warps take 208, the others 80 (63488 of 64512)
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (warp < 4)
+      kt_rows<T, HDP, 0>(p, w, bars, tmem, qs, ring, hk, split);
+    else if (w.tokens1 > 0)
+      kt_rows<T, HDP, 1>(p, w, bars, tmem, qs, ring, hk, split);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8 && lane == 0 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS));
+  }
+}
+
+// out = the joined states of all slots, one 16-byte vector of a row a thread; rows that belong to no
+// sequence are left alone.
+template <typename T>
+__global__ void __launch_bounds__(128)
+    kv_rows_join_kernel(const int32_t* __restrict__ cu, int64_t batch, int64_t tokens, int32_t q_heads, int32_t head_dim,
+                        const float2* __restrict__ row_ml, const float* __restrict__ row_o, int32_t slots, KvRows out) {
+  const int vecs = head_dim >> 2;
+  const int64_t it = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t row = it / vecs;
+  const int col = int(it - row * vecs) << 2;
+  if (row >= tokens * q_heads) return;
+  const int64_t token = row / q_heads;
+  if (cu != nullptr && (token < cu[0] || token >= cu[batch])) return;
+  const int64_t slot_rows = tokens * q_heads;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < slots; ++i) {
+    const float2 ml = row_ml[i * slot_rows + row];
+    if (ml.x == -INFINITY) continue;
+    const float4 v = *reinterpret_cast<const float4*>(row_o + (i * slot_rows + row) * head_dim + col);
+    const float n = fmaxf(m, ml.x);
+    const float fo = m == -INFINITY ? 0.f : exp2_fast(m - n), fn = exp2_fast(ml.x - n);
+    m = n;
+    l = l * fo + ml.y * fn;
+    o.x = o.x * fo + v.x * fn;
+    o.y = o.y * fo + v.y * fn;
+    o.z = o.z * fo + v.z * fn;
+    o.w = o.w * fo + v.w * fn;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int head = int(row - token * q_heads);
+  *reinterpret_cast<uint2*>(static_cast<T*>(out.ptr) + token * out.token + head * out.head + col) =
+      make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+}
+
+}  // namespace lng

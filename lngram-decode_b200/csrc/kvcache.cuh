@@ -181,49 +181,4 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// ------------------------------------------------------------------ attention, one warp a row
-// The plain form of the attention: one warp per (token, query head) walks the prefix's keys, then the
-// sequence's own visible ones, with the running maximum and sum of the softmax; 4 values of the head a lane.
-template <typename T>
-__global__ void __launch_bounds__(128)
-    kv_attend_rows_kernel(KvView c, KvRows q, KvRows o, int32_t q_heads, float scale, int32_t window, int32_t sinks,
-                          const int32_t* __restrict__ prefix_table, int32_t prefix_len) {
-  const int64_t item = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (item >= c.tokens * q_heads) return;
-  const int64_t t = item / q_heads;
-  const int h = int(item - t * q_heads), hk = h / (q_heads / c.kv_heads);
-  const int64_t b = kv_sequence_of(c, t);
-  if (b < 0 || b >= c.batch) return;
-  const SeqSpan s = kv_span(c, b);
-  if (t < s.first || t >= s.first + s.n) return;
-  const int32_t p = s.len - s.n + int32_t(t - s.first);
-  const int d0 = lane * 4;
-  const bool in = d0 < c.head_dim;
-  float qv[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  if (in)
-    for (int i = 0; i < 4; ++i) qv[i] = scale * to_f32<T>(static_cast<const T*>(q.ptr)[t * q.token + h * q.head + d0 + i]);
-  auto visit = [&](const int32_t* table, int32_t j) {
-    const int32_t page = page_of(table, j, c.page_shift, c.num_pages), slot = j & ((1 << c.page_shift) - 1);
-    if (page < 0) kv_range_error();
-    const T* kp = static_cast<const T*>(c.k) + page * c.k_page + hk * c.k_head + slot * c.k_slot + d0;
-    const T* vp = static_cast<const T*>(c.v) + page * c.v_page + hk * c.v_head + slot * c.v_slot + d0;
-    float dot = 0.f;
-    if (in && page >= 0)
-      for (int i = 0; i < 4; ++i) dot += qv[i] * to_f32<T>(kp[i]);
-    dot = warp_sum(dot);
-    const float mn = fmaxf(m, dot), f = m == -INFINITY ? 0.f : expf(m - mn), w = expf(dot - mn);
-    l = l * f + w;
-    m = mn;
-    for (int i = 0; i < 4; ++i) acc[i] = acc[i] * f + (in && page >= 0 ? w * to_f32<T>(vp[i]) : 0.f);
-  };
-  for (int32_t j = 0; j < prefix_len; ++j) visit(prefix_table, j);
-  const KeySpan ks = key_span(p, p, window, sinks);
-  for (int32_t j = 0; j < ks.sink_end; ++j) visit(c.table + b * c.table_stride, j);
-  for (int32_t j = ks.lo; j < ks.hi; ++j) visit(c.table + b * c.table_stride, j);
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  if (in)
-    for (int i = 0; i < 4; ++i) static_cast<T*>(o.ptr)[t * o.token + h * o.head + d0 + i] = from_f32<T>(acc[i] * inv);
-}
-
 }  // namespace lng

@@ -24,6 +24,7 @@
 #include "online.cuh"
 #include "kvcache.cuh"
 #include "kv_step.cuh"
+#include "kv_tile.cuh"
 
 static int scratch_alloc(void** p, size_t bytes, cudaStream_t stream);
 
@@ -1748,26 +1749,95 @@ static int kv_page_maps(CUtensorMap* k, CUtensorMap* v, const lng_kv_cache* c, i
   return st ? st : kv_page_map(v, c, c->v, c->v_page_stride, c->v_head_stride, c->v_slot_stride, box);
 }
 
+// The tensor map of a step's queries: [tokens][heads][head_dim], the heads of one key head and as many tokens
+// as fill a tile of 128 rows a copy.
+static int kv_query_map(CUtensorMap* map, const lng_kv_cache* c, const lng_kv_rows* q, int64_t tokens, int group, int tile_tokens) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (driver entry point)");
+  const cuuint64_t dims[3] = {cuuint64_t(c->head_dim), cuuint64_t(q->heads), cuuint64_t(tokens)};
+  const cuuint64_t strides[2] = {cuuint64_t(q->head_stride) * 2, cuuint64_t(q->token_stride) * 2};
+  const cuuint32_t box[3] = {64, cuuint32_t(group), cuuint32_t(tile_tokens)}, one[3] = {1, 1, 1};
+  const auto type = c->dtype == LNG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult r = enc(map, type, 3, q->ptr, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+  return LNG_OK;
+}
+
+// Into how many key ranges `units` CTAs with up to `tiles` key tiles each are divided: the count with the
+// least estimated time, in tiles -- waves of CTAs (one an SM) times (a range's tiles + 3 for a CTA's start and
+// end), plus the join of the ranges' states.
+static int kv_splits(int64_t units, int64_t tiles) {
+  const int64_t sms = num_sms();
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 32 && s <= tiles; ++s) {
+    const double cost = double(ceil_div(units * s, sms)) * (ceil_div(tiles, s) + 3) + (s > 1 ? 4 + s * 0.25 : 0.0);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // How an attention call is carried out, and what it needs of the workspace.
 struct KvPlan {
-  bool step;              // at most 16 rows a key head and sequence: kv_step_kernel
-  int shares;             // its CTAs
-  size_t piece_ml, piece_o, bytes;
+  bool step;          // the sequences' own keys by kv_step_kernel (at most 16 rows a key head), else by kv_tile_kernel
+  int shares;         // CTAs of the step kernel
+  int64_t units;      // CTAs of the tile kernel per key head and range
+  int splits;         // key ranges of the tile kernel
+  int prefix_splits;  // key ranges of a shared prefix (0: there is none)
+  int slots;          // row states that are joined (0: rows are written directly or by the step's join)
+  size_t piece_ml, piece_o, row_ml, row_o, bytes;
 };
 static KvPlan kv_plan(const lng_kv_cache* c, int64_t prefix_len, int64_t tokens, int64_t max_new, int64_t max_len, int32_t q_heads,
                       int32_t window, int32_t sinks) {
   KvPlan p{};
-  if (!c || tokens <= 0 || c->batch <= 0 || c->num_kv_heads <= 0 || q_heads <= 0) return p;
-  const int64_t group = q_heads / c->num_kv_heads;
-  p.step = group * max_new <= KS_ROWS && prefix_len == 0;
+  if (!c || tokens <= 0 || c->batch <= 0 || c->num_kv_heads <= 0 || q_heads < c->num_kv_heads || max_new <= 0) return p;
+  const int64_t group = q_heads / c->num_kv_heads, span = 2 * std::max<int64_t>(1, KT_BM / group);
+  int64_t keys = c->max_pages * c->page_size;
+  if (max_len > 0) keys = std::min(keys, max_len);
+  if (window > 0) keys = std::min(keys, int64_t(window) + sinks + span + KT_BK);
+  p.step = group * max_new <= KS_ROWS;
   if (p.step) {
     p.shares = num_sms();
-    const size_t rows = size_t(2) * p.shares * KS_ROWS;
-    p.piece_ml = 0;
-    p.piece_o = al256(rows * 8);
-    p.bytes = p.piece_o + al256(rows * c->head_dim * 4);
+  } else {
+    // ragged steps: at most one unit a sequence is not full
+    p.units = c->batch * ceil_div(max_new, span);
+    const int64_t ragged = tokens / span + std::min(c->batch, tokens);
+    if (ragged < p.units) p.units = ragged;
+    p.splits = kv_splits(std::max<int64_t>(1, ceil_div(tokens, span)) * c->num_kv_heads, std::max<int64_t>(1, ceil_div(keys, KT_BK)));
   }
+  if (prefix_len > 0) p.prefix_splits = kv_splits(ceil_div(tokens, span) * c->num_kv_heads, ceil_div(prefix_len, KT_BK));
+  if (p.prefix_splits)
+    p.slots = p.prefix_splits + (p.step ? 1 : p.splits);
+  else if (!p.step && p.splits > 1)
+    p.slots = p.splits;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += al256(bytes);
+    return here;
+  };
+  const size_t pieces = size_t(2) * p.shares * KS_ROWS, rows = size_t(p.slots) * tokens * q_heads;
+  p.piece_ml = take(pieces * 8);
+  p.piece_o = take(pieces * c->head_dim * 4);
+  p.row_ml = take(rows * 8);
+  p.row_o = take(rows * c->head_dim * 4);
+  p.bytes = at;
   return p;
+}
+
+template <typename T, int HDP>
+static int launch_kv_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const KtParams& p, int64_t units,
+                          cudaStream_t s) {
+  using Cfg = KtCfg<HDP>;
+  auto kern = kv_tile_kernel<T, HDP>;
+  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  kern<<<dim3(unsigned(units * p.c.kv_heads), unsigned(p.splits)), KT_THREADS, Cfg::SMEM, s>>>(tq, tk, tv, p);
+  LNG_LAUNCHED("kv_tile_kernel");
+  return LNG_OK;
 }
 
 template <typename T, int HDP>
@@ -1817,38 +1887,79 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   window = std::min(window, 1 << 30);
   sinks = std::min(sinks, 1 << 30);
   const KvView v = kv_view(cache, cu, tokens, max_new);
+  const cudaStream_t cs = S(stream);
+  const bool bf16 = cache->dtype == LNG_BF16, wide = cache->head_dim > 64;
+  const int group = q->heads / cache->num_kv_heads, tile_tokens = KT_BM / group;
+  const float scale_log2 = scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  if (plan.step) {
-    KsParams p{};
+  float2* row_ml = plan.slots ? reinterpret_cast<float2*>(ws + plan.row_ml) : nullptr;
+  float* row_o = plan.slots ? reinterpret_cast<float*>(ws + plan.row_o) : nullptr;
+
+  if (plan.prefix_splits > 0 || !plan.step) {
+    CUtensorMap tq, tk, tv;
+    KtParams p{};
     p.c = v;
-    p.q = kv_rows(q);
     p.o = kv_rows(out);
     p.q_heads = q->heads;
-    p.group = q->heads / cache->num_kv_heads;
-    p.scale_log2 = scale * 1.4426950408889634f;
-    p.window = window;
-    p.sinks = sinks;
-    p.box = std::min(cache->page_size, KS_BK);
-    p.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
-    p.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
-    p.shares = plan.shares;
-    CUtensorMap tk, tv;
-    if ((st = kv_page_maps(&tk, &tv, cache, p.box))) return st;
-    const bool wide = cache->head_dim > 64;
-    if (cache->dtype == LNG_BF16)
-      return wide ? launch_kv_step<__nv_bfloat16, 128>(tk, tv, p, S(stream)) : launch_kv_step<__nv_bfloat16, 64>(tk, tv, p, S(stream));
-    return wide ? launch_kv_step<__half, 128>(tk, tv, p, S(stream)) : launch_kv_step<__half, 64>(tk, tv, p, S(stream));
+    p.group = group;
+    p.tile_tokens = tile_tokens;
+    p.scale_log2 = scale_log2;
+    p.box = std::min(cache->page_size, KT_BK);
+    p.row_ml = row_ml;
+    p.row_o = row_o;
+    if ((st = kv_query_map(&tq, cache, q, tokens, group, tile_tokens)) || (st = kv_page_maps(&tk, &tv, cache, p.box))) return st;
+    auto launch = [&](int64_t units) {
+      if (bf16)
+        return wide ? launch_kv_tile<__nv_bfloat16, 128>(tq, tk, tv, p, units, cs)
+                    : launch_kv_tile<__nv_bfloat16, 64>(tq, tk, tv, p, units, cs);
+      return wide ? launch_kv_tile<__half, 128>(tq, tk, tv, p, units, cs) : launch_kv_tile<__half, 64>(tq, tk, tv, p, units, cs);
+    };
+    if (plan.prefix_splits > 0) {
+      KtParams own = p;
+      p.prefix_table = prefix_table;
+      p.prefix_len = int32_t(prefix_len);
+      p.splits = plan.prefix_splits;
+      if ((st = launch(ceil_div(tokens, 2 * tile_tokens)))) return st;
+      p = own;
+      p.slot0 = plan.prefix_splits;
+    }
+    if (!plan.step) {
+      p.window = window;
+      p.sinks = sinks;
+      p.splits = plan.splits;
+      if ((st = launch(plan.units))) return st;
+      if (plan.slots == 0) return LNG_OK;
+      const unsigned grid = unsigned(ceil_div(tokens * q->heads * (cache->head_dim / 4), 128));
+      if (bf16)
+        kv_rows_join_kernel<__nv_bfloat16><<<grid, 128, 0, cs>>>(cu, cache->batch, tokens, q->heads, cache->head_dim, row_ml, row_o,
+                                                                 plan.slots, kv_rows(out));
+      else
+        kv_rows_join_kernel<__half><<<grid, 128, 0, cs>>>(cu, cache->batch, tokens, q->heads, cache->head_dim, row_ml, row_o,
+                                                          plan.slots, kv_rows(out));
+      LNG_LAUNCHED("kv_rows_join_kernel");
+      return LNG_OK;
+    }
   }
-  const int64_t warps = tokens * q->heads;
-  const unsigned grid = unsigned(ceil_div(warps, 4));
-  if (cache->dtype == LNG_BF16)
-    kv_attend_rows_kernel<__nv_bfloat16><<<grid, 128, 0, S(stream)>>>(v, kv_rows(q), kv_rows(out), q->heads, scale, window,
-                                                                    sinks, prefix_table, int32_t(prefix_len));
-  else
-    kv_attend_rows_kernel<__half><<<grid, 128, 0, S(stream)>>>(v, kv_rows(q), kv_rows(out), q->heads, scale, window, sinks,
-                                                              prefix_table, int32_t(prefix_len));
-  LNG_LAUNCHED("kv_attend_rows_kernel");
-  return LNG_OK;
+  KsParams p{};
+  p.c = v;
+  p.q = kv_rows(q);
+  p.o = kv_rows(out);
+  p.q_heads = q->heads;
+  p.group = group;
+  p.scale_log2 = scale_log2;
+  p.window = window;
+  p.sinks = sinks;
+  p.box = std::min(cache->page_size, KS_BK);
+  p.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
+  p.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
+  p.shares = plan.shares;
+  p.row_ml = row_ml;
+  p.row_o = row_o;
+  p.prefix_slots = plan.prefix_splits;
+  CUtensorMap tk, tv;
+  if ((st = kv_page_maps(&tk, &tv, cache, p.box))) return st;
+  if (bf16) return wide ? launch_kv_step<__nv_bfloat16, 128>(tk, tv, p, cs) : launch_kv_step<__nv_bfloat16, 64>(tk, tv, p, cs);
+  return wide ? launch_kv_step<__half, 128>(tk, tv, p, cs) : launch_kv_step<__half, 64>(tk, tv, p, cs);
 }
 
 }  // namespace lng
