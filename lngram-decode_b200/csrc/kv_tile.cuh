@@ -19,7 +19,7 @@
 
 namespace lng {
 
-constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 384;
+constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 288;
 
 template <int HDP>
 struct KtCfg {
@@ -187,10 +187,6 @@ struct KtWork {
   KeySpan span;
   KeyTiles tiles;
 };
-template <int G> __device__ __forceinline__ int32_t kt_tokens(const KtWork& w) { return G ? w.tokens1 : w.tokens0; }
-template <int G> __device__ __forceinline__ int32_t kt_first(const KtWork& w) { return G ? w.pos1 : w.pos0; }
-template <int G> __device__ __forceinline__ int32_t kt_last(const KtWork& w) { return G ? w.last1 : w.last0; }
-template <int G> __device__ __forceinline__ int32_t kt_cnt(const KtWork& w) { return G ? w.cnt1 : w.cnt0; }
 
 __device__ __forceinline__ int32_t kt_count(const KeyTiles& t, int32_t last, int32_t tokens, int32_t j0, int32_t j1) {
   const int32_t end = last >= 0 && tokens > 0 ? last / KT_BK + 1 : 0;  // tiles of the keys up to `last`
@@ -209,12 +205,70 @@ struct KtBars {
   uint32_t tmem, abort;
 };
 
+// Bounded wait that also gives up when another role has (an expired wait records the device error).
 template <int HDP>
 __device__ __forceinline__ bool kt_wait(KtBars<HDP>* bars, uint64_t* bar, uint32_t parity) {
-  if (*reinterpret_cast<volatile uint32_t*>(&bars->abort)) return false;
-  if (mbar_wait_bounded(bar, parity, &g_error_word, DEV_ERR_WAIT_TIMEOUT)) return true;
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 63 && *reinterpret_cast<volatile uint32_t*>(&bars->abort)) return false;
+  }
+  atomicCAS(&g_error_word, 0u, (unsigned int)DEV_ERR_WAIT_TIMEOUT);
   *reinterpret_cast<volatile uint32_t*>(&bars->abort) = 1u;
   return false;
+}
+
+// Two fp32 operations an instruction (sm_100).
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// -inf in the columns of a 32-column piece (from column `base` of the tile) that the row does not see.
+__device__ __forceinline__ void kt_mask(uint32_t (&s)[32], int32_t base, int32_t hi, int32_t lo, int32_t sink) {
+#pragma unroll
+  for (int x = 0; x < 32; ++x)
+    if (base + x > hi || (base + x <= lo && base + x >= sink)) s[x] = 0xff800000u;
+}
+__device__ __forceinline__ float kt_max(const uint32_t (&s)[32], float m0) {
+  float m1 = m0;
+#pragma unroll
+  for (int x = 0; x < 32; x += 4) {
+    m0 = fmaxf(m0, fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 1])));
+    m1 = fmaxf(m1, fmaxf(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])));
+  }
+  return fmaxf(m0, m1);
+}
+// Weights of a 32-column piece: 2^(s * scale - ref), summed in fp32 and packed to the cache's type (rounded for
+// the matrix unit; the sum keeps the unrounded weights).
+template <typename T>
+__device__ __forceinline__ void kt_weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t ref2, uint64_t& sum0, uint64_t& sum1,
+                                           uint32_t (&w)[16]) {
+#pragma unroll
+  for (int y = 0; y < 16; ++y) {
+    float a, b;
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), scale2, ref2), a, b);
+    a = exp2_fast(a);
+    b = exp2_fast(b);
+    if (y & 1)
+      sum1 = f2_add(sum1, f2_pack(a, b));
+    else
+      sum0 = f2_add(sum0, f2_pack(a, b));
+    w[y] = pack2<T>(a, b);
+  }
 }
 
 // One thread: queries once, then keys and values of every tile, page by page, into the ring.
@@ -270,18 +324,18 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
 //   S = Q K^T -> softmax in registers, P over S -> O += P V,
 // each committed to an mbarrier and waited for before its operands are touched again (the ISA orders products
 // of unlike operands only through their completion).  The other row tile's products run meanwhile.
-template <typename T, int HDP, int G>
+template <typename T, int HDP>
 __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBars<HDP>* bars, uint32_t tmem, const uint8_t* qs,
-                                        uint8_t* ring, int hk, int split) {
+                                        uint8_t* ring, int hk, int split, int G) {
   using Cfg = KtCfg<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const KvView& c = p.c;
   const int quad = (threadIdx.x >> 5) & 3, r = quad * 32 + (threadIdx.x & 31);
   const bool leader = r == 0;
   const int32_t tok = r / p.group, head = hk * p.group + (r - tok * p.group);
-  const bool mine = tok < kt_tokens<G>(w);
+  const bool mine = tok < (G ? w.tokens1 : w.tokens0);
   const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
-  const int32_t first = kt_first<G>(w), last = kt_last<G>(w), cnt = kt_cnt<G>(w);
+  const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0, cnt = G ? w.cnt1 : w.cnt0;
   const int32_t pos = w.shared ? last : first + tok;
   const int ksteps = (c.head_dim + 15) >> 4;
   const uint32_t t_s = tmem + Cfg::TMEM_S + G * 128, t_o = tmem + Cfg::TMEM_O + G * HDP;
@@ -334,26 +388,31 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBa
     ok = ok && kt_wait(bars, &bars->s_full[G], i & 1);
     __syncwarp();
     tc_fence_after();
-    uint32_t s[4][32];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) tmem_ld32(ts + x * 32, s[x]);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) tmem_wait32(s[x]);
-    if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
-      // visible columns of this row: x <= hi and (x > lo or x < sink)
-      const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
-#pragma unroll
-      for (int x = 0; x < 128; ++x)
-        if (x > hi || (x <= lo && x >= sink)) s[x >> 5][x & 31] = 0xff800000u;
+    // S in pieces of 32 columns, read twice (maximum, then weights): the body stays small enough for the
+    // instruction cache and the next piece is under way while one is worked on
+    const bool masked = !all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks);
+    // visible columns of this row: x <= hi and (x > lo or x < sink)
+    const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
+    uint32_t s0[32], s1[32];
+    float top = -INFINITY;
+    tmem_ld32(ts, s0);
+#pragma unroll 1
+    for (int x = 0; x < 128; x += 64) {
+      tmem_wait32(s0);
+      tmem_ld32(ts + x + 32, s1);
+      if (masked) kt_mask(s0, x, hi, lo, sink);
+      top = kt_max(s0, top);
+      tmem_wait32(s1);
+      tmem_ld32(ts + ((x + 64) & 127), s0);  // behind the last piece: the first one again, for the second reading
+      if (masked) kt_mask(s1, x + 32, hi, lo, sink);
+      top = kt_max(s1, top);
     }
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int x = 0; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(s[x >> 5][x & 31]));
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+    top *= p.scale_log2;
     const bool grow = top > m + 8.f || (i == 0 && top > m);
     if (i > 0 && __any_sync(0xffffffffu, grow)) {
       const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
       l *= f;
+      tmem_wait32(s0);  // (no other load may be pending when O's are waited for)
 #pragma unroll 1
       for (int x = 0; x < HDP; x += 32) {
         uint32_t o[32];
@@ -366,21 +425,26 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBa
     }
     if (grow) m = top;
     const float ref = m == -INFINITY ? 0.f : m;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), ref2 = f2_pack(-ref, -ref);
+    uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll 1
+    for (int x = 0; x < 128; x += 64) {
       uint32_t w16[16];
-#pragma unroll
-      for (int y = 0; y < 16; ++y) {
-        const float a = exp2_fast(fmaf(__uint_as_float(s[x][2 * y]), p.scale_log2, -ref));
-        const float b = exp2_fast(fmaf(__uint_as_float(s[x][2 * y + 1]), p.scale_log2, -ref));
-        sum[(2 * y) & 3] += a;
-        sum[(2 * y + 1) & 3] += b;
-        w16[y] = pack2<T>(a, b);  // rounded for the matrix unit; the sum keeps the unrounded weights
-      }
-      tmem_store16(ts + x * 16, w16);
+      tmem_wait32(s0);
+      tmem_ld32(ts + x + 32, s1);
+      if (masked) kt_mask(s0, x, hi, lo, sink);
+      kt_weights<T>(s0, scale2, ref2, sum0, sum1, w16);
+      tmem_wait32(s1);
+      if (x == 0) tmem_ld32(ts + 64, s0);
+      tmem_store16(ts + (x >> 1), w16);  // (columns that have been read)
+      if (masked) kt_mask(s1, x + 32, hi, lo, sink);
+      kt_weights<T>(s1, scale2, ref2, sum0, sum1, w16);
+      tmem_store16(ts + (x >> 1) + 16, w16);
     }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    float a0, a1, b0, b1;
+    f2_unpack(sum0, a0, a1);
+    f2_unpack(sum1, b0, b1);
+    l += (a0 + a1) + (b0 + b1);
     tmem_wait_st();
     tc_fence_before();
     asm volatile("bar.sync %0, 128;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
@@ -515,16 +579,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem);
 
-  // registers: 384 threads x 168 at launch; the row tiles' warps take 208, the others 80 (63488 of 64512)
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    if (warp < 4)
-      kt_rows<T, HDP, 0>(p, w, bars, tmem, qs, ring, hk, split);
-    else if (w.tokens1 > 0)
-      kt_rows<T, HDP, 1>(p, w, bars, tmem, qs, ring, hk, split);
+    if (warp < 4 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, tmem, qs, ring, hk, split, warp >> 2);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8 && lane == 0 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+    if (lane == 0 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
   }
   tc_fence_before();
   __syncwarp();
