@@ -3,8 +3,8 @@
 //
 // A CTA takes two tiles of up to 128 (token, head of the key head's group) rows -- the group's heads share
 // every key they load -- and walks the tiles of 128 keys that any of its tokens sees.  Roles:
-//   warp 8   one thread loads: queries once, then keys and values of each tile by TMA, page by page, into a ring;
-//   warps 0-3, 4-7  a row tile each, one row a thread: the first thread issues tcgen05.mma for S = Q K^T (fp32 in
+//   warp 16  one thread loads: queries once, then keys and values of each tile by TMA, page by page, into a ring;
+//   warps 0-7, 8-15  a row tile each, two threads a row: the first thread issues tcgen05.mma for S = Q K^T (fp32 in
 //            TMEM), all take S from TMEM, keep the running maximum and sum in fp32 and write P, rounded to the
 //            cache's type, over S's columns; the first thread issues O += P V with P read from TMEM.
 // While one row tile's softmax runs, the tensor cores work on the other's: per 128 x 128 block at head size 128
@@ -19,15 +19,15 @@
 
 namespace lng {
 
-constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 288;
+constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 640;
 
 template <int HDP>
 struct KtCfg {
   static constexpr uint32_t TILE_BYTES = 128 * HDP * 2;  // 128 rows of queries, keys or values
   static constexpr uint32_t HALF_BYTES = 128 * 128;      // 64 columns of them
-  static constexpr int SLOTS = HDP == 128 ? 5 : 8;
+  static constexpr int SLOTS = HDP == 128 ? 4 : 8;
   static constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;
-  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE_BYTES + 1024 + 256;
+  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE_BYTES + 1024 + 3072;
 };
 
 struct KtParams {
@@ -61,11 +61,8 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
       LNG_I8(r, 8), LNG_I8(r, 16), LNG_I8(r, 24), "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::LNG_I8(r, 0),
-      LNG_I8(r, 8), "r"(addr)
-      : "memory");
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::LNG_I8(r, 0), "r"(addr) : "memory");
 }
 #undef LNG_I8
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -79,11 +76,11 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       "r"(tmem_a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
-// B operand with N contiguous (one block of 64 columns), 128-byte swizzle: groups of 8 rows of K 1024 bytes
-// apart.
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(const void* tile) {
-  uint64_t d = (smem_addr(tile) >> 4) & 0x3FFFull;
-  d |= uint64_t(1) << 16;  // leading byte offset (unused: one block)
+// A 128-byte swizzled operand, groups of 8 rows 1024 bytes apart: K-major (queries, keys: K contiguous, 16 a
+// step of 32 bytes), or with N contiguous (values: one block of 64 columns, 16 rows of K a step of 2048 bytes).
+__device__ __forceinline__ uint64_t umma_desc_at(uint32_t tile) {
+  uint64_t d = (tile >> 4) & 0x3FFFull;
+  d |= uint64_t(1) << 16;  // leading byte offset (unused: one block of 64 columns)
   d |= uint64_t(1024 >> 4) << 32;
   d |= uint64_t(1) << 46;
   d |= uint64_t(2) << 61;
@@ -94,11 +91,17 @@ __device__ __forceinline__ uint32_t umma_idesc(int M, int N, bool b_mn) {
   const uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
   return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(b_mn) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint64_t* bar) {
+__device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_at(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w,
+                                               uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
 }
 
@@ -195,25 +198,71 @@ __device__ __forceinline__ int32_t kt_count(const KeyTiles& t, int32_t last, int
   return n > j0 ? n : j0;
 }
 
-// Shared memory behind the tiles.
+// Shared memory behind the tiles, by 32-bit shared addresses (offsets from the block's).
 template <int HDP>
 struct KtBars {
-  uint64_t kv_full[KtCfg<HDP>::SLOTS], kv_empty[KtCfg<HDP>::SLOTS];  // empty: one arrival a row tile
-  uint64_t q_full;
-  uint64_t s_full[2];   // a row tile's scores are in TMEM
-  uint64_t pv_done[2];  // its O += P V is done: O may be read, P overwritten
-  uint32_t tmem, abort;
+  static constexpr uint32_t NS = KtCfg<HDP>::SLOTS;
+  static constexpr uint32_t kv_full = 0, kv_empty = 8 * NS;  // [NS] each; empty: one arrival a row tile
+  static constexpr uint32_t q_full = 16 * NS;
+  static constexpr uint32_t s_full = q_full + 8;    // [2] a row tile's scores are in TMEM
+  static constexpr uint32_t pv_done = s_full + 16;  // [2] its O += P V is done: O may be read, P overwritten
+  static constexpr uint32_t tmem = pv_done + 16, abort = tmem + 4;
+  static constexpr uint32_t row_max = (abort + 4 + 1023) & ~1023u;  // fp32 [2 row tiles][2 halves][128]
+  static constexpr uint32_t BYTES = row_max + 2 * 2 * 128 * 4;
 };
 
+// One lane of the (converged) warp.  Products are issued by whole warps with uniform operands and one elected
+// lane: operands that the compiler cannot see to be uniform cost a hundred cycles a product.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok)::"memory");
+  return ok != 0;
+}
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
+  asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ void sts_zero16(uint32_t a) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void mbar_init_at(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void umma_commit_at(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait that also gives up when another role has (an expired wait records the device error).
 template <int HDP>
-__device__ __forceinline__ bool kt_wait(KtBars<HDP>* bars, uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 22); ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63) == 63 && *reinterpret_cast<volatile uint32_t*>(&bars->abort)) return false;
+    if (mbar_try_at(bars + bar, parity)) return true;
+    if ((i & 63) == 63 && lds32(bars + KtBars<HDP>::abort)) return false;
   }
   atomicCAS(&g_error_word, 0u, (unsigned int)DEV_ERR_WAIT_TIMEOUT);
-  *reinterpret_cast<volatile uint32_t*>(&bars->abort) = 1u;
+  sts32(bars + KtBars<HDP>::abort, 1u);
   return false;
 }
 
@@ -241,50 +290,62 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 __device__ __forceinline__ void kt_mask(uint32_t (&s)[32], int32_t base, int32_t hi, int32_t lo, int32_t sink) {
 #pragma unroll
   for (int x = 0; x < 32; ++x)
-    if (base + x > hi || (base + x <= lo && base + x >= sink)) s[x] = 0xff800000u;
-}
-__device__ __forceinline__ float kt_max(const uint32_t (&s)[32], float m0) {
-  float m1 = m0;
+    if (base + x > hi) s[x] = 0xff800000u;
+  if (base <= lo) {
 #pragma unroll
-  for (int x = 0; x < 32; x += 4) {
-    m0 = fmaxf(m0, fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 1])));
-    m1 = fmaxf(m1, fmaxf(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])));
+    for (int x = 0; x < 32; ++x)
+      if (base + x <= lo && base + x >= sink) s[x] = 0xff800000u;
   }
-  return fmaxf(m0, m1);
 }
-// Weights of a 32-column piece: 2^(s * scale - ref), summed in fp32 and packed to the cache's type (rounded for
-// the matrix unit; the sum keeps the unrounded weights).
+__device__ __forceinline__ float kt_max(const uint32_t (&s)[32]) {
+  float m0 = __uint_as_float(s[0]), m1 = __uint_as_float(s[1]);
+#pragma unroll
+  for (int x = 2; x < 30; x += 4) {
+    m0 = fmaxf(fmaxf(m0, __uint_as_float(s[x])), __uint_as_float(s[x + 1]));
+    m1 = fmaxf(fmaxf(m1, __uint_as_float(s[x + 2])), __uint_as_float(s[x + 3]));
+  }
+  return fmaxf(fmaxf(fmaxf(m0, __uint_as_float(s[30])), __uint_as_float(s[31])), m1);
+}
+// Weights of a 32-column piece to TMEM column tp: 2^(s * scale - ref), summed in fp32 and packed to the cache's
+// type (rounded for the matrix unit; the sum keeps the unrounded weights).
 template <typename T>
 __device__ __forceinline__ void kt_weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t ref2, uint64_t& sum0, uint64_t& sum1,
-                                           uint32_t (&w)[16]) {
+                                           uint32_t tp) {
 #pragma unroll
-  for (int y = 0; y < 16; ++y) {
-    float a, b;
-    f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), scale2, ref2), a, b);
-    a = exp2_fast(a);
-    b = exp2_fast(b);
-    if (y & 1)
-      sum1 = f2_add(sum1, f2_pack(a, b));
-    else
-      sum0 = f2_add(sum0, f2_pack(a, b));
-    w[y] = pack2<T>(a, b);
+  for (int z = 0; z < 2; ++z) {
+    uint32_t w[8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+      const int x = z * 16 + y * 2;
+      float a, b;
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, ref2), a, b);
+      a = exp2_fast(a);
+      b = exp2_fast(b);
+      if (y & 1)
+        sum1 = f2_add(sum1, f2_pack(a, b));
+      else
+        sum0 = f2_add(sum0, f2_pack(a, b));
+      w[y] = pack2<T>(a, b);
+    }
+    tmem_store8(tp + z * 8, w);
   }
 }
 
 // One thread: queries once, then keys and values of every tile, page by page, into the ring.
 template <int HDP>
 __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv, const KtParams& p,
-                                        const KtWork& w, KtBars<HDP>* bars, uint8_t* qs, uint8_t* ring, int hk) {
+                                        const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int hk) {
   using Cfg = KtCfg<HDP>;
+  using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const KvView& c = p.c;
   const int tiles_q = w.tokens1 > 0 ? 2 : 1;
-  mbar_arrive_expect_tx(&bars->q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
+  mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
   for (int g = 0; g < tiles_q; ++g)
 #pragma unroll
     for (int hh = 0; hh < HDP / 64; ++hh)
-      tma_load_3d(qs + g * Cfg::TILE_BYTES + hh * Cfg::HALF_BYTES, tmq, hh * 64, hk * p.group,
-                  int32_t(w.s.first + w.t0 + g * p.tile_tokens), &bars->q_full);
+      tma_load_3d_at(qs + g * Cfg::TILE_BYTES + hh * Cfg::HALF_BYTES, tmq, hh * 64, hk * p.group,
+                     int32_t(w.s.first + w.t0 + g * p.tile_tokens), bars + B::q_full);
   const int32_t* row = w.shared ? p.prefix_table : c.table + w.b * c.table_stride;
   uint32_t it = 0;
   bool ok = true;
@@ -295,10 +356,10 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
       if (any_needed(w.span, key0 + r, key0 + r + p.box)) bytes += uint32_t(p.box) * 128u * (HDP / 64);
     auto fill = [&](const CUtensorMap* map) -> bool {
       const uint32_t s = it % NS;
-      if (it >= NS && !kt_wait(bars, &bars->kv_empty[s], (it / NS - 1) & 1)) return false;
+      if (it >= NS && !kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1)) return false;
       ++it;
-      mbar_arrive_expect_tx(&bars->kv_full[s], bytes);
-      uint8_t* dst = ring + s * Cfg::TILE_BYTES;
+      mbar_expect_at(bars + B::kv_full + 8 * s, bytes);
+      const uint32_t dst = ring + s * Cfg::TILE_BYTES;
       for (int32_t r = 0; r < KT_BK; r += p.box) {
         const int32_t key = key0 + r;
         if (!any_needed(w.span, key, key + p.box)) continue;
@@ -310,111 +371,114 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
         const int32_t slot = key & ((1 << c.page_shift) - 1);
 #pragma unroll
         for (int hh = 0; hh < HDP / 64; ++hh)
-          tma_load_4d(dst + hh * Cfg::HALF_BYTES + r * 128, map, hh * 64, slot, hk, page, &bars->kv_full[s]);
+          tma_load_4d_at(dst + hh * Cfg::HALF_BYTES + r * 128, map, hh * 64, slot, hk, page, bars + B::kv_full + 8 * s);
       }
       return true;
     };
     ok = fill(tmk) && fill(tmv);
   }
   // the last uses of the ring's slots: behind them no copy and no product is in flight
-  for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait(bars, &bars->kv_empty[k % NS], (k / NS) & 1);
+  for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
 }
 
-// The 128 threads of row tile G.  Thread 0 of them issues the tile's products; per key tile
+// The 256 threads of row tile G, two a row (64 columns of S each, so that eight warps a row tile hide each
+// other's latencies).  Warp 0 of them issues the tile's products; per key tile
 //   S = Q K^T -> softmax in registers, P over S -> O += P V,
 // each committed to an mbarrier and waited for before its operands are touched again (the ISA orders products
 // of unlike operands only through their completion).  The other row tile's products run meanwhile.
 template <typename T, int HDP>
-__device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBars<HDP>* bars, uint32_t tmem, const uint8_t* qs,
-                                        uint8_t* ring, int hk, int split, int G) {
+__device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int hk, int split,
+                                        int warp) {
   using Cfg = KtCfg<HDP>;
+  using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
+  constexpr int OC = HDP / 2;  // columns of O a thread rescales and stores
   const KvView& c = p.c;
-  const int quad = (threadIdx.x >> 5) & 3, r = quad * 32 + (threadIdx.x & 31);
-  const bool leader = r == 0;
-  const int32_t tok = r / p.group, head = hk * p.group + (r - tok * p.group);
-  const bool mine = tok < (G ? w.tokens1 : w.tokens0);
-  const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
-  const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0, cnt = G ? w.cnt1 : w.cnt0;
+  const int G = warp >> 3, quad = warp & 3, half = (warp >> 2) & 1, r = quad * 32 + (threadIdx.x & 31);
+  const bool issues = (warp & 7) == 0;
+  const int32_t tok = r / p.group, n = uniform(w.jend - w.j0), cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
+  const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
   const int32_t pos = w.shared ? last : first + tok;
-  const int ksteps = (c.head_dim + 15) >> 4;
-  const uint32_t t_s = tmem + Cfg::TMEM_S + G * 128, t_o = tmem + Cfg::TMEM_O + G * HDP;
-  const uint32_t ts = tmem_at(t_s, quad, 0), to = tmem_at(t_o, quad, 0);
+  const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
+  const uint32_t ts = tmem_at(t_s, quad, half * 64), tp = tmem_at(t_s, quad, half * 32), to = tmem_at(t_o, quad, half * OC);
+  const uint32_t mine_x = bars + B::row_max + ((G * 2 + half) * 128 + r) * 4, other_x = mine_x ^ 512u;
+  const uint32_t s_bar = B::s_full + 8 * G, pv_bar = B::pv_done + 8 * G;
   float m = -INFINITY, l = 0.f;
   bool ok = true;
-  for (int32_t j = w.j0; j < w.jend; ++j) {
-    const uint32_t i = uint32_t(j - w.j0), ik = 2 * i, iv = 2 * i + 1;
-    const uint32_t sk = ik % NS, sv = iv % NS;
-    if (j >= cnt) {  // none of this row tile's tokens sees a key of the tile
-      if (leader) {
-        mbar_arrive(&bars->kv_empty[sk]);
-        mbar_arrive(&bars->kv_empty[sv]);
+#pragma unroll 1
+  for (int32_t i = 0; i < n; ++i) {
+    const uint32_t ik = 2 * i, iv = 2 * i + 1, sk = ik % NS, sv = iv % NS;
+    if (i >= cnt) {  // none of this row tile's tokens sees a key of the tile
+      if (issues && elect_lane()) {
+        mbar_arrive_at(bars + B::kv_empty + 8 * sk);
+        mbar_arrive_at(bars + B::kv_empty + 8 * sv);
       }
+      __syncwarp();
       continue;
     }
-    const int32_t key0 = tile_index(w.tiles, j) * KT_BK;
-    if (leader) {
-      if (i == 0) ok = ok && kt_wait(bars, &bars->q_full, 0);
-      ok = ok && kt_wait(bars, &bars->kv_full[sk], (ik / NS) & 1);
-      if (i > 0) ok = ok && kt_wait(bars, &bars->pv_done[G], (i - 1) & 1);
+    const int32_t key0 = tile_index(w.tiles, w.j0 + i) * KT_BK;
+    if (issues) {
+      if (i == 0) ok = kt_wait<HDP>(bars, B::q_full, 0);
+      ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1);
+      if (i > 0) ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
-        const uint64_t dq = umma_desc_sw128(qs + G * Cfg::TILE_BYTES), dk = umma_desc_sw128(ring + sk * Cfg::TILE_BYTES);
+        if (elect_lane()) {
+          const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
+          const uint64_t dq = umma_desc_at(qs + G * Cfg::TILE_BYTES), dk = umma_desc_at(ring + sk * Cfg::TILE_BYTES);
+          const int ksteps = (c.head_dim + 15) >> 4;
 #pragma unroll
-        for (int k = 0; k < HDP / 16; ++k)
-          if (k < ksteps) {
-            const uint64_t off = uint64_t((k >> 2) * int(Cfg::HALF_BYTES >> 4) + (k & 3) * 2);
-            umma_bf16(t_s, dq + off, dk + off, idesc, k > 0 ? 1u : 0u);
-          }
-        umma_commit(&bars->s_full[G]);
-        umma_commit(&bars->kv_empty[sk]);
+          for (int k = 0; k < HDP / 16; ++k)
+            if (k < ksteps) {
+              const uint64_t off = uint64_t((k >> 2) * int(Cfg::HALF_BYTES >> 4) + (k & 3) * 2);
+              umma_bf16(t_s, dq + off, dk + off, idesc, k > 0 ? 1u : 0u);
+            }
+          umma_commit_at(bars + s_bar);
+          umma_commit_at(bars + B::kv_empty + 8 * sk);
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1));  // for the product with V
       }
     }
-    __syncwarp();
     if (!all_needed(w.span, key0, key0 + KT_BK)) {
       // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
       // tiles clear them, each before its own product)
-      ok = ok && kt_wait(bars, &bars->kv_full[sv], (iv / NS) & 1);
+      ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1);
       if (ok && !key_needed(w.span, key0 + r)) {
-        uint8_t* v = ring + sv * Cfg::TILE_BYTES + r * 128;
+        const uint32_t v = ring + sv * Cfg::TILE_BYTES + r * 128 + half * 64;
 #pragma unroll
         for (int hh = 0; hh < HDP / 64; ++hh)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(v + hh * Cfg::HALF_BYTES + x * 16) = make_uint4(0, 0, 0, 0);
+          for (int x = 0; x < 4; ++x) sts_zero16(v + hh * Cfg::HALF_BYTES + x * 16);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    ok = ok && kt_wait(bars, &bars->s_full[G], i & 1);
+    ok = ok && kt_wait<HDP>(bars, s_bar, i & 1);
     __syncwarp();
     tc_fence_after();
-    // S in pieces of 32 columns, read twice (maximum, then weights): the body stays small enough for the
-    // instruction cache and the next piece is under way while one is worked on
-    const bool masked = !all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks);
-    // visible columns of this row: x <= hi and (x > lo or x < sink)
-    const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
     uint32_t s0[32], s1[32];
-    float top = -INFINITY;
     tmem_ld32(ts, s0);
-#pragma unroll 1
-    for (int x = 0; x < 128; x += 64) {
-      tmem_wait32(s0);
-      tmem_ld32(ts + x + 32, s1);
-      if (masked) kt_mask(s0, x, hi, lo, sink);
-      top = kt_max(s0, top);
-      tmem_wait32(s1);
-      tmem_ld32(ts + ((x + 64) & 127), s0);  // behind the last piece: the first one again, for the second reading
-      if (masked) kt_mask(s1, x + 32, hi, lo, sink);
-      top = kt_max(s1, top);
+    tmem_ld32(ts + 32, s1);
+    tmem_wait32(s0);
+    tmem_wait32(s1);
+    if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
+      // visible columns of this row: x <= hi and (x > lo or x < sink)
+      const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
+      kt_mask(s0, half * 64, hi, lo, sink);
+      kt_mask(s1, half * 64 + 32, hi, lo, sink);
     }
-    top *= p.scale_log2;
+    // the row's maximum over both halves (behind the barrier all of S has been read: P may overwrite it)
+    const float here = fmaxf(kt_max(s0), kt_max(s1));
+    sts32(mine_x, __float_as_uint(here));
+    asm volatile("bar.sync %0, 256;" ::"r"(1 + G) : "memory");
+    const float top = fmaxf(here, __uint_as_float(lds32(other_x))) * p.scale_log2;
     const bool grow = top > m + 8.f || (i == 0 && top > m);
     if (i > 0 && __any_sync(0xffffffffu, grow)) {
       const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
       l *= f;
-      tmem_wait32(s0);  // (no other load may be pending when O's are waited for)
 #pragma unroll 1
-      for (int x = 0; x < HDP; x += 32) {
+      for (int x = 0; x < OC; x += 32) {
         uint32_t o[32];
         tmem_ld32(to + x, o);
         tmem_wait32(o);
@@ -427,55 +491,49 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBa
     const float ref = m == -INFINITY ? 0.f : m;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), ref2 = f2_pack(-ref, -ref);
     uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll 1
-    for (int x = 0; x < 128; x += 64) {
-      uint32_t w16[16];
-      tmem_wait32(s0);
-      tmem_ld32(ts + x + 32, s1);
-      if (masked) kt_mask(s0, x, hi, lo, sink);
-      kt_weights<T>(s0, scale2, ref2, sum0, sum1, w16);
-      tmem_wait32(s1);
-      if (x == 0) tmem_ld32(ts + 64, s0);
-      tmem_store16(ts + (x >> 1), w16);  // (columns that have been read)
-      if (masked) kt_mask(s1, x + 32, hi, lo, sink);
-      kt_weights<T>(s1, scale2, ref2, sum0, sum1, w16);
-      tmem_store16(ts + (x >> 1) + 16, w16);
-    }
+    kt_weights<T>(s0, scale2, ref2, sum0, sum1, tp);
+    kt_weights<T>(s1, scale2, ref2, sum0, sum1, tp + 16);
     float a0, a1, b0, b1;
     f2_unpack(sum0, a0, a1);
     f2_unpack(sum1, b0, b1);
     l += (a0 + a1) + (b0 + b1);
     tmem_wait_st();
     tc_fence_before();
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
-    if (leader) {
-      ok = ok && kt_wait(bars, &bars->kv_full[sv], (iv / NS) & 1);
-      if (ok) {
-        tc_fence_after();
+    asm volatile("bar.sync %0, 256;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
+    if (issues && __all_sync(0xffffffffu, ok)) {
+      tc_fence_after();
+      if (elect_lane()) {
         const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
-        const uint64_t dv = umma_desc_mn_sw128(ring + sv * Cfg::TILE_BYTES);
+        const uint64_t dv = umma_desc_at(ring + sv * Cfg::TILE_BYTES);
 #pragma unroll
         for (int k = 0; k < KT_BK / 16; ++k)  // 16 keys: 16 rows of 128 bytes
 #pragma unroll
           for (int hh = 0; hh < HDP / 64; ++hh)  // one product per block of 64 columns
             umma_f16_ts(t_o + hh * 64, t_s + k * 8, dv + uint64_t(k * 128 + hh * int(Cfg::HALF_BYTES >> 4)), idesc,
                         i > 0 || k > 0 ? 1u : 0u);
-        umma_commit(&bars->pv_done[G]);
-        umma_commit(&bars->kv_empty[sv]);
+        umma_commit_at(bars + pv_bar);
+        umma_commit_at(bars + B::kv_empty + 8 * sv);
       }
+      __syncwarp();
     }
-    __syncwarp();
   }
-  const bool any = cnt > w.j0;
-  if (any) ok = ok && kt_wait(bars, &bars->pv_done[G], uint32_t(cnt - w.j0 - 1) & 1);
+  const bool any = cnt > 0;
+  if (any) ok = ok && kt_wait<HDP>(bars, pv_bar, uint32_t(cnt - 1) & 1);
   __syncwarp();
   tc_fence_after();
+  sts32(mine_x, __float_as_uint(l));
+  asm volatile("bar.sync %0, 256;" ::"r"(1 + G) : "memory");
+  l += __uint_as_float(lds32(other_x));
+  const int32_t head = hk * p.group + (r - tok * p.group);
+  const bool mine = tok < (G ? w.tokens1 : w.tokens0);
+  const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
   const int64_t row = int64_t(p.slot0 + split) * c.tokens * p.q_heads + token * p.q_heads + head;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const bool state = p.row_ml != nullptr;
-  if (state && mine && ok) p.row_ml[row] = make_float2(any ? m : -INFINITY, l);
+  if (state && mine && ok && half == 0) p.row_ml[row] = make_float2(any ? m : -INFINITY, l);
 #pragma unroll 1
-  for (int x = 0; x < HDP; x += 32) {
+  for (int x = 0; x < OC; x += 32) {
+    const int col = half * OC + x;
     uint32_t o[32];
     __syncwarp();
     if (any) {
@@ -488,18 +546,18 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, KtBa
     if (!mine || !ok) continue;
     if (state) {
       if (any) {  // (a state of sum 0 is not read)
-        float* dst = p.row_o + row * c.head_dim + x;
+        float* dst = p.row_o + row * c.head_dim + col;
 #pragma unroll
         for (int y = 0; y < 32; y += 4)
-          if (x + y < c.head_dim)
+          if (col + y < c.head_dim)
             *reinterpret_cast<float4*>(dst + y) = make_float4(__uint_as_float(o[y]), __uint_as_float(o[y + 1]),
                                                               __uint_as_float(o[y + 2]), __uint_as_float(o[y + 3]));
       }
     } else {
-      T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + x;
+      T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + col;
 #pragma unroll
       for (int y = 0; y < 32; y += 8) {
-        if (x + y < c.head_dim) {
+        if (col + y < c.head_dim) {
           uint32_t w4[4];
 #pragma unroll
           for (int z = 0; z < 4; ++z)
@@ -516,14 +574,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
     kv_tile_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                    const __grid_constant__ CUtensorMap tmv, const __grid_constant__ KtParams p) {
   using Cfg = KtCfg<HDP>;
+  using B = KtBars<HDP>;
   extern __shared__ uint8_t kt_smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kt_smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* qs = base;
-  uint8_t* ring = base + 2 * Cfg::TILE_BYTES;
-  auto* bars = reinterpret_cast<KtBars<HDP>*>(ring + Cfg::SLOTS * Cfg::TILE_BYTES);
+  const uint32_t qs = (smem_addr(kt_smem_raw) + 1023) & ~1023u, ring = qs + 2 * Cfg::TILE_BYTES;
+  const uint32_t bars = ring + Cfg::SLOTS * Cfg::TILE_BYTES;
   __shared__ int64_t warp_tot[KT_THREADS / 32];
   __shared__ KtUnit found;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int64_t unit = blockIdx.x / p.c.kv_heads;
   const int hk = int(blockIdx.x - unit * p.c.kv_heads), split = blockIdx.y;
   const int32_t tt = p.tile_tokens;
@@ -557,19 +614,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   if (tid == 0) {
     const uint32_t row_tiles = w.tokens1 > 0 ? 2 : 1;
     for (int s = 0; s < Cfg::SLOTS; ++s) {
-      mbar_init(&bars->kv_full[s], 1);
-      mbar_init(&bars->kv_empty[s], row_tiles);
+      mbar_init_at(bars + B::kv_full + 8 * s, 1);
+      mbar_init_at(bars + B::kv_empty + 8 * s, row_tiles);
     }
-    mbar_init(&bars->q_full, 1);
+    mbar_init_at(bars + B::q_full, 1);
     for (int g = 0; g < 2; ++g) {
-      mbar_init(&bars->s_full[g], 1);
-      mbar_init(&bars->pv_done[g], 1);
+      mbar_init_at(bars + B::s_full + 8 * g, 1);
+      mbar_init_at(bars + B::pv_done + 8 * g, 1);
     }
-    bars->abort = 0u;
+    sts32(bars + B::abort, 0u);
     fence_mbar_init();
   }
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars->tmem)),
+  if (warp == 16) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bars + B::tmem),
                  "r"(Cfg::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -577,17 +634,20 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem);
+  const uint32_t tmem = lds32(bars + B::tmem);
 
-  if (warp < 8) {
-    if (warp < 4 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, tmem, qs, ring, hk, split, warp >> 2);
+  // registers: 640 threads x 96 at launch; the row tiles' warps take 104, the others 64 (61440 in all)
+  if (warp < 16) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    if (warp < 8 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, qs, ring, hk, split, warp);
   } else {
-    if (lane == 0 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 16 && lane == 0 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
   }
   tc_fence_before();
   __syncwarp();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS));
   }
