@@ -434,8 +434,9 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       lb += __shfl_xor_sync(0xffffffffu, lb, o);
     }
     if (t4 == 0) {
-      merge_ml[warp * KS_ROWS + g] = make_float2(ma, la);
-      merge_ml[warp * KS_ROWS + g + 8] = make_float2(mb, lb);
+      // (scores that are all NaN leave the maximum at -inf: their NaN sum must not be taken for an empty state)
+      merge_ml[warp * KS_ROWS + g] = make_float2(la == la ? ma : 0.f, la);
+      merge_ml[warp * KS_ROWS + g + 8] = make_float2(lb == lb ? mb : 0.f, lb);
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {

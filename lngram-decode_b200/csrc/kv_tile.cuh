@@ -306,8 +306,32 @@ __device__ __forceinline__ float kt_max(const uint32_t (&s)[32]) {
   }
   return fmaxf(fmaxf(fmaxf(m0, __uint_as_float(s[30])), __uint_as_float(s[31])), m1);
 }
+// 2^x of a pair on the fma pipe: x = n + f with n the nearest integer (by adding 1.5 * 2^23, whose last place is
+// 1) and |f| <= 1/2, 2^f by a polynomial of degree 4 (least-squares fit of the relative error, reweighted towards
+// its peaks: at most 2.7e-6 = 2^-18.5 off), n added to the exponent.  x <= 8 here; below -126, and for the -inf
+// of a masked key, the result is 2^-126.
+__device__ __forceinline__ void exp2_fma(uint64_t x2, float& a, float& b) {
+  float x0, x1;
+  f2_unpack(x2, x0, x1);
+  x2 = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const float big = 12582912.f;
+  const uint64_t t2 = f2_add(x2, f2_pack(big, big));
+  const uint64_t f2 = f2_fma(f2_add(t2, f2_pack(-big, -big)), f2_pack(-1.f, -1.f), x2);
+  uint64_t r2 = f2_fma(f2, f2_pack(0.009570100344717503f, 0.009570100344717503f), f2_pack(0.05591785907745361f, 0.05591785907745361f));
+  r2 = f2_fma(r2, f2, f2_pack(0.240247443318367f, 0.240247443318367f));
+  r2 = f2_fma(r2, f2, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+  r2 = f2_fma(r2, f2, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1;
+  f2_unpack(t2, t0, t1);
+  f2_unpack(r2, a, b);
+  a = __int_as_float(__float_as_int(a) + (__float_as_int(t0) << 23));
+  b = __int_as_float(__float_as_int(b) + (__float_as_int(t1) << 23));
+}
+
 // Weights of a 32-column piece to TMEM column tp: 2^(s * scale - ref), summed in fp32 and packed to the cache's
-// type (rounded for the matrix unit; the sum keeps the unrounded weights).
+// type (rounded for the matrix unit; the sum keeps the unrounded weights).  Every second pair goes to the fma
+// pipe: the special-function unit alone (16 a cycle and SM) would take as long as the products at head
+// size 128 and twice as long at 64.
 template <typename T>
 __device__ __forceinline__ void kt_weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t ref2, uint64_t& sum0, uint64_t& sum1,
                                            uint32_t tp) {
@@ -317,21 +341,25 @@ __device__ __forceinline__ void kt_weights(const uint32_t (&s)[32], uint64_t sca
 #pragma unroll
     for (int y = 0; y < 8; ++y) {
       const int x = z * 16 + y * 2;
+      const uint64_t v = f2_fma(f2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, ref2);
       float a, b;
-      f2_unpack(f2_fma(f2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, ref2), a, b);
-      a = exp2_fast(a);
-      b = exp2_fast(b);
-      if (y & 1)
+      if (y & 1) {
+        exp2_fma(v, a, b);
         sum1 = f2_add(sum1, f2_pack(a, b));
-      else
+      } else {
+        f2_unpack(v, a, b);
+        a = exp2_fast(a);
+        b = exp2_fast(b);
         sum0 = f2_add(sum0, f2_pack(a, b));
+      }
       w[y] = pack2<T>(a, b);
     }
     tmem_store8(tp + z * 8, w);
   }
 }
 
-// One thread: queries once, then keys and values of every tile, page by page, into the ring.
+// One warp: queries once, then keys and values of every tile, page by page, into the ring.  The lanes look up a
+// tile's pages side by side, a tile ahead; one elected lane issues the copies.
 template <int HDP>
 __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv, const KtParams& p,
                                         const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int hk) {
@@ -339,43 +367,59 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const KvView& c = p.c;
-  const int tiles_q = w.tokens1 > 0 ? 2 : 1;
-  mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
-  for (int g = 0; g < tiles_q; ++g)
+  const int lane = threadIdx.x & 31;
+  const int tiles_q = uniform(w.tokens1 > 0 ? 2 : 1), n = uniform(w.jend - w.j0), box = p.box, boxes = KT_BK / box;
+  const int32_t q0 = uniform(int32_t(w.s.first + w.t0));
+  if (elect_lane()) {
+    mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
+    for (int g = 0; g < tiles_q; ++g)
 #pragma unroll
-    for (int hh = 0; hh < HDP / 64; ++hh)
-      tma_load_3d_at(qs + g * Cfg::TILE_BYTES + hh * Cfg::HALF_BYTES, tmq, hh * 64, hk * p.group,
-                     int32_t(w.s.first + w.t0 + g * p.tile_tokens), bars + B::q_full);
+      for (int hh = 0; hh < HDP / 64; ++hh)
+        tma_load_3d_at(qs + g * Cfg::TILE_BYTES + hh * Cfg::HALF_BYTES, tmq, hh * 64, hk * p.group, q0 + g * p.tile_tokens,
+                       bars + B::q_full);
+  }
+  __syncwarp();
   const int32_t* row = w.shared ? p.prefix_table : c.table + w.b * c.table_stride;
+  // the page of this lane's piece of a tile (-1: no token sees a key of it)
+  auto look_up = [&](int32_t i) -> int32_t {
+    const int32_t key = tile_index(w.tiles, w.j0 + i) * KT_BK + lane * box;
+    if (lane >= boxes || !any_needed(w.span, key, key + box)) return -1;
+    const int32_t page = page_of(row, key, c.page_shift, c.num_pages);
+    if (page >= 0) return page;
+    kv_range_error();
+    return int32_t(c.num_pages);  // behind the last page: the copy fills zeros
+  };
   uint32_t it = 0;
   bool ok = true;
-  for (int32_t j = w.j0; j < w.jend && ok; ++j) {
-    const int32_t key0 = tile_index(w.tiles, j) * KT_BK;
-    uint32_t bytes = 0;
-    for (int32_t r = 0; r < KT_BK; r += p.box)
-      if (any_needed(w.span, key0 + r, key0 + r + p.box)) bytes += uint32_t(p.box) * 128u * (HDP / 64);
-    auto fill = [&](const CUtensorMap* map) -> bool {
-      const uint32_t s = it % NS;
-      if (it >= NS && !kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1)) return false;
-      ++it;
-      mbar_expect_at(bars + B::kv_full + 8 * s, bytes);
-      const uint32_t dst = ring + s * Cfg::TILE_BYTES;
-      for (int32_t r = 0; r < KT_BK; r += p.box) {
-        const int32_t key = key0 + r;
-        if (!any_needed(w.span, key, key + p.box)) continue;
-        int32_t page = page_of(row, key, c.page_shift, c.num_pages);
-        if (page < 0) {
-          kv_range_error();
-          page = int32_t(c.num_pages);  // behind the last page: the copy fills zeros
-        }
-        const int32_t slot = key & ((1 << c.page_shift) - 1);
+  int32_t next = n > 0 ? look_up(0) : -1;
+#pragma unroll 1
+  for (int32_t i = 0; i < n && ok; ++i) {
+    const int32_t page = next;
+    const int32_t slot0 = uniform((tile_index(w.tiles, w.j0 + i) * KT_BK) & ((1 << c.page_shift) - 1));
+    if (i + 1 < n) next = look_up(i + 1);
+    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+    const uint32_t bytes = uint32_t(__popc(there)) * uint32_t(box) * 128u * (HDP / 64);
 #pragma unroll
-        for (int hh = 0; hh < HDP / 64; ++hh)
-          tma_load_4d_at(dst + hh * Cfg::HALF_BYTES + r * 128, map, hh * 64, slot, hk, page, bars + B::kv_full + 8 * s);
+    for (int kv = 0; kv < 2; ++kv, ++it) {
+      const uint32_t s = it % NS;
+      if (it >= NS) ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
+      if (!ok) break;
+      const uint32_t bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::TILE_BYTES;
+      if (elect_lane()) mbar_expect_at(bar, bytes);
+      __syncwarp();
+#pragma unroll 1
+      for (int r = 0; r < boxes; ++r) {
+        const int32_t pg = __shfl_sync(0xffffffffu, page, r);
+        if (pg < 0) continue;
+        if (elect_lane()) {
+#pragma unroll
+          for (int hh = 0; hh < HDP / 64; ++hh)
+            tma_load_4d_at(dst + hh * Cfg::HALF_BYTES + r * box * 128, kv ? tmv : tmk, hh * 64, (slot0 + r * box) & ((1 << c.page_shift) - 1),
+                           hk, pg, bar);
+        }
+        __syncwarp();
       }
-      return true;
-    };
-    ok = fill(tmk) && fill(tmv);
+    }
   }
   // the last uses of the ring's slots: behind them no copy and no product is in flight
   for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
@@ -420,20 +464,23 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
     if (issues) {
       if (i == 0) ok = kt_wait<HDP>(bars, B::q_full, 0);
       ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1);
-      if (i > 0) ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 1) & 1);
+      // (the second row tile starts behind the first one's first scores, so that one's exponentials run beside the
+      // other's products)
+      if (i > 0)
+        ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 1) & 1);
+      else if (G == 1 && w.cnt0 > w.j0)
+        ok = ok && kt_wait<HDP>(bars, B::pv_done, 0);
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
         if (elect_lane()) {
           const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
           const uint64_t dq = umma_desc_at(qs + G * Cfg::TILE_BYTES), dk = umma_desc_at(ring + sk * Cfg::TILE_BYTES);
-          const int ksteps = (c.head_dim + 15) >> 4;
 #pragma unroll
-          for (int k = 0; k < HDP / 16; ++k)
-            if (k < ksteps) {
-              const uint64_t off = uint64_t((k >> 2) * int(Cfg::HALF_BYTES >> 4) + (k & 3) * 2);
-              umma_bf16(t_s, dq + off, dk + off, idesc, k > 0 ? 1u : 0u);
-            }
+          for (int k = 0; k < HDP / 16; ++k) {  // (columns behind head_dim are zeros)
+            const uint64_t off = uint64_t((k >> 2) * int(Cfg::HALF_BYTES >> 4) + (k & 3) * 2);
+            umma_bf16(t_s, dq + off, dk + off, idesc, k > 0 ? 1u : 0u);
+          }
           umma_commit_at(bars + s_bar);
           umma_commit_at(bars + B::kv_empty + 8 * sk);
         }
@@ -528,9 +575,11 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
   const bool mine = tok < (G ? w.tokens1 : w.tokens0);
   const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
   const int64_t row = int64_t(p.slot0 + split) * c.tokens * p.q_heads + token * p.q_heads + head;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  // no key seen: zeros (weights of masked keys are 2^-126, not 0); scores that are NaN leave m alone and make l NaN
+  const bool none = m == -INFINITY && l == l;
+  const float inv = none ? 0.f : 1.f / l;
   const bool state = p.row_ml != nullptr;
-  if (state && mine && ok && half == 0) p.row_ml[row] = make_float2(any ? m : -INFINITY, l);
+  if (state && mine && ok && half == 0) p.row_ml[row] = make_float2(l == l ? m : 0.f, l);
 #pragma unroll 1
   for (int x = 0; x < OC; x += 32) {
     const int col = half * OC + x;
@@ -580,7 +629,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   const uint32_t bars = ring + Cfg::SLOTS * Cfg::TILE_BYTES;
   __shared__ int64_t warp_tot[KT_THREADS / 32];
   __shared__ KtUnit found;
-  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5);
   const int64_t unit = blockIdx.x / p.c.kv_heads;
   const int hk = int(blockIdx.x - unit * p.c.kv_heads), split = blockIdx.y;
   const int32_t tt = p.tile_tokens;
@@ -642,7 +691,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
     if (warp < 8 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, qs, ring, hk, split, warp);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 16 && lane == 0 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+    if (warp == 16 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
   }
   tc_fence_before();
   __syncwarp();
