@@ -3,8 +3,8 @@
 //
 // A CTA takes two tiles of up to 128 (token, head of the key head's group) rows -- the group's heads share
 // every key they load -- and walks the tiles of 128 keys that any of its tokens sees.  Roles:
-//   warp 16  one thread loads: queries once, then keys and values of each tile by TMA, page by page, into a ring;
-//   warps 0-7, 8-15  a row tile each, two threads a row: the first thread issues tcgen05.mma for S = Q K^T (fp32 in
+//   warp 8   one thread loads: queries once, then keys and values of each tile by TMA, page by page, into a ring;
+//   warps 0-3, 4-7  a row tile each, one row a thread: the first warp issues tcgen05.mma for S = Q K^T (fp32 in
 //            TMEM), all take S from TMEM, keep the running maximum and sum in fp32 and write P, rounded to the
 //            cache's type, over S's columns; the first thread issues O += P V with P read from TMEM.
 // While one row tile's softmax runs, the tensor cores work on the other's: per 128 x 128 block at head size 128
@@ -19,7 +19,10 @@
 
 namespace lng {
 
-constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 640;
+constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 384;
+#ifndef KT_FMA_EXP
+#define KT_FMA_EXP 0x52  // of 8 pairs of exponentials, those on the fma pipe
+#endif
 
 template <int HDP>
 struct KtCfg {
@@ -27,7 +30,7 @@ struct KtCfg {
   static constexpr uint32_t HALF_BYTES = 128 * 128;      // 64 columns of them
   static constexpr int SLOTS = HDP == 128 ? 4 : 8;
   static constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;
-  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE_BYTES + 1024 + 3072;
+  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE_BYTES + 1024 + 256;
 };
 
 struct KtParams {
@@ -61,8 +64,11 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
       LNG_I8(r, 8), LNG_I8(r, 16), LNG_I8(r, 24), "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::LNG_I8(r, 0), "r"(addr) : "memory");
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::LNG_I8(r, 0),
+      LNG_I8(r, 8), "r"(addr)
+      : "memory");
 }
 #undef LNG_I8
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -207,8 +213,6 @@ struct KtBars {
   static constexpr uint32_t s_full = q_full + 8;    // [2] a row tile's scores are in TMEM
   static constexpr uint32_t pv_done = s_full + 16;  // [2] its O += P V is done: O may be read, P overwritten
   static constexpr uint32_t tmem = pv_done + 16, abort = tmem + 4;
-  static constexpr uint32_t row_max = (abort + 4 + 1023) & ~1023u;  // fp32 [2 row tiles][2 halves][128]
-  static constexpr uint32_t BYTES = row_max + 2 * 2 * 128 * 4;
 };
 
 // One lane of the (converged) warp.  Products are issued by whole warps with uniform operands and one elected
@@ -333,28 +337,35 @@ __device__ __forceinline__ void exp2_fma(uint64_t x2, float& a, float& b) {
 // pipe: the special-function unit alone (16 a cycle and SM) would take as long as the products at head
 // size 128 and twice as long at 64.
 template <typename T>
-__device__ __forceinline__ void kt_weights(const uint32_t (&s)[32], uint64_t scale2, uint64_t ref2, uint64_t& sum0, uint64_t& sum1,
+__device__ __forceinline__ void kt_weights(uint32_t (&s)[32], uint64_t scale2, uint64_t ref2, uint64_t& sum0, uint64_t& sum1,
                                            uint32_t tp) {
+  uint64_t v[16];
 #pragma unroll
-  for (int z = 0; z < 2; ++z) {
-    uint32_t w[8];
+  for (int y = 0; y < 16; ++y) v[y] = f2_fma(f2_pack(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), scale2, ref2);
 #pragma unroll
-    for (int y = 0; y < 8; ++y) {
-      const int x = z * 16 + y * 2;
-      const uint64_t v = f2_fma(f2_pack(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), scale2, ref2);
-      float a, b;
-      if (y & 1) {
-        exp2_fma(v, a, b);
-        sum1 = f2_add(sum1, f2_pack(a, b));
-      } else {
-        f2_unpack(v, a, b);
-        a = exp2_fast(a);
-        b = exp2_fast(b);
-        sum0 = f2_add(sum0, f2_pack(a, b));
-      }
-      w[y] = pack2<T>(a, b);
+  for (int y = 0; y < 16; ++y) {
+    float a, b;
+    if (KT_FMA_EXP >> (y & 7) & 1) {
+      exp2_fma(v[y], a, b);
+    } else {
+      f2_unpack(v[y], a, b);
+      a = exp2_fast(a);
+      b = exp2_fast(b);
     }
-    tmem_store8(tp + z * 8, w);
+    v[y] = f2_pack(a, b);
+  }
+  uint32_t w[16];
+#pragma unroll
+  for (int y = 0; y < 16; ++y) {
+    float a, b;
+    f2_unpack(v[y], a, b);
+    w[y] = pack2<T>(a, b);
+  }
+  tmem_store16(tp, w);
+#pragma unroll
+  for (int y = 0; y < 16; y += 2) {
+    sum0 = f2_add(sum0, v[y]);
+    sum1 = f2_add(sum1, v[y + 1]);
   }
 }
 
@@ -425,8 +436,7 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
   for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
 }
 
-// The 256 threads of row tile G, two a row (64 columns of S each, so that eight warps a row tile hide each
-// other's latencies).  Warp 0 of them issues the tile's products; per key tile
+// The 128 threads of row tile G, one a row.  Warp 0 of them issues the tile's products; per key tile
 //   S = Q K^T -> softmax in registers, P over S -> O += P V,
 // each committed to an mbarrier and waited for before its operands are touched again (the ISA orders products
 // of unlike operands only through their completion).  The other row tile's products run meanwhile.
@@ -436,16 +446,14 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
-  constexpr int OC = HDP / 2;  // columns of O a thread rescales and stores
   const KvView& c = p.c;
-  const int G = warp >> 3, quad = warp & 3, half = (warp >> 2) & 1, r = quad * 32 + (threadIdx.x & 31);
-  const bool issues = (warp & 7) == 0;
+  const int G = warp >> 2, quad = warp & 3, r = quad * 32 + (threadIdx.x & 31);
+  const bool issues = (warp & 3) == 0;
   const int32_t tok = r / p.group, n = uniform(w.jend - w.j0), cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
   const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
   const int32_t pos = w.shared ? last : first + tok;
   const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
-  const uint32_t ts = tmem_at(t_s, quad, half * 64), tp = tmem_at(t_s, quad, half * 32), to = tmem_at(t_o, quad, half * OC);
-  const uint32_t mine_x = bars + B::row_max + ((G * 2 + half) * 128 + r) * 4, other_x = mine_x ^ 512u;
+  const uint32_t ts = tmem_at(t_s, quad, 0), to = tmem_at(t_o, quad, 0);
   const uint32_t s_bar = B::s_full + 8 * G, pv_bar = B::pv_done + 8 * G;
   float m = -INFINITY, l = 0.f;
   bool ok = true;
@@ -493,39 +501,35 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
       // tiles clear them, each before its own product)
       ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1);
       if (ok && !key_needed(w.span, key0 + r)) {
-        const uint32_t v = ring + sv * Cfg::TILE_BYTES + r * 128 + half * 64;
+        const uint32_t v = ring + sv * Cfg::TILE_BYTES + r * 128;
 #pragma unroll
         for (int hh = 0; hh < HDP / 64; ++hh)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sts_zero16(v + hh * Cfg::HALF_BYTES + x * 16);
+          for (int x = 0; x < 8; ++x) sts_zero16(v + hh * Cfg::HALF_BYTES + x * 16);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     ok = ok && kt_wait<HDP>(bars, s_bar, i & 1);
     __syncwarp();
     tc_fence_after();
-    uint32_t s0[32], s1[32];
-    tmem_ld32(ts, s0);
-    tmem_ld32(ts + 32, s1);
-    tmem_wait32(s0);
-    tmem_wait32(s1);
+    uint32_t s[4][32];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tmem_ld32(ts + x * 32, s[x]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tmem_wait32(s[x]);
     if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
       // visible columns of this row: x <= hi and (x > lo or x < sink)
       const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
-      kt_mask(s0, half * 64, hi, lo, sink);
-      kt_mask(s1, half * 64 + 32, hi, lo, sink);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) kt_mask(s[x], x * 32, hi, lo, sink);
     }
-    // the row's maximum over both halves (behind the barrier all of S has been read: P may overwrite it)
-    const float here = fmaxf(kt_max(s0), kt_max(s1));
-    sts32(mine_x, __float_as_uint(here));
-    asm volatile("bar.sync %0, 256;" ::"r"(1 + G) : "memory");
-    const float top = fmaxf(here, __uint_as_float(lds32(other_x))) * p.scale_log2;
+    const float top = fmaxf(fmaxf(kt_max(s[0]), kt_max(s[1])), fmaxf(kt_max(s[2]), kt_max(s[3]))) * p.scale_log2;
     const bool grow = top > m + 8.f || (i == 0 && top > m);
     if (i > 0 && __any_sync(0xffffffffu, grow)) {
       const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
       l *= f;
 #pragma unroll 1
-      for (int x = 0; x < OC; x += 32) {
+      for (int x = 0; x < HDP; x += 32) {
         uint32_t o[32];
         tmem_ld32(to + x, o);
         tmem_wait32(o);
@@ -538,15 +542,15 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
     const float ref = m == -INFINITY ? 0.f : m;
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), ref2 = f2_pack(-ref, -ref);
     uint64_t sum0 = 0, sum1 = 0;
-    kt_weights<T>(s0, scale2, ref2, sum0, sum1, tp);
-    kt_weights<T>(s1, scale2, ref2, sum0, sum1, tp + 16);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) kt_weights<T>(s[x], scale2, ref2, sum0, sum1, ts + x * 16);
     float a0, a1, b0, b1;
     f2_unpack(sum0, a0, a1);
     f2_unpack(sum1, b0, b1);
     l += (a0 + a1) + (b0 + b1);
     tmem_wait_st();
     tc_fence_before();
-    asm volatile("bar.sync %0, 256;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
     if (issues && __all_sync(0xffffffffu, ok)) {
       tc_fence_after();
       if (elect_lane()) {
@@ -568,9 +572,6 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
   if (any) ok = ok && kt_wait<HDP>(bars, pv_bar, uint32_t(cnt - 1) & 1);
   __syncwarp();
   tc_fence_after();
-  sts32(mine_x, __float_as_uint(l));
-  asm volatile("bar.sync %0, 256;" ::"r"(1 + G) : "memory");
-  l += __uint_as_float(lds32(other_x));
   const int32_t head = hk * p.group + (r - tok * p.group);
   const bool mine = tok < (G ? w.tokens1 : w.tokens0);
   const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
@@ -579,14 +580,13 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
   const bool none = m == -INFINITY && l == l;
   const float inv = none ? 0.f : 1.f / l;
   const bool state = p.row_ml != nullptr;
-  if (state && mine && ok && half == 0) p.row_ml[row] = make_float2(l == l ? m : 0.f, l);
+  if (state && mine && ok) p.row_ml[row] = make_float2(l == l ? m : 0.f, l);
 #pragma unroll 1
-  for (int x = 0; x < OC; x += 32) {
-    const int col = half * OC + x;
+  for (int col = 0; col < HDP; col += 32) {
     uint32_t o[32];
     __syncwarp();
     if (any) {
-      tmem_ld32(to + x, o);
+      tmem_ld32(to + col, o);
       tmem_wait32(o);
     } else {
 #pragma unroll
@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
     sts32(bars + B::abort, 0u);
     fence_mbar_init();
   }
-  if (warp == 16) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bars + B::tmem),
                  "r"(Cfg::TMEM_COLS)
                  : "memory");
@@ -685,18 +685,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = lds32(bars + B::tmem);
 
-  // registers: 640 threads x 96 at launch; the row tiles' warps take 104, the others 64 (61440 in all)
-  if (warp < 16) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    if (warp < 8 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, qs, ring, hk, split, warp);
+  // registers: 384 threads x 168 at launch; the row tiles' warps take 208 (128 of them a row of S), the others
+  // 80 (63488 of 64512)
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (warp < 4 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, qs, ring, hk, split, warp);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 16 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
   }
   tc_fence_before();
   __syncwarp();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS));
   }
