@@ -19,18 +19,18 @@
 
 namespace lng {
 
-constexpr int KT_BM = 128, KT_BK = 128, KT_THREADS = 384;
+constexpr int KT_BM = 128, KT_BK = 64, KT_THREADS = 384;
 #ifndef KT_FMA_EXP
 #define KT_FMA_EXP 0x52  // of 8 pairs of exponentials, those on the fma pipe
 #endif
 
 template <int HDP>
 struct KtCfg {
-  static constexpr uint32_t TILE_BYTES = 128 * HDP * 2;  // 128 rows of queries, keys or values
-  static constexpr uint32_t HALF_BYTES = 128 * 128;      // 64 columns of them
-  static constexpr int SLOTS = HDP == 128 ? 4 : 8;
+  static constexpr uint32_t Q_BYTES = 128 * HDP * 2, Q_HALF = 128 * 128;        // a row tile of queries; 64 columns of it
+  static constexpr uint32_t KV_BYTES = KT_BK * HDP * 2, KV_HALF = KT_BK * 128;  // a tile of keys or values
+  static constexpr int SLOTS = HDP == 128 ? 8 : 16;
   static constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;
-  static constexpr size_t SMEM = size_t(2 + SLOTS) * TILE_BYTES + 1024 + 256;
+  static constexpr size_t SMEM = size_t(2) * Q_BYTES + size_t(SLOTS) * KV_BYTES + 1024 + 512;
 };
 
 struct KtParams {
@@ -210,8 +210,9 @@ struct KtBars {
   static constexpr uint32_t NS = KtCfg<HDP>::SLOTS;
   static constexpr uint32_t kv_full = 0, kv_empty = 8 * NS;  // [NS] each; empty: one arrival a row tile
   static constexpr uint32_t q_full = 16 * NS;
-  static constexpr uint32_t s_full = q_full + 8;    // [2] a row tile's scores are in TMEM
-  static constexpr uint32_t pv_done = s_full + 16;  // [2] its O += P V is done: O may be read, P overwritten
+  static constexpr uint32_t s_full = q_full + 8;    // [2 row tiles][2]: scores of an even / odd key tile are in TMEM
+  static constexpr uint32_t p_full = s_full + 32;   // [2][2], 128 arrivals: the tile's weights are, O is rescaled
+  static constexpr uint32_t pv_done = p_full + 32;  // [2] O += P V is done
   static constexpr uint32_t tmem = pv_done + 16, abort = tmem + 4;
 };
 
@@ -261,6 +262,7 @@ __device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
 // Bounded wait that also gives up when another role has (an expired wait records the device error).
 template <int HDP>
 __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t parity) {
+  if (mbar_try_at(bars + bar, parity)) return true;
   for (uint32_t i = 0; i < (1u << 22); ++i) {
     if (mbar_try_at(bars + bar, parity)) return true;
     if ((i & 63) == 63 && lds32(bars + KtBars<HDP>::abort)) return false;
@@ -386,7 +388,7 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
     for (int g = 0; g < tiles_q; ++g)
 #pragma unroll
       for (int hh = 0; hh < HDP / 64; ++hh)
-        tma_load_3d_at(qs + g * Cfg::TILE_BYTES + hh * Cfg::HALF_BYTES, tmq, hh * 64, hk * p.group, q0 + g * p.tile_tokens,
+        tma_load_3d_at(qs + g * Cfg::Q_BYTES + hh * Cfg::Q_HALF, tmq, hh * 64, hk * p.group, q0 + g * p.tile_tokens,
                        bars + B::q_full);
   }
   __syncwarp();
@@ -415,7 +417,7 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
       const uint32_t s = it % NS;
       if (it >= NS) ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
       if (!ok) break;
-      const uint32_t bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::TILE_BYTES;
+      const uint32_t bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::KV_BYTES;
       if (elect_lane()) mbar_expect_at(bar, bytes);
       __syncwarp();
 #pragma unroll 1
@@ -425,7 +427,7 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
         if (elect_lane()) {
 #pragma unroll
           for (int hh = 0; hh < HDP / 64; ++hh)
-            tma_load_4d_at(dst + hh * Cfg::HALF_BYTES + r * box * 128, kv ? tmv : tmk, hh * 64, (slot0 + r * box) & ((1 << c.page_shift) - 1),
+            tma_load_4d_at(dst + hh * Cfg::KV_HALF + r * box * 128, kv ? tmv : tmk, hh * 64, (slot0 + r * box) & ((1 << c.page_shift) - 1),
                            hk, pg, bar);
         }
         __syncwarp();
@@ -436,98 +438,126 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
   for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
 }
 
-// The 128 threads of row tile G, one a row.  Warp 0 of them issues the tile's products; per key tile
-//   S = Q K^T -> softmax in registers, P over S -> O += P V,
-// each committed to an mbarrier and waited for before its operands are touched again (the ISA orders products
-// of unlike operands only through their completion).  The other row tile's products run meanwhile.
+// One warp a row tile issues its products: the scores of the next key tile (into the other of two S buffers) ahead
+// of O += P V of this one, so that the softmax finds its scores waiting.  P lies over its tile's scores; a product's
+// operands are only overwritten once an mbarrier has shown it done (the ISA orders products of unlike operands
+// through their completion alone).
 template <typename T, int HDP>
-__device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int hk, int split,
-                                        int warp) {
+__device__ __forceinline__ void kt_multiply(const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int G) {
+  using Cfg = KtCfg<HDP>;
+  using B = KtBars<HDP>;
+  constexpr uint32_t NS = Cfg::SLOTS;
+  const int32_t n = uniform(w.jend - w.j0), cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
+  const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
+  const uint32_t pv_bar = B::pv_done + 8 * G;
+  auto scores = [&](int32_t i) -> bool {
+    const uint32_t ik = 2 * i, sk = ik % NS;
+    bool ok = kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1);
+    if (i >= 2) ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 2) & 1);  // P of tile i - 2 lies where the scores go
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    if (ok && elect_lane()) {
+      const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
+      const uint64_t dq = umma_desc_at(qs + G * Cfg::Q_BYTES), dk = umma_desc_at(ring + sk * Cfg::KV_BYTES);
+#pragma unroll
+      for (int k = 0; k < HDP / 16; ++k)  // (columns behind head_dim are zeros)
+        umma_bf16(t_s + (i & 1) * KT_BK, dq + uint64_t((k >> 2) * int(Cfg::Q_HALF >> 4) + (k & 3) * 2),
+                  dk + uint64_t((k >> 2) * int(Cfg::KV_HALF >> 4) + (k & 3) * 2), idesc, k > 0 ? 1u : 0u);
+      umma_commit_at(bars + B::s_full + 16 * G + 8 * (i & 1));
+      umma_commit_at(bars + B::kv_empty + 8 * sk);
+    }
+    __syncwarp();
+    return ok;
+  };
+  bool ok = cnt <= 0 || kt_wait<HDP>(bars, B::q_full, 0);
+  if (cnt > 0) ok = __all_sync(0xffffffffu, ok) && scores(0);
+#pragma unroll 1
+  for (int32_t i = 0; i < cnt && ok; ++i) {
+    if (i + 1 < cnt) ok = scores(i + 1);
+    const uint32_t iv = 2 * i + 1, sv = iv % NS;
+    ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1) && kt_wait<HDP>(bars, B::p_full + 16 * G + 8 * (i & 1), (i >> 1) & 1);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    if (ok && elect_lane()) {
+      const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
+      const uint64_t dv = umma_desc_at(ring + sv * Cfg::KV_BYTES);
+#pragma unroll
+      for (int k = 0; k < KT_BK / 16; ++k)  // 16 keys: 16 rows of 128 bytes
+#pragma unroll
+        for (int hh = 0; hh < HDP / 64; ++hh)  // one product per block of 64 columns
+          umma_f16_ts(t_o + hh * 64, t_s + (i & 1) * KT_BK + k * 8, dv + uint64_t(k * 128 + hh * int(Cfg::KV_HALF >> 4)), idesc,
+                      i > 0 || k > 0 ? 1u : 0u);
+      umma_commit_at(bars + pv_bar);
+      umma_commit_at(bars + B::kv_empty + 8 * sv);
+    }
+    __syncwarp();
+  }
+  // key tiles that none of this row tile's tokens sees: given back once they are there (not before: the slot's
+  // last use by the other row tile may still be going on)
+  for (int32_t k = 2 * (cnt > 0 ? cnt : 0); k < 2 * n && ok; ++k) {
+    const uint32_t sl = uint32_t(k) % NS;
+    ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sl, (uint32_t(k) / NS) & 1));
+    if (ok && elect_lane()) mbar_arrive_at(bars + B::kv_empty + 8 * sl);
+    __syncwarp();
+  }
+}
+
+// The 128 threads of row tile G, one a row: softmax of every key tile's scores, then the result.
+template <typename T, int HDP>
+__device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint32_t bars, uint32_t ring, int hk, int split, int warp) {
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const KvView& c = p.c;
   const int G = warp >> 2, quad = warp & 3, r = quad * 32 + (threadIdx.x & 31);
-  const bool issues = (warp & 3) == 0;
-  const int32_t tok = r / p.group, n = uniform(w.jend - w.j0), cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
+  const int32_t tok = r / p.group, cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
   const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
   const int32_t pos = w.shared ? last : first + tok;
-  const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
-  const uint32_t ts = tmem_at(t_s, quad, 0), to = tmem_at(t_o, quad, 0);
-  const uint32_t s_bar = B::s_full + 8 * G, pv_bar = B::pv_done + 8 * G;
+  const uint32_t ts = tmem_at(Cfg::TMEM_S + G * 128, quad, 0), to = tmem_at(Cfg::TMEM_O + G * HDP, quad, 0);
+  const uint32_t pv_bar = B::pv_done + 8 * G;
+  const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
   float m = -INFINITY, l = 0.f;
   bool ok = true;
 #pragma unroll 1
-  for (int32_t i = 0; i < n; ++i) {
-    const uint32_t ik = 2 * i, iv = 2 * i + 1, sk = ik % NS, sv = iv % NS;
-    if (i >= cnt) {  // none of this row tile's tokens sees a key of the tile
-      if (issues && elect_lane()) {
-        mbar_arrive_at(bars + B::kv_empty + 8 * sk);
-        mbar_arrive_at(bars + B::kv_empty + 8 * sv);
-      }
-      __syncwarp();
-      continue;
-    }
+  for (int32_t i = 0; i < cnt; ++i) {
     const int32_t key0 = tile_index(w.tiles, w.j0 + i) * KT_BK;
-    if (issues) {
-      if (i == 0) ok = kt_wait<HDP>(bars, B::q_full, 0);
-      ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1);
-      // (the second row tile starts behind the first one's first scores, so that one's exponentials run beside the
-      // other's products)
-      if (i > 0)
-        ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 1) & 1);
-      else if (G == 1 && w.cnt0 > w.j0)
-        ok = ok && kt_wait<HDP>(bars, B::pv_done, 0);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        tc_fence_after();
-        if (elect_lane()) {
-          const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
-          const uint64_t dq = umma_desc_at(qs + G * Cfg::TILE_BYTES), dk = umma_desc_at(ring + sk * Cfg::TILE_BYTES);
-#pragma unroll
-          for (int k = 0; k < HDP / 16; ++k) {  // (columns behind head_dim are zeros)
-            const uint64_t off = uint64_t((k >> 2) * int(Cfg::HALF_BYTES >> 4) + (k & 3) * 2);
-            umma_bf16(t_s, dq + off, dk + off, idesc, k > 0 ? 1u : 0u);
-          }
-          umma_commit_at(bars + s_bar);
-          umma_commit_at(bars + B::kv_empty + 8 * sk);
-        }
-        __syncwarp();
-        ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1));  // for the product with V
-      }
-    }
     if (!all_needed(w.span, key0, key0 + KT_BK)) {
       // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
       // tiles clear them, each before its own product)
+      const uint32_t iv = 2 * i + 1, sv = iv % NS;
       ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1);
-      if (ok && !key_needed(w.span, key0 + r)) {
-        const uint32_t v = ring + sv * Cfg::TILE_BYTES + r * 128;
+      if (ok && !key_needed(w.span, key0 + (r & 63))) {
+        const uint32_t v = ring + sv * Cfg::KV_BYTES + (r & 63) * 128 + (r >> 6) * 64;
 #pragma unroll
         for (int hh = 0; hh < HDP / 64; ++hh)
 #pragma unroll
-          for (int x = 0; x < 8; ++x) sts_zero16(v + hh * Cfg::HALF_BYTES + x * 16);
+          for (int x = 0; x < 4; ++x) sts_zero16(v + hh * Cfg::KV_HALF + x * 16);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    ok = ok && kt_wait<HDP>(bars, s_bar, i & 1);
+    ok = ok && kt_wait<HDP>(bars, B::s_full + 16 * G + 8 * (i & 1), (i >> 1) & 1);
     __syncwarp();
     tc_fence_after();
-    uint32_t s[4][32];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) tmem_ld32(ts + x * 32, s[x]);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) tmem_wait32(s[x]);
+    const uint32_t tb = ts + (i & 1) * KT_BK;
+    uint32_t s0[32], s1[32];
+    tmem_ld32(tb, s0);
+    tmem_ld32(tb + 32, s1);
+    tmem_wait32(s0);
+    tmem_wait32(s1);
     if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
       // visible columns of this row: x <= hi and (x > lo or x < sink)
       const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) kt_mask(s[x], x * 32, hi, lo, sink);
+      kt_mask(s0, 0, hi, lo, sink);
+      kt_mask(s1, 32, hi, lo, sink);
     }
-    const float top = fmaxf(fmaxf(kt_max(s[0]), kt_max(s[1])), fmaxf(kt_max(s[2]), kt_max(s[3]))) * p.scale_log2;
+    const float top = fmaxf(kt_max(s0), kt_max(s1)) * p.scale_log2;
     const bool grow = top > m + 8.f || (i == 0 && top > m);
     if (i > 0 && __any_sync(0xffffffffu, grow)) {
       const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
       l *= f;
+      ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 1) & 1);  // the product before this one is done with O
+      __syncwarp();
+      tc_fence_after();
 #pragma unroll 1
       for (int x = 0; x < HDP; x += 32) {
         uint32_t o[32];
@@ -540,35 +570,22 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
     }
     if (grow) m = top;
     const float ref = m == -INFINITY ? 0.f : m;
-    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), ref2 = f2_pack(-ref, -ref);
+    const uint64_t ref2 = f2_pack(-ref, -ref);
     uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) kt_weights<T>(s[x], scale2, ref2, sum0, sum1, ts + x * 16);
+    kt_weights<T>(s0, scale2, ref2, sum0, sum1, tb);
+    kt_weights<T>(s1, scale2, ref2, sum0, sum1, tb + 16);
     float a0, a1, b0, b1;
     f2_unpack(sum0, a0, a1);
     f2_unpack(sum1, b0, b1);
     l += (a0 + a1) + (b0 + b1);
     tmem_wait_st();
     tc_fence_before();
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + G) : "memory");  // the row tile's P and zeroed values are there
-    if (issues && __all_sync(0xffffffffu, ok)) {
-      tc_fence_after();
-      if (elect_lane()) {
-        const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
-        const uint64_t dv = umma_desc_at(ring + sv * Cfg::TILE_BYTES);
-#pragma unroll
-        for (int k = 0; k < KT_BK / 16; ++k)  // 16 keys: 16 rows of 128 bytes
-#pragma unroll
-          for (int hh = 0; hh < HDP / 64; ++hh)  // one product per block of 64 columns
-            umma_f16_ts(t_o + hh * 64, t_s + k * 8, dv + uint64_t(k * 128 + hh * int(Cfg::HALF_BYTES >> 4)), idesc,
-                        i > 0 || k > 0 ? 1u : 0u);
-        umma_commit_at(bars + pv_bar);
-        umma_commit_at(bars + B::kv_empty + 8 * sv);
-      }
-      __syncwarp();
-    }
+    mbar_arrive_at(bars + B::p_full + 16 * G + 8 * (i & 1));
   }
   const bool any = cnt > 0;
+  // the last two products may be under way (the last scores have shown the one before them done): one phase of
+  // the barrier after the other, since a parity only tells neighbouring phases apart
+  if (cnt > 1) ok = ok && kt_wait<HDP>(bars, pv_bar, uint32_t(cnt - 2) & 1);
   if (any) ok = ok && kt_wait<HDP>(bars, pv_bar, uint32_t(cnt - 1) & 1);
   __syncwarp();
   tc_fence_after();
@@ -625,8 +642,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   extern __shared__ uint8_t kt_smem_raw[];
-  const uint32_t qs = (smem_addr(kt_smem_raw) + 1023) & ~1023u, ring = qs + 2 * Cfg::TILE_BYTES;
-  const uint32_t bars = ring + Cfg::SLOTS * Cfg::TILE_BYTES;
+  const uint32_t qs = (smem_addr(kt_smem_raw) + 1023) & ~1023u, ring = qs + 2 * Cfg::Q_BYTES;
+  const uint32_t bars = ring + Cfg::SLOTS * Cfg::KV_BYTES;
   __shared__ int64_t warp_tot[KT_THREADS / 32];
   __shared__ KtUnit found;
   const int tid = threadIdx.x, warp = uniform(tid >> 5);
@@ -668,7 +685,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
     }
     mbar_init_at(bars + B::q_full, 1);
     for (int g = 0; g < 2; ++g) {
-      mbar_init_at(bars + B::s_full + 8 * g, 1);
+      mbar_init_at(bars + B::s_full + 16 * g, 1);
+      mbar_init_at(bars + B::s_full + 16 * g + 8, 1);
+      mbar_init_at(bars + B::p_full + 16 * g, 128);
+      mbar_init_at(bars + B::p_full + 16 * g + 8, 128);
       mbar_init_at(bars + B::pv_done + 8 * g, 1);
     }
     sts32(bars + B::abort, 0u);
@@ -685,14 +705,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = lds32(bars + B::tmem);
 
-  // registers: 384 threads x 168 at launch; the row tiles' warps take 208 (128 of them a row of S), the others
-  // 80 (63488 of 64512)
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    if (warp < 4 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, qs, ring, hk, split, warp);
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 8 && w.jend > w.j0) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+    if (warp < 4 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, ring, hk, split, warp);
+  } else if (w.jend > w.j0) {
+    if (warp == 8) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
+    if (warp == 9 || (warp == 10 && w.tokens1 > 0)) kt_multiply<T, HDP>(w, bars, qs, ring, warp - 9);
   }
   tc_fence_before();
   __syncwarp();
