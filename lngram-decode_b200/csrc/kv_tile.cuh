@@ -30,7 +30,7 @@ struct KtCfg {
   static constexpr uint32_t KV_BYTES = KT_BK * HDP * 2, KV_HALF = KT_BK * 128;  // a tile of keys or values
   static constexpr int SLOTS = HDP == 128 ? 8 : 16;
   static constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;
-  static constexpr size_t SMEM = size_t(2) * Q_BYTES + size_t(SLOTS) * KV_BYTES + 1024 + 512;
+  static constexpr size_t SMEM = size_t(2) * Q_BYTES + size_t(SLOTS) * KV_BYTES + 8 * 4096 + 1024 + 512;
 };
 
 struct KtParams {
@@ -40,7 +40,8 @@ struct KtParams {
   float scale_log2;
   int32_t window, sinks;
   int32_t box;              // keys a TMA copy: min(page size, 128)
-  int32_t splits;           // key ranges a unit's tiles are divided into (grid z)
+  int32_t splits;           // key ranges a unit's tiles are divided into
+  int64_t total;            // units
   const int32_t* prefix_table;  // not null: all tokens against the shared prefix, every key visible
   int32_t prefix_len;
   float2* row_ml;           // split or prefix: states to [slot0 + split][row], row = token * q_heads + head
@@ -111,19 +112,54 @@ __device__ __forceinline__ void tma_load_4d_at(uint32_t dst, const CUtensorMap* 
       : "memory");
 }
 
-// The unit (2 * tile_tokens tokens of one sequence) of a CTA: tokens t0 .. of the span, or n = 0 when there is
-// none.  Steps of equal n: the last units of all sequences, which see the most keys, come first.  Ragged
-// steps: the sequences' units in a line, last units first within a sequence.
-struct KtUnit {
+// A unit of work: 2 * tile_tokens tokens of one sequence (two row tiles), one key head, one range of the keys.
+// Every warp of a CTA walks the CTA's units by itself.
+struct KtWork {
   SeqSpan s;
   int64_t b;
-  int32_t t0;
+  int32_t hk, split;
+  int32_t t0, window, sinks;
+  int32_t tokens0, tokens1;          // tokens of the two row tiles
+  int32_t pos0, pos1, last0, last1;  // first and last position of each row tile
+  int32_t cnt0, cnt1;                // key tiles [j0, j0 + cnt) are visited for a row tile
+  int32_t j0, n;                     // [j0, j0 + n) for either
+  bool shared;
+  KeySpan span;
+  KeyTiles tiles;
 };
 
-__device__ inline KtUnit kt_find(const KvView& c, const int32_t* prefix_table, int32_t prefix_len, int64_t u, int32_t span,
-                                 int nthreads, int64_t* warp_tot, KtUnit* found) {
-  KtUnit r{};
-  if (prefix_table != nullptr) {  // all tokens of the step are one sequence
+// Of the key tiles [j0, j1) those (a leading run) that hold keys up to `last`.
+__device__ __forceinline__ int32_t kt_count(const KeyTiles& t, int32_t last, int32_t tokens, int32_t j0, int32_t j1) {
+  const int32_t end = last >= 0 && tokens > 0 ? last / KT_BK + 1 : 0;
+  int32_t n = end <= t.first ? (end < t.sink_tiles ? end : t.sink_tiles) : t.sink_tiles + end - t.first;
+  n = n < j1 ? n : j1;
+  return n > j0 ? n - j0 : 0;
+}
+
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// The CTA's units: unit i of round k is k * grid + i, every second round backwards, so that each CTA's sum of units
+// of falling size evens out.  Steps of equal n: the last units of all sequences, which see the most keys, come
+// first.  Ragged steps: the sequences' units in a line, last units first within a sequence; the line is
+// searched forward from where the last unit was found.
+struct KtWalk {
+  int64_t round, b, base;  // base: units of the sequences before b
+};
+
+__device__ __forceinline__ bool kt_next(const KtParams& p, KtWalk& walk, KtWork& w, bool& there) {
+  const KvView& c = p.c;
+  const int64_t grid = gridDim.x, k = walk.round++;
+  const int64_t idx = k * grid + (k & 1 ? grid - 1 - int64_t(blockIdx.x) : int64_t(blockIdx.x));
+  there = false;
+  if (k * grid >= p.total) return false;
+  if (idx >= p.total) return true;
+  const int64_t u = idx / (int64_t(c.kv_heads) * p.splits);
+  const int32_t rest = int32_t(idx - u * c.kv_heads * p.splits);
+  w.hk = rest / p.splits;
+  w.split = rest - w.hk * p.splits;
+  w.shared = p.prefix_table != nullptr;
+  const int32_t tt = p.tile_tokens, span = 2 * tt;
+  if (w.shared) {  // all tokens of the step are one sequence, standing behind the prefix's last key
     int64_t first = 0, end = c.tokens;
     if (c.cu != nullptr) {
       first = c.cu[0];
@@ -134,74 +170,66 @@ __device__ inline KtUnit kt_find(const KvView& c, const int32_t* prefix_table, i
         end = end > c.tokens ? c.tokens : end < first ? first : end;
       }
     }
-    r.b = 0;
-    r.s.first = first;
-    r.s.n = int32_t(end - first);
-    r.s.len = prefix_len;
-    r.t0 = int32_t(u * span < r.s.n ? u * span : r.s.n);
-    return r;
-  }
-  if (c.cu == nullptr) {
-    const int64_t per = (c.max_new + span - 1) / span;
-    r.b = u % c.batch;
-    r.s = kv_span(c, r.b);
-    const int64_t k = u / c.batch;
-    r.t0 = k < per ? int32_t((per - 1 - k) * span) : r.s.n;
-    return r;
-  }
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t run = (c.batch + nthreads - 1) / nthreads;
-  const int64_t b0 = tid * run, b1 = b0 + run < c.batch ? b0 + run : c.batch;
-  int64_t mine = 0;
-  for (int64_t b = b0; b < b1; ++b) mine += (kv_span(c, b).n + span - 1) / span;
-  int64_t incl = mine;
+    w.b = 0;
+    w.s.first = first;
+    w.s.n = int32_t(end - first);
+    w.s.len = p.prefix_len;
+    if (u * span >= w.s.n) return true;
+    w.t0 = int32_t(u * span);
+  } else if (c.cu == nullptr) {
+    const int64_t per = (c.max_new + span - 1) / span, r = u / c.batch;
+    if (r >= per) return true;
+    w.b = u - r * c.batch;
+    w.s = kv_span(c, w.b);
+    w.t0 = int32_t((per - 1 - r) * span);
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (;;) {  // 32 sequences a step
+      if (walk.b >= c.batch) return true;
+      const int64_t b = walk.b + lane;
+      SeqSpan s{};
+      if (b < c.batch) s = kv_span(c, b);
+      const int32_t mine = (s.n + span - 1) / span;
+      int64_t incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) warp_tot[warp] = incl;
-  if (tid == 0) found->b = -1;
-  __syncthreads();
-  int64_t at = incl - mine;
-  for (int w = 0; w < warp; ++w) at += warp_tot[w];
-  if (u >= at && u < at + mine) {
-    for (int64_t b = b0; b < b1; ++b) {
-      const SeqSpan s = kv_span(c, b);
-      const int64_t n = (s.n + span - 1) / span;
-      if (u < at + n) {
-        found->s = s;
-        found->b = b;
-        found->t0 = int32_t((n - 1 - (u - at)) * span);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      incl += walk.base;
+      const uint32_t hit = __ballot_sync(0xffffffffu, u >= incl - mine && u < incl);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        w.b = walk.b + src;
+        w.s.first = __shfl_sync(0xffffffffu, s.first, src);
+        w.s.n = __shfl_sync(0xffffffffu, s.n, src);
+        w.s.len = __shfl_sync(0xffffffffu, s.len, src);
+        w.t0 = __shfl_sync(0xffffffffu, int32_t((incl - 1 - u) * span), src);
         break;
       }
-      at += n;
+      walk.base = __shfl_sync(0xffffffffu, incl, 31);
+      walk.b += 32;
     }
   }
-  __syncthreads();
-  if (found->b < 0) return r;
-  return *found;
-}
-
-// What every role of a CTA knows about its unit: the two row tiles' tokens, positions and key tiles.
-struct KtWork {
-  SeqSpan s;
-  int64_t b;
-  int32_t t0, window, sinks;
-  int32_t tokens0, tokens1;  // tokens of the two row tiles
-  int32_t pos0, pos1, last0, last1;  // first and last position of each row tile
-  int32_t cnt0, cnt1;        // key tiles [j0, cnt) are visited for a row tile
-  int32_t j0, jend;
-  bool shared;
-  KeySpan span;
-  KeyTiles tiles;
-};
-
-__device__ __forceinline__ int32_t kt_count(const KeyTiles& t, int32_t last, int32_t tokens, int32_t j0, int32_t j1) {
-  const int32_t end = last >= 0 && tokens > 0 ? last / KT_BK + 1 : 0;  // tiles of the keys up to `last`
-  int32_t n = end <= t.first ? (end < t.sink_tiles ? end : t.sink_tiles) : t.sink_tiles + end - t.first;
-  n = n < j1 ? n : j1;
-  return n > j0 ? n : j0;
+  there = true;
+  w.window = w.shared ? 0 : p.window;
+  w.sinks = w.shared ? 0 : p.sinks;
+  const int32_t left = w.s.n - w.t0;
+  w.tokens0 = left < tt ? left : tt;
+  w.tokens1 = left <= tt ? 0 : (left < span ? left - tt : tt);
+  const int32_t at = w.s.len - w.s.n + w.t0;
+  w.pos0 = w.shared ? w.s.len - 1 : at;
+  w.last0 = w.shared ? w.s.len - 1 : at + w.tokens0 - 1;
+  w.pos1 = w.shared ? w.s.len - 1 : at + tt;
+  w.last1 = w.shared ? w.s.len - 1 : at + tt + w.tokens1 - 1;
+  w.span = key_span(w.pos0, w.tokens1 > 0 ? w.last1 : w.last0, w.window, w.sinks);
+  w.tiles = key_tiles(w.span, KT_BK);
+  w.j0 = int32_t(int64_t(w.tiles.count) * w.split / p.splits);
+  const int32_t j1 = int32_t(int64_t(w.tiles.count) * (w.split + 1) / p.splits);
+  w.cnt0 = uniform(kt_count(w.tiles, w.last0, w.tokens0, w.j0, j1));
+  w.cnt1 = uniform(kt_count(w.tiles, w.last1, w.tokens1, w.j0, j1));
+  w.n = w.cnt0 > w.cnt1 ? w.cnt0 : w.cnt1;
+  return true;
 }
 
 // Shared memory behind the tiles, by 32-bit shared addresses (offsets from the block's).
@@ -209,11 +237,14 @@ template <int HDP>
 struct KtBars {
   static constexpr uint32_t NS = KtCfg<HDP>::SLOTS;
   static constexpr uint32_t kv_full = 0, kv_empty = 8 * NS;  // [NS] each; empty: one arrival a row tile
-  static constexpr uint32_t q_full = 16 * NS;
-  static constexpr uint32_t s_full = q_full + 8;    // [2 row tiles][2]: scores of an even / odd key tile are in TMEM
+  static constexpr uint32_t q_full = 16 * NS, q_empty = q_full + 8;  // empty: one arrival a row tile
+  static constexpr uint32_t s_full = q_empty + 8;    // [2 row tiles][2]: scores of an even / odd key tile are in TMEM
   static constexpr uint32_t p_full = s_full + 32;   // [2][2], 128 arrivals: the tile's weights are, O is rescaled
-  static constexpr uint32_t pv_done = p_full + 32;  // [2] O += P V is done
-  static constexpr uint32_t tmem = pv_done + 16, abort = tmem + 4;
+  static constexpr uint32_t pv_done = p_full + 32;  // [2] O += P V is done, a phase a tile
+  static constexpr uint32_t o_full = pv_done + 16;  // [2] the unit's last one is
+  static constexpr uint32_t tmem = o_full + 16, abort = tmem + 4;
+  // A wait names a phase by its parity alone, so a role may only wait for a phase while the barrier can be in that
+  // one or the next: every role waits for the phases of its barriers one after the other.
 };
 
 // One lane of the (converged) warp.  Products are issued by whole warps with uniform operands and one elected
@@ -223,8 +254,6 @@ __device__ __forceinline__ bool elect_lane() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok)::"memory");
   return ok != 0;
 }
-__device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
-
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -232,6 +261,14 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 }
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) {
   asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
 }
 __device__ __forceinline__ void sts_zero16(uint32_t a) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0u) : "memory");
@@ -259,13 +296,19 @@ __device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait that also gives up when another role has (an expired wait records the device error).
+// Wait bounded by time (two seconds; the longest wait of a working kernel is a unit's, milliseconds), which also
+// gives up when another role has.  An expired wait records the device error.
 template <int HDP>
 __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t parity) {
   if (mbar_try_at(bars + bar, parity)) return true;
-  for (uint32_t i = 0; i < (1u << 22); ++i) {
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(start));
+  for (uint32_t i = 0;; ++i) {
     if (mbar_try_at(bars + bar, parity)) return true;
-    if ((i & 63) == 63 && lds32(bars + KtBars<HDP>::abort)) return false;
+    if ((i & 63) != 63) continue;
+    if (lds32(bars + KtBars<HDP>::abort)) return false;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+    if (now - start > 2000000000ull) break;
   }
   atomicCAS(&g_error_word, 0u, (unsigned int)DEV_ERR_WAIT_TIMEOUT);
   sts32(bars + KtBars<HDP>::abort, 1u);
@@ -371,71 +414,80 @@ __device__ __forceinline__ void kt_weights(uint32_t (&s)[32], uint64_t scale2, u
   }
 }
 
-// One warp: queries once, then keys and values of every tile, page by page, into the ring.  The lanes look up a
-// tile's pages side by side, a tile ahead; one elected lane issues the copies.
+// One warp: for every unit its queries, then keys and values of every tile, page by page, into the ring.  The lanes
+// look up a tile's pages side by side, a tile ahead; one elected lane issues the copies.
 template <int HDP>
 __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv, const KtParams& p,
-                                        const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int hk) {
+                                        uint32_t bars, uint32_t qs, uint32_t ring) {
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const KvView& c = p.c;
-  const int lane = threadIdx.x & 31;
-  const int tiles_q = uniform(w.tokens1 > 0 ? 2 : 1), n = uniform(w.jend - w.j0), box = p.box, boxes = KT_BK / box;
-  const int32_t q0 = uniform(int32_t(w.s.first + w.t0));
-  if (elect_lane()) {
-    mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
-    for (int g = 0; g < tiles_q; ++g)
+  const int lane = threadIdx.x & 31, box = p.box, boxes = KT_BK / box;
+  const int32_t page_mask = (1 << c.page_shift) - 1;
+  uint32_t it = 0, units = 0;  // copies into the ring, units with keys
+  bool ok = true, there;
+  KtWalk walk{};
+  KtWork w;
+  while (ok && kt_next(p, walk, w, there)) {
+    if (!there || w.n == 0) continue;
+    const int32_t* row = w.shared ? p.prefix_table : c.table + w.b * c.table_stride;
+    // the page of this lane's piece of a tile (-1: no token sees a key of it)
+    auto look_up = [&](int32_t i) -> int32_t {
+      const int32_t key = tile_index(w.tiles, w.j0 + i) * KT_BK + lane * box;
+      if (lane >= boxes || !any_needed(w.span, key, key + box)) return -1;
+      const int32_t page = page_of(row, key, c.page_shift, c.num_pages);
+      if (page >= 0) return page;
+      kv_range_error();
+      return int32_t(c.num_pages);  // behind the last page: the copy fills zeros
+    };
+    int32_t next = look_up(0);
+    if (units > 0) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1));
+    if (!ok) break;
+    ++units;
+    if (elect_lane()) {
+      const int32_t tiles_q = w.tokens1 > 0 ? 2 : 1, q0 = int32_t(w.s.first + w.t0);
+      mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
+      for (int g = 0; g < tiles_q; ++g)
 #pragma unroll
-      for (int hh = 0; hh < HDP / 64; ++hh)
-        tma_load_3d_at(qs + g * Cfg::Q_BYTES + hh * Cfg::Q_HALF, tmq, hh * 64, hk * p.group, q0 + g * p.tile_tokens,
-                       bars + B::q_full);
-  }
-  __syncwarp();
-  const int32_t* row = w.shared ? p.prefix_table : c.table + w.b * c.table_stride;
-  // the page of this lane's piece of a tile (-1: no token sees a key of it)
-  auto look_up = [&](int32_t i) -> int32_t {
-    const int32_t key = tile_index(w.tiles, w.j0 + i) * KT_BK + lane * box;
-    if (lane >= boxes || !any_needed(w.span, key, key + box)) return -1;
-    const int32_t page = page_of(row, key, c.page_shift, c.num_pages);
-    if (page >= 0) return page;
-    kv_range_error();
-    return int32_t(c.num_pages);  // behind the last page: the copy fills zeros
-  };
-  uint32_t it = 0;
-  bool ok = true;
-  int32_t next = n > 0 ? look_up(0) : -1;
+        for (int hh = 0; hh < HDP / 64; ++hh)
+          tma_load_3d_at(qs + g * Cfg::Q_BYTES + hh * Cfg::Q_HALF, tmq, hh * 64, w.hk * p.group, q0 + g * p.tile_tokens,
+                         bars + B::q_full);
+    }
+    __syncwarp();
 #pragma unroll 1
-  for (int32_t i = 0; i < n && ok; ++i) {
-    const int32_t page = next;
-    const int32_t slot0 = uniform((tile_index(w.tiles, w.j0 + i) * KT_BK) & ((1 << c.page_shift) - 1));
-    if (i + 1 < n) next = look_up(i + 1);
-    const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-    const uint32_t bytes = uint32_t(__popc(there)) * uint32_t(box) * 128u * (HDP / 64);
+    for (int32_t i = 0; i < w.n && ok; ++i) {
+      const int32_t page = next;
+      const int32_t slot0 = uniform((tile_index(w.tiles, w.j0 + i) * KT_BK) & page_mask);
+      if (i + 1 < w.n) next = look_up(i + 1);
+      const uint32_t there_boxes = __ballot_sync(0xffffffffu, page >= 0);
+      const uint32_t bytes = uint32_t(__popc(there_boxes)) * uint32_t(box) * 128u * (HDP / 64);
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv, ++it) {
-      const uint32_t s = it % NS;
-      if (it >= NS) ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
-      if (!ok) break;
-      const uint32_t bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::KV_BYTES;
-      if (elect_lane()) mbar_expect_at(bar, bytes);
-      __syncwarp();
-#pragma unroll 1
-      for (int r = 0; r < boxes; ++r) {
-        const int32_t pg = __shfl_sync(0xffffffffu, page, r);
-        if (pg < 0) continue;
-        if (elect_lane()) {
-#pragma unroll
-          for (int hh = 0; hh < HDP / 64; ++hh)
-            tma_load_4d_at(dst + hh * Cfg::KV_HALF + r * box * 128, kv ? tmv : tmk, hh * 64, (slot0 + r * box) & ((1 << c.page_shift) - 1),
-                           hk, pg, bar);
-        }
+      for (int kv = 0; kv < 2; ++kv, ++it) {
+        const uint32_t s = it % NS;
+        if (it >= NS) ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
+        if (!ok) break;
+        const uint32_t bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::KV_BYTES;
+        if (elect_lane()) mbar_expect_at(bar, bytes);
         __syncwarp();
+#pragma unroll 1
+        for (int r = 0; r < boxes; ++r) {
+          const int32_t pg = __shfl_sync(0xffffffffu, page, r);
+          if (pg < 0) continue;
+          if (elect_lane()) {
+#pragma unroll
+            for (int hh = 0; hh < HDP / 64; ++hh)
+              tma_load_4d_at(dst + hh * Cfg::KV_HALF + r * box * 128, kv ? tmv : tmk, hh * 64, (slot0 + r * box) & page_mask, w.hk, pg,
+                             bar);
+          }
+          __syncwarp();
+        }
       }
     }
   }
   // the last uses of the ring's slots: behind them no copy and no product is in flight
   for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
+  if (units > 0) kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1);
 }
 
 // One warp a row tile issues its products: the scores of the next key tile (into the other of two S buffers) ahead
@@ -443,89 +495,190 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
 // operands are only overwritten once an mbarrier has shown it done (the ISA orders products of unlike operands
 // through their completion alone).
 template <typename T, int HDP>
-__device__ __forceinline__ void kt_multiply(const KtWork& w, uint32_t bars, uint32_t qs, uint32_t ring, int G) {
+__device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, uint32_t qs, uint32_t ring, int G) {
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
-  const int32_t n = uniform(w.jend - w.j0), cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
   const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
   const uint32_t pv_bar = B::pv_done + 8 * G;
-  auto scores = [&](int32_t i) -> bool {
-    const uint32_t ik = 2 * i, sk = ik % NS;
-    bool ok = kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1);
-    if (i >= 2) ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 2) & 1);  // P of tile i - 2 lies where the scores go
-    ok = __all_sync(0xffffffffu, ok);
+  uint32_t base = 0, tile = 0, units = 0;  // ring copies before this unit, tiles of this row tile so far, units
+  bool ok = true, there;
+  // scores of ring copy ik, the row tile's tile t: they go where P of tile t - 2 lay, whose product is done
+  auto scores = [&](uint32_t ik, uint32_t t) -> bool {
+    const uint32_t sk = ik % NS;
+    // (the values too: whoever has seen the scores may touch them)
+    const bool good = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1) &&
+                                                  kt_wait<HDP>(bars, B::kv_full + 8 * ((ik + 1) % NS), ((ik + 1) / NS) & 1));
     tc_fence_after();
-    if (ok && elect_lane()) {
+    if (good && elect_lane()) {
       const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
       const uint64_t dq = umma_desc_at(qs + G * Cfg::Q_BYTES), dk = umma_desc_at(ring + sk * Cfg::KV_BYTES);
 #pragma unroll
       for (int k = 0; k < HDP / 16; ++k)  // (columns behind head_dim are zeros)
-        umma_bf16(t_s + (i & 1) * KT_BK, dq + uint64_t((k >> 2) * int(Cfg::Q_HALF >> 4) + (k & 3) * 2),
+        umma_bf16(t_s + (t & 1) * KT_BK, dq + uint64_t((k >> 2) * int(Cfg::Q_HALF >> 4) + (k & 3) * 2),
                   dk + uint64_t((k >> 2) * int(Cfg::KV_HALF >> 4) + (k & 3) * 2), idesc, k > 0 ? 1u : 0u);
-      umma_commit_at(bars + B::s_full + 16 * G + 8 * (i & 1));
+      umma_commit_at(bars + B::s_full + 16 * G + 8 * (t & 1));
       umma_commit_at(bars + B::kv_empty + 8 * sk);
     }
     __syncwarp();
-    return ok;
+    return good;
   };
-  bool ok = cnt <= 0 || kt_wait<HDP>(bars, B::q_full, 0);
-  if (cnt > 0) ok = __all_sync(0xffffffffu, ok) && scores(0);
+  KtWalk walk{};
+  KtWork w;
+  while (ok && kt_next(p, walk, w, there)) {
+    if (!there || w.n == 0) continue;
+    const int32_t cnt = G ? w.cnt1 : w.cnt0;
+    ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::q_full, units & 1));
+    ++units;
+    if (cnt > 0 && ok) ok = scores(base, tile);
 #pragma unroll 1
-  for (int32_t i = 0; i < cnt && ok; ++i) {
-    if (i + 1 < cnt) ok = scores(i + 1);
-    const uint32_t iv = 2 * i + 1, sv = iv % NS;
-    ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1) && kt_wait<HDP>(bars, B::p_full + 16 * G + 8 * (i & 1), (i >> 1) & 1);
-    ok = __all_sync(0xffffffffu, ok);
-    tc_fence_after();
-    if (ok && elect_lane()) {
-      const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
-      const uint64_t dv = umma_desc_at(ring + sv * Cfg::KV_BYTES);
+    for (int32_t i = 0; i < cnt && ok; ++i) {
+      if (tile + i > 0) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, pv_bar, (tile + i - 1) & 1));
+      if (i + 1 < cnt) {
+        ok = ok && scores(base + 2 * (i + 1), tile + i + 1);
+      } else if (elect_lane()) {
+        umma_commit_at(bars + B::q_empty);  // behind the unit's last scores
+      }
+      __syncwarp();
+      const uint32_t iv = base + 2 * i + 1, sv = iv % NS, t = tile + i;
+      ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::p_full + 16 * G + 8 * (t & 1), (t >> 1) & 1));
+      tc_fence_after();
+      if (ok && elect_lane()) {
+        const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
+        const uint64_t dv = umma_desc_at(ring + sv * Cfg::KV_BYTES);
 #pragma unroll
-      for (int k = 0; k < KT_BK / 16; ++k)  // 16 keys: 16 rows of 128 bytes
+        for (int k = 0; k < KT_BK / 16; ++k)  // 16 keys: 16 rows of 128 bytes
 #pragma unroll
-        for (int hh = 0; hh < HDP / 64; ++hh)  // one product per block of 64 columns
-          umma_f16_ts(t_o + hh * 64, t_s + (i & 1) * KT_BK + k * 8, dv + uint64_t(k * 128 + hh * int(Cfg::KV_HALF >> 4)), idesc,
-                      i > 0 || k > 0 ? 1u : 0u);
-      umma_commit_at(bars + pv_bar);
-      umma_commit_at(bars + B::kv_empty + 8 * sv);
+          for (int hh = 0; hh < HDP / 64; ++hh)  // one product per block of 64 columns
+            umma_f16_ts(t_o + hh * 64, t_s + (t & 1) * KT_BK + k * 8, dv + uint64_t(k * 128 + hh * int(Cfg::KV_HALF >> 4)), idesc,
+                        i > 0 || k > 0 ? 1u : 0u);
+        umma_commit_at(bars + pv_bar);
+        umma_commit_at(bars + B::kv_empty + 8 * sv);
+        if (i + 1 == cnt) umma_commit_at(bars + B::o_full + 8 * G);
+      }
+      __syncwarp();
     }
+    if (cnt == 0 && elect_lane()) mbar_arrive_at(bars + B::q_empty);
     __syncwarp();
-  }
-  // key tiles that none of this row tile's tokens sees: given back once they are there (not before: the slot's
-  // last use by the other row tile may still be going on)
-  for (int32_t k = 2 * (cnt > 0 ? cnt : 0); k < 2 * n && ok; ++k) {
-    const uint32_t sl = uint32_t(k) % NS;
-    ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sl, (uint32_t(k) / NS) & 1));
-    if (ok && elect_lane()) mbar_arrive_at(bars + B::kv_empty + 8 * sl);
-    __syncwarp();
+    // key tiles that none of this row tile's tokens sees: given back once they are there (not before: the slot's
+    // last use by the other row tile may still be going on)
+    for (uint32_t k = base + 2 * cnt; k < base + 2 * w.n && ok; ++k) {
+      const uint32_t sl = k % NS;
+      ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sl, (k / NS) & 1));
+      if (ok && elect_lane()) mbar_arrive_at(bars + B::kv_empty + 8 * sl);
+      __syncwarp();
+    }
+    base += 2 * w.n;
+    tile += cnt;
   }
 }
 
-// The 128 threads of row tile G, one a row: softmax of every key tile's scores, then the result.
+// A warp's 32 rows of a unit's result, from TMEM columns `to` of its lanes: to the output, or with their maximum and
+// sum as a state.  Rows pass through 4 KB of shared memory (16-byte pieces swizzled by row), so that eight lanes
+// write 128 contiguous bytes of a row.
 template <typename T, int HDP>
-__device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint32_t bars, uint32_t ring, int hk, int split, int warp) {
+__device__ __forceinline__ void kt_result(const KtParams& p, const KtWork& w, uint32_t to, uint32_t stage, int G, int quad, bool any,
+                                          bool ok, float m, float l) {
+  const KvView& c = p.c;
+  const int lane = threadIdx.x & 31;
+  const int32_t tokens = ok ? (G ? w.tokens1 : w.tokens0) : 0, rows = tokens * p.group;
+  const int64_t token0 = w.s.first + w.t0 + G * p.tile_tokens;
+  const bool state = p.row_ml != nullptr;
+  // no key seen: zeros (weights of masked keys are 2^-126, not 0); scores that are NaN leave m alone and make l NaN
+  const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
+  auto row_of = [&](int r, int64_t& token, int32_t& head) {
+    const int32_t tok = r / p.group;
+    token = token0 + tok;
+    head = w.hk * p.group + (r - tok * p.group);
+  };
+  const int64_t state0 = int64_t(p.slot0 + w.split) * c.tokens * p.q_heads;
+  if (state && quad * 32 + lane < rows) {
+    int64_t token;
+    int32_t head;
+    row_of(quad * 32 + lane, token, head);
+    p.row_ml[state0 + token * p.q_heads + head] = make_float2(l == l ? m : 0.f, l);
+  }
+  if (state && !any) return;  // (a state of sum 0 is not read)
+  const int sub = lane >> 3, piece = lane & 7;
+  const uint32_t mine = stage + lane * 128;
+#pragma unroll 1
+  for (int col = 0; col < HDP; col += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    if (any) {
+      tmem_ld32(to + col, o);
+      tmem_wait32(o);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 32; ++y) o[y] = 0u;
+    }
+    if (state) {
+#pragma unroll
+      for (int y = 0; y < 8; ++y) sts128(mine + ((y ^ (lane & 7)) << 4), o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        uint32_t w4[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          w4[z] = pack2<T>(__uint_as_float(o[8 * y + 2 * z]) * inv, __uint_as_float(o[8 * y + 2 * z + 1]) * inv);
+        const int at = (col >> 3 & 4) + y;  // two rounds of 32 columns fill the rows' 128 bytes
+        sts128(mine + ((at ^ (lane & 7)) << 4), w4[0], w4[1], w4[2], w4[3]);
+      }
+      if (!(col & 32)) continue;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int rr = x * 4 + sub, r = quad * 32 + rr;
+      if (r >= rows) continue;
+      const uint4 v = lds128(stage + rr * 128 + ((piece ^ (rr & 7)) << 4));
+      int64_t token;
+      int32_t head;
+      row_of(r, token, head);
+      if (state) {
+        const int d = col + piece * 4;
+        if (d < c.head_dim) *reinterpret_cast<uint4*>(p.row_o + (state0 + token * p.q_heads + head) * c.head_dim + d) = v;
+      } else {
+        const int d = col - 32 + piece * 8;
+        if (d < c.head_dim) *reinterpret_cast<uint4*>(static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + d) = v;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// The 128 threads of row tile G, one a row: softmax of every key tile's scores, then the unit's result.
+template <typename T, int HDP>
+__device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32_t ring, uint32_t stage, int warp) {
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
-  const KvView& c = p.c;
-  const int G = warp >> 2, quad = warp & 3, r = quad * 32 + (threadIdx.x & 31);
-  const int32_t tok = r / p.group, cnt = uniform((G ? w.cnt1 : w.cnt0) - w.j0);
-  const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
-  const int32_t pos = w.shared ? last : first + tok;
+  const int G = warp >> 2, quad = warp & 3, lane = threadIdx.x & 31, r = quad * 32 + lane;
+  const int32_t tok = r / p.group;
   const uint32_t ts = tmem_at(Cfg::TMEM_S + G * 128, quad, 0), to = tmem_at(Cfg::TMEM_O + G * HDP, quad, 0);
   const uint32_t pv_bar = B::pv_done + 8 * G;
   const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+  uint32_t base = 0, tile = 0, results = 0;  // ring copies before this unit, this row tile's tiles and results so far
+  bool ok = true, there;
+  KtWalk walk{};
+  KtWork w;
+#pragma unroll 1
+  while (kt_next(p, walk, w, there)) {
+  if (!there) continue;
+  const int32_t cnt = G ? w.cnt1 : w.cnt0;
+  const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
+  const int32_t pos = w.shared ? last : first + tok;
   float m = -INFINITY, l = 0.f;
-  bool ok = true;
 #pragma unroll 1
   for (int32_t i = 0; i < cnt; ++i) {
+    const uint32_t t = tile + i;
     const int32_t key0 = tile_index(w.tiles, w.j0 + i) * KT_BK;
+    ok = ok && kt_wait<HDP>(bars, B::s_full + 16 * G + 8 * (t & 1), (t >> 1) & 1);
     if (!all_needed(w.span, key0, key0 + KT_BK)) {
       // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
       // tiles clear them, each before its own product)
-      const uint32_t iv = 2 * i + 1, sv = iv % NS;
-      ok = ok && kt_wait<HDP>(bars, B::kv_full + 8 * sv, (iv / NS) & 1);
+      const uint32_t iv = base + 2 * i + 1, sv = iv % NS;
       if (ok && !key_needed(w.span, key0 + (r & 63))) {
         const uint32_t v = ring + sv * Cfg::KV_BYTES + (r & 63) * 128 + (r >> 6) * 64;
 #pragma unroll
@@ -535,10 +688,9 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    ok = ok && kt_wait<HDP>(bars, B::s_full + 16 * G + 8 * (i & 1), (i >> 1) & 1);
     __syncwarp();
     tc_fence_after();
-    const uint32_t tb = ts + (i & 1) * KT_BK;
+    const uint32_t tb = ts + (t & 1) * KT_BK;
     uint32_t s0[32], s1[32];
     tmem_ld32(tb, s0);
     tmem_ld32(tb + 32, s1);
@@ -555,7 +707,7 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
     if (i > 0 && __any_sync(0xffffffffu, grow)) {
       const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
       l *= f;
-      ok = ok && kt_wait<HDP>(bars, pv_bar, (i - 1) & 1);  // the product before this one is done with O
+      ok = ok && kt_wait<HDP>(bars, pv_bar, (t - 1) & 1);  // the product before this one is done with O
       __syncwarp();
       tc_fence_after();
 #pragma unroll 1
@@ -580,58 +732,16 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, const KtWork& w, uint
     l += (a0 + a1) + (b0 + b1);
     tmem_wait_st();
     tc_fence_before();
-    mbar_arrive_at(bars + B::p_full + 16 * G + 8 * (i & 1));
+    mbar_arrive_at(bars + B::p_full + 16 * G + 8 * (t & 1));
   }
   const bool any = cnt > 0;
-  // the last two products may be under way (the last scores have shown the one before them done): one phase of
-  // the barrier after the other, since a parity only tells neighbouring phases apart
-  if (cnt > 1) ok = ok && kt_wait<HDP>(bars, pv_bar, uint32_t(cnt - 2) & 1);
-  if (any) ok = ok && kt_wait<HDP>(bars, pv_bar, uint32_t(cnt - 1) & 1);
+  tile += cnt;
+  base += 2 * w.n;
+  if (any) ok = ok && kt_wait<HDP>(bars, B::o_full + 8 * G, results++ & 1);
   __syncwarp();
   tc_fence_after();
-  const int32_t head = hk * p.group + (r - tok * p.group);
-  const bool mine = tok < (G ? w.tokens1 : w.tokens0);
-  const int64_t token = w.s.first + w.t0 + G * p.tile_tokens + tok;
-  const int64_t row = int64_t(p.slot0 + split) * c.tokens * p.q_heads + token * p.q_heads + head;
-  // no key seen: zeros (weights of masked keys are 2^-126, not 0); scores that are NaN leave m alone and make l NaN
-  const bool none = m == -INFINITY && l == l;
-  const float inv = none ? 0.f : 1.f / l;
-  const bool state = p.row_ml != nullptr;
-  if (state && mine && ok) p.row_ml[row] = make_float2(l == l ? m : 0.f, l);
-#pragma unroll 1
-  for (int col = 0; col < HDP; col += 32) {
-    uint32_t o[32];
-    __syncwarp();
-    if (any) {
-      tmem_ld32(to + col, o);
-      tmem_wait32(o);
-    } else {
-#pragma unroll
-      for (int y = 0; y < 32; ++y) o[y] = 0u;
-    }
-    if (!mine || !ok) continue;
-    if (state) {
-      if (any) {  // (a state of sum 0 is not read)
-        float* dst = p.row_o + row * c.head_dim + col;
-#pragma unroll
-        for (int y = 0; y < 32; y += 4)
-          if (col + y < c.head_dim)
-            *reinterpret_cast<float4*>(dst + y) = make_float4(__uint_as_float(o[y]), __uint_as_float(o[y + 1]),
-                                                              __uint_as_float(o[y + 2]), __uint_as_float(o[y + 3]));
-      }
-    } else {
-      T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + col;
-#pragma unroll
-      for (int y = 0; y < 32; y += 8) {
-        if (col + y < c.head_dim) {
-          uint32_t w4[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            w4[z] = pack2<T>(__uint_as_float(o[y + 2 * z]) * inv, __uint_as_float(o[y + 2 * z + 1]) * inv);
-          *reinterpret_cast<uint4*>(dst + y) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-        }
-      }
-    }
+  kt_result<T, HDP>(p, w, to, stage, G, quad, any, __all_sync(0xffffffffu, ok), m, l);
+  tc_fence_before();
   }
 }
 
@@ -643,60 +753,28 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   using B = KtBars<HDP>;
   extern __shared__ uint8_t kt_smem_raw[];
   const uint32_t qs = (smem_addr(kt_smem_raw) + 1023) & ~1023u, ring = qs + 2 * Cfg::Q_BYTES;
-  const uint32_t bars = ring + Cfg::SLOTS * Cfg::KV_BYTES;
-  __shared__ int64_t warp_tot[KT_THREADS / 32];
-  __shared__ KtUnit found;
-  const int tid = threadIdx.x, warp = uniform(tid >> 5);
-  const int64_t unit = blockIdx.x / p.c.kv_heads;
-  const int hk = int(blockIdx.x - unit * p.c.kv_heads), split = blockIdx.y;
-  const int32_t tt = p.tile_tokens;
-
-  const KtUnit un = kt_find(p.c, p.prefix_table, p.prefix_len, unit, 2 * tt, KT_THREADS, warp_tot, &found);
-  if (un.t0 >= un.s.n) return;  // (the same for all threads: no unit here)
-  KtWork w;
-  w.s = un.s;
-  w.b = un.b;
-  w.t0 = un.t0;
-  w.shared = p.prefix_table != nullptr;
-  w.window = w.shared ? 0 : p.window;
-  w.sinks = w.shared ? 0 : p.sinks;
-  const int32_t left = un.s.n - un.t0;
-  w.tokens0 = left < tt ? left : tt;
-  w.tokens1 = left <= tt ? 0 : (left < 2 * tt ? left - tt : tt);
-  // against a prefix all rows stand behind its last key
-  const int32_t at = un.s.len - un.s.n + un.t0;
-  w.pos0 = w.shared ? un.s.len - 1 : at;
-  w.last0 = w.shared ? un.s.len - 1 : at + w.tokens0 - 1;
-  w.pos1 = w.shared ? un.s.len - 1 : at + tt;
-  w.last1 = w.shared ? un.s.len - 1 : at + tt + w.tokens1 - 1;
-  w.span = key_span(w.pos0, w.tokens1 > 0 ? w.last1 : w.last0, w.window, w.sinks);
-  w.tiles = key_tiles(w.span, KT_BK);
-  w.j0 = int32_t(int64_t(w.tiles.count) * split / p.splits);
-  const int32_t j1 = int32_t(int64_t(w.tiles.count) * (split + 1) / p.splits);
-  w.cnt0 = kt_count(w.tiles, w.last0, w.tokens0, w.j0, j1);
-  w.cnt1 = kt_count(w.tiles, w.last1, w.tokens1, w.j0, j1);
-  w.jend = w.cnt0 > w.cnt1 ? w.cnt0 : w.cnt1;
-
-  if (tid == 0) {
-    const uint32_t row_tiles = w.tokens1 > 0 ? 2 : 1;
+  const uint32_t stage = ring + Cfg::SLOTS * Cfg::KV_BYTES, bars = stage + 8 * 4096;
+  const int warp = uniform(int(threadIdx.x) >> 5);
+  if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::SLOTS; ++s) {
       mbar_init_at(bars + B::kv_full + 8 * s, 1);
-      mbar_init_at(bars + B::kv_empty + 8 * s, row_tiles);
+      mbar_init_at(bars + B::kv_empty + 8 * s, 2);
     }
     mbar_init_at(bars + B::q_full, 1);
+    mbar_init_at(bars + B::q_empty, 2);
     for (int g = 0; g < 2; ++g) {
-      mbar_init_at(bars + B::s_full + 16 * g, 1);
-      mbar_init_at(bars + B::s_full + 16 * g + 8, 1);
-      mbar_init_at(bars + B::p_full + 16 * g, 128);
-      mbar_init_at(bars + B::p_full + 16 * g + 8, 128);
+      for (int x = 0; x < 16; x += 8) {
+        mbar_init_at(bars + B::s_full + 16 * g + x, 1);
+        mbar_init_at(bars + B::p_full + 16 * g + x, 128);
+      }
       mbar_init_at(bars + B::pv_done + 8 * g, 1);
+      mbar_init_at(bars + B::o_full + 8 * g, 1);
     }
     sts32(bars + B::abort, 0u);
     fence_mbar_init();
   }
   if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bars + B::tmem),
-                 "r"(Cfg::TMEM_COLS)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bars + B::tmem), "r"(Cfg::TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -704,12 +782,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = lds32(bars + B::tmem);
-
   if (warp < 8) {
-    if (warp < 4 || w.tokens1 > 0) kt_rows<T, HDP>(p, w, bars, ring, hk, split, warp);
-  } else if (w.jend > w.j0) {
-    if (warp == 8) kt_load<HDP>(&tmq, &tmk, &tmv, p, w, bars, qs, ring, hk);
-    if (warp == 9 || (warp == 10 && w.tokens1 > 0)) kt_multiply<T, HDP>(w, bars, qs, ring, warp - 9);
+    kt_rows<T, HDP>(p, bars, ring, stage + warp * 4096, warp);
+  } else if (warp == 8) {
+    kt_load<HDP>(&tmq, &tmk, &tmv, p, bars, qs, ring);
+  } else if (warp < 11) {
+    kt_multiply<T, HDP>(p, bars, qs, ring, warp - 9);
   }
   tc_fence_before();
   __syncwarp();

@@ -1764,15 +1764,16 @@ static int kv_query_map(CUtensorMap* map, const lng_kv_cache* c, const lng_kv_ro
   return LNG_OK;
 }
 
-// Into how many key ranges `units` CTAs with up to `tiles` key tiles each are divided: the count with the
-// least estimated time, in tiles -- waves of CTAs (one an SM) times (a range's tiles + 3 for a CTA's start and
-// end), plus the join of the ranges' states.
+// Into how many key ranges units with up to `tiles` key tiles each are divided: one where the units alone fill the
+// SMs, else the count with the least estimated time, in tiles -- waves of units (one an SM) times (a range's
+// tiles + 8 for a unit's start and its state's way out), plus the join of the states.
 static int kv_splits(int64_t units, int64_t tiles) {
   const int64_t sms = num_sms();
   int best = 1;
+  if (units >= sms) return best;
   double least = 1e300;
   for (int s = 1; s <= 32 && s <= tiles; ++s) {
-    const double cost = double(ceil_div(units * s, sms)) * (ceil_div(tiles, s) + 3) + (s > 1 ? 4 + s * 0.25 : 0.0);
+    const double cost = double(ceil_div(units * s, sms)) * (ceil_div(tiles, s) + 8) + (s > 1 ? 4 + s * 0.5 : 0.0);
     if (cost < least) {
       least = cost;
       best = s;
@@ -1807,7 +1808,7 @@ static KvPlan kv_plan(const lng_kv_cache* c, int64_t prefix_len, int64_t tokens,
     p.units = c->batch * ceil_div(max_new, span);
     const int64_t ragged = tokens / span + std::min(c->batch, tokens);
     if (ragged < p.units) p.units = ragged;
-    p.splits = kv_splits(std::max<int64_t>(1, ceil_div(tokens, span)) * c->num_kv_heads, std::max<int64_t>(1, ceil_div(keys, KT_BK)));
+    p.splits = kv_splits(p.units * c->num_kv_heads, std::max<int64_t>(1, ceil_div(keys, KT_BK)));
   }
   if (prefix_len > 0) p.prefix_splits = kv_splits(ceil_div(tokens, span) * c->num_kv_heads, ceil_div(prefix_len, KT_BK));
   if (p.prefix_splits)
@@ -1835,7 +1836,9 @@ static int launch_kv_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CU
   using Cfg = KtCfg<HDP>;
   auto kern = kv_tile_kernel<T, HDP>;
   LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
-  kern<<<dim3(unsigned(units * p.c.kv_heads), unsigned(p.splits)), KT_THREADS, Cfg::SMEM, s>>>(tq, tk, tv, p);
+  KtParams q = p;
+  q.total = units * p.c.kv_heads * p.splits;
+  kern<<<unsigned(std::min<int64_t>(q.total, num_sms())), KT_THREADS, Cfg::SMEM, s>>>(tq, tk, tv, q);
   LNG_LAUNCHED("kv_tile_kernel");
   return LNG_OK;
 }

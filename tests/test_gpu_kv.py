@@ -484,3 +484,35 @@ def test_a_decode_loop_beside_the_memory_layer(lngram):
     check_attend(again, want.view(B, total, heads, dim)[:, -2:].reshape(-1, heads, dim),
                  tol.view(B, total, heads, dim)[:, -2:].reshape(-1, heads, dim))
     assert u > 0 and lngram._lib.device_error() == 0
+
+
+@pytest.mark.parametrize("ctx, new, heads, kv, dim", [
+    ([5] * 90, [17] * 90, 8, 4, 64),                                   # several units a CTA, one row tile each
+    (list(range(0, 600, 6)), [40 + i % 50 for i in range(100)], 4, 2, 128),  # ragged, two row tiles
+    ([0] * 3, [900, 1, 1300], 16, 8, 64),
+])
+def test_many_units(lngram, ctx, new, heads, kv, dim):
+    """More units of work than SMs: every CTA of the tile kernel walks several."""
+    s = Setup(lngram, ctx, new, heads, kv, dim, 32, seed=len(ctx)).fill()
+    q = s.normal(*s.lead, heads, dim)
+    want = s.want(q)
+    for _ in range(5):
+        check_attend(lngram.kv_attend(s.cache, q, **s.kw()), *want)
+    check_attend(lngram.kv_attend(s.cache, q, window=100, sinks=3, **s.kw()), *s.want(q, 100, 3))
+    assert lngram._lib.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [1, 60])
+def test_nan_queries_stay_nan_and_alone(lngram, n):
+    """A query of NaN (a padded row, say) gives NaN for its row and head, and no other."""
+    s = Setup(lngram, [300, 20], [n, n], 8, 2, 64, 16, prefix=90).fill()
+    q = s.normal(*s.lead, 8, 64)
+    runs = (lambda x: lngram.kv_attend(s.cache, x), lambda x: lngram.kv_prefix_attend(s.cache, x, s.prefix_table, 90))
+    clean = [f(q) for f in runs]
+    q2 = q.clone()
+    q2[1, n // 2, 3] = math.nan
+    for f, a in zip(runs, clean):
+        b = f(q2)
+        assert torch.isnan(b[1, n // 2, 3]).all()
+        b[1, n // 2, 3] = a[1, n // 2, 3]
+        assert torch.equal(a, b)
