@@ -414,18 +414,19 @@ __device__ __forceinline__ void kt_weights(uint32_t (&s)[32], uint64_t scale2, u
   }
 }
 
-// One warp: for every unit its queries, then keys and values of every tile, page by page, into the ring.  The lanes
-// look up a tile's pages side by side, a tile ahead; one elected lane issues the copies.
+// Two warps, one for keys (and the units' queries), one for values: every tile's into the ring, page by page.  The
+// lanes look up a tile's pages side by side, a tile ahead; one elected lane issues the copies, four pieces in a row
+// without anything between (small pages make 16 copies a tile: one at a time they were slower than the products).
 template <int HDP>
-__device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMap* tmk, const CUtensorMap* tmv, const KtParams& p,
-                                        uint32_t bars, uint32_t qs, uint32_t ring) {
+__device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMap* map, const KtParams& p, uint32_t bars, uint32_t qs,
+                                        uint32_t ring, const uint32_t kv) {
   using Cfg = KtCfg<HDP>;
   using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const KvView& c = p.c;
   const int lane = threadIdx.x & 31, box = p.box, boxes = KT_BK / box;
   const int32_t page_mask = (1 << c.page_shift) - 1;
-  uint32_t it = 0, units = 0;  // copies into the ring, units with keys
+  uint32_t it = kv, units = 0;  // this warp's next copy into the ring, units with keys
   bool ok = true, there;
   KtWalk walk{};
   KtWork w;
@@ -442,52 +443,54 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
       return int32_t(c.num_pages);  // behind the last page: the copy fills zeros
     };
     int32_t next = look_up(0);
-    if (units > 0) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1));
-    if (!ok) break;
-    ++units;
-    if (elect_lane()) {
-      const int32_t tiles_q = w.tokens1 > 0 ? 2 : 1, q0 = int32_t(w.s.first + w.t0);
-      mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
-      for (int g = 0; g < tiles_q; ++g)
+    if (kv == 0) {
+      if (units > 0) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1));
+      if (!ok) break;
+      if (elect_lane()) {
+        const int32_t tiles_q = w.tokens1 > 0 ? 2 : 1, q0 = int32_t(w.s.first + w.t0);
+        mbar_expect_at(bars + B::q_full, uint32_t(p.group * p.tile_tokens) * 128u * (HDP / 64) * tiles_q);
+        for (int g = 0; g < tiles_q; ++g)
 #pragma unroll
-        for (int hh = 0; hh < HDP / 64; ++hh)
-          tma_load_3d_at(qs + g * Cfg::Q_BYTES + hh * Cfg::Q_HALF, tmq, hh * 64, w.hk * p.group, q0 + g * p.tile_tokens,
-                         bars + B::q_full);
+          for (int hh = 0; hh < HDP / 64; ++hh)
+            tma_load_3d_at(qs + g * Cfg::Q_BYTES + hh * Cfg::Q_HALF, tmq, hh * 64, w.hk * p.group, q0 + g * p.tile_tokens,
+                           bars + B::q_full);
+      }
+      __syncwarp();
     }
-    __syncwarp();
+    ++units;
 #pragma unroll 1
-    for (int32_t i = 0; i < w.n && ok; ++i) {
+    for (int32_t i = 0; i < w.n; ++i, it += 2) {
       const int32_t page = next;
       const int32_t slot0 = uniform((tile_index(w.tiles, w.j0 + i) * KT_BK) & page_mask);
       if (i + 1 < w.n) next = look_up(i + 1);
-      const uint32_t there_boxes = __ballot_sync(0xffffffffu, page >= 0);
-      const uint32_t bytes = uint32_t(__popc(there_boxes)) * uint32_t(box) * 128u * (HDP / 64);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv, ++it) {
-        const uint32_t s = it % NS;
-        if (it >= NS) ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
-        if (!ok) break;
-        const uint32_t bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::KV_BYTES;
-        if (elect_lane()) mbar_expect_at(bar, bytes);
-        __syncwarp();
+      const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, page >= 0))) * uint32_t(box) * 128u * (HDP / 64);
+      const uint32_t s = it % NS, bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::KV_BYTES;
+      if (it >= NS) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
+      if (!ok) break;
+      if (elect_lane()) mbar_expect_at(bar, bytes);
+      __syncwarp();
 #pragma unroll 1
-        for (int r = 0; r < boxes; ++r) {
-          const int32_t pg = __shfl_sync(0xffffffffu, page, r);
-          if (pg < 0) continue;
-          if (elect_lane()) {
+      for (int r = 0; r < boxes; r += 4) {
+        int32_t pg[4];
 #pragma unroll
-            for (int hh = 0; hh < HDP / 64; ++hh)
-              tma_load_4d_at(dst + hh * Cfg::KV_HALF + r * box * 128, kv ? tmv : tmk, hh * 64, (slot0 + r * box) & page_mask, w.hk, pg,
-                             bar);
-          }
-          __syncwarp();
+        for (int x = 0; x < 4; ++x) pg[x] = __shfl_sync(0xffffffffu, page, (r + x) & 31);
+        if (elect_lane()) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (r + x < boxes && pg[x] >= 0) {
+              const int32_t slot = (slot0 + (r + x) * box) & page_mask;
+#pragma unroll
+              for (int hh = 0; hh < HDP / 64; ++hh)
+                tma_load_4d_at(dst + hh * Cfg::KV_HALF + (r + x) * box * 128, map, hh * 64, slot, w.hk, pg[x], bar);
+            }
         }
+        __syncwarp();
       }
     }
   }
   // the last uses of the ring's slots: behind them no copy and no product is in flight
-  for (uint32_t k = it > NS ? it - NS : 0; k < it; ++k) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
-  if (units > 0) kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1);
+  for (uint32_t k = it >= NS ? it - NS : kv; k < it; k += 2) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
+  if (kv == 0 && units > 0) kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1);
 }
 
 // One warp a row tile issues its products: the scores of the next key tile (into the other of two S buffers) ahead
@@ -785,9 +788,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   if (warp < 8) {
     kt_rows<T, HDP>(p, bars, ring, stage + warp * 4096, warp);
   } else if (warp == 8) {
-    kt_load<HDP>(&tmq, &tmk, &tmv, p, bars, qs, ring);
-  } else if (warp < 11) {
-    kt_multiply<T, HDP>(p, bars, qs, ring, warp - 9);
+    kt_load<HDP>(&tmq, &tmk, p, bars, qs, ring, 0);
+  } else if (warp == 9) {
+    kt_load<HDP>(&tmq, &tmv, p, bars, qs, ring, 1);
+  } else {
+    kt_multiply<T, HDP>(p, bars, qs, ring, warp - 10);
   }
   tc_fence_before();
   __syncwarp();
