@@ -73,7 +73,8 @@ class PagedKVCache:
                                   table_stride=max(table.stride(0), table.shape[1]), max_pages=table.shape[1],
                                   lengths=lengths.data_ptr(), batch=table.shape[0])
         self._ref = C.byref(self._desc)
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.dtype, self.index = k.device, k.dtype, k.get_device()
+        self._sizes: dict = {}
         self.batch, self.page_size, self.num_kv_heads, self.head_dim = table.shape[0], size, heads, dim
         self.capacity = table.shape[1] * size
 
@@ -105,47 +106,67 @@ class PagedKVCache:
             self._lengths.clamp_(max=int(lengths))
 
 
-def _rows(t: Tensor, what: str, cache: PagedKVCache, shape=None, heads: int | None = None) -> _lib.KvRows:
-    """The descriptor of a step's rows; ``shape``: the leading shape they must have."""
-    _require(t.dtype == cache.dtype, f"{what} must have the cache's dtype {cache.dtype}")
-    _require(t.dim() in (3, 4) and t.shape[-1] == cache.head_dim,
-             f"{what} must be [B, n, heads, {cache.head_dim}] or [tokens, heads, {cache.head_dim}]")
-    if shape is not None:
-        _require(t.shape[:-2] == shape, f"{what} must have the step's leading shape {tuple(shape)}")
-    if heads is not None:
-        _require(t.shape[-2] == heads, f"{what} must have {heads} heads")
-    st = t.stride()
-    n = t.shape[-2]
+def _strides(t: Tensor, what: str, cache: PagedKVCache) -> tuple[int, int]:
+    """(token stride, head stride) of a step's rows whose shape has been checked."""
+    st, n = t.stride(), t.shape[-2]
     head = st[-2] if n > 1 else cache.head_dim
     token = st[-3] if t.shape[-3] > 1 else (st[0] if t.dim() == 4 and t.shape[0] > 1 else n * cache.head_dim)
     if t.dim() == 4 and t.shape[0] > 1 and t.shape[1] > 1:
         _require(st[0] == st[1] * t.shape[1], f"{what}: the tokens of all sequences must lie at one stride")
-    _require(st[-1] == 1 and head > 0 and head % 8 == 0 and token > 0 and token % 8 == 0 and t.data_ptr() % 16 == 0,
+    _require(st[-1] == 1 and head > 0 and head % 8 == 0 and token > 0 and token % 8 == 0,
              f"{what} must be 16-byte aligned with a contiguous head dimension and strides of positive multiples of 8")
-    _require(t.device == cache.device, f"{what} must be on the cache's device")
-    return _lib.KvRows(t.data_ptr(), token, head, n)
+    return token, head
+
+
+def _rows(t: Tensor, what: str, cache: PagedKVCache, shape=None, heads: int | None = None) -> _lib.KvRows:
+    """The descriptor of a step's rows; ``shape``: the leading shape they must have."""
+    # (messages are only made when they are needed: a decode step's host time is spent in lines like these)
+    ts = t.shape
+    if t.dtype is not cache.dtype:
+        raise ValueError(f"{what} must have the cache's dtype {cache.dtype}")
+    if len(ts) not in (3, 4) or ts[-1] != cache.head_dim:
+        raise ValueError(f"{what} must be [B, n, heads, {cache.head_dim}] or [tokens, heads, {cache.head_dim}]")
+    if shape is not None and ts[:-2] != shape:
+        raise ValueError(f"{what} must have the step's leading shape {tuple(shape)}")
+    n = ts[-2]
+    if heads is not None and n != heads:
+        raise ValueError(f"{what} must have {heads} heads")
+    if t.is_contiguous():
+        token, head = max(n, 1) * cache.head_dim, cache.head_dim
+    else:
+        token, head = _strides(t, what, cache)
+    p = t.data_ptr()
+    if p % 16:
+        raise ValueError(f"{what} must be 16-byte aligned with a contiguous head dimension and strides of positive multiples of 8")
+    if t.get_device() != cache.index:
+        raise ValueError(f"{what} must be on the cache's device")
+    return _lib.KvRows(p, token, head, n)
 
 
 def _step(cache: PagedKVCache, t: Tensor, cu: Tensor | None, max_new: int | None):
     """(tokens, max_new) of a step whose rows are shaped like t."""
+    ts = t.shape
     if cu is None:
-        _require(t.dim() == 4 and t.shape[0] == cache.batch,
-                 f"without cu the step's rows must be [B = {cache.batch}, n, heads, {cache.head_dim}]")
-        _require(max_new is None or max_new == t.shape[1], "max_new must be the step's n when there is no cu")
-        return t.shape[0] * t.shape[1], t.shape[1]
-    _require(t.dim() == 3, "with cu the step's rows must be [tokens, heads, head_dim]")
-    _require(cu.dtype == torch.int32 and cu.dim() == 1 and cu.shape[0] == cache.batch + 1 and cu.is_contiguous()
-             and cu.device == cache.device, f"cu must be contiguous int32 [{cache.batch + 1}] on the cache's device")
-    _require(max_new is not None and max_new >= 0, "a step with cu needs max_new")
-    return t.shape[0], int(max_new)
+        if len(ts) != 4 or ts[0] != cache.batch:
+            raise ValueError(f"without cu the step's rows must be [B = {cache.batch}, n, heads, {cache.head_dim}]")
+        if max_new is not None and max_new != ts[1]:
+            raise ValueError("max_new must be the step's n when there is no cu")
+        return ts[0] * ts[1], ts[1]
+    if len(ts) != 3:
+        raise ValueError("with cu the step's rows must be [tokens, heads, head_dim]")
+    if cu.dtype is not torch.int32 or cu.shape != (cache.batch + 1,) or not cu.is_contiguous() or cu.get_device() != cache.index:
+        raise ValueError(f"cu must be contiguous int32 [{cache.batch + 1}] on the cache's device")
+    if max_new is None or max_new < 0:
+        raise ValueError("a step with cu needs max_new")
+    return ts[0], int(max_new)
 
 
-def _on_gpu(cache: PagedKVCache) -> None:
-    if cache.device.type != "cuda":
+def _library(cache: PagedKVCache):
+    if cache.index < 0:
         raise RuntimeError("the cache must be on a CUDA device: lngram_b200 has no CPU path")
+    return _lib._LIB if cache.index in _lib._DEVICE_OK else _lib.library()
 
 
-@torch.no_grad()
 def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None, *, cu: Tensor | None = None,
               max_new: int | None = None, positions: Tensor | None = None, inv_freq: Tensor | None = None,
               interleaved: bool = False, q_out: Tensor | None = None) -> Tensor | None:
@@ -153,7 +174,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     ``lengths - n + i`` (``extend`` first).  With ``inv_freq`` (fp32 ``[rotary_dim / 2]``) the first rotary_dim
     values of keys and queries are rotated by the token's position -- ``positions`` (int64, the step's leading
     shape) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
-    Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``."""
+    Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``.  No gradients."""
     tokens, max_new = _step(cache, k, cu, max_new)
     lead = k.shape[:-2]
     kr = _rows(k, "k", cache, lead, cache.num_kv_heads)
@@ -162,45 +183,58 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     if q is not None:
         qr = C.byref(_rows(q, "q", cache, lead))
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = q.new_empty(q.shape)
         qo = C.byref(_rows(q_out, "q_out", cache, lead, q.shape[-2]))
-    else:
-        _require(q_out is None, "q_out without q")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
     rotary = 0
     if inv_freq is not None:
-        _require(inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
-                 and inv_freq.device == cache.device, "inv_freq must be contiguous fp32 [rotary_dim / 2] on the cache's device")
+        if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous() \
+                or inv_freq.get_device() != cache.index:
+            raise ValueError("inv_freq must be contiguous fp32 [rotary_dim / 2] on the cache's device")
         rotary = 2 * inv_freq.shape[0]
-        _require(rotary <= cache.head_dim, "inv_freq has more pairs than the head")
-    if positions is not None:
-        _require(positions.dtype == torch.int64 and positions.shape == lead and positions.is_contiguous()
-                 and positions.device == cache.device, "positions must be contiguous int64 of the step's leading shape")
-    _on_gpu(cache)
+        if rotary > cache.head_dim:
+            raise ValueError("inv_freq has more pairs than the head")
+    if positions is not None and (positions.dtype is not torch.int64 or positions.shape != lead or not positions.is_contiguous()
+                                  or positions.get_device() != cache.index):
+        raise ValueError("positions must be contiguous int64 of the step's leading shape")
+    lib = _library(cache)
     with _lib.on_device(cache.device):
-        check(_lib.library().lng_kv_append(cache._ref, ptr(cu), tokens, max_new, C.byref(kr), C.byref(vr), qr, qo,
-                                           ptr(positions), ptr(inv_freq) if rotary else None, rotary, int(bool(interleaved)),
-                                           stream_ptr()), "kv_append")
+        check(lib.lng_kv_append(cache._ref, ptr(cu), tokens, max_new, C.byref(kr), C.byref(vr), qr, qo, ptr(positions),
+                                ptr(inv_freq) if rotary else None, rotary, 1 if interleaved else 0, stream_ptr()), "kv_append")
     return q_out
 
 
 def _attend_args(cache, q, cu, max_new, max_len, scale, out):
     tokens, max_new = _step(cache, q, cu, max_new)
     qr = _rows(q, "q", cache)
-    heads = q.shape[-2]
-    _require(heads % cache.num_kv_heads == 0 and 1 <= heads // cache.num_kv_heads <= 128,
-             "query heads must be a multiple of the key heads, at most 128 a key head")
+    heads = qr.heads
+    if heads % cache.num_kv_heads or not 1 <= heads // cache.num_kv_heads <= 128:
+        raise ValueError("query heads must be a multiple of the key heads, at most 128 a key head")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     orow = _rows(out, "out", cache, q.shape[:-2], heads)
-    _require(tokens == 0 or out.data_ptr() != q.data_ptr(), "out must not overlap q")
+    if tokens and orow.ptr == qr.ptr:
+        raise ValueError("out must not overlap q")
     max_len = cache.capacity if max_len is None else int(max_len)
-    _require(max_len >= 0, "max_len must not be negative")
+    if max_len < 0:
+        raise ValueError("max_len must not be negative")
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-    _require(0.0 < scale < 3e38, "scale must be positive and finite")
+    if not 0.0 < scale < 3e38:
+        raise ValueError("scale must be positive and finite")
     return tokens, max_new, max_len, qr, heads, scale, out, orow
 
 
-@torch.no_grad()
+def _workspace(cache: PagedKVCache, key: tuple, size) -> Tensor | None:
+    """A workspace of its own for this call, of the size that ``size()`` gives (kept by the call's arguments)."""
+    need = cache._sizes.get(key)
+    if need is None:
+        if len(cache._sizes) > 256:
+            cache._sizes.clear()
+        need = cache._sizes[key] = size()
+    return torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+
+
 def kv_attend(cache: PagedKVCache, q: Tensor, *, cu: Tensor | None = None, max_new: int | None = None,
               max_len: int | None = None, window: int = 0, sinks: int = 0, scale: float | None = None,
               out: Tensor | None = None) -> Tensor:
@@ -208,42 +242,43 @@ def kv_attend(cache: PagedKVCache, q: Tensor, *, cu: Tensor | None = None, max_n
     token at position p sees keys j <= p; with ``window`` > 0 only its last ``window`` keys and the first
     ``sinks`` of the sequence.  softmax(scale q . k) v with ``scale`` = head_dim^-1/2 by default; a token
     that sees no key gets zeros.  ``max_len`` (a host bound of the lengths) only guides how the work is split.
-    Rows of ``q`` that belong to no sequence are skipped: their rows of ``out`` stay as they are."""
+    Rows of ``q`` that belong to no sequence are skipped: their rows of ``out`` stay as they are.  No gradients."""
     tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
     window, sinks = int(window), int(sinks)
-    _require(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
     window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
-    _on_gpu(cache)
-    lib = _lib.library()
+    lib = _library(cache)
     with _lib.on_device(cache.device):
-        need = lib.lng_kv_attend_workspace_bytes(cache._ref, tokens, max_new, max_len, heads, window, sinks)
-        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        ws = _workspace(cache, (tokens, max_new, max_len, heads, window, sinks), lambda: lib.lng_kv_attend_workspace_bytes(
+            cache._ref, tokens, max_new, max_len, heads, window, sinks))
         check(lib.lng_kv_attend(cache._ref, ptr(cu), tokens, max_new, max_len, C.byref(qr), scale, window, sinks,
-                                C.byref(orow), ptr(ws), need, stream_ptr()), "kv_attend")
+                                C.byref(orow), ptr(ws), 0 if ws is None else ws.numel(), stream_ptr()), "kv_attend")
     return out
 
 
-@torch.no_grad()
 def kv_prefix_attend(cache: PagedKVCache, q: Tensor, prefix_table: Tensor, prefix_len: int, *, cu: Tensor | None = None,
                      max_new: int | None = None, max_len: int | None = None, scale: float | None = None,
                      out: Tensor | None = None) -> Tensor:
     """``kv_attend`` (without a window) for a batch whose sequences all begin with the ``prefix_len`` keys in the
     pages ``prefix_table`` (int32 ``[>= ceil(prefix_len / page_size)]``) of the same cache; ``table`` and
-    ``lengths`` hold what each sequence adds to it.  The prefix is read once for the whole batch."""
+    ``lengths`` hold what each sequence adds to it.  The prefix is read once for the whole batch.  No gradients."""
     tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
     prefix_len = int(prefix_len)
-    _require(0 <= prefix_len < 1 << 30, "prefix_len must be in [0, 2^30)")
-    _require(prefix_table.dtype == torch.int32 and prefix_table.dim() == 1 and prefix_table.is_contiguous()
-             and prefix_table.device == cache.device, "prefix_table must be contiguous int32 on the cache's device")
-    _require(prefix_table.shape[0] * cache.page_size >= prefix_len, "prefix_table has too few pages for prefix_len")
-    _on_gpu(cache)
-    lib = _lib.library()
+    if not 0 <= prefix_len < 1 << 30:
+        raise ValueError("prefix_len must be in [0, 2^30)")
+    if prefix_table.dtype is not torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() \
+            or prefix_table.get_device() != cache.index:
+        raise ValueError("prefix_table must be contiguous int32 on the cache's device")
+    if prefix_table.shape[0] * cache.page_size < prefix_len:
+        raise ValueError("prefix_table has too few pages for prefix_len")
+    lib = _library(cache)
     with _lib.on_device(cache.device):
-        need = lib.lng_kv_prefix_workspace_bytes(cache._ref, prefix_len, tokens, max_new, max_len, heads)
-        ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+        ws = _workspace(cache, (prefix_len, tokens, max_new, max_len, heads), lambda: lib.lng_kv_prefix_workspace_bytes(
+            cache._ref, prefix_len, tokens, max_new, max_len, heads))
         check(lib.lng_kv_prefix_attend(cache._ref, ptr(prefix_table) if prefix_len else None, prefix_len, ptr(cu), tokens,
-                                       max_new, max_len, C.byref(qr), scale, C.byref(orow), ptr(ws), need, stream_ptr()),
-              "kv_prefix_attend")
+                                       max_new, max_len, C.byref(qr), scale, C.byref(orow), ptr(ws),
+                                       0 if ws is None else ws.numel(), stream_ptr()), "kv_prefix_attend")
     return out
 
 
