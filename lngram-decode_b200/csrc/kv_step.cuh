@@ -22,18 +22,20 @@
 
 namespace lng {
 
-constexpr int KS_ROWS = 16, KS_BK = 32, KS_STAGES = 3;
+constexpr int KS_ROWS = 16, KS_STAGES = 3;
 
 template <int HDP>  // head size padded to 64 or 128
 struct KsCfg {
-  static constexpr int WARPS = 512 / HDP;
-  static constexpr int THREADS = WARPS * 32;
-  static constexpr uint32_t HALF_BYTES = KS_BK * 128;               // 32 keys x 64 values
-  static constexpr uint32_t KV_BYTES = HALF_BYTES * (HDP / 64);     // K (or V) of a stage
+  // (blocks of 16 keys on eight warps at head size 128 were slower, 0.46 against 0.39 ms a step of 64 long
+  // sequences: what a block costs besides its keys counts twice)
+  static constexpr int BK = 32, WARPS = 512 / HDP, THREADS = 32 * WARPS;
+  static constexpr uint32_t HALF_BYTES = BK * 128;               // BK keys x 64 values
+  static constexpr uint32_t KV_BYTES = HALF_BYTES * (HDP / 64);  // K (or V) of a stage
   static constexpr uint32_t STAGE_BYTES = 2 * KV_BYTES;
-  static constexpr uint32_t RING_BYTES = STAGE_BYTES * KS_STAGES;   // one warp's
-  static constexpr uint32_t MERGE_BYTES = WARPS * KS_ROWS * HDP * 4;
-  static constexpr size_t SMEM = size_t(WARPS) * RING_BYTES + MERGE_BYTES + WARPS * KS_ROWS * 8 + WARPS * KS_STAGES * 8 + 64 + 1024;
+  static constexpr uint32_t RING_BYTES = STAGE_BYTES * KS_STAGES;  // one warp's
+  static constexpr uint32_t MERGE_BYTES = 4 * KS_ROWS * HDP * 4;  // the products of four warps
+  static constexpr size_t SMEM =
+      size_t(WARPS) * RING_BYTES + MERGE_BYTES + WARPS * KS_ROWS * 8 + WARPS * KS_STAGES * 8 + 64 + 1024;
 };
 
 struct KsParams {
@@ -59,15 +61,15 @@ struct KsPlan {
   int64_t total, per;  // blocks in all, blocks a share
 };
 
+template <int BK>
 __device__ __forceinline__ int32_t ks_blocks(const KvView& c, const SeqSpan& s, int32_t window, int32_t sinks) {
   if (s.n <= 0) return 0;
-  return key_tiles(key_span(s.len - s.n, s.len - 1, window, sinks), KS_BK).count;
+  return key_tiles(key_span(s.len - s.n, s.len - 1, window, sinks), BK).count;
 }
 
-// A share is at least one block a warp, so that short steps use fewer CTAs and have fewer pieces.
-__device__ __forceinline__ int64_t ks_share(int64_t total, int shares, int warps) {
+__device__ __forceinline__ int64_t ks_share(int64_t total, int shares) {
   const int64_t per = (total + shares - 1) / shares;
-  return per < warps ? warps : per;
+  return per > 0 ? per : 1;
 }
 
 // Sums blocks(b) * KV over all sequences and finds the sequence in which block `want` of the line falls and
@@ -77,13 +79,14 @@ struct KsFound {
   int64_t total, b, start;
 };
 
-__device__ inline KsFound ks_find(const KvView& c, int32_t window, int32_t sinks, int nthreads, int shares, int warps,
-                                  int64_t* warp_tot, int64_t* found, int64_t cta) {
+template <int BK>
+__device__ inline KsFound ks_find(const KvView& c, int32_t window, int32_t sinks, int nthreads, int shares, int64_t* warp_tot,
+                                  int64_t* found, int64_t cta) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t run = (c.batch + nthreads - 1) / nthreads;
   const int64_t b0 = tid * run, b1 = b0 + run < c.batch ? b0 + run : c.batch;
   int64_t mine = 0;
-  for (int64_t b = b0; b < b1; ++b) mine += int64_t(ks_blocks(c, kv_span(c, b), window, sinks)) * c.kv_heads;
+  for (int64_t b = b0; b < b1; ++b) mine += int64_t(ks_blocks<BK>(c, kv_span(c, b), window, sinks)) * c.kv_heads;
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -102,11 +105,11 @@ __device__ inline KsFound ks_find(const KvView& c, int32_t window, int32_t sinks
     total += warp_tot[w];
   }
   const int64_t at = before + incl - mine;
-  const int64_t want = cta * ks_share(total, shares, warps);
+  const int64_t want = cta * ks_share(total, shares);
   if (want >= at && want < at + mine) {
     int64_t pos = at;
     for (int64_t b = b0; b < b1; ++b) {
-      const int64_t n = int64_t(ks_blocks(c, kv_span(c, b), window, sinks)) * c.kv_heads;
+      const int64_t n = int64_t(ks_blocks<BK>(c, kv_span(c, b), window, sinks)) * c.kv_heads;
       if (want < pos + n) {
         found[0] = b;
         found[1] = pos;
@@ -166,6 +169,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 
 // A walk along a CTA's share: the current pair, its sequence and the blocks [k0, k1) of it that belong to
 // the share.
+template <int BK>
 struct KsWalk {
   int64_t pos, end;  // in the line
   int64_t b;
@@ -177,7 +181,7 @@ struct KsWalk {
   __device__ __forceinline__ void enter(const KvView& c, int32_t window, int32_t sinks) {
     s = kv_span(c, b);
     span = key_span(s.len - s.n, s.len - 1, window, sinks);
-    tiles = key_tiles(span, KS_BK);
+    tiles = key_tiles(span, BK);
     blocks = s.n > 0 ? tiles.count : 0;
   }
   __device__ __forceinline__ void clip() {
@@ -215,7 +219,7 @@ template <typename T, int HDP>
 __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     kv_step_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const KsParams p) {
   using Cfg = KsCfg<HDP>;
-  constexpr int WARPS = Cfg::WARPS, KSTEPS = HDP / 16, NT = HDP / 8;
+  constexpr int WARPS = Cfg::WARPS, BK = Cfg::BK, KSTEPS = HDP / 16, NT = HDP / 8, ST = BK / 8;
   extern __shared__ uint8_t ks_smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ks_smem_raw) + 1023) & ~uintptr_t(1023));
   float* merge_o = reinterpret_cast<float*>(base + WARPS * Cfg::RING_BYTES);  // [WARPS][16][HDP]
@@ -235,50 +239,63 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       tma_prefetch_desc(&tmv);
     }
   }
-  const KsFound f = ks_find(c, p.window, p.sinks, Cfg::THREADS, p.shares, WARPS, warp_tot, found, blockIdx.x);
-  const int64_t per = ks_share(f.total, p.shares, WARPS);
+  const KsFound f = ks_find<BK>(c, p.window, p.sinks, Cfg::THREADS, p.shares, warp_tot, found, blockIdx.x);
+  const int64_t per = ks_share(f.total, p.shares);
   const int64_t p0 = int64_t(blockIdx.x) * per, p1 = p0 + per < f.total ? p0 + per : f.total;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the loading walk runs KS_STAGES blocks of this warp ahead of the computing walk
-  KsWalk ld, cw;
+  KsWalk<BK> ld, cw;
   ld.start(c, p.window, p.sinks, f, p0, p1);
   cw = ld;
   int32_t ld_k = ld.done() ? 0 : ld.k0 + warp;
   uint32_t issued = 0, taken = 0;
+  // pages of the warp's next blocks of the pair, a piece (of `box` keys) a lane: looked up together, since a
+  // look-up of one block's page takes longer than its copies
+  const int boxes = BK / p.box, ahead = 32 / boxes;
+  int32_t pages = -1, seen = ahead;  // -1: no row sees a key of the piece; blocks issued out of the looked-up ones
+  auto look_up = [&]() {
+    const int32_t k = ld_k + (lane / boxes) * WARPS;
+    pages = -1;
+    if (k < ld.k1) {
+      const int32_t key = tile_index(ld.tiles, k) * BK + (lane % boxes) * p.box;
+      if (any_needed(ld.span, key, key + p.box)) {
+        pages = page_of(c.table + ld.b * c.table_stride, key, c.page_shift, c.num_pages);
+        if (pages < 0) {
+          kv_range_error();
+          pages = int32_t(c.num_pages);  // behind the last page: the copy fills zeros
+        }
+      }
+    }
+    seen = 0;
+  };
   auto issue = [&]() {  // the warp's next block into the ring (all lanes keep the walk; lane 0 copies)
     while (!ld.done() && ld_k >= ld.k1) {
       ld.next(c, p.window, p.sinks);
       if (!ld.done()) ld_k = ld.k0 + warp;
+      seen = ahead;
     }
     if (ld.done()) return;
-    if (lane == 0) {
-      const uint32_t s = issued % KS_STAGES;
-      uint8_t* dk = ring + s * Cfg::STAGE_BYTES;
-      uint8_t* dv = dk + Cfg::KV_BYTES;
-      const int32_t key0 = tile_index(ld.tiles, ld_k) * KS_BK;
-      const int32_t* row = c.table + ld.b * c.table_stride;
-      uint32_t bytes = 0;
-      for (int32_t r = 0; r < KS_BK; r += p.box)
-        if (any_needed(ld.span, key0 + r, key0 + r + p.box)) bytes += uint32_t(p.box) * 128 * (HDP / 64) * 2;
-      mbar_arrive_expect_tx(&bar[s], bytes);
-      for (int32_t r = 0; r < KS_BK; r += p.box) {
-        const int32_t key = key0 + r;
-        if (!any_needed(ld.span, key, key + p.box)) continue;
-        int32_t page = page_of(row, key, c.page_shift, c.num_pages);
-        if (page < 0) {
-          kv_range_error();
-          page = int32_t(c.num_pages);  // behind the last page: the copy fills zeros
-        }
-        const int32_t slot = key & ((1 << c.page_shift) - 1);
+    if (seen == ahead) look_up();
+    const uint32_t s = issued % KS_STAGES, mine = boxes == 32 ? 0xffffffffu : ((1u << boxes) - 1u);
+    const uint32_t there = (__ballot_sync(0xffffffffu, pages >= 0) >> (seen * boxes)) & mine;
+    uint8_t* dk = ring + s * Cfg::STAGE_BYTES;
+    uint8_t* dv = dk + Cfg::KV_BYTES;
+    const int32_t slot0 = (tile_index(ld.tiles, ld_k) * BK) & ((1 << c.page_shift) - 1);
+    if (lane == 0) mbar_arrive_expect_tx(&bar[s], uint32_t(__popc(there)) * uint32_t(p.box) * 128 * (HDP / 64) * 2);
+    for (int r = 0; r < boxes; ++r) {
+      const int32_t page = __shfl_sync(0xffffffffu, pages, seen * boxes + r);
+      if (page < 0 || lane != 0) continue;
+      const int32_t slot = (slot0 + r * p.box) & ((1 << c.page_shift) - 1);
 #pragma unroll
-        for (int hh = 0; hh < HDP / 64; ++hh) {
-          tma_load_4d(dk + hh * Cfg::HALF_BYTES + r * 128, &tmk, hh * 64, slot, ld.h, page, &bar[s]);
-          tma_load_4d(dv + hh * Cfg::HALF_BYTES + r * 128, &tmv, hh * 64, slot, ld.h, page, &bar[s]);
-        }
+      for (int hh = 0; hh < HDP / 64; ++hh) {
+        tma_load_4d(dk + hh * Cfg::HALF_BYTES + r * p.box * 128, &tmk, hh * 64, slot, ld.h, page, &bar[s]);
+        tma_load_4d(dv + hh * Cfg::HALF_BYTES + r * p.box * 128, &tmv, hh * 64, slot, ld.h, page, &bar[s]);
       }
     }
+    __syncwarp();
     ++issued;
+    ++seen;
     ld_k += WARPS;
   };
 #pragma unroll 1
@@ -324,24 +341,26 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       if (!ok) break;
       uint8_t* sk = ring + s * Cfg::STAGE_BYTES;
       uint8_t* sv = sk + Cfg::KV_BYTES;
-      const int32_t key0 = tile_index(cw.tiles, k) * KS_BK;
-      const bool whole = all_needed(cw.span, key0, key0 + KS_BK);
+      const int32_t key0 = tile_index(cw.tiles, k) * BK;
+      const bool whole = all_needed(cw.span, key0, key0 + BK);
       if (!whole) {
         // values of keys that no row sees may be anything in memory: zero weights must not meet a NaN
-        if (!key_needed(cw.span, key0 + lane)) {
+        constexpr int PARTS = 32 / BK;  // lanes a row
+        const int key = lane % BK, part = lane / BK;
+        if (!key_needed(cw.span, key0 + key)) {
 #pragma unroll
           for (int hh = 0; hh < HDP / 64; ++hh)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<uint4*>(sv + hh * Cfg::HALF_BYTES + lane * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 8 / PARTS; ++i)
+              *reinterpret_cast<uint4*>(sv + hh * Cfg::HALF_BYTES + key * 128 + (part * (8 / PARTS) + i) * 16) = make_uint4(0, 0, 0, 0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this stage
         __syncwarp();
       }
-      // S = Q K^T: 16 rows x 32 keys
-      float sacc[4][4];
+      // S = Q K^T: 16 rows x BK keys
+      float sacc[ST][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < ST; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) sacc[i][j] = 0.f;
       const uint32_t skb = smem_addr(sk), svb = smem_addr(sv);
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       for (int kk = 0; kk < KSTEPS; ++kk) {
         if (kk * 16 < c.head_dim) {
 #pragma unroll
-          for (int np = 0; np < 2; ++np) {  // keys 16 np .. + 15
+          for (int np = 0; np < ST / 2; ++np) {  // keys 16 np .. + 15
             const int key = np * 16 + (lane & 7) + ((lane >> 4) << 3);
             const int chunk = (kk & 3) * 2 + ((lane >> 3) & 1);
             uint32_t b[4];
@@ -359,9 +378,9 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
           }
         }
       }
-      if (!all_visible(key0, key0 + KS_BK, pos0, cw.s.len - 1, p.window, p.sinks)) {
+      if (!all_visible(key0, key0 + BK, pos0, cw.s.len - 1, p.window, p.sinks)) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < ST; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int32_t key = key0 + n * 8 + t4 * 2 + (j & 1);
@@ -371,7 +390,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       // running maximum and sum of the two rows (base 2)
       float xa = -INFINITY, xb = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int n = 0; n < ST; ++n) {
         xa = fmaxf(xa, fmaxf(sacc[n][0], sacc[n][1]));
         xb = fmaxf(xb, fmaxf(sacc[n][2], sacc[n][3]));
       }
@@ -397,7 +416,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       }
       const float ra = ma == -INFINITY ? 0.f : ma, rb = mb == -INFINITY ? 0.f : mb;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+      for (int n = 0; n < ST; ++n) {
         sacc[n][0] = exp2_fast(sacc[n][0] * p.scale_log2 - ra);
         sacc[n][1] = exp2_fast(sacc[n][1] * p.scale_log2 - ra);
         sacc[n][2] = exp2_fast(sacc[n][2] * p.scale_log2 - rb);
@@ -407,7 +426,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       }
       // O += P V; the weights are rounded to the cache's type for the matrix unit, their sum is not
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
+      for (int kk = 0; kk < BK / 16; ++kk) {
         uint32_t a[4] = {pack2<T>(sacc[2 * kk][0], sacc[2 * kk][1]), pack2<T>(sacc[2 * kk][2], sacc[2 * kk][3]),
                          pack2<T>(sacc[2 * kk + 1][0], sacc[2 * kk + 1][1]), pack2<T>(sacc[2 * kk + 1][2], sacc[2 * kk + 1][3])};
 #pragma unroll
@@ -438,12 +457,38 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       merge_ml[warp * KS_ROWS + g] = make_float2(la == la ? ma : 0.f, la);
       merge_ml[warp * KS_ROWS + g + 8] = make_float2(lb == lb ? mb : 0.f, lb);
     }
+    // (16-byte vectors swizzled by row, so that the eight rows of a store lie in different banks)
+    float* slot_o = merge_o + (warp & 3) * KS_ROWS * HDP;
+    auto at = [&](int row, int i) { return slot_o + row * HDP + (((i * 2 + (t4 >> 1)) ^ g) << 2) + (t4 & 1) * 2; };
+    if (WARPS == 4 || warp >= 4) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      // 16-byte vectors swizzled by row, so that the eight rows of a store lie in different banks
-      const int col = (((i * 2 + (t4 >> 1)) ^ g) << 2) + (t4 & 1) * 2;
-      *reinterpret_cast<float2*>(merge_o + (warp * KS_ROWS + g) * HDP + col) = make_float2(oacc[i][0], oacc[i][1]);
-      *reinterpret_cast<float2*>(merge_o + (warp * KS_ROWS + g + 8) * HDP + col) = make_float2(oacc[i][2], oacc[i][3]);
+      for (int i = 0; i < NT; ++i) {
+        *reinterpret_cast<float2*>(at(g, i)) = make_float2(oacc[i][0], oacc[i][1]);
+        *reinterpret_cast<float2*>(at(g + 8, i)) = make_float2(oacc[i][2], oacc[i][3]);
+      }
+    }
+    if constexpr (WARPS > 4) {  // eight warps: the upper four's states join the lower four's
+    __syncthreads();
+    if (warp < 4) {
+      const float2 xa2 = merge_ml[(warp + 4) * KS_ROWS + g], xb2 = merge_ml[(warp + 4) * KS_ROWS + g + 8];
+      const float2 ya2 = merge_ml[warp * KS_ROWS + g], yb2 = merge_ml[warp * KS_ROWS + g + 8];
+      const float na = fmaxf(xa2.x, ya2.x), nb = fmaxf(xb2.x, yb2.x);
+      const float ea = xa2.x == -INFINITY ? 0.f : exp2_fast(xa2.x - na), eb = xb2.x == -INFINITY ? 0.f : exp2_fast(xb2.x - nb);
+      const float fa = ya2.x == -INFINITY ? 0.f : exp2_fast(ya2.x - na), fb = yb2.x == -INFINITY ? 0.f : exp2_fast(yb2.x - nb);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float2* pa = reinterpret_cast<float2*>(at(g, i));
+        float2* pb = reinterpret_cast<float2*>(at(g + 8, i));
+        const float2 va = *pa, vb = *pb;
+        *pa = make_float2(oacc[i][0] * fa + va.x * ea, oacc[i][1] * fa + va.y * ea);
+        *pb = make_float2(oacc[i][2] * fb + vb.x * eb, oacc[i][3] * fb + vb.y * eb);
+      }
+      __syncwarp();
+      if (t4 == 0) {
+        merge_ml[warp * KS_ROWS + g] = make_float2(na, ya2.y * fa + xa2.y * ea);
+        merge_ml[warp * KS_ROWS + g + 8] = make_float2(nb, yb2.y * fb + xb2.y * eb);
+      }
+    }
     }
     __syncthreads();
     const bool begins = cw.k0 == 0, ends = cw.k1 == cw.blocks, finished = begins && ends;
@@ -453,10 +498,10 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       const int r = it / vecs, col = (it - r * vecs) << 2;
       float m = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, merge_ml[w * KS_ROWS + r].x);
+      for (int w = 0; w < 4; ++w) m = fmaxf(m, merge_ml[w * KS_ROWS + r].x);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
+      for (int w = 0; w < 4; ++w) {
         const float2 ml = merge_ml[w * KS_ROWS + r];
         const float e = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
         const float4 v = *reinterpret_cast<const float4*>(merge_o + (w * KS_ROWS + r) * HDP + (col ^ ((r & 7) << 2)));
@@ -489,21 +534,67 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     }
     __syncthreads();
   }
+  // launched beside the prefix's kernel, this one must not be complete before it: the join waits for this one only
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins what the step kernel left in pieces: one CTA a (sequence, key head) pair, one 16-byte vector of a row
-// a thread.  Rows of pairs without a key become zero (they are in nobody's share).  With a prefix every row
-// also takes in the states of the prefix's ranges.
+// One row's states, `count` of them, state i at (ml(i), o(i)): the lanes of a warp take a 16-byte vector of the row
+// each, the warp every `stride`-th state from `begin`; maximum first, so that the loads of the products do not
+// wait for one another.
+struct KsRow {
+  float m, l;
+  float4 o;
+};
+template <typename ML, typename O>
+__device__ __forceinline__ KsRow ks_join_states(int begin, int stride, int count, int lane, bool on, ML ml, O o) {
+  KsRow r{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i = begin + lane * stride; i < count; i += 32 * stride) r.m = fmaxf(r.m, ml(i)->x);
+  r.m = warp_max(r.m);
+#pragma unroll 4
+  for (int i = begin; i < count; i += stride) {
+    const float2 s = *ml(i);
+    const bool there = s.x != -INFINITY;
+    const float4 v = there && on ? *reinterpret_cast<const float4*>(o(i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float e = there ? exp2_fast(s.x - r.m) : 0.f;
+    r.l += e * s.y;
+    r.o.x += e * v.x;
+    r.o.y += e * v.y;
+    r.o.z += e * v.z;
+    r.o.w += e * v.w;
+  }
+  return r;
+}
+__device__ __forceinline__ void ks_join_two(KsRow& a, const KsRow& b) {
+  const float n = fmaxf(a.m, b.m);
+  const float ea = a.m == -INFINITY ? 0.f : exp2_fast(a.m - n), eb = b.m == -INFINITY ? 0.f : exp2_fast(b.m - n);
+  a.m = n;
+  a.l = a.l * ea + b.l * eb;
+  a.o.x = a.o.x * ea + b.o.x * eb;
+  a.o.y = a.o.y * ea + b.o.y * eb;
+  a.o.z = a.o.z * ea + b.o.z * eb;
+  a.o.w = a.o.w * ea + b.o.w * eb;
+}
 template <typename T>
-__global__ void __launch_bounds__(128) kv_step_join_kernel(const KsParams p, int step_warps) {
+__device__ __forceinline__ void ks_store_row(const KsRow& r, T* dst) {
+  const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(r.o.x * inv, r.o.y * inv), pack2<T>(r.o.z * inv, r.o.w * inv));
+}
+
+// Joins what the step kernel left in pieces: one CTA a (sequence, key head) pair, its eight warps shared out over
+// the pair's rows (several a row when the rows are few).  Rows of pairs without a key become zero (they are
+// in nobody's share).  With a prefix every row also takes in the states of the prefix's ranges.
+template <typename T, int BK>
+__global__ void __launch_bounds__(256) kv_step_join_kernel(const KsParams p) {
+  __shared__ int64_t sums[8][2];
+  __shared__ KsRow part[8][32];
   const KvView& c = p.c;
   const int64_t b = blockIdx.x / c.kv_heads;
   const int h = int(blockIdx.x - b * c.kv_heads);
   // blocks of all sequences, and of those before b
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int64_t total = 0, before = 0;
-  for (int64_t i = tid; i < c.batch; i += 128) {
-    const int64_t n = int64_t(ks_blocks(c, kv_span(c, i), p.window, p.sinks)) * c.kv_heads;
+  for (int64_t i = tid; i < c.batch; i += 256) {
+    const int64_t n = int64_t(ks_blocks<BK>(c, kv_span(c, i), p.window, p.sinks)) * c.kv_heads;
     total += n;
     if (i < b) before += n;
   }
@@ -512,54 +603,57 @@ __global__ void __launch_bounds__(128) kv_step_join_kernel(const KsParams p, int
     total += __shfl_xor_sync(0xffffffffu, total, o);
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
-  __shared__ int64_t sums[4][2];
   if (lane == 0) {
     sums[warp][0] = total;
     sums[warp][1] = before;
   }
   __syncthreads();
-  total = sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0];
-  before = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
+  total = before = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    total += sums[i][0];
+    before += sums[i][1];
+  }
   const SeqSpan s = kv_span(c, b);
-  const int32_t blocks = ks_blocks(c, s, p.window, p.sinks);
-  const int64_t per = ks_share(total, p.shares, step_warps);
+  const int32_t blocks = ks_blocks<BK>(c, s, p.window, p.sinks);
+  const int64_t per = ks_share(total, p.shares);
   const int64_t first = before + int64_t(h) * blocks;
   const int64_t c0 = first / per, c1 = blocks > 0 ? (first + blocks - 1) / per : c0;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool whole = blocks > 0 && c0 == c1;
   if (whole && p.row_ml == nullptr) return;
-  const int rows = p.group * s.n, vecs = c.head_dim >> 2;
+  const int rows = p.group * s.n;
+  if (rows == 0) return;
   const int64_t slot_rows = c.tokens * p.q_heads;
-  for (int it = tid; it < rows * vecs; it += 128) {
-    const int r = it / vecs, col = (it - r * vecs) << 2;
+  // states of a row: those of the prefix's ranges, the own one if one CTA finished the pair, else the pieces
+  const int shared_n = p.row_ml != nullptr ? p.prefix_slots + (whole ? 1 : 0) : 0;
+  const int count = shared_n + (blocks > 0 && !whole ? int(c1 - c0) + 1 : 0);
+  int per_row = 1;  // warps a row
+  while (per_row * 2 * rows <= 8) per_row *= 2;
+  const int at_once = 8 / per_row, sub = warp % per_row, col = lane * 4;
+  const bool on = col < c.head_dim;
+  for (int r0 = 0; r0 < rows; r0 += at_once) {
+    const int r = r0 + warp / per_row;
+    const bool live = r < rows;
     const int tok = r / p.group, head = h * p.group + (r - tok * p.group);
     const int64_t token = s.first + tok, row = token * p.q_heads + head;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto take = [&](const float2* ml_p, const float* o_p) {
-      const float2 ml = *ml_p;
-      if (ml.x == -INFINITY) return;
-      const float4 v = *reinterpret_cast<const float4*>(o_p + col);
-      const float n = fmaxf(m, ml.x);
-      const float fo = m == -INFINITY ? 0.f : exp2_fast(m - n), fn = exp2_fast(ml.x - n);
-      m = n;
-      l = l * fo + ml.y * fn;
-      o.x = o.x * fo + v.x * fn;
-      o.y = o.y * fo + v.y * fn;
-      o.z = o.z * fo + v.z * fn;
-      o.w = o.w * fo + v.w * fn;
-    };
-    if (p.row_ml != nullptr)
-      for (int i = 0; i < p.prefix_slots + (whole ? 1 : 0); ++i)
-        take(p.row_ml + i * slot_rows + row, p.row_o + (i * slot_rows + row) * c.head_dim);
-    if (blocks > 0 && !whole)
-      for (int64_t i = c0; i <= c1; ++i) {
-        const int64_t piece = (2 * i + (i == c0 ? 1 : 0)) * KS_ROWS + r;
-        take(p.piece_ml + piece, p.piece_o + piece * c.head_dim);
-      }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const uint2 w2 = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + col) = w2;
+    auto piece = [&](int i) { return (2 * (c0 + i) + (i == 0 ? 1 : 0)) * KS_ROWS + r; };
+    KsRow x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    if (live)
+      x = ks_join_states(
+          sub, per_row, count, lane, on,
+          [&](int i) { return i < shared_n ? p.row_ml + i * slot_rows + row : p.piece_ml + piece(i - shared_n); },
+          [&](int i) {
+            return (i < shared_n ? p.row_o + (i * slot_rows + row) * c.head_dim : p.piece_o + piece(i - shared_n) * c.head_dim) + col;
+          });
+    if (per_row > 1) {
+      part[warp][lane] = x;
+      __syncthreads();
+      if (sub == 0)
+        for (int i = 1; i < per_row; ++i) ks_join_two(x, part[warp + i][lane]);
+      __syncthreads();
+    }
+    if (live && sub == 0 && on) ks_store_row(x, static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + col);
   }
 }
 

@@ -794,6 +794,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   } else {
     kt_multiply<T, HDP>(p, bars, qs, ring, warp - 10);
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   tc_fence_before();
   __syncwarp();
   __syncthreads();
@@ -803,39 +804,23 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   }
 }
 
-// out = the joined states of all slots, one 16-byte vector of a row a thread; rows that belong to no
-// sequence are left alone.
+// out = the joined states of all slots, a warp a row; rows that belong to no sequence are left alone.
 template <typename T>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
     kv_rows_join_kernel(const int32_t* __restrict__ cu, int64_t batch, int64_t tokens, int32_t q_heads, int32_t head_dim,
                         const float2* __restrict__ row_ml, const float* __restrict__ row_o, int32_t slots, KvRows out) {
-  const int vecs = head_dim >> 2;
-  const int64_t it = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t row = it / vecs;
-  const int col = int(it - row * vecs) << 2;
+  const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31, col = lane * 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (row >= tokens * q_heads) return;
   const int64_t token = row / q_heads;
   if (cu != nullptr && (token < cu[0] || token >= cu[batch])) return;
   const int64_t slot_rows = tokens * q_heads;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < slots; ++i) {
-    const float2 ml = row_ml[i * slot_rows + row];
-    if (ml.x == -INFINITY) continue;
-    const float4 v = *reinterpret_cast<const float4*>(row_o + (i * slot_rows + row) * head_dim + col);
-    const float n = fmaxf(m, ml.x);
-    const float fo = m == -INFINITY ? 0.f : exp2_fast(m - n), fn = exp2_fast(ml.x - n);
-    m = n;
-    l = l * fo + ml.y * fn;
-    o.x = o.x * fo + v.x * fn;
-    o.y = o.y * fo + v.y * fn;
-    o.z = o.z * fo + v.z * fn;
-    o.w = o.w * fo + v.w * fn;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const KsRow x = ks_join_states(
+      0, 1, slots, lane, col < head_dim, [&](int i) { return row_ml + i * slot_rows + row; },
+      [&](int i) { return row_o + (i * slot_rows + row) * head_dim + col; });
   const int head = int(row - token * q_heads);
-  *reinterpret_cast<uint2*>(static_cast<T*>(out.ptr) + token * out.token + head * out.head + col) =
-      make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  if (col < head_dim) ks_store_row(x, static_cast<T*>(out.ptr) + token * out.token + head * out.head + col);
 }
 
 }  // namespace lng

@@ -1843,26 +1843,37 @@ static int launch_kv_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CU
   return LNG_OK;
 }
 
-template <typename T, int HDP>
-static int launch_kv_step(const CUtensorMap& tk, const CUtensorMap& tv, const KsParams& p, cudaStream_t s) {
-  using Cfg = KsCfg<HDP>;
-  auto kern = kv_step_kernel<T, HDP>;
-  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
-  kern<<<p.shares, Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
-  LNG_LAUNCHED("kv_step_kernel");
-  // the join is a programmatic dependent: it finds its pieces while the step kernel runs and waits for
-  // it before it reads them
+// A launch that may start while the kernel before it in the stream still runs (griddepcontrol in both).
+template <typename... Params, typename... Args>
+static int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, Args... args) {
   cudaLaunchAttribute pdl[1];
   pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(p.c.batch * p.c.kv_heads));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = pdl;
   cfg.numAttrs = 1;
-  LNG_CUDA(cudaLaunchKernelEx(&cfg, kv_step_join_kernel<T>, p, int(Cfg::WARPS)));
+  LNG_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
   return LNG_OK;
+}
+
+// behind_prefix: the kernel before is the prefix's, which this one needs nothing of
+template <typename T, int HDP>
+static int launch_kv_step(const CUtensorMap& tk, const CUtensorMap& tv, const KsParams& p, bool behind_prefix, cudaStream_t s) {
+  using Cfg = KsCfg<HDP>;
+  auto kern = kv_step_kernel<T, HDP>;
+  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  if (behind_prefix) {
+    if (const int st = launch_dependent(kern, unsigned(p.shares), Cfg::THREADS, Cfg::SMEM, s, tk, tv, p)) return st;
+  } else {
+    kern<<<p.shares, Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
+    LNG_LAUNCHED("kv_step_kernel");
+  }
+  // the join finds its pieces while the step kernel runs and waits for it before it reads them
+  return launch_dependent(kv_step_join_kernel<T, Cfg::BK>, unsigned(p.c.batch * p.c.kv_heads), 256u, size_t(0), s, p);
 }
 
 static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len, const int32_t* cu,
@@ -1932,15 +1943,10 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
       p.splits = plan.splits;
       if ((st = launch(plan.units))) return st;
       if (plan.slots == 0) return LNG_OK;
-      const unsigned grid = unsigned(ceil_div(tokens * q->heads * (cache->head_dim / 4), 128));
-      if (bf16)
-        kv_rows_join_kernel<__nv_bfloat16><<<grid, 128, 0, cs>>>(cu, cache->batch, tokens, q->heads, cache->head_dim, row_ml, row_o,
-                                                                 plan.slots, kv_rows(out));
-      else
-        kv_rows_join_kernel<__half><<<grid, 128, 0, cs>>>(cu, cache->batch, tokens, q->heads, cache->head_dim, row_ml, row_o,
-                                                          plan.slots, kv_rows(out));
-      LNG_LAUNCHED("kv_rows_join_kernel");
-      return LNG_OK;
+      auto join = bf16 ? kv_rows_join_kernel<__nv_bfloat16> : kv_rows_join_kernel<__half>;
+      return launch_dependent(join, unsigned(ceil_div(tokens * q->heads, 8)), 256u, size_t(0), cs, cu, cache->batch, tokens, q->heads,
+                              cache->head_dim, static_cast<const float2*>(row_ml), static_cast<const float*>(row_o), plan.slots,
+                              kv_rows(out));
     }
   }
   KsParams p{};
@@ -1952,7 +1958,7 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   p.scale_log2 = scale_log2;
   p.window = window;
   p.sinks = sinks;
-  p.box = std::min(cache->page_size, KS_BK);
+  p.box = std::min(cache->page_size, KsCfg<64>::BK);
   p.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
   p.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
   p.shares = plan.shares;
@@ -1961,8 +1967,10 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   p.prefix_slots = plan.prefix_splits;
   CUtensorMap tk, tv;
   if ((st = kv_page_maps(&tk, &tv, cache, p.box))) return st;
-  if (bf16) return wide ? launch_kv_step<__nv_bfloat16, 128>(tk, tv, p, cs) : launch_kv_step<__nv_bfloat16, 64>(tk, tv, p, cs);
-  return wide ? launch_kv_step<__half, 128>(tk, tv, p, cs) : launch_kv_step<__half, 64>(tk, tv, p, cs);
+  const bool behind = plan.prefix_splits > 0;
+  if (bf16)
+    return wide ? launch_kv_step<__nv_bfloat16, 128>(tk, tv, p, behind, cs) : launch_kv_step<__nv_bfloat16, 64>(tk, tv, p, behind, cs);
+  return wide ? launch_kv_step<__half, 128>(tk, tv, p, behind, cs) : launch_kv_step<__half, 64>(tk, tv, p, behind, cs);
 }
 
 }  // namespace lng
