@@ -45,10 +45,10 @@ struct KsParams {
   float scale_log2;  // scale * log2(e): the softmax runs in base 2
   int32_t window, sinks;
   int32_t box;       // keys a TMA copy: min(page size, 32)
-  // pieces: slot 2 * cta (a pair begun before the CTA's share) and 2 * cta + 1 (one that goes on behind it)
-  float2* piece_ml;  // [2 * grid][16] (maximum, sum), base 2
-  float* piece_o;    // [2 * grid][16][head_dim]
-  int32_t shares;    // CTAs of the step kernel
+  // pieces: slot 2 * share (a pair begun before the share) and 2 * share + 1 (one that goes on behind it)
+  float2* piece_ml;  // [2 * shares][16] (maximum, sum), base 2
+  float* piece_o;    // [2 * shares][16][head_dim]
+  int32_t shares;    // into which the line is cut
   // a shared prefix: states of `prefix_slots` ranges of it, [slot][row][..] with row = token * q_heads + head;
   // pairs finished by one CTA then go to slot prefix_slots (null: to o)
   float2* row_ml;
@@ -72,16 +72,17 @@ __device__ __forceinline__ int64_t ks_share(int64_t total, int shares) {
   return per > 0 ? per : 1;
 }
 
-// Sums blocks(b) * KV over all sequences and finds the sequence in which block `want` of the line falls and
-// the line's position where that sequence starts (b = batch when want >= total).  All `nthreads` threads
-// take part; thread t sums a contiguous run of sequences.
+// Sums blocks(b) * KV over all sequences and finds, for the CTA's FINDS shares from share0 on, the sequence in which
+// the share's first block falls and the line's position where that sequence starts (b = batch behind the line's
+// end); returns that of share share0 + mine_of.  All `nthreads` threads take part; thread t sums a contiguous run
+// of sequences.
 struct KsFound {
   int64_t total, b, start;
 };
 
-template <int BK>
+template <int BK, int FINDS>
 __device__ inline KsFound ks_find(const KvView& c, int32_t window, int32_t sinks, int nthreads, int shares, int64_t* warp_tot,
-                                  int64_t* found, int64_t cta) {
+                                  int64_t (*found)[2], int64_t share0, int mine_of) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t run = (c.batch + nthreads - 1) / nthreads;
   const int64_t b0 = tid * run, b1 = b0 + run < c.batch ? b0 + run : c.batch;
@@ -94,9 +95,9 @@ __device__ inline KsFound ks_find(const KvView& c, int32_t window, int32_t sinks
     if (lane >= o) incl += v;
   }
   if (lane == 31) warp_tot[warp] = incl;
-  if (tid == 0) {
-    found[0] = c.batch;
-    found[1] = 0;
+  if (tid < FINDS) {
+    found[tid][0] = c.batch;
+    found[tid][1] = 0;
   }
   __syncthreads();
   int64_t before = 0, total = 0;
@@ -105,21 +106,23 @@ __device__ inline KsFound ks_find(const KvView& c, int32_t window, int32_t sinks
     total += warp_tot[w];
   }
   const int64_t at = before + incl - mine;
-  const int64_t want = cta * ks_share(total, shares);
-  if (want >= at && want < at + mine) {
+  const int64_t per = ks_share(total, shares);
+  for (int f = 0; f < FINDS; ++f) {
+    const int64_t want = (share0 + f) * per;
+    if (want < at || want >= at + mine) continue;
     int64_t pos = at;
     for (int64_t b = b0; b < b1; ++b) {
       const int64_t n = int64_t(ks_blocks<BK>(c, kv_span(c, b), window, sinks)) * c.kv_heads;
       if (want < pos + n) {
-        found[0] = b;
-        found[1] = pos;
+        found[f][0] = b;
+        found[f][1] = pos;
         break;
       }
       pos += n;
     }
   }
   __syncthreads();
-  return KsFound{total, found[0], found[1]};
+  return KsFound{total, found[mine_of][0], found[mine_of][1]};
 }
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w,
@@ -215,7 +218,9 @@ struct KsWalk {
   }
 };
 
-template <typename T, int HDP>
+// WS: a share a warp (many pairs: no meeting of warps at each pair's end), else a share a CTA (few pairs: fewer
+// pieces a pair).
+template <typename T, int HDP, bool WS>
 __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     kv_step_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const KsParams p) {
   using Cfg = KsCfg<HDP>;
@@ -225,7 +230,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
   float* merge_o = reinterpret_cast<float*>(base + WARPS * Cfg::RING_BYTES);  // [WARPS][16][HDP]
   float2* merge_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(merge_o) + Cfg::MERGE_BYTES);  // [WARPS][16]
   uint64_t* bars = reinterpret_cast<uint64_t*>(merge_ml + WARPS * KS_ROWS);   // [WARPS][STAGES]
-  __shared__ int64_t warp_tot[WARPS], found[2];
+  __shared__ int64_t warp_tot[WARPS], found[WS ? WARPS : 1][2];
   const KvView& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = base + warp * Cfg::RING_BYTES;
@@ -239,23 +244,27 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       tma_prefetch_desc(&tmv);
     }
   }
-  const KsFound f = ks_find<BK>(c, p.window, p.sinks, Cfg::THREADS, p.shares, warp_tot, found, blockIdx.x);
+  // blocks of a pair that are this warp's: all of its share's, or every WARPS-th of the CTA's
+  constexpr int STRIDE = WS ? 1 : WARPS;
+  const int start = WS ? 0 : warp;
+  const int64_t share0 = int64_t(blockIdx.x) * (WS ? WARPS : 1), share = share0 + (WS ? warp : 0);
+  const KsFound f = ks_find<BK, WS ? WARPS : 1>(c, p.window, p.sinks, Cfg::THREADS, p.shares, warp_tot, found, share0, WS ? warp : 0);
   const int64_t per = ks_share(f.total, p.shares);
-  const int64_t p0 = int64_t(blockIdx.x) * per, p1 = p0 + per < f.total ? p0 + per : f.total;
+  const int64_t p0 = share * per, p1 = p0 + per < f.total ? p0 + per : f.total;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the loading walk runs KS_STAGES blocks of this warp ahead of the computing walk
   KsWalk<BK> ld, cw;
   ld.start(c, p.window, p.sinks, f, p0, p1);
   cw = ld;
-  int32_t ld_k = ld.done() ? 0 : ld.k0 + warp;
+  int32_t ld_k = ld.done() ? 0 : ld.k0 + start;
   uint32_t issued = 0, taken = 0;
   // pages of the warp's next blocks of the pair, a piece (of `box` keys) a lane: looked up together, since a
   // look-up of one block's page takes longer than its copies
   const int boxes = BK / p.box, ahead = 32 / boxes;
   int32_t pages = -1, seen = ahead;  // -1: no row sees a key of the piece; blocks issued out of the looked-up ones
   auto look_up = [&]() {
-    const int32_t k = ld_k + (lane / boxes) * WARPS;
+    const int32_t k = ld_k + (lane / boxes) * STRIDE;
     pages = -1;
     if (k < ld.k1) {
       const int32_t key = tile_index(ld.tiles, k) * BK + (lane % boxes) * p.box;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
   auto issue = [&]() {  // the warp's next block into the ring (all lanes keep the walk; lane 0 copies)
     while (!ld.done() && ld_k >= ld.k1) {
       ld.next(c, p.window, p.sinks);
-      if (!ld.done()) ld_k = ld.k0 + warp;
+      if (!ld.done()) ld_k = ld.k0 + start;
       seen = ahead;
     }
     if (ld.done()) return;
@@ -296,7 +305,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     __syncwarp();
     ++issued;
     ++seen;
-    ld_k += WARPS;
+    ld_k += STRIDE;
   };
 #pragma unroll 1
   for (int i = 0; i < KS_STAGES; ++i) issue();
@@ -334,7 +343,7 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       for (int j = 0; j < 4; ++j) oacc[i][j] = 0.f;
     float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
 
-    for (int32_t k = cw.k0 + warp; k < cw.k1; k += WARPS) {
+    for (int32_t k = cw.k0 + start; k < cw.k1; k += STRIDE) {
       const uint32_t s = taken % KS_STAGES;
       if (ok) ok = mbar_wait_bounded(&bar[s], (taken / KS_STAGES) & 1, &g_error_word, DEV_ERR_WAIT_TIMEOUT);
       ok = __all_sync(0xffffffffu, ok);
@@ -446,12 +455,42 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
       issue();
     }
 
-    // the warps' states meet: maximum and sum first, then the products, each scaled to the common maximum
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       la += __shfl_xor_sync(0xffffffffu, la, o);
       lb += __shfl_xor_sync(0xffffffffu, lb, o);
     }
+    const bool begins = cw.k0 == 0, ends = cw.k1 == cw.blocks, finished = begins && ends;
+    const int64_t piece = 2 * share + (begins ? 1 : 0);
+    if constexpr (WS) {
+      if (!ok) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = g + 8 * i;
+        if (r >= rows) continue;
+        const float m = i ? mb : ma, l = i ? lb : la;
+        const int tok = r / rows_of_n, head = cw.h * p.group + (r - tok * rows_of_n);
+        const int64_t token = cw.s.first + tok;
+        if (finished && p.row_ml == nullptr) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + t4 * 2;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            if (n * 8 < c.head_dim) *reinterpret_cast<uint32_t*>(dst + n * 8) = pack2<T>(oacc[n][2 * i] * inv, oacc[n][2 * i + 1] * inv);
+        } else {
+          const int64_t row = int64_t(p.prefix_slots) * c.tokens * p.q_heads + token * p.q_heads + head;
+          float2* ml = finished ? p.row_ml + row : p.piece_ml + piece * KS_ROWS + r;
+          float* po = (finished ? p.row_o + row * c.head_dim : p.piece_o + (piece * KS_ROWS + r) * c.head_dim) + t4 * 2;
+          // (scores that are all NaN leave the maximum at -inf: their NaN sum must not be taken for an empty state)
+          if (t4 == 0) *ml = make_float2(l == l ? m : 0.f, l);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            if (n * 8 < c.head_dim) *reinterpret_cast<float2*>(po + n * 8) = make_float2(oacc[n][2 * i], oacc[n][2 * i + 1]);
+        }
+      }
+      continue;
+    }
+    // the warps' states meet: maximum and sum first, then the products, each scaled to the common maximum
     if (t4 == 0) {
       // (scores that are all NaN leave the maximum at -inf: their NaN sum must not be taken for an empty state)
       merge_ml[warp * KS_ROWS + g] = make_float2(la == la ? ma : 0.f, la);
@@ -491,8 +530,6 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     }
     }
     __syncthreads();
-    const bool begins = cw.k0 == 0, ends = cw.k1 == cw.blocks, finished = begins && ends;
-    const int64_t piece = 2 * int64_t(blockIdx.x) + (begins ? 1 : 0);
     const int vecs = c.head_dim >> 2;
     for (int it = threadIdx.x; it < rows * vecs; it += Cfg::THREADS) {
       const int r = it / vecs, col = (it - r * vecs) << 2;

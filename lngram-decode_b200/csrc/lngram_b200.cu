@@ -1785,7 +1785,8 @@ static int kv_splits(int64_t units, int64_t tiles) {
 // How an attention call is carried out, and what it needs of the workspace.
 struct KvPlan {
   bool step;          // the sequences' own keys by kv_step_kernel (at most 16 rows a key head), else by kv_tile_kernel
-  int shares;         // CTAs of the step kernel
+  int shares;         // into which its work is cut
+  bool warp_shares;   // a share a warp, not a CTA
   int64_t units;      // CTAs of the tile kernel per key head and range
   int splits;         // key ranges of the tile kernel
   int prefix_splits;  // key ranges of a shared prefix (0: there is none)
@@ -1802,7 +1803,10 @@ static KvPlan kv_plan(const lng_kv_cache* c, int64_t prefix_len, int64_t tokens,
   if (window > 0) keys = std::min(keys, int64_t(window) + sinks + span + KT_BK);
   p.step = group * max_new <= KS_ROWS;
   if (p.step) {
-    p.shares = num_sms();
+    // many pairs: a share a warp, so that pairs end without the CTA's warps meeting (64 sequences of 300 keys, 8 key
+    // heads: 37 -> 31 us; 64 of 2000 keys: 107 -> 98); few pairs: a share a CTA, which leaves an eighth or a quarter of the pieces to join
+    p.warp_shares = c->batch * c->num_kv_heads >= num_sms();
+    p.shares = num_sms() * (p.warp_shares ? (c->head_dim > 64 ? KsCfg<128>::WARPS : KsCfg<64>::WARPS) : 1);
   } else {
     // ragged steps: at most one unit a sequence is not full
     p.units = c->batch * ceil_div(max_new, span);
@@ -1861,15 +1865,16 @@ static int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned thr
 }
 
 // behind_prefix: the kernel before is the prefix's, which this one needs nothing of
-template <typename T, int HDP>
+template <typename T, int HDP, bool WS>
 static int launch_kv_step(const CUtensorMap& tk, const CUtensorMap& tv, const KsParams& p, bool behind_prefix, cudaStream_t s) {
   using Cfg = KsCfg<HDP>;
-  auto kern = kv_step_kernel<T, HDP>;
+  auto kern = kv_step_kernel<T, HDP, WS>;
   LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  const unsigned grid = unsigned(p.shares / (WS ? Cfg::WARPS : 1));
   if (behind_prefix) {
-    if (const int st = launch_dependent(kern, unsigned(p.shares), Cfg::THREADS, Cfg::SMEM, s, tk, tv, p)) return st;
+    if (const int st = launch_dependent(kern, grid, Cfg::THREADS, Cfg::SMEM, s, tk, tv, p)) return st;
   } else {
-    kern<<<p.shares, Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
+    kern<<<grid, Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
     LNG_LAUNCHED("kv_step_kernel");
   }
   // the join finds its pieces while the step kernel runs and waits for it before it reads them
@@ -1968,9 +1973,13 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   CUtensorMap tk, tv;
   if ((st = kv_page_maps(&tk, &tv, cache, p.box))) return st;
   const bool behind = plan.prefix_splits > 0;
-  if (bf16)
-    return wide ? launch_kv_step<__nv_bfloat16, 128>(tk, tv, p, behind, cs) : launch_kv_step<__nv_bfloat16, 64>(tk, tv, p, behind, cs);
-  return wide ? launch_kv_step<__half, 128>(tk, tv, p, behind, cs) : launch_kv_step<__half, 64>(tk, tv, p, behind, cs);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (plan.warp_shares)
+      return wide ? launch_kv_step<T, 128, true>(tk, tv, p, behind, cs) : launch_kv_step<T, 64, true>(tk, tv, p, behind, cs);
+    return wide ? launch_kv_step<T, 128, false>(tk, tv, p, behind, cs) : launch_kv_step<T, 64, false>(tk, tv, p, behind, cs);
+  };
+  return bf16 ? launch(__nv_bfloat16()) : launch(__half());
 }
 
 }  // namespace lng
