@@ -34,7 +34,8 @@ __device__ __forceinline__ SeqSpan kv_span(const KvView& c, int64_t b) {
 
 // The sequence whose rows hold `token`, or -1: division for uniform steps, else a binary search of cu.
 __device__ __forceinline__ int64_t kv_sequence_of(const KvView& c, int64_t token) {
-  if (c.cu == nullptr) return token / c.max_new;
+  if (c.cu == nullptr)  // (a 64-bit division takes some 40 instructions more)
+    return token < (int64_t(1) << 32) ? int64_t(uint32_t(token) / uint32_t(c.max_new)) : token / c.max_new;
   if (token < c.cu[0] || token >= c.cu[c.batch]) return -1;
   int64_t lo = 0, hi = c.batch;  // cu[lo] <= token < cu[hi]
   while (hi - lo > 1) {
@@ -48,136 +49,127 @@ __device__ __forceinline__ int64_t kv_sequence_of(const KvView& c, int64_t token
 }
 
 // ------------------------------------------------------------------ append
-// Memory bound: every row is read once and written once, 16 bytes a thread.  A 256-thread CTA takes TPC
-// tokens: first one thread per (token, pair) forms cos and sin -- the angle p * f needs more than fp32's
-// 24 bits for far positions (p = 10^6 would leave an error of 0.06 rad), so the product and its reduction
-// by 2 pi are 64-bit, once per token and not per head, and sine and cosine of the reduced angle fp32 --
-// then the threads walk the tokens' (head, column) vectors.  Pairs (j, j + half) are both handled by the
-// thread of column j, so rotating q in place is safe.
-template <typename T, int TPC>
-__global__ void __launch_bounds__(256)
-    kv_append_kernel(KvView c, KvRows kr, KvRows vr, KvRows qr, KvRows qo, int32_t q_heads,
-                     const int64_t* __restrict__ positions, const float* __restrict__ inv_freq, int32_t rotary,
-                     int32_t interleaved) {
-  constexpr int MAX_HALF = 64;  // head_dim <= 128
-  __shared__ float2 cs[TPC][MAX_HALF];
-  __shared__ int64_t k_base[TPC], v_base[TPC];  // element offsets of the token's slot (head 0), -1: none
-  __shared__ int64_t row[TPC];                  // -1: the token belongs to no sequence
-  __shared__ double pos[TPC];
-  const int half = rotary >> 1, tid = threadIdx.x;
-  for (int64_t t0 = int64_t(blockIdx.x) * TPC; t0 < c.tokens; t0 += int64_t(gridDim.x) * TPC) {
-    if (tid < TPC) {
-      const int64_t t = t0 + tid;
-      int64_t kb = -1, vb = -1, rw = -1;
-      double p = 0.0;
-      const int64_t b = t < c.tokens ? kv_sequence_of(c, t) : -1;
-      if (b >= 0 && b < c.batch) {
-        const SeqSpan s = kv_span(c, b);
-        const int64_t i = t - s.first;
-        if (i >= 0 && i < s.n) {
-          rw = t;
-          const int32_t key = s.len - s.n + int32_t(i);
-          p = positions ? double(positions[t]) : double(key);
-          const int32_t page = key >= 0 ? page_of(c.table + b * c.table_stride, key, c.page_shift, c.num_pages) : -1;
-          if (page >= 0) {
-            const int32_t slot = key & ((1 << c.page_shift) - 1);
-            kb = page * c.k_page + slot * c.k_slot;
-            vb = page * c.v_page + slot * c.v_slot;
-          } else {
-            kv_range_error();
-          }
-        }
-      }
-      k_base[tid] = kb;
-      v_base[tid] = vb;
-      row[tid] = rw;
-      pos[tid] = p;
-    }
-    __syncthreads();
-    for (int i = tid; i < TPC * half; i += 256) {
-      const int t = i / half, j = i - t * half;
-      const double a = pos[t] * double(inv_freq[j]);
-      const float r = float(fma(-rint(a * 0.15915494309189533577), 6.283185307179586476925, a));
+// Memory bound: every row is read once and written once.  A warp takes a token (or one of `parts` of it, when
+// the step has few tokens) and meets no other: its lanes look up the token's slot, form cos and sin of the token's
+// pairs once for all heads, and then move the token's items, an item being two 16-byte vectors of a head -- the two
+// halves of eight pairs where pairs are (j, j + half), so rotating q in place is safe.  The angle p * f needs more
+// than fp32's 24 bits for far positions (p = 10^6 would leave an error of 0.06 rad): it is formed in turns and
+// reduced to the nearest whole one in 64 bits, sine and cosine of the rest fp32.
+// What counts is how many warps have loads in flight: CTAs of two warps are replaced as soon as both are through,
+// and registers for 48 warps an SM (one item at a time a thread) beat items in pairs.  32 prompts of 2048 tokens, 16
+// query and 4 key heads of 64 (403 MB): 8 warps a CTA 86 us, 4 warps 80, 2 warps 77, 1 warp 80; 2 warps with 42
+// registers a thread instead of 60: 70 us, 5.8 TB/s.  28 query heads of 128, half rotated: 98 us, 5.4 TB/s.
+constexpr int KA_WARPS = 2;
+constexpr int KA_MAX_HALF = 64;  // head_dim <= 128
+
+struct KaParams {
+  KvView c;
+  KvRows kr, vr, qr, qo;
+  int32_t q_heads, rotary, interleaved;
+  int32_t parts;         // warps a token
+  int32_t items;         // of a head: half its vectors, rounded up
+  uint32_t items_magic;  // i / items = __umulhi(i, items_magic) where items > 1
+  const int64_t* positions;
+  const float* inv_freq;
+};
+
+template <typename T>
+__device__ __forceinline__ void ka_rotate(T& a, T& b, float2 cs) {
+  const float x = to_f32<T>(a), y = to_f32<T>(b);
+  a = from_f32<T>(x * cs.x - y * cs.y);
+  b = from_f32<T>(y * cs.x + x * cs.y);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(KA_WARPS * 32, 24) kv_append_kernel(const KaParams p) {
+  __shared__ __align__(16) float2 cs_all[KA_WARPS][KA_MAX_HALF];
+  const KvView& c = p.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t w = int64_t(blockIdx.x) * KA_WARPS + warp;
+  const int64_t token = p.parts == 1 ? w : int64_t(uint32_t(w) / uint32_t(p.parts));  // (parted only when few)
+  if (token >= c.tokens) return;
+  const int part = int(w - token * p.parts);
+  float2* cs = cs_all[warp];
+  const int64_t b = kv_sequence_of(c, token);
+  if (b < 0 || b >= c.batch) return;
+  const SeqSpan s = kv_span(c, b);
+  const int64_t i = token - s.first;
+  if (i < 0 || i >= s.n) return;
+  const int32_t key = s.len - s.n + int32_t(i);
+  const int32_t page = key >= 0 ? page_of(c.table + b * c.table_stride, key, c.page_shift, c.num_pages) : -1;
+  if (page < 0) kv_range_error();
+  const int32_t slot = key & ((1 << c.page_shift) - 1);
+  const int half = p.rotary >> 1;
+  if (half > 0) {
+    const double pos = p.positions ? double(p.positions[token]) : double(key);
+    for (int j = lane; j < half; j += 32) {
+      const double turns = pos * double(p.inv_freq[j]) * 0.15915494309189533577;  // 1 / (2 pi)
       float sn, cn;
-      sincosf(r, &sn, &cn);
-      cs[t][j] = make_float2(cn, sn);
+      sincospif(float(2.0 * (turns - rint(turns))), &sn, &cn);
+      cs[j] = make_float2(cn, sn);
     }
-    __syncthreads();
-    // columns of 8 values; in the split form columns of the first half of the rotated part also do
-    // their partners, and a half that is no multiple of 8 is rotated value by value
-    const int cols = c.head_dim >> 3;
-    const bool split_vec = !interleaved && half > 0 && (half & 7) == 0;
-    const bool split_any = !interleaved && half > 0 && (half & 7) != 0;
-    const int heads = 2 * c.kv_heads + q_heads;
-    const int items = TPC * heads * cols;
-    for (int it = tid; it < items; it += 256) {
-      const int t = it / (heads * cols);
-      const int rem = it - t * heads * cols;
-      const int h = rem / cols, col = (rem - h * cols) << 3;
-      if (row[t] < 0) continue;
-      const T* src;
-      T* dst;
-      bool rot = rotary > 0 && col < rotary;
-      if (h < c.kv_heads) {
-        if (k_base[t] < 0) continue;
-        src = static_cast<const T*>(kr.ptr) + row[t] * kr.token + h * kr.head;
-        dst = static_cast<T*>(c.k) + k_base[t] + h * c.k_head;
-      } else if (h < 2 * c.kv_heads) {
-        if (v_base[t] < 0) continue;
-        const int hv = h - c.kv_heads;
-        src = static_cast<const T*>(vr.ptr) + row[t] * vr.token + hv * vr.head;
-        dst = static_cast<T*>(c.v) + v_base[t] + hv * c.v_head;
-        rot = false;
-      } else {
-        const int hq = h - 2 * c.kv_heads;
-        src = static_cast<const T*>(qr.ptr) + row[t] * qr.token + hq * qr.head;
-        dst = static_cast<T*>(qo.ptr) + row[t] * qo.token + hq * qo.head;
-      }
-      if (!rot) {
-        *reinterpret_cast<uint4*>(dst + col) = *reinterpret_cast<const uint4*>(src + col);
-      } else if (interleaved) {
-        uint4 w = *reinterpret_cast<const uint4*>(src + col);
-        T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          if (col + i < rotary) {
-            const float2 r = cs[t][(col + i) >> 1];
-            const float a = to_f32<T>(e[i]), b = to_f32<T>(e[i + 1]);
-            e[i] = from_f32<T>(a * r.x - b * r.y);
-            e[i + 1] = from_f32<T>(b * r.x + a * r.y);
-          }
-        }
-        *reinterpret_cast<uint4*>(dst + col) = w;
-      } else if (split_vec) {
-        if (col >= half) continue;  // the partner column does it
-        uint4 w0 = *reinterpret_cast<const uint4*>(src + col);
-        uint4 w1 = *reinterpret_cast<const uint4*>(src + col + half);
-        T* e0 = reinterpret_cast<T*>(&w0);
-        T* e1 = reinterpret_cast<T*>(&w1);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 r = cs[t][col + i];
-          const float a = to_f32<T>(e0[i]), b = to_f32<T>(e1[i]);
-          e0[i] = from_f32<T>(a * r.x - b * r.y);
-          e1[i] = from_f32<T>(b * r.x + a * r.y);
-        }
-        *reinterpret_cast<uint4*>(dst + col) = w0;
-        *reinterpret_cast<uint4*>(dst + col + half) = w1;
-      } else if (split_any) {
-        for (int i = 0; i < 8; ++i) {
-          const int j = col + i;
-          if (j < half) {
-            const float2 r = cs[t][j];
-            const float a = to_f32<T>(src[j]), b = to_f32<T>(src[j + half]);
-            dst[j] = from_f32<T>(a * r.x - b * r.y);
-            dst[j + half] = from_f32<T>(b * r.x + a * r.y);
-          } else if (j >= rotary) {
-            dst[j] = src[j];
-          }
+    __syncwarp();
+  }
+  const bool split = !p.interleaved && half > 0, split_vec = split && (half & 7) == 0;
+  const int total = (2 * c.kv_heads + p.q_heads) * p.items;
+#pragma unroll 1
+  for (int it = part * 32 + lane; it < total; it += p.parts * 32) {
+    const int h = p.items > 1 ? int(__umulhi(uint32_t(it), p.items_magic)) : it;
+    const int item = it - h * p.items;
+    const T* src;
+    T* dst;
+    bool rot = half > 0;
+    if (h < c.kv_heads) {
+      src = static_cast<const T*>(p.kr.ptr) + token * p.kr.token + h * p.kr.head;
+      dst = static_cast<T*>(c.k) + page * c.k_page + slot * c.k_slot + h * c.k_head;
+    } else if (h < 2 * c.kv_heads) {
+      const int hv = h - c.kv_heads;
+      src = static_cast<const T*>(p.vr.ptr) + token * p.vr.token + hv * p.vr.head;
+      dst = static_cast<T*>(c.v) + page * c.v_page + slot * c.v_slot + hv * c.v_head;
+      rot = false;
+    } else {
+      const int hq = h - 2 * c.kv_heads;
+      src = static_cast<const T*>(p.qr.ptr) + token * p.qr.token + hq * p.qr.head;
+      dst = static_cast<T*>(p.qo.ptr) + token * p.qo.token + hq * p.qo.head;
+    }
+    if (h < 2 * c.kv_heads && page < 0) continue;
+    if (rot && split && !split_vec) {  // halves that are no multiple of 8: value by value
+      for (int j = item * 16; j < item * 16 + 16 && j < c.head_dim; ++j) {
+        if (j < half) {
+          T x = src[j], y = src[j + half];
+          ka_rotate<T>(x, y, cs[j]);
+          dst[j] = x;
+          dst[j + half] = y;
+        } else if (j >= p.rotary) {
+          dst[j] = src[j];
         }
       }
+      continue;
     }
-    __syncthreads();
+    // the item's columns: partners first, then what is not rotated, two vectors each
+    int c0 = item * 16, c1 = c0 + 8;
+    const bool pair = rot && split && item * 8 < half;
+    if (pair) c0 = item * 8, c1 = c0 + half;
+    const bool two = c1 < c.head_dim;
+    uint4 w0 = __ldcs(reinterpret_cast<const uint4*>(src + c0)), w1 = make_uint4(0, 0, 0, 0);
+    if (two) w1 = __ldcs(reinterpret_cast<const uint4*>(src + c1));
+    T *e0 = reinterpret_cast<T*>(&w0), *e1 = reinterpret_cast<T*>(&w1);
+    if (pair) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float4 r = *reinterpret_cast<const float4*>(cs + c0 + e);
+        ka_rotate<T>(e0[e], e1[e], make_float2(r.x, r.y));
+        ka_rotate<T>(e0[e + 1], e1[e + 1], make_float2(r.z, r.w));
+      }
+    } else if (rot && p.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        if (c0 + e < p.rotary) ka_rotate<T>(e0[e], e0[e + 1], cs[(c0 + e) >> 1]);
+        if (c1 + e < p.rotary) ka_rotate<T>(e1[e], e1[e + 1], cs[(c1 + e) >> 1]);
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + c0) = w0;
+    if (two) *reinterpret_cast<uint4*>(dst + c1) = w1;
   }
 }
 
