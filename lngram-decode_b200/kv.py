@@ -60,6 +60,7 @@ class PagedKVCache:
             _require(t.data_ptr() % 16 == 0, "k and v must be 16-byte aligned")
         _require(table.dim() == 2 and table.dtype == torch.int32 and (table.shape[1] <= 1 or table.stride(1) == 1),
                  "table must be int32 [B, max_pages] with contiguous rows")
+        _require(table.shape[0] <= 1 or table.stride(0) >= table.shape[1], "table: the sequences' rows must not overlap")
         _require(lengths.dim() == 1 and lengths.dtype == torch.int32 and lengths.is_contiguous(),
                  "lengths must be contiguous int32 [B]")
         _require(lengths.shape[0] == table.shape[0], "table and lengths must have one row a sequence")
@@ -161,6 +162,11 @@ def _step(cache: PagedKVCache, t: Tensor, cu: Tensor | None, max_new: int | None
     return ts[0], int(max_new)
 
 
+def _no_grad(*tensors: Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the paged cache's operators have no backward: call them under torch.no_grad()")
+
+
 def _library(cache: PagedKVCache):
     if cache.index < 0:
         raise RuntimeError("the cache must be on a CUDA device: lngram_b200 has no CPU path")
@@ -175,6 +181,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     values of keys and queries are rotated by the token's position -- ``positions`` (int64, the step's leading
     shape) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
     Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``.  No gradients."""
+    _no_grad(k, v, q)
     tokens, max_new = _step(cache, k, cu, max_new)
     lead = k.shape[:-2]
     kr = _rows(k, "k", cache, lead, cache.num_kv_heads)
@@ -206,6 +213,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
 
 
 def _attend_args(cache, q, cu, max_new, max_len, scale, out):
+    _no_grad(q)
     tokens, max_new = _step(cache, q, cu, max_new)
     qr = _rows(q, "q", cache)
     heads = qr.heads
@@ -287,8 +295,13 @@ def attention_step(cache: PagedKVCache, q: Tensor, k: Tensor, v: Tensor, *, cu: 
                    interleaved: bool = False, max_len: int | None = None, window: int = 0, sinks: int = 0,
                    scale: float | None = None, out: Tensor | None = None) -> Tensor:
     """The attention part of a decode step, beside ``seams.memory_step``: the lengths count the step's tokens,
-    keys and values are appended, and the rotated queries attend."""
+    keys and values are appended, and the rotated queries attend.  A refused step leaves the lengths as they were."""
     _step(cache, q, cu, max_new)
-    cache.extend(q.shape[1] if cu is None else cu[1:] - cu[:-1])
-    q = kv_append(cache, k, v, q, cu=cu, max_new=max_new, positions=positions, inv_freq=inv_freq, interleaved=interleaved)
-    return kv_attend(cache, q, cu=cu, max_new=max_new, max_len=max_len, window=window, sinks=sinks, scale=scale, out=out)
+    n = q.shape[1] if cu is None else cu[1:] - cu[:-1]
+    cache.extend(n)
+    try:
+        q = kv_append(cache, k, v, q, cu=cu, max_new=max_new, positions=positions, inv_freq=inv_freq, interleaved=interleaved)
+        return kv_attend(cache, q, cu=cu, max_new=max_new, max_len=max_len, window=window, sinks=sinks, scale=scale, out=out)
+    except (ValueError, RuntimeError):
+        cache.extend(-n)
+        raise

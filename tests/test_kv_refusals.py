@@ -134,3 +134,39 @@ def test_c_entries_refuse_before_any_launch(lngram):
                 dict(q=dict(heads=4), qo=dict(heads=4, token_stride=512))):
         assert append(**bad) == _lib.ERR_ARGUMENT, bad
     assert append(tokens=0, max_new=0) == _lib.OK
+
+
+def test_overlapping_table_rows(lngram):
+    # one row expanded over the batch, and rows that overlap: the kernels would walk past the row's end
+    with pytest.raises(ValueError, match="overlap"):
+        make(lngram, table=torch.zeros(1, 2, dtype=torch.int32).expand(2, 2))
+    with pytest.raises(ValueError, match="overlap"):
+        make(lngram, table=torch.zeros(4, dtype=torch.int32).as_strided((2, 3), (1, 1)))
+    make(lngram, batch=1, table=torch.zeros(3, dtype=torch.int32).as_strided((1, 3), (1, 1)), lengths=torch.zeros(1, dtype=torch.int32))
+
+
+def test_no_gradients(lngram):
+    c = make(lngram)
+    bf = dict(dtype=torch.bfloat16)
+    q, k = torch.zeros(2, 3, 4, 64, **bf), torch.zeros(2, 3, 2, 64, **bf)
+    qg, kg = q.clone().requires_grad_(), k.clone().requires_grad_()
+    for call in (lambda: lngram.kv_attend(c, qg), lambda: lngram.kv_append(c, k, kg), lambda: lngram.kv_append(c, k, k, qg),
+                 lambda: lngram.kv_prefix_attend(c, qg, torch.zeros(1, dtype=torch.int32), 3),
+                 lambda: lngram.attention_step(c, q, kg, k)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_refused_step_leaves_lengths(lngram):
+    c = make(lngram)
+    bf = dict(dtype=torch.bfloat16)
+    q, k = torch.zeros(2, 3, 4, 64, **bf), torch.zeros(2, 3, 2, 64, **bf)
+    c.lengths.copy_(torch.tensor([5, 7], dtype=torch.int32))
+    with pytest.raises(ValueError, match="dtype"):
+        lngram.attention_step(c, q, k.half(), k)
+    cu = torch.tensor([0, 1, 6], dtype=torch.int32)
+    with pytest.raises(ValueError, match="dtype"):
+        lngram.attention_step(c, q.view(6, 4, 64), k.view(6, 2, 64), k.view(6, 2, 64).half(), cu=cu, max_new=5)
+    assert c.lengths.tolist() == [5, 7]
