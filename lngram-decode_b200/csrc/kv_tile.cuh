@@ -1,18 +1,26 @@
 // Attention of many rows over the paged cache on the tensor cores: prompts, chunks of prompts, batches of
 // drafts, and a whole batch against the prefix that it shares.
 //
-// A CTA takes two tiles of up to 128 (token, head of the key head's group) rows -- the group's heads share
-// every key they load -- and walks the tiles of 128 keys that any of its tokens sees.  Roles:
-//   warp 8   one thread loads: queries once, then keys and values of each tile by TMA, page by page, into a ring;
-//   warps 0-3, 4-7  a row tile each, one row a thread: the first warp issues tcgen05.mma for S = Q K^T (fp32 in
-//            TMEM), all take S from TMEM, keep the running maximum and sum in fp32 and write P, rounded to the
-//            cache's type, over S's columns; the first thread issues O += P V with P read from TMEM.
-// While one row tile's softmax runs, the tensor cores work on the other's: per 128 x 128 block at head size 128
-// both take about 1024 cycles (2 x 128^3 x 2 flops at 8192 a cycle; 16384 exponentials at 16 a cycle).
-// TMEM: S of both tiles (2 x 128 columns, P in the same ones) and O of both (2 x head size) fill its 512 columns.
+// A unit of work is two tiles of up to 128 (token, head of the key head's group) rows -- the group's heads share
+// every key they load -- against the tiles of 64 keys that any of its tokens sees (or one range of them).  One CTA an
+// SM takes units in turn, so that a unit's loads and first scores start under the one before.  Roles:
+//   warps 0-3, 4-7  a row tile each, one row a thread: S from TMEM, the running maximum and sum in fp32, P, rounded to
+//             the cache's type, over its S's columns;
+//   warps 8, 9      load by TMA, page by page, into a ring: queries and keys, values;
+//   warps 10, 11    issue a row tile's tcgen05.mma: S = Q K^T (fp32 in TMEM) a key tile ahead, O += P V, P from TMEM.
+// TMEM: two S buffers of 64 columns a row tile (P in the same ones) and O of both (2 x head size).
 // O is rescaled only when a row's maximum has grown by more than 2^8 (8 in base 2): the old reference stays
 // valid, weights reach at most 256, exact in fp32 and in range for fp16, and the quotient is the same.
 // Values are the B operand with the head dimension contiguous (MN-major), just as the pages hold them.
+//
+// What bounds it: at head size 64 a row tile's own softmax, about 1500 of the 1700 cycles that a pair of 64-key tiles
+// takes (64 exponentials a thread, with the loads and the maximum before them); at head size 128 what warps 10 and 11
+// do in a row, about 2000 cycles (sixteen products, four commits, four waits of a hundred cycles or more).  Key
+// tiles of 128 with one S buffer were slower (32 prompts of 2048 tokens, 16 query and 4 key heads of 64: 0.63 against
+// 0.55 ms), and so were: scores and products issued by a warp each (0.56 against 0.54 ms; two prompts of 8000
+// tokens and 28 heads of 128: 0.75 against 0.76), sixteen row warps, two groups taking a row tile's key tiles in turn
+// (0.73 and 0.87 ms), and the next scores loaded while the weights are formed (0.63 and 0.92 ms).
+// Measured: 0.54 ms, 511 TFLOP/s, for the former; 0.74 to 0.78 ms, 900 to 950 TFLOP/s, for the latter (window of 4096).
 #pragma once
 
 #include "kv_step.cuh"
@@ -20,9 +28,9 @@
 namespace lng {
 
 constexpr int KT_BM = 128, KT_BK = 64, KT_THREADS = 384;
-#ifndef KT_FMA_EXP
-#define KT_FMA_EXP 0x52  // of 8 pairs of exponentials, those on the fma pipe
-#endif
+// Of eight pairs of exponentials, those on the fma pipe.  None, one, two, three (32 prompts of 2048 tokens, heads of
+// 64): 564, 559, 561, 537 us, and four was slower than three by 16; at heads of 128 they are alike.
+constexpr uint32_t KT_FMA_EXP = 0x52;
 
 template <int HDP>
 struct KtCfg {
@@ -39,7 +47,7 @@ struct KtParams {
   int32_t q_heads, group, tile_tokens;  // tile_tokens = 128 / group
   float scale_log2;
   int32_t window, sinks;
-  int32_t box;              // keys a TMA copy: min(page size, 128)
+  int32_t box;              // keys a TMA copy: min(page size, 64)
   int32_t splits;           // key ranges a unit's tiles are divided into
   int64_t total;            // units
   const int32_t* prefix_table;  // not null: all tokens against the shared prefix, every key visible
@@ -378,9 +386,9 @@ __device__ __forceinline__ void exp2_fma(uint64_t x2, float& a, float& b) {
 }
 
 // Weights of a 32-column piece to TMEM column tp: 2^(s * scale - ref), summed in fp32 and packed to the cache's
-// type (rounded for the matrix unit; the sum keeps the unrounded weights).  Every second pair goes to the fma
-// pipe: the special-function unit alone (16 a cycle and SM) would take as long as the products at head
-// size 128 and twice as long at 64.
+// type (rounded for the matrix unit; the sum keeps the unrounded weights).  Three of eight pairs go to the fma pipe:
+// the special-function unit alone (16 a cycle and SM) would take as long as the products at head size 128 and
+// twice as long at 64.
 template <typename T>
 __device__ __forceinline__ void kt_weights(uint32_t (&s)[32], uint64_t scale2, uint64_t ref2, uint64_t& sum0, uint64_t& sum1,
                                            uint32_t tp) {
@@ -668,83 +676,83 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32
   KtWork w;
 #pragma unroll 1
   while (kt_next(p, walk, w, there)) {
-  if (!there) continue;
-  const int32_t cnt = G ? w.cnt1 : w.cnt0;
-  const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
-  const int32_t pos = w.shared ? last : first + tok;
-  float m = -INFINITY, l = 0.f;
+    if (!there) continue;
+    const int32_t cnt = G ? w.cnt1 : w.cnt0;
+    const int32_t first = G ? w.pos1 : w.pos0, last = G ? w.last1 : w.last0;
+    const int32_t pos = w.shared ? last : first + tok;
+    float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-  for (int32_t i = 0; i < cnt; ++i) {
-    const uint32_t t = tile + i;
-    const int32_t key0 = tile_index(w.tiles, w.j0 + i) * KT_BK;
-    ok = ok && kt_wait<HDP>(bars, B::s_full + 16 * G + 8 * (t & 1), (t >> 1) & 1);
-    if (!all_needed(w.span, key0, key0 + KT_BK)) {
-      // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
-      // tiles clear them, each before its own product)
-      const uint32_t iv = base + 2 * i + 1, sv = iv % NS;
-      if (ok && !key_needed(w.span, key0 + (r & 63))) {
-        const uint32_t v = ring + sv * Cfg::KV_BYTES + (r & 63) * 128 + (r >> 6) * 64;
+    for (int32_t i = 0; i < cnt; ++i) {
+      const uint32_t t = tile + i;
+      const int32_t key0 = tile_index(w.tiles, w.j0 + i) * KT_BK;
+      ok = ok && kt_wait<HDP>(bars, B::s_full + 16 * G + 8 * (t & 1), (t >> 1) & 1);
+      if (!all_needed(w.span, key0, key0 + KT_BK)) {
+        // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
+        // tiles clear them, each before its own product)
+        const uint32_t iv = base + 2 * i + 1, sv = iv % NS;
+        if (ok && !key_needed(w.span, key0 + (r & 63))) {
+          const uint32_t v = ring + sv * Cfg::KV_BYTES + (r & 63) * 128 + (r >> 6) * 64;
 #pragma unroll
-        for (int hh = 0; hh < HDP / 64; ++hh)
+          for (int hh = 0; hh < HDP / 64; ++hh)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sts_zero16(v + hh * Cfg::KV_HALF + x * 16);
+            for (int x = 0; x < 4; ++x) sts_zero16(v + hh * Cfg::KV_HALF + x * 16);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    __syncwarp();
-    tc_fence_after();
-    const uint32_t tb = ts + (t & 1) * KT_BK;
-    uint32_t s0[32], s1[32];
-    tmem_ld32(tb, s0);
-    tmem_ld32(tb + 32, s1);
-    tmem_wait32(s0);
-    tmem_wait32(s1);
-    if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
-      // visible columns of this row: x <= hi and (x > lo or x < sink)
-      const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
-      kt_mask(s0, 0, hi, lo, sink);
-      kt_mask(s1, 32, hi, lo, sink);
-    }
-    const float top = fmaxf(kt_max(s0), kt_max(s1)) * p.scale_log2;
-    const bool grow = top > m + 8.f || (i == 0 && top > m);
-    if (i > 0 && __any_sync(0xffffffffu, grow)) {
-      const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
-      l *= f;
-      ok = ok && kt_wait<HDP>(bars, pv_bar, (t - 1) & 1);  // the product before this one is done with O
       __syncwarp();
       tc_fence_after();
-#pragma unroll 1
-      for (int x = 0; x < HDP; x += 32) {
-        uint32_t o[32];
-        tmem_ld32(to + x, o);
-        tmem_wait32(o);
-#pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-        tmem_store32(to + x, o);
+      const uint32_t tb = ts + (t & 1) * KT_BK;
+      uint32_t s0[32], s1[32];
+      tmem_ld32(tb, s0);
+      tmem_ld32(tb + 32, s1);
+      tmem_wait32(s0);
+      tmem_wait32(s1);
+      if (!all_visible(key0, key0 + KT_BK, first, last, w.window, w.sinks)) {
+        // visible columns of this row: x <= hi and (x > lo or x < sink)
+        const int32_t hi = pos - key0, lo = w.window > 0 ? pos - w.window - key0 : -1, sink = w.sinks - key0;
+        kt_mask(s0, 0, hi, lo, sink);
+        kt_mask(s1, 32, hi, lo, sink);
       }
+      const float top = fmaxf(kt_max(s0), kt_max(s1)) * p.scale_log2;
+      const bool grow = top > m + 8.f || (i == 0 && top > m);
+      if (i > 0 && __any_sync(0xffffffffu, grow)) {
+        const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
+        l *= f;
+        ok = ok && kt_wait<HDP>(bars, pv_bar, (t - 1) & 1);  // the product before this one is done with O
+        __syncwarp();
+        tc_fence_after();
+#pragma unroll 1
+        for (int x = 0; x < HDP; x += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + x, o);
+          tmem_wait32(o);
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+          tmem_store32(to + x, o);
+        }
+      }
+      if (grow) m = top;
+      const float ref = m == -INFINITY ? 0.f : m;
+      const uint64_t ref2 = f2_pack(-ref, -ref);
+      uint64_t sum0 = 0, sum1 = 0;
+      kt_weights<T>(s0, scale2, ref2, sum0, sum1, tb);
+      kt_weights<T>(s1, scale2, ref2, sum0, sum1, tb + 16);
+      float a0, a1, b0, b1;
+      f2_unpack(sum0, a0, a1);
+      f2_unpack(sum1, b0, b1);
+      l += (a0 + a1) + (b0 + b1);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive_at(bars + B::p_full + 16 * G + 8 * (t & 1));
     }
-    if (grow) m = top;
-    const float ref = m == -INFINITY ? 0.f : m;
-    const uint64_t ref2 = f2_pack(-ref, -ref);
-    uint64_t sum0 = 0, sum1 = 0;
-    kt_weights<T>(s0, scale2, ref2, sum0, sum1, tb);
-    kt_weights<T>(s1, scale2, ref2, sum0, sum1, tb + 16);
-    float a0, a1, b0, b1;
-    f2_unpack(sum0, a0, a1);
-    f2_unpack(sum1, b0, b1);
-    l += (a0 + a1) + (b0 + b1);
-    tmem_wait_st();
+    const bool any = cnt > 0;
+    tile += cnt;
+    base += 2 * w.n;
+    if (any) ok = ok && kt_wait<HDP>(bars, B::o_full + 8 * G, results++ & 1);
+    __syncwarp();
+    tc_fence_after();
+    kt_result<T, HDP>(p, w, to, stage, G, quad, any, __all_sync(0xffffffffu, ok), m, l);
     tc_fence_before();
-    mbar_arrive_at(bars + B::p_full + 16 * G + 8 * (t & 1));
-  }
-  const bool any = cnt > 0;
-  tile += cnt;
-  base += 2 * w.n;
-  if (any) ok = ok && kt_wait<HDP>(bars, B::o_full + 8 * G, results++ & 1);
-  __syncwarp();
-  tc_fence_after();
-  kt_result<T, HDP>(p, w, to, stage, G, quad, any, __all_sync(0xffffffffu, ok), m, l);
-  tc_fence_before();
   }
 }
 

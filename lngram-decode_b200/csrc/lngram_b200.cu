@@ -1784,7 +1784,7 @@ static int kv_splits(int64_t units, int64_t tiles) {
 
 // How an attention call is carried out, and what it needs of the workspace.
 struct KvPlan {
-  bool step;          // the sequences' own keys by kv_step_kernel (at most 16 rows a key head), else by kv_tile_kernel
+  bool step;          // the sequences' own keys by kv_step_kernel (few rows a key head), else by kv_tile_kernel
   int shares;         // into which its work is cut
   bool warp_shares;   // a share a warp, not a CTA
   int64_t units;      // CTAs of the tile kernel per key head and range
@@ -1801,10 +1801,16 @@ static KvPlan kv_plan(const lng_kv_cache* c, int64_t prefix_len, int64_t tokens,
   int64_t keys = c->max_pages * c->page_size;
   if (max_len > 0) keys = std::min(keys, max_len);
   if (window > 0) keys = std::min(keys, int64_t(window) + sinks + span + KT_BK);
-  p.step = group * max_new <= KS_ROWS;
+  // up to 16 rows a key head: the step kernel, a third faster where there is much to read (64 sequences of 2000 keys, 8
+  // key heads of 128: 99 against 146 us with 4 rows, 104 against 148 with 16) -- but not more than four rows of so few
+  // pairs that each falls into more than 16 pieces, whose join then counts more (one sequence of 4000 keys, 4 key heads
+  // of 64, 16 rows: 37 us against 17 by the tile kernel; with 4 rows 19 against 17, four sequences of 16 rows 22
+  // against 21)
+  p.step = group * max_new <= KS_ROWS && (group * max_new <= 4 || c->batch * c->num_kv_heads * 16 >= num_sms());
   if (p.step) {
     // many pairs: a share a warp, so that pairs end without the CTA's warps meeting (64 sequences of 300 keys, 8 key
-    // heads: 37 -> 31 us; 64 of 2000 keys: 107 -> 98); few pairs: a share a CTA, which leaves an eighth or a quarter of the pieces to join
+    // heads: 31 us against 37; 64 of 500 to 16000: 358 against 389); few pairs: a share a CTA, which leaves an
+    // eighth or a quarter of the pieces to join (one sequence of 4096 keys, 4 key heads: 16 us against 35)
     p.warp_shares = c->batch * c->num_kv_heads >= num_sms();
     p.shares = num_sms() * (p.warp_shares ? (c->head_dim > 64 ? KsCfg<128>::WARPS : KsCfg<64>::WARPS) : 1);
   } else {

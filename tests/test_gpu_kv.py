@@ -516,3 +516,15 @@ def test_nan_queries_stay_nan_and_alone(lngram, n):
         assert torch.isnan(b[1, n // 2, 3]).all()
         b[1, n // 2, 3] = a[1, n // 2, 3]
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch, n, heads", [(1, 1, 8), (1, 4, 8), (1, 3, 10), (4, 2, 16), (5, 2, 16), (5, 1, 32), (80, 1, 14), (80, 4, 8)])
+def test_few_rows_of_few_and_many_pairs(lngram, batch, n, heads, dim):
+    """Up to 16 rows for each of 2 key heads, over both sides of every choice of kernel and share."""
+    ctx = [(i * 389) % 700 for i in range(batch)] if batch > 1 else [2500]
+    s = Setup(lngram, ctx, [n] * batch, heads, 2, dim, 16, "bf16", seed=batch + n).fill()
+    q = s.normal(*s.lead, heads, dim)
+    check_attend(lngram.kv_attend(s.cache, q, **s.kw()), *s.want(q))
+    check_attend(lngram.kv_attend(s.cache, q, window=90, sinks=5, **s.kw()), *s.want(q, 90, 5))
+    assert lngram._lib.device_error() == 0
