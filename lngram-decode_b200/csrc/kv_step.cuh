@@ -15,7 +15,7 @@
 // joins the pieces in order.  A share has at most two pieces (its first and its last pair).
 //
 // Measured (one token a sequence): 64 sequences of 500 to 16000 keys, 32 query and 8 key heads of 128 (2.24 GB of
-// keys and values): 0.36 ms, 6.3 TB/s; 24 sequences, window of 4096 and pages of 16: 91 us, 4.4 TB/s; 64 sequences
+// keys and values): 0.34 ms, 6.5 TB/s; 24 sequences, window of 4096 and pages of 16: 79 us, 5.1 TB/s; 64 sequences
 // of 300 keys: 31 us, 2.6 TB/s (a pair's start and end, not its keys); one sequence of 4096 keys, 4 heads of 64: 16 us.
 #pragma once
 
@@ -159,6 +159,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// One lane of the (converged) warp.  Copies and products are issued by whole warps with uniform operands and one
+// elected lane: operands that the compiler cannot see to be uniform cost a hundred cycles each.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok)::"memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -291,18 +298,27 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     uint8_t* dk = ring + s * Cfg::STAGE_BYTES;
     uint8_t* dv = dk + Cfg::KV_BYTES;
     const int32_t slot0 = (tile_index(ld.tiles, ld_k) * BK) & ((1 << c.page_shift) - 1);
-    if (lane == 0) mbar_arrive_expect_tx(&bar[s], uint32_t(__popc(there)) * uint32_t(p.box) * 128 * (HDP / 64) * 2);
-    for (int r = 0; r < boxes; ++r) {
-      const int32_t page = __shfl_sync(0xffffffffu, pages, seen * boxes + r);
-      if (page < 0 || lane != 0) continue;
-      const int32_t slot = (slot0 + r * p.box) & ((1 << c.page_shift) - 1);
-#pragma unroll
-      for (int hh = 0; hh < HDP / 64; ++hh) {
-        tma_load_4d(dk + hh * Cfg::HALF_BYTES + r * p.box * 128, &tmk, hh * 64, slot, ld.h, page, &bar[s]);
-        tma_load_4d(dv + hh * Cfg::HALF_BYTES + r * p.box * 128, &tmv, hh * 64, slot, ld.h, page, &bar[s]);
-      }
-    }
+    if (elect_lane()) mbar_arrive_expect_tx(&bar[s], uint32_t(__popc(there)) * uint32_t(p.box) * 128 * (HDP / 64) * 2);
     __syncwarp();
+#pragma unroll 1
+    for (int r = 0; r < boxes; r += 2) {  // (two pieces, or the only one, without anything between)
+      int32_t pg[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) pg[x] = __shfl_sync(0xffffffffu, pages, (seen * boxes + r + x) & 31);
+      if (elect_lane()) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (r + x < boxes && pg[x] >= 0) {
+            const int32_t slot = (slot0 + (r + x) * p.box) & ((1 << c.page_shift) - 1);
+#pragma unroll
+            for (int hh = 0; hh < HDP / 64; ++hh) {
+              tma_load_4d(dk + hh * Cfg::HALF_BYTES + (r + x) * p.box * 128, &tmk, hh * 64, slot, ld.h, pg[x], &bar[s]);
+              tma_load_4d(dv + hh * Cfg::HALF_BYTES + (r + x) * p.box * 128, &tmv, hh * 64, slot, ld.h, pg[x], &bar[s]);
+            }
+          }
+      }
+      __syncwarp();
+    }
     ++issued;
     ++seen;
     ld_k += STRIDE;

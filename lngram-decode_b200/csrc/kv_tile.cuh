@@ -255,13 +255,6 @@ struct KtBars {
   // one or the next: every role waits for the phases of its barriers one after the other.
 };
 
-// One lane of the (converged) warp.  Products are issued by whole warps with uniform operands and one elected
-// lane: operands that the compiler cannot see to be uniform cost a hundred cycles a product.
-__device__ __forceinline__ bool elect_lane() {
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok)::"memory");
-  return ok != 0;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");

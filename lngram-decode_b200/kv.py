@@ -180,7 +180,8 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     ``lengths - n + i`` (``extend`` first).  With ``inv_freq`` (fp32 ``[rotary_dim / 2]``) the first rotary_dim
     values of keys and queries are rotated by the token's position -- ``positions`` (int64, the step's leading
     shape) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
-    Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``.  No gradients."""
+    Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``.  Pages that several
+    sequences name are for reading: no two tokens of a step may go to one slot.  No gradients."""
     _no_grad(k, v, q)
     tokens, max_new = _step(cache, k, cu, max_new)
     lead = k.shape[:-2]
@@ -190,7 +191,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     if q is not None:
         qr = C.byref(_rows(q, "q", cache, lead))
         if q_out is None:
-            q_out = q.new_empty(q.shape)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qo = C.byref(_rows(q_out, "q_out", cache, lead, q.shape[-2]))
     elif q_out is not None:
         raise ValueError("q_out without q")
@@ -220,7 +221,7 @@ def _attend_args(cache, q, cu, max_new, max_len, scale, out):
     if heads % cache.num_kv_heads or not 1 <= heads // cache.num_kv_heads <= 128:
         raise ValueError("query heads must be a multiple of the key heads, at most 128 a key head")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     orow = _rows(out, "out", cache, q.shape[:-2], heads)
     if tokens and orow.ptr == qr.ptr:
         raise ValueError("out must not overlap q")
