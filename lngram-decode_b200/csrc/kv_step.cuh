@@ -15,7 +15,7 @@
 // joins the pieces in order.  A share has at most two pieces (its first and its last pair).
 //
 // Measured (one token a sequence): 64 sequences of 500 to 16000 keys, 32 query and 8 key heads of 128 (2.24 GB of
-// keys and values): 0.34 ms, 6.5 TB/s; 24 sequences, window of 4096 and pages of 16: 79 us, 5.1 TB/s; 64 sequences
+// keys and values): 0.34 ms, 6.5 TB/s (0.37 with a cold L2); 24 sequences, window of 4096 and pages of 16: 79 us, 5.1 TB/s; 64 sequences
 // of 300 keys: 31 us, 2.6 TB/s (a pair's start and end, not its keys); one sequence of 4096 keys, 4 heads of 64: 16 us.
 #pragma once
 
