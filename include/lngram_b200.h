@@ -454,9 +454,11 @@ int lng_online_counts_mix(const int64_t* codes, int64_t T, int64_t R, const int3
  * sequence b lives in page table[b * table_stride + j / page_size], slot j % page_size.  lengths[b] counts
  * the keys of sequence b INCLUDING the step's new tokens: a step first raises lengths, then appends, then
  * attends.  table and lengths are device memory and are read when the kernels run, so a captured graph
- * replays with their current values.  Page numbers outside [0, num_pages) of needed keys, lengths outside
- * [0, max_pages * page_size] and bad row offsets record device error 4; such keys read as zeros and are not
- * written.  dtype LNG_BF16 or LNG_F16; k, v 16-byte aligned, strides multiples of 8 elements; head_dim a
+ * replays with their current values.  Page numbers outside [0, num_pages) of needed keys record device
+ * error 4; such keys read as zeros and are not written.  Lengths outside [0, max_pages * page_size] and bad row
+ * offsets record it too: every token keeps the key index that its sequence's given length and count say, and is
+ * written only where that lies in the sequence's pages; attention sees no keys of a sequence with such a length (zeros,
+ * or the shared prefix alone); of more than max_new rows a sequence the first max_new are taken.  dtype LNG_BF16 or LNG_F16; k, v 16-byte aligned, strides multiples of 8 elements; head_dim a
  * multiple of 8 up to 128; page_size a power of two in [8, 4096]; max_pages * page_size < 2^30. */
 typedef struct {
   void* k;

@@ -13,39 +13,43 @@
 
 namespace lng {
 
-// The new tokens of sequence b: rows [first, first + n) of the step's tokens, at positions
-// len - n .. len - 1 of the sequence, which then holds `len` keys.
+// The new tokens of sequence b: rows [first, first + n) of the step's tokens, at positions pos .. pos + n - 1 of the
+// sequence (its length less its count of tokens, both as given).  `len` is what attention reads: the keys up to the
+// last of these rows, so that pos == len - n, or 0 -- no keys -- when the length is out of range.
 struct SeqSpan {
-  int64_t first;
+  int64_t first, pos;
   int32_t n, len;
-  int32_t bad;  // the offsets or the length were out of range (and have been cut to it)
+  int32_t bad;  // the offsets or the length were out of range
 };
 
 // cu (offsets [batch + 1] into `tokens` rows) may be null: every sequence then adds max_new tokens.
-// Values out of range give an empty or a shorter span, never one outside the caller's rows or table.
+// Offsets out of range give an empty or a shorter span, never one outside the caller's rows, and leave every token
+// that is kept at its own position; what a length out of range does is said above.
 LNG_HD SeqSpan seq_span(const int32_t* cu, const int32_t* lengths, int64_t b, int64_t tokens, int32_t max_new,
                         int32_t capacity) {
   SeqSpan s;
-  s.bad = 0;
-  int32_t len = lengths[b];
-  if (len < 0 || len > capacity) {
-    s.bad = 1;
-    len = len < 0 ? 0 : capacity;
-  }
-  s.len = len;
+  const int32_t len = lengths[b];
+  s.bad = len < 0 || len > capacity;
+  s.len = s.bad ? 0 : len;
   if (cu == nullptr) {
     s.first = b * int64_t(max_new);
     s.n = max_new;
+    s.pos = int64_t(len) - max_new;
     return s;
   }
-  int64_t first = cu[b], end = cu[b + 1];
+  const int64_t begin = cu[b], stop = cu[b + 1];
+  int64_t first = begin, end = stop;
+  s.pos = int64_t(len) - (end - first);
   if (first < 0 || end < first || end > tokens || end - first > max_new) {
-    s.bad = 1;
     if (first < 0) first = 0;
     if (first > tokens) first = tokens;
     if (end > tokens) end = tokens;
     if (end < first) end = first;
     if (end - first > max_new) end = first + max_new;
+    s.pos += first - begin;
+    const int64_t keys = s.pos + (end - first);
+    s.len = s.bad || keys < 0 ? 0 : keys < capacity ? int32_t(keys) : capacity;
+    s.bad = 1;
   }
   s.first = first;
   s.n = int32_t(end - first);

@@ -95,13 +95,15 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 24) kv_append_kernel(const KaPa
   const SeqSpan s = kv_span(c, b);
   const int64_t i = token - s.first;
   if (i < 0 || i >= s.n) return;
-  const int32_t key = s.len - s.n + int32_t(i);
+  // a key outside the sequence's pages (a step past the capacity, say) goes nowhere: every slot there belongs to another
+  const int64_t place = s.pos + i;
+  const int32_t key = place >= 0 && place < c.capacity ? int32_t(place) : -1;
   const int32_t page = key >= 0 ? page_of(c.table + b * c.table_stride, key, c.page_shift, c.num_pages) : -1;
   if (page < 0) kv_range_error();
   const int32_t slot = key & ((1 << c.page_shift) - 1);
   const int half = p.rotary >> 1;
   if (half > 0) {
-    const double pos = p.positions ? double(p.positions[token]) : double(key);
+    const double pos = p.positions ? double(p.positions[token]) : double(place);
     for (int j = lane; j < half; j += 32) {
       const double turns = pos * double(p.inv_freq[j]) * 0.15915494309189533577;  // 1 / (2 pi)
       float sn, cn;

@@ -96,7 +96,9 @@ class PagedKVCache:
                    torch.zeros(batch, dtype=torch.int32, device=device))
 
     def extend(self, n) -> None:
-        """Count n (an int, or int32 [B] on the device) new tokens a sequence."""
+        """Count n (an int, or int32 [B] on the device) new tokens a sequence.  The lengths are on the device and not
+        looked at here: past ``capacity`` ``kv_append`` drops the tokens that do not fit, attention gives zeros for the
+        sequence, and device error 4 is recorded (``lng_device_error``)."""
         self._lengths.add_(n)
 
     def truncate(self, lengths) -> None:
