@@ -805,17 +805,35 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
   }
 }
 
-// out = the joined states of all slots, a warp a row; rows that belong to no sequence are left alone.
+// The sequence whose rows hold `token`, found by a whole warp, which leaves a 32nd of them after each round of
+// loads.  (Offsets that do not ascend give some sequence of the batch.)
+__device__ __forceinline__ int64_t kt_sequence_of(const KvView& c, int64_t token, int lane) {
+  int64_t lo = 0, hi = c.batch;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+    const int found = __popc(__ballot_sync(0xffffffffu, at < hi && c.cu[at] <= token));
+    lo += found * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  return lo;
+}
+
+// out = the joined states of all slots, a warp a row; rows that belong to no sequence (they have no states, or only
+// the prefix's) are left alone.
 template <typename T>
 __global__ void __launch_bounds__(256)
-    kv_rows_join_kernel(const int32_t* __restrict__ cu, int64_t batch, int64_t tokens, int32_t q_heads, int32_t head_dim,
-                        const float2* __restrict__ row_ml, const float* __restrict__ row_o, int32_t slots, KvRows out) {
-  const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31, col = lane * 4;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= tokens * q_heads) return;
+    kv_rows_join_kernel(const KvView c, int32_t q_heads, const float2* __restrict__ row_ml, const float* __restrict__ row_o,
+                        int32_t slots, KvRows out) {
+  const int64_t row = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5, tokens = c.tokens;
+  const int lane = threadIdx.x & 31, col = lane * 4, head_dim = c.head_dim;
   const int64_t token = row / q_heads;
-  if (cu != nullptr && (token < cu[0] || token >= cu[batch])) return;
+  bool mine = token < tokens;
+  if (c.cu != nullptr && mine) {
+    const SeqSpan s = kv_span(c, kt_sequence_of(c, token, lane));
+    mine = token >= s.first && token < s.first + s.n;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
   const int64_t slot_rows = tokens * q_heads;
   const KsRow x = ks_join_states(
       0, 1, slots, lane, col < head_dim, [&](int i) { return row_ml + i * slot_rows + row; },

@@ -1955,9 +1955,8 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
       if ((st = launch(plan.units))) return st;
       if (plan.slots == 0) return LNG_OK;
       auto join = bf16 ? kv_rows_join_kernel<__nv_bfloat16> : kv_rows_join_kernel<__half>;
-      return launch_dependent(join, unsigned(ceil_div(tokens * q->heads, 8)), 256u, size_t(0), cs, cu, cache->batch, tokens, q->heads,
-                              cache->head_dim, static_cast<const float2*>(row_ml), static_cast<const float*>(row_o), plan.slots,
-                              kv_rows(out));
+      return launch_dependent(join, unsigned(ceil_div(tokens * q->heads, 8)), 256u, size_t(0), cs, v, q->heads,
+                              static_cast<const float2*>(row_ml), static_cast<const float*>(row_o), plan.slots, kv_rows(out));
     }
   }
   KsParams p{};

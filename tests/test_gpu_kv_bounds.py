@@ -97,3 +97,25 @@ def test_a_loop_that_runs_too_long_leaves_the_cache_whole(lngram):
     assert torch.equal(cache.k[cache.table[0, j // 16].long(), :, j % 16], x[1, 0, :32])
     assert all((o == 0).all() for o in outs[32:]) and not any((o == 0).all() for o in outs[:32])
     assert math.isfinite(outs[31].float().sum().item())
+
+
+@pytest.mark.parametrize("take", [1, 4, 40])
+@pytest.mark.parametrize("ctx", [[15, 9, 30], [700, 0, 1500]])
+@pytest.mark.parametrize("batch", [3, 99])
+def test_rows_past_max_new_stay_as_they_are(lngram, take, ctx, batch):
+    """They belong to no sequence: neither written from states that nothing has made nor from the prefix's alone."""
+    new, ctx = [take + 1, take, take + 5] * (batch // 3), ctx * (batch // 3)
+    s = Setup(lngram, ctx, new, 4, 2, 64, 16, uniform=False, prefix=90, gap=2).fill()
+    q = s.normal(*s.lead, 4, 64)
+    at = torch.cat([torch.arange(n, device="cuda") for n in new] + [torch.full((2,), take, device="cuda")])
+    kept = at < take
+    prefix, out = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    torch.full((64 << 20,), math.nan, device="cuda")  # what a workspace made next finds in its memory
+    lngram.kv_attend(s.cache, q, cu=s.cu, max_new=take, out=out)
+    lngram.kv_prefix_attend(s.cache, q, s.prefix_table, 90, cu=s.cu, max_new=take, out=prefix)
+    assert lngram._lib.device_error() == 4
+    assert (out[~kept] == 7).all() and (prefix[~kept] == 7).all()
+    for got, n in ((prefix, 90), (out, 0)):
+        s.prefix = n
+        want, tol = s.want(q[:s.tokens])
+        check_attend(got[kept], want[kept[:s.tokens]], tol[kept[:s.tokens]])
