@@ -501,8 +501,9 @@ int lng_kv_append(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, 
  * sequence sees keys j <= p, with window > 0 only j > p - window or j < sinks; out = softmax(scale q . k) v
  * with fp32 scores and sums (weights rounded to the cache's dtype for the product with v); 0 where a
  * token sees no key.  Query head h reads key head h / (q.heads / num_kv_heads); at most 128 query heads a key
- * head.  Pages that hold no visible key are not touched (their table entries may be stale).  Visible
- * keys and values must be finite.  max_len: an upper bound of lengths that only guides how the work is split
+ * head.  Pages that hold no visible key are not touched (their table entries may be stale).  Scores
+ * of NaN or +inf make their row NaN, and no other.  Values that any of the step's tokens sees must be finite (a weight
+ * of zero times NaN is NaN, for the tokens before it too).  max_len: an upper bound of lengths that only guides how the work is split
  * (0 = max_pages * page_size).  q and out must not overlap.  workspace: 256-byte aligned,
  * lng_kv_attend_workspace_bytes bytes, used by this call alone until it has finished. */
 size_t lng_kv_attend_workspace_bytes(const lng_kv_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,

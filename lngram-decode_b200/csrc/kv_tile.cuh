@@ -347,19 +347,25 @@ __device__ __forceinline__ void kt_mask(uint32_t (&s)[32], int32_t base, int32_t
       if (base + x <= lo && base + x >= sink) s[x] = 0xff800000u;
   }
 }
+// The larger value, or NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float kt_max(const uint32_t (&s)[32]) {
   float m0 = __uint_as_float(s[0]), m1 = __uint_as_float(s[1]);
 #pragma unroll
   for (int x = 2; x < 30; x += 4) {
-    m0 = fmaxf(fmaxf(m0, __uint_as_float(s[x])), __uint_as_float(s[x + 1]));
-    m1 = fmaxf(fmaxf(m1, __uint_as_float(s[x + 2])), __uint_as_float(s[x + 3]));
+    m0 = max_nan(max_nan(m0, __uint_as_float(s[x])), __uint_as_float(s[x + 1]));
+    m1 = max_nan(max_nan(m1, __uint_as_float(s[x + 2])), __uint_as_float(s[x + 3]));
   }
-  return fmaxf(fmaxf(fmaxf(m0, __uint_as_float(s[30])), __uint_as_float(s[31])), m1);
+  return max_nan(max_nan(max_nan(m0, __uint_as_float(s[30])), __uint_as_float(s[31])), m1);
 }
 // 2^x of a pair on the fma pipe: x = n + f with n the nearest integer (by adding 1.5 * 2^23, whose last place is
 // 1) and |f| <= 1/2, 2^f by a polynomial of degree 4 (least-squares fit of the relative error, reweighted towards
 // its peaks: at most 2.7e-6 = 2^-18.5 off), n added to the exponent.  x <= 8 here; below -126, and for the -inf
-// of a masked key, the result is 2^-126.
+// of a masked key, the result is 2^-126.  NaN gives 2^-126 too: it is the row's maximum that carries a NaN score.
 __device__ __forceinline__ void exp2_fma(uint64_t x2, float& a, float& b) {
   float x0, x1;
   f2_unpack(x2, x0, x1);
@@ -588,7 +594,7 @@ __device__ __forceinline__ void kt_result(const KtParams& p, const KtWork& w, ui
   const int32_t tokens = ok ? (G ? w.tokens1 : w.tokens0) : 0, rows = tokens * p.group;
   const int64_t token0 = w.s.first + w.t0 + G * p.tile_tokens;
   const bool state = p.row_ml != nullptr;
-  // no key seen: zeros (weights of masked keys are 2^-126, not 0); scores that are NaN leave m alone and make l NaN
+  // no key seen: zeros (weights of masked keys are 2^-126, not 0); a row with a NaN score has l NaN
   const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
   auto row_of = [&](int r, int64_t& token, int32_t& head) {
     const int32_t tok = r / p.group;
@@ -706,7 +712,8 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32
         kt_mask(s0, 0, hi, lo, sink);
         kt_mask(s1, 32, hi, lo, sink);
       }
-      const float top = fmaxf(kt_max(s0), kt_max(s1)) * p.scale_log2;
+      // (NaN when one of the row's scores is: it is never a new reference, and makes the sum NaN below)
+      const float top = max_nan(kt_max(s0), kt_max(s1)) * p.scale_log2;
       const bool grow = top > m + 8.f || (i == 0 && top > m);
       if (i > 0 && __any_sync(0xffffffffu, grow)) {
         const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
@@ -734,6 +741,8 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32
       f2_unpack(sum0, a0, a1);
       f2_unpack(sum1, b0, b1);
       l += (a0 + a1) + (b0 + b1);
+      // a NaN score, and one of +inf (inf - inf), makes the row NaN whichever pipe its own weight went through
+      if (!(top < INFINITY)) l = NAN;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive_at(bars + B::p_full + 16 * G + 8 * (t & 1));

@@ -252,7 +252,8 @@ def kv_attend(cache: PagedKVCache, q: Tensor, *, cu: Tensor | None = None, max_n
     """Causal attention of a step's tokens over the cache, whose lengths count them (``kv_append`` first): the
     token at position p sees keys j <= p; with ``window`` > 0 only its last ``window`` keys and the first
     ``sinks`` of the sequence.  softmax(scale q . k) v with ``scale`` = head_dim^-1/2 by default; a token
-    that sees no key gets zeros.  ``max_len`` (a host bound of the lengths) only guides how the work is split.
+    that sees no key gets zeros, one with a score of NaN or +inf NaN.  Values that any token of the step sees must be
+    finite.  ``max_len`` (a host bound of the lengths) only guides how the work is split.
     Rows of ``q`` that belong to no sequence are skipped: their rows of ``out`` stay as they are.  No gradients."""
     tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
     window, sinks = int(window), int(sinks)
