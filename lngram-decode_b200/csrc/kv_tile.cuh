@@ -23,6 +23,7 @@
 // Measured: 0.54 ms, 511 TFLOP/s, for the former; 0.74 to 0.78 ms, 900 to 950 TFLOP/s, for the latter (window of 4096).
 #pragma once
 
+#include "exp2_poly.cuh"
 #include "kv_step.cuh"
 
 namespace lng {
@@ -362,21 +363,18 @@ __device__ __forceinline__ float kt_max(const uint32_t (&s)[32]) {
   }
   return max_nan(max_nan(max_nan(m0, __uint_as_float(s[30])), __uint_as_float(s[31])), m1);
 }
-// 2^x of a pair on the fma pipe: x = n + f with n the nearest integer (by adding 1.5 * 2^23, whose last place is
-// 1) and |f| <= 1/2, 2^f by a polynomial of degree 4 (least-squares fit of the relative error, reweighted towards
-// its peaks: at most 2.7e-6 = 2^-18.5 off), n added to the exponent.  x <= 8 here; below -126, and for the -inf
-// of a masked key, the result is 2^-126.  NaN gives 2^-126 too: it is the row's maximum that carries a NaN score.
+// 2^x of a pair on the fma pipe (exp2_poly.cuh has the steps).  x <= 8 here; below -126, and for the -inf of a masked
+// key, the result is 2^-126.  NaN gives 2^-126 too: it is the row's maximum that carries a NaN score.
 __device__ __forceinline__ void exp2_fma(uint64_t x2, float& a, float& b) {
   float x0, x1;
   f2_unpack(x2, x0, x1);
-  x2 = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const float big = 12582912.f;
-  const uint64_t t2 = f2_add(x2, f2_pack(big, big));
-  const uint64_t f2 = f2_fma(f2_add(t2, f2_pack(-big, -big)), f2_pack(-1.f, -1.f), x2);
-  uint64_t r2 = f2_fma(f2, f2_pack(0.009570100344717503f, 0.009570100344717503f), f2_pack(0.05591785907745361f, 0.05591785907745361f));
-  r2 = f2_fma(r2, f2, f2_pack(0.240247443318367f, 0.240247443318367f));
-  r2 = f2_fma(r2, f2, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-  r2 = f2_fma(r2, f2, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+  x2 = f2_pack(fmaxf(x0, EXP2_LOW), fmaxf(x1, EXP2_LOW));
+  const uint64_t t2 = f2_add(x2, f2_pack(EXP2_ROUND, EXP2_ROUND));
+  const uint64_t f2 = f2_fma(f2_add(t2, f2_pack(-EXP2_ROUND, -EXP2_ROUND)), f2_pack(-1.f, -1.f), x2);
+  uint64_t r2 = f2_fma(f2, f2_pack(EXP2_C4, EXP2_C4), f2_pack(EXP2_C3, EXP2_C3));
+  r2 = f2_fma(r2, f2, f2_pack(EXP2_C2, EXP2_C2));
+  r2 = f2_fma(r2, f2, f2_pack(EXP2_C1, EXP2_C1));
+  r2 = f2_fma(r2, f2, f2_pack(EXP2_C0, EXP2_C0));
   float t0, t1;
   f2_unpack(t2, t0, t1);
   f2_unpack(r2, a, b);
