@@ -1895,7 +1895,8 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   if (st) return st;
   LNG_REQUIRE(max_len >= 0, "max_len must not be negative");
   LNG_REQUIRE(window >= 0 && sinks >= 0, "window and sinks must not be negative");
-  LNG_REQUIRE(scale > 0.f && scale <= 3.0e38f, "scale must be positive and finite");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  LNG_REQUIRE(scale > 0.f && std::isfinite(scale_log2), "scale must be positive, and scale * log2(e) finite");
   LNG_REQUIRE(prefix_len >= 0 && prefix_len < (int64_t(1) << 30), "prefix_len must be in [0, 2^30)");
   if (tokens == 0 || cache->batch == 0) return LNG_OK;
   LNG_REQUIRE(prefix_len == 0 || prefix_table != nullptr, "prefix_table is NULL");
@@ -1915,7 +1916,6 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   const cudaStream_t cs = S(stream);
   const bool bf16 = cache->dtype == LNG_BF16, wide = cache->head_dim > 64;
   const int group = q->heads / cache->num_kv_heads, tile_tokens = KT_BM / group;
-  const float scale_log2 = scale * 1.4426950408889634f;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float2* row_ml = plan.slots ? reinterpret_cast<float2*>(ws + plan.row_ml) : nullptr;
   float* row_o = plan.slots ? reinterpret_cast<float*>(ws + plan.row_o) : nullptr;

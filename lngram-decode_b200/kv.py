@@ -231,8 +231,8 @@ def _attend_args(cache, q, cu, max_new, max_len, scale, out):
     if max_len < 0:
         raise ValueError("max_len must not be negative")
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError("scale must be positive and finite")
+    if not 0.0 < scale < 2.35e38:  # (scores are kept in base 2: scale * log2(e) must be finite in fp32)
+        raise ValueError("scale must be positive and below 2.35e38")
     return tokens, max_new, max_len, qr, heads, scale, out, orow
 
 

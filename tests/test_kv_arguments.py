@@ -1,0 +1,35 @@
+"""Arguments of the paged cache's calls at the edges of what they take, without a GPU."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+from tests.test_kv_refusals import make
+
+BF = dict(dtype=torch.bfloat16)
+
+
+def test_scales_whose_base_2_form_overflows(lngram):
+    """Scores are kept in base 2: scale * log2(e) has to be finite in fp32, 2.35e38 at most for the scale."""
+    c, q = make(lngram), torch.zeros(2, 3, 4, 64, **BF)
+    for scale in (2.4e38, 2.9e38, 3.3e38, 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            lngram.kv_attend(c, q, scale=scale)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        lngram.kv_attend(c, q, scale=2.3e38)
+    _lib = lngram._lib
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built")
+    lib = _lib.library(require_device=False)
+    cache = _lib.KvCache(k=4096, v=8192, dtype=_lib.BF16, page_size=16, num_pages=4, num_kv_heads=2, head_dim=64,
+                         k_page_stride=2048, k_head_stride=1024, k_slot_stride=64, v_page_stride=2048, v_head_stride=1024,
+                         v_slot_stride=64, table=256, table_stride=2, max_pages=2, lengths=512, batch=2)
+    rows = [_lib.KvRows(ptr=1 << p, token_stride=256, head_stride=64, heads=4) for p in (20, 21)]
+    # (addresses that are never read: the scale is judged before anything is launched)
+    for scale in (2.4e38, 2.9e38):
+        assert lib.lng_kv_attend(C.byref(cache), None, 6, 3, 0, C.byref(rows[0]), scale, 0, 0, C.byref(rows[1]), None, 0,
+                                 None) == _lib.ERR_ARGUMENT
+        assert b"scale" in lib.lng_last_error()
