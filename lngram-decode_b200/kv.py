@@ -306,6 +306,6 @@ def attention_step(cache: PagedKVCache, q: Tensor, k: Tensor, v: Tensor, *, cu: 
     try:
         q = kv_append(cache, k, v, q, cu=cu, max_new=max_new, positions=positions, inv_freq=inv_freq, interleaved=interleaved)
         return kv_attend(cache, q, cu=cu, max_new=max_new, max_len=max_len, window=window, sinks=sinks, scale=scale, out=out)
-    except (ValueError, RuntimeError):
+    except BaseException:
         cache.extend(-n)
         raise

@@ -33,3 +33,19 @@ def test_scales_whose_base_2_form_overflows(lngram):
         assert lib.lng_kv_attend(C.byref(cache), None, 6, 3, 0, C.byref(rows[0]), scale, 0, 0, C.byref(rows[1]), None, 0,
                                  None) == _lib.ERR_ARGUMENT
         assert b"scale" in lib.lng_last_error()
+
+
+@pytest.mark.parametrize("kw, error", [(dict(window=None), TypeError), (dict(sinks="x"), ValueError), (dict(scale=[]), TypeError),
+                                       (dict(max_len=float("inf")), OverflowError), (dict(out=3), AttributeError)])
+def test_a_step_refused_after_the_append_leaves_lengths(lngram, monkeypatch, kw, error):
+    """Whatever ends the step behind ``extend``; the append is a stand-in that takes everything."""
+    import sys
+    monkeypatch.setattr(sys.modules[lngram.kv_append.__module__], "kv_append", lambda cache, k, v, q, **_: q)
+    c, q, k = make(lngram), torch.zeros(2, 3, 4, 64, **BF), torch.zeros(2, 3, 2, 64, **BF)
+    c.lengths.copy_(torch.tensor([5, 7], dtype=torch.int32))
+    with pytest.raises(error):
+        lngram.attention_step(c, q, k, k, **kw)
+    cu = torch.tensor([0, 1, 6], dtype=torch.int32)
+    with pytest.raises(error):
+        lngram.attention_step(c, q.view(6, 4, 64), k.view(6, 2, 64), k.view(6, 2, 64), cu=cu, max_new=5, **kw)
+    assert c.lengths.tolist() == [5, 7]
