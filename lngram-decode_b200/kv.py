@@ -29,6 +29,7 @@ import ctypes as C
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr, stream_ptr
@@ -164,9 +165,13 @@ def _step(cache: PagedKVCache, t: Tensor, cu: Tensor | None, max_new: int | None
     return ts[0], int(max_new)
 
 
-def _no_grad(*tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(cache: PagedKVCache, *tensors: Tensor | None) -> None:
+    if torch.is_grad_enabled() and (cache._k.requires_grad or cache._v.requires_grad
+                                    or any(t is not None and t.requires_grad for t in tensors)):
         raise RuntimeError("the paged cache's operators have no backward: call them under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (cache._k, cache._v) + tensors):
+        raise RuntimeError("the paged cache's operators carry no tangent: give them the primal values")
 
 
 def _library(cache: PagedKVCache):
@@ -184,7 +189,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     shape) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
     Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``.  Pages that several
     sequences name are for reading: no two tokens of a step may go to one slot.  No gradients."""
-    _no_grad(k, v, q)
+    _no_grad(cache, k, v, q, inv_freq, q_out)
     tokens, max_new = _step(cache, k, cu, max_new)
     lead = k.shape[:-2]
     kr = _rows(k, "k", cache, lead, cache.num_kv_heads)
@@ -216,7 +221,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
 
 
 def _attend_args(cache, q, cu, max_new, max_len, scale, out):
-    _no_grad(q)
+    _no_grad(cache, q, out)
     tokens, max_new = _step(cache, q, cu, max_new)
     qr = _rows(q, "q", cache)
     heads = qr.heads

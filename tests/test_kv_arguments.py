@@ -49,3 +49,31 @@ def test_a_step_refused_after_the_append_leaves_lengths(lngram, monkeypatch, kw,
     with pytest.raises(error):
         lngram.attention_step(c, q.view(6, 4, 64), k.view(6, 2, 64), k.view(6, 2, 64), cu=cu, max_new=5, **kw)
     assert c.lengths.tolist() == [5, 7]
+
+
+def test_no_gradients_of_anything(lngram):
+    """Not of the frequencies, the pages, the outputs or a tangent either: nothing is lost without a word."""
+    import torch.autograd.forward_ad as fwd
+    q, k = torch.zeros(2, 3, 4, 64, **BF), torch.zeros(2, 3, 2, 64, **BF)
+    freq, table = torch.ones(32), torch.zeros(1, dtype=torch.int32)
+    c, cg = make(lngram), make(lngram, k=torch.zeros(4, 2, 16, 64, **BF).requires_grad_())
+    qg, freqg = q.clone().requires_grad_(), freq.clone().requires_grad_()
+    calls = [lambda: lngram.kv_append(c, k, k, q, inv_freq=freqg), lambda: lngram.kv_append(c, k, k, q, q_out=qg),
+             lambda: lngram.kv_append(cg, k, k), lambda: lngram.kv_attend(cg, q), lambda: lngram.kv_attend(c, q, out=qg),
+             lambda: lngram.kv_prefix_attend(cg, q, table, 3), lambda: lngram.kv_prefix_attend(c, q, table, 3, out=qg),
+             lambda: lngram.attention_step(c, q, k, k, inv_freq=freqg)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+    with fwd.dual_level():
+        qd, kd, fd = (fwd.make_dual(x, torch.ones_like(x)) for x in (q, k, freq))
+        for call in (lambda: lngram.kv_attend(c, qd), lambda: lngram.kv_append(c, kd, k), lambda: lngram.kv_append(c, k, kd),
+                     lambda: lngram.kv_append(c, k, k, q, inv_freq=fd), lambda: lngram.kv_prefix_attend(c, qd, table, 3)):
+            for mode in (torch.no_grad(), torch.enable_grad()):
+                with mode, pytest.raises(RuntimeError, match="tangent"):
+                    call()
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            lngram.kv_attend(c, q)
+    assert c.lengths.tolist() == [0, 0]
