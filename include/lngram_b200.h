@@ -515,7 +515,8 @@ int lng_kv_attend(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, 
 /* lng_kv_attend (no window) for a batch whose sequences all begin with the same prefix_len keys, kept once in
  * the pages prefix_table[0 .. ceil(prefix_len / page_size) - 1] (i32, device): every token sees the whole
  * prefix and, causally, its own sequence's keys (table, lengths), which come after it.  The prefix is read
- * once for the batch. */
+ * once for the batch.  Where keys are rotated, lng_kv_append must be given positions that count the prefix (its
+ * default, a token's key index, does not). */
 size_t lng_kv_prefix_workspace_bytes(const lng_kv_cache* cache, int64_t prefix_len, int64_t tokens, int64_t max_new,
                                      int64_t max_len, int32_t q_heads);
 int lng_kv_prefix_attend(const lng_kv_cache* cache, const int32_t* prefix_table, int64_t prefix_len, const int32_t* cu,

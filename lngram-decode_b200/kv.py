@@ -186,7 +186,7 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
     """Write a step's keys and values to the cache: token i of the n new ones of a sequence becomes key
     ``lengths - n + i`` (``extend`` first).  With ``inv_freq`` (fp32 ``[rotary_dim / 2]``) the first rotary_dim
     values of keys and queries are rotated by the token's position -- ``positions`` (int64, the step's leading
-    shape) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
+    shape; needed behind a shared prefix) or its place in the sequence -- in pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) if ``interleaved``.
     Returns the rotated queries (``q_out`` if given; it may be ``q``) or None without ``q``.  Pages that several
     sequences name are for reading: no two tokens of a step may go to one slot.  No gradients."""
     _no_grad(cache, k, v, q, inv_freq, q_out)
@@ -279,7 +279,10 @@ def kv_prefix_attend(cache: PagedKVCache, q: Tensor, prefix_table: Tensor, prefi
                      out: Tensor | None = None) -> Tensor:
     """``kv_attend`` (without a window) for a batch whose sequences all begin with the ``prefix_len`` keys in the
     pages ``prefix_table`` (int32 ``[>= ceil(prefix_len / page_size)]``) of the same cache; ``table`` and
-    ``lengths`` hold what each sequence adds to it.  The prefix is read once for the whole batch.  No gradients."""
+    ``lengths`` hold what each sequence adds to it.  The prefix is read once for the whole batch.  ``kv_append``'s own
+    positions count a sequence's own keys only: behind a prefix give it ``positions`` that count the prefix too
+    (prefix_len + the key's place).  The prefix itself is appended once, through a cache of one sequence over the same
+    pages whose table is ``prefix_table``.  No gradients."""
     tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
     prefix_len = int(prefix_len)
     if not 0 <= prefix_len < 1 << 30:
