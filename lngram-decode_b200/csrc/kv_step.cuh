@@ -587,6 +587,10 @@ __global__ void __launch_bounds__(KsCfg<HDP>::THREADS, 1)
     }
     __syncthreads();
   }
+  // a wait has run out: behind this warp's copies in flight, which must not outlive the CTA
+  if (!ok)
+    for (; taken != issued; ++taken)
+      mbar_wait_bounded(&bar[taken % KS_STAGES], (taken / KS_STAGES) & 1, &g_error_word, DEV_ERR_WAIT_TIMEOUT);
   // launched beside the prefix's kernel, this one must not be complete before it: the join waits for this one only
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

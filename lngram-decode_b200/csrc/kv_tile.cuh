@@ -251,7 +251,8 @@ struct KtBars {
   static constexpr uint32_t p_full = s_full + 32;   // [2][2], 128 arrivals: the tile's weights are, O is rescaled
   static constexpr uint32_t pv_done = p_full + 32;  // [2] O += P V is done, a phase a tile
   static constexpr uint32_t o_full = pv_done + 16;  // [2] the unit's last one is
-  static constexpr uint32_t tmem = o_full + 16, abort = tmem + 4;
+  static constexpr uint32_t idle = o_full + 16;     // [2] no product of the row tile is in flight
+  static constexpr uint32_t tmem = idle + 16, abort = tmem + 4;
   // A wait names a phase by its parity alone, so a role may only wait for a phase while the barrier can be in that
   // one or the next: every role waits for the phases of its barriers one after the other.
 };
@@ -299,8 +300,9 @@ __device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 // Wait bounded by time (two seconds; the longest wait of a working kernel is a unit's, milliseconds), which also
-// gives up when another role has.  An expired wait records the device error.
-template <int HDP>
+// gives up when another role has -- but for the waits (ALONE) with which a role ends: whatever has happened, its own
+// copies and products must not outlive the CTA.  An expired wait records the device error.
+template <int HDP, bool ALONE = false>
 __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t parity) {
   if (mbar_try_at(bars + bar, parity)) return true;
   uint64_t start, now;
@@ -308,7 +310,7 @@ __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t pa
   for (uint32_t i = 0;; ++i) {
     if (mbar_try_at(bars + bar, parity)) return true;
     if ((i & 63) != 63) continue;
-    if (lds32(bars + KtBars<HDP>::abort)) return false;
+    if (!ALONE && lds32(bars + KtBars<HDP>::abort)) return false;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
     if (now - start > 2000000000ull) break;
   }
@@ -494,8 +496,14 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
     }
   }
   // the last uses of the ring's slots: behind them no copy and no product is in flight
-  for (uint32_t k = it >= NS ? it - NS : kv; k < it; k += 2) kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1);
-  if (kv == 0 && units > 0) kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1);
+  const uint32_t k0 = it >= NS ? it - NS : kv;
+  bool used = true;
+  for (uint32_t k = k0; k < it; k += 2) used = kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1) && used;
+  if (kv == 0 && units > 0) used = kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1) && used;
+  if (__all_sync(0xffffffffu, used)) return;
+  // (a role has given up: behind the copies themselves)
+  for (uint32_t k = k0; k < it; k += 2) kt_wait<HDP, true>(bars, B::kv_full + 8 * (k % NS), (k / NS) & 1);
+  if (kv == 0 && units > 0) kt_wait<HDP, true>(bars, B::q_full, (units - 1) & 1);
 }
 
 // One warp a row tile issues its products: the scores of the next key tile (into the other of two S buffers) ahead
@@ -578,6 +586,12 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
     }
     base += 2 * w.n;
     tile += cnt;
+  }
+  // a role has given up: behind this warp's products (else the loading warps have seen the last of them done)
+  if (__any_sync(0xffffffffu, !ok || lds32(bars + B::abort) != 0)) {
+    if (elect_lane()) umma_commit_at(bars + B::idle + 8 * G);
+    __syncwarp();
+    kt_wait<HDP, true>(bars, B::idle + 8 * G, 0);
   }
 }
 
@@ -780,6 +794,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
       }
       mbar_init_at(bars + B::pv_done + 8 * g, 1);
       mbar_init_at(bars + B::o_full + 8 * g, 1);
+      mbar_init_at(bars + B::idle + 8 * g, 1);
     }
     sts32(bars + B::abort, 0u);
     fence_mbar_init();
