@@ -5,7 +5,7 @@
 // every key they load -- against the tiles of 64 keys that any of its tokens sees (or one range of them).  One CTA an
 // SM takes units in turn, so that a unit's loads and first scores start under the one before.  Roles:
 //   warps 0-3, 4-7  a row tile each, one row a thread: S from TMEM, the running maximum and sum in fp32, P, rounded to
-//             the cache's type, over its S's columns;
+//             the cache's type (as the step kernel's weights, and with its errors), over its S's columns;
 //   warps 8, 9      load by TMA, page by page, into a ring: queries and keys, values;
 //   warps 10, 11    issue a row tile's tcgen05.mma: S = Q K^T (fp32 in TMEM) a key tile ahead, O += P V, P from TMEM.
 // TMEM: two S buffers of 64 columns a row tile (P in the same ones) and O of both (2 x head size).
@@ -20,7 +20,8 @@
 // 0.55 ms), and so were: scores and products issued by a warp each (0.56 against 0.54 ms; two prompts of 8000
 // tokens and 28 heads of 128: 0.75 against 0.76), sixteen row warps, two groups taking a row tile's key tiles in turn
 // (0.73 and 0.87 ms), and the next scores loaded while the weights are formed (0.63 and 0.92 ms).
-// Measured: 0.54 ms, 511 TFLOP/s, for the former; 0.74 to 0.78 ms, 900 to 950 TFLOP/s, for the latter (window of 4096).
+// Measured: 0.534 ms, 515 TFLOP/s, for the former; 0.87 ms, 809 TFLOP/s, for the latter (window of 4096) in a long
+// loop, where power sets the clock (0.75 ms, 930 TFLOP/s, in the first few milliseconds).
 #pragma once
 
 #include "exp2_poly.cuh"
@@ -29,8 +30,8 @@
 namespace lng {
 
 constexpr int KT_BM = 128, KT_BK = 64, KT_THREADS = 384;
-// Of eight pairs of exponentials, those on the fma pipe.  None, one, two, three (32 prompts of 2048 tokens, heads of
-// 64): 564, 559, 561, 537 us, and four was slower than three by 16; at heads of 128 they are alike.
+// Of eight pairs of exponentials, those on the fma pipe.  None, one, two, three, four (32 prompts of 2048 tokens, heads
+// of 64): 571, 559, 551, 533, 555 us; two prompts of 8000 tokens, heads of 128: 736, 727, 761, 755, 754.
 constexpr uint32_t KT_FMA_EXP = 0x52;
 
 template <int HDP>

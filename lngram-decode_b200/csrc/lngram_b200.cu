@@ -1870,7 +1870,8 @@ static int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned thr
   return LNG_OK;
 }
 
-// behind_prefix: the kernel before is the prefix's, which this one needs nothing of
+// behind_prefix: the kernel before is the prefix's, which this one needs nothing of; it starts as that one's CTAs end
+// (each takes nearly all of an SM's shared memory)
 template <typename T, int HDP, bool WS>
 static int launch_kv_step(const CUtensorMap& tk, const CUtensorMap& tv, const KsParams& p, bool behind_prefix, cudaStream_t s) {
   using Cfg = KsCfg<HDP>;
@@ -1883,7 +1884,8 @@ static int launch_kv_step(const CUtensorMap& tk, const CUtensorMap& tv, const Ks
     kern<<<grid, Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
     LNG_LAUNCHED("kv_step_kernel");
   }
-  // the join finds its pieces while the step kernel runs and waits for it before it reads them
+  // the join finds its pieces while the step kernel's last CTAs run (at head size 64 there is room for it beside them,
+  // at 128 where one has ended) and waits for the whole kernel before it reads them
   return launch_dependent(kv_step_join_kernel<T, Cfg::BK>, unsigned(p.c.batch * p.c.kv_heads), 256u, size_t(0), s, p);
 }
 
