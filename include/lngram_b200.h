@@ -458,8 +458,9 @@ int lng_online_counts_mix(const int64_t* codes, int64_t T, int64_t R, const int3
  * error 4; such keys read as zeros and are not written.  Lengths outside [0, max_pages * page_size] and bad row
  * offsets record it too: every token keeps the key index that its sequence's given length and count say, and is
  * written only where that lies in the sequence's pages; attention sees no keys of a sequence with such a length (zeros,
- * or the shared prefix alone); of more than max_new rows a sequence the first max_new are taken.  dtype LNG_BF16 or LNG_F16; k, v 16-byte aligned, strides multiples of 8 elements; head_dim a
- * multiple of 8 up to 128; page_size a power of two in [8, 4096]; max_pages * page_size < 2^30. */
+ * or the shared prefix alone); of more than max_new rows a sequence the first max_new are taken.  dtype LNG_BF16 or
+ * LNG_F16; k, v 16-byte aligned, strides multiples of 8 elements; head_dim a multiple of 8 up to 128; page_size a power
+ * of two in [8, 4096]; max_pages * page_size < 2^30. */
 typedef struct {
   void* k;
   void* v;
@@ -503,9 +504,9 @@ int lng_kv_append(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, 
  * token sees no key.  Query head h reads key head h / (q.heads / num_kv_heads); at most 128 query heads a key
  * head.  Pages that hold no visible key are not touched (their table entries may be stale).  Scores
  * of NaN or +inf make their row NaN, and no other.  Values that any of the step's tokens sees must be finite (a weight
- * of zero times NaN is NaN, for the tokens before it too).  max_len: an upper bound of lengths that only guides how the work is split
- * (0 = max_pages * page_size).  q and out must not overlap.  workspace: 256-byte aligned,
- * lng_kv_attend_workspace_bytes bytes, used by this call alone until it has finished. */
+ * of zero times NaN is NaN, for the tokens before it too).  scale * log2(e) must be finite in fp32.  max_len: an upper
+ * bound of lengths that only guides how the work is split (0 = max_pages * page_size).  q and out must not overlap.
+ * workspace: 256-byte aligned, lng_kv_attend_workspace_bytes bytes, used by this call alone until it has finished. */
 size_t lng_kv_attend_workspace_bytes(const lng_kv_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
                                      int32_t q_heads, int32_t window, int32_t sinks);
 int lng_kv_attend(const lng_kv_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,

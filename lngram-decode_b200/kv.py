@@ -169,8 +169,8 @@ def _no_grad(cache: PagedKVCache, *tensors: Tensor | None) -> None:
     if torch.is_grad_enabled() and (cache._k.requires_grad or cache._v.requires_grad
                                     or any(t is not None and t.requires_grad for t in tensors)):
         raise RuntimeError("the paged cache's operators have no backward: call them under torch.no_grad()")
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                              for t in (cache._k, cache._v) + tensors):
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (cache._k, cache._v) + tensors):
         raise RuntimeError("the paged cache's operators carry no tangent: give them the primal values")
 
 
