@@ -524,6 +524,92 @@ int lng_kv_prefix_attend(const lng_kv_cache* cache, const int32_t* prefix_table,
                          int64_t tokens, int64_t max_new, int64_t max_len, const lng_kv_rows* q, float scale,
                          const lng_kv_rows* out, void* workspace, size_t workspace_bytes, lng_stream_t stream);
 
+/* ------------------------------------------------------------------ keys and values in 8 bits */
+
+/* A paged cache whose slots are e4m3 bytes: page p of head h holds value * 2^k_exp[p * k_exp_stride + h] (v likewise),
+ * int8 exponents in [-40, 40].  pages: as above with k, v e4m3, all strides in bytes and multiples of 16, head_dim a
+ * multiple of 16 up to 128, page_size a power of two in [8, 256]; pages.dtype is the type of the rows (LNG_BF16 or
+ * LNG_F16) that are appended and attended with.  For lng_kv_pages_* k_exp = v_exp = NULL says that the pages are those
+ * of an lng_kv_cache. */
+typedef struct {
+  lng_kv_cache pages;
+  int8_t* k_exp;
+  int8_t* v_exp;
+  int64_t k_exp_stride, v_exp_stride;
+} lng_kv8_cache;
+
+/* lng_kv_append into 8 bits.  Keys are rotated in fp32 and rounded once, to e4m3 under their page's and head's exponent:
+ * the least e for which every finite new value of the page has |x| <= 448 * 2^e, at least -40 and at most 40 (larger
+ * values saturate); NaN and infinities are stored as NaN and do not count.  A page whose first slot is among the new
+ * ones takes that exponent; else the page keeps the larger of its exponent and that one, and the slots before
+ * the new ones are rounded again where it grew (exact but for what becomes subnormal).  The slots behind are left as
+ * they are.  No two sequences of a step may write to one page. */
+int lng_kv8_append(const lng_kv8_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, const lng_kv_rows* k,
+                   const lng_kv_rows* v, const lng_kv_rows* q, const lng_kv_rows* q_out, const int64_t* positions,
+                   const float* inv_freq, int32_t rotary_dim, int32_t interleaved, lng_stream_t stream);
+
+/* lng_kv_attend over a cache in 8 bits.  Products in fp16, in which e4m3 is exact (queries are scaled by a power of two
+ * a row), exponents, scores, sums and states in fp32; weights are rounded to fp16 for the product with the values. */
+size_t lng_kv8_attend_workspace_bytes(const lng_kv8_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
+                                      int32_t q_heads, int32_t window, int32_t sinks);
+int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,
+                   const lng_kv_rows* q, float scale, int32_t window, int32_t sinks, const lng_kv_rows* out,
+                   void* workspace, size_t workspace_bytes, lng_stream_t stream);
+
+/* What the slots of all pages stand for, in bf16 (which holds every such value exactly): k_out, v_out
+ * [num_pages, num_kv_heads, page_size, head_dim], 16-byte aligned; either may be NULL. */
+int lng_kv8_values(const lng_kv8_cache* cache, void* k_out, void* v_out, lng_stream_t stream);
+
+/* ------------------------------------------------------------------ pages from lengths */
+
+/* Tables and slots of a paged cache made on the GPU.  refs i32 [num_pages] counts the table rows that hold a page;
+ * pages with 0 are free.  cache.pages.table and .lengths are written by these calls; table entries behind a
+ * sequence's keys are -1.  A length below 0 is that of a suspended sequence of -1 - length keys: attention sees no keys
+ * of it, lng_kv_append drops its tokens, nothing of it is lost; the next extend or truncate takes it up again.
+ * At most 8192 sequences and 2^22 pages. */
+
+/* Every sequence grows by its tokens of the step (cu or max_new as for lng_kv_append).  New pages are the lowest
+ * free ones, in order of sequence and then of column.  A partly filled last page that other rows hold too is replaced by
+ * a page of the sequence's own, and its copy noted.  A sequence that does not fit its table's row, or for which too few
+ * pages are free once those before it have theirs, is suspended (served = 0); one that needs no page is served always.
+ * slots i64 [tokens]: page * page_size + slot of every new token, -1 where it has none.  copies i32 [batch, 4]:
+ * (source page, target page, filled slots, 0), target -1 where nothing is copied. */
+int lng_kv_pages_extend(const lng_kv8_cache* cache, int32_t* refs, const int32_t* cu, int64_t tokens, int64_t max_new,
+                        int64_t* slots, uint8_t* served, int32_t* copies, lng_stream_t stream);
+/* Carries out an extend's copies in one cache (one call a layer, where layers share the table), before its append. */
+int lng_kv_pages_copy(const lng_kv8_cache* cache, const int32_t* copies, lng_stream_t stream);
+/* Sequence b keeps its first min(lengths[b], its length) keys (most for all where lengths is NULL); the pages behind
+ * them are given back. */
+int lng_kv_pages_truncate(const lng_kv8_cache* cache, int32_t* refs, const int32_t* lengths, int64_t most, lng_stream_t stream);
+/* Row g * beams + k takes over the pages and the length of row g * beams + parents[g * beams + k] (i64, device;
+ * groups * beams = batch); pages are shared, those that no row holds any more become free.  A parent out of range
+ * records device error 4 and leaves its row as it is. */
+int lng_kv_pages_reorder(const lng_kv8_cache* cache, int32_t* refs, const int64_t* parents, int64_t groups, int64_t beams,
+                         lng_stream_t stream);
+
+/* ------------------------------------------------------------------ beams */
+
+/* One step of beam search: of the candidates scores[g, k] + logits[g, k, v] - log sum_v exp logits[g, k, v] of a
+ * group the `width` largest, in falling order, ties to the lowest k * vocab + v.  logits f32, bf16 or f16, rows of
+ * `vocab` values row_stride elements apart; scores f32 [groups, beams]; done (u8, may be NULL): a beam that has ended
+ * offers token eos at its own score and -inf for every other.  A row that holds a NaN, +inf or nothing but -inf
+ * offers -inf throughout.  Outputs [groups, width]: f32, i64, i64.  beams, width <= 32, width <= beams * vocab,
+ * vocab < 2^30.  workspace: 256-byte aligned, used by this call alone until it has finished. */
+size_t lng_beam_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t width);
+int lng_beam_select(const void* logits, int32_t dtype, int64_t row_stride, int64_t groups, int64_t beams, int64_t vocab,
+                    const float* scores, const uint8_t* done, int64_t eos, int64_t width, float* out_scores,
+                    int64_t* tokens, int64_t* parents, void* workspace, size_t workspace_bytes, lng_stream_t stream);
+
+/* Rows of a state, in place: the first `bytes` bytes of row g * beams + k become those of row g * beams +
+ * parents[g, k] (i64, device; a parent out of range records device error 4 and leaves its row as it is).  beams <= 32;
+ * at most 8 states a call, whose rows are `stride` bytes apart, stride >= bytes. */
+typedef struct {
+  void* ptr;
+  int64_t stride, bytes;
+} lng_beam_state;
+int lng_beam_reorder(const int64_t* parents, int64_t groups, int64_t beams, const lng_beam_state* states_host,
+                     int32_t count, lng_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,10 @@ from . import serving, sharded  # noqa: E402
 from .sharded import RouteShardedMemory  # noqa: E402
 
 __all__ += ["RouteShardedMemory", "serving", "sharded"]
-from .kv import PagedKVCache, attention_step, kv_append, kv_attend, kv_prefix_attend  # noqa: E402
+from .kv import PagedKVCache, PagedKVCache8, attention_step, kv_append, kv_attend, kv_prefix_attend  # noqa: E402
 
-__all__ += ["PagedKVCache", "attention_step", "kv_append", "kv_attend", "kv_prefix_attend"]
+__all__ += ["PagedKVCache", "PagedKVCache8", "attention_step", "kv_append", "kv_attend", "kv_prefix_attend"]
+from .beams import beam_reorder, beam_select  # noqa: E402
+from .pages import PagePool  # noqa: E402
+
+__all__ += ["PagePool", "beam_reorder", "beam_select"]

@@ -73,10 +73,19 @@ class KvRows(C.Structure):
     _fields_ = [("ptr", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32)]
 
 
+class KvCache8(C.Structure):
+    _fields_ = [("pages", KvCache), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p), ("k_exp_stride", C.c_int64),
+                ("v_exp_stride", C.c_int64)]
+
+
+class BeamState(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride", C.c_int64), ("bytes", C.c_int64)]
+
+
 P = C.c_void_p
 i32, i64, f32, sz = C.c_int32, C.c_int64, C.c_float, C.c_size_t
 PT, PR = C.POINTER(Tables), C.POINTER(Readout)
-PK, PW = C.POINTER(KvCache), C.POINTER(KvRows)
+PK, PW, PK8 = C.POINTER(KvCache), C.POINTER(KvRows), C.POINTER(KvCache8)
 
 # name -> (restype, argtypes); mirrors include/lngram_b200.h
 SIGNATURES = {
@@ -138,6 +147,17 @@ SIGNATURES = {
     "lng_kv_attend": (C.c_int, [PK, P, i64, i64, i64, PW, f32, i32, i32, PW, P, sz, P]),
     "lng_kv_prefix_workspace_bytes": (sz, [PK, i64, i64, i64, i64, i32]),
     "lng_kv_prefix_attend": (C.c_int, [PK, P, i64, P, i64, i64, i64, PW, f32, PW, P, sz, P]),
+    "lng_kv8_append": (C.c_int, [PK8, P, i64, i64, PW, PW, PW, PW, P, P, i32, i32, P]),
+    "lng_kv8_attend_workspace_bytes": (sz, [PK8, i64, i64, i64, i32, i32, i32]),
+    "lng_kv8_attend": (C.c_int, [PK8, P, i64, i64, i64, PW, f32, i32, i32, PW, P, sz, P]),
+    "lng_kv8_values": (C.c_int, [PK8, P, P, P]),
+    "lng_kv_pages_extend": (C.c_int, [PK8, P, P, i64, i64, P, P, P, P]),
+    "lng_kv_pages_copy": (C.c_int, [PK8, P, P]),
+    "lng_kv_pages_truncate": (C.c_int, [PK8, P, P, i64, P]),
+    "lng_kv_pages_reorder": (C.c_int, [PK8, P, P, i64, i64, P]),
+    "lng_beam_workspace_bytes": (sz, [i64, i64, i64, i64]),
+    "lng_beam_select": (C.c_int, [P, i32, i64, i64, i64, i64, P, P, i64, i64, P, P, P, P, sz, P]),
+    "lng_beam_reorder": (C.c_int, [P, i64, i64, C.POINTER(BeamState), i32, P]),
     "lng_online_counts_mix": (C.c_int, [P, i64, i64, P, i32, i32, P, P, P, i64, i64, P, P, i64, f32, P, P]),
 }
 

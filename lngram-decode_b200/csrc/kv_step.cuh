@@ -27,8 +27,8 @@
 
 #include <type_traits>
 
-#include "gemm_tc.cuh"
 #include "kvcache.cuh"
+#include "tc_prims.cuh"
 
 namespace lng {
 

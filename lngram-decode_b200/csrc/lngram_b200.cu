@@ -1,5 +1,5 @@
-// lngram_b200: the C ABI of include/lngram_b200.h (one translation unit, so every kernel shares
-// the device error word and inlines the addressing helpers).
+// lngram_b200: the C ABI of include/lngram_b200.h (kv8.cu and kv_pages.cu hold the entries of the 8-bit
+// cache and of page pools and beams).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -25,6 +25,7 @@
 #include "kvcache.cuh"
 #include "kv_step.cuh"
 #include "kv_tile.cuh"
+#include "kv_host.cuh"
 
 static int scratch_alloc(void** p, size_t bytes, cudaStream_t stream);
 
@@ -53,8 +54,6 @@ static int grid_for(int64_t work, int threads, int per_sm = 8) {
   const int64_t want = ceil_div(std::max<int64_t>(work, 1), threads);
   return int(std::max<int64_t>(1, std::min<int64_t>(want, int64_t(num_sms()) * per_sm)));
 }
-
-static cudaStream_t S(lng_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 static int check_tables(const lng_tables* t) {
   LNG_REQUIRE(t != nullptr, "tables descriptor is NULL");
@@ -116,13 +115,14 @@ extern "C" int lng_device_ok(void) {
 }
 
 extern "C" int lng_device_error(int clear) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_error_word, sizeof(v)) != cudaSuccess) return -1;
-  if (clear && v) {
-    const unsigned int z = 0;
-    cudaMemcpyToSymbol(g_error_word, &z, sizeof(z));
+  // a word a translation unit: the first one that holds a code is reported, all are cleared
+  int first = 0;
+  for (int (*word)(int) : {error_word_here, error_word_kv8, error_word_pages}) {
+    const int v = word(clear);
+    if (v < 0) return -1;
+    if (first == 0) first = v;
   }
-  return int(v);
+  return first;
 }
 
 // ====================================================================== router
@@ -1665,70 +1665,6 @@ extern "C" int lng_online_counts_mix(const int64_t* codes, int64_t T, int64_t R,
 // ====================================================================== paged keys and values
 namespace lng {
 
-static int check_kv(const lng_kv_cache* c, const int32_t* cu, int64_t tokens, int64_t max_new) {
-  LNG_REQUIRE(c != nullptr, "cache descriptor is NULL");
-  LNG_REQUIRE(c->dtype == LNG_BF16 || c->dtype == LNG_F16, "cache dtype must be bf16 or f16");
-  LNG_REQUIRE(c->page_size >= 8 && c->page_size <= 4096 && (c->page_size & (c->page_size - 1)) == 0,
-              "page_size must be a power of two in [8, 4096]");
-  LNG_REQUIRE(c->num_pages >= 1 && c->num_pages < (int64_t(1) << 31), "num_pages must be in [1, 2^31)");
-  LNG_REQUIRE(c->num_kv_heads >= 1 && c->num_kv_heads <= 65535, "num_kv_heads must be in [1, 65535]");
-  LNG_REQUIRE(c->head_dim >= 8 && c->head_dim <= 128 && c->head_dim % 8 == 0, "head_dim must be a multiple of 8 up to 128");
-  LNG_REQUIRE(c->batch >= 0 && c->max_pages >= 0, "batch and max_pages must not be negative");
-  LNG_REQUIRE(c->max_pages < (int64_t(1) << 30) / c->page_size, "max_pages * page_size must be below 2^30");
-  LNG_REQUIRE(c->table_stride >= c->max_pages, "table_stride must be at least max_pages");
-  LNG_REQUIRE(max_new >= 0 && max_new < (int64_t(1) << 30), "max_new must be in [0, 2^30)");
-  LNG_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 31), "tokens must be in [0, 2^31)");
-  LNG_REQUIRE(cu != nullptr || tokens == c->batch * max_new, "without cu, tokens must be batch * max_new");
-  if (tokens == 0 || c->batch == 0) return LNG_OK;
-  LNG_REQUIRE(max_new >= 1, "max_new must be positive");
-  LNG_REQUIRE(c->k && c->v && c->lengths && (c->table || c->max_pages == 0), "NULL pointer in the cache descriptor");
-  LNG_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) == 0,
-              "k and v must be 16-byte aligned");
-  for (int64_t s : {c->k_page_stride, c->k_head_stride, c->k_slot_stride, c->v_page_stride, c->v_head_stride, c->v_slot_stride})
-    LNG_REQUIRE(s > 0 && s % 8 == 0 && s < (int64_t(1) << 38), "cache strides must be positive multiples of 8 elements");
-  return LNG_OK;
-}
-
-static int check_kv_rows(const lng_kv_rows* r, int64_t heads, const char* what) {
-  const std::string w(what);
-  LNG_REQUIRE(r != nullptr && r->ptr != nullptr, w + " is NULL");
-  LNG_REQUIRE(heads <= 0 || r->heads == heads, w + ": wrong number of heads");
-  LNG_REQUIRE(r->heads >= 1 && r->heads <= (1 << 20), w + ": heads must be positive");
-  LNG_REQUIRE((reinterpret_cast<uintptr_t>(r->ptr) & 15) == 0, w + " must be 16-byte aligned");
-  LNG_REQUIRE(r->token_stride > 0 && r->token_stride % 8 == 0 && r->head_stride > 0 && r->head_stride % 8 == 0 &&
-                  r->token_stride < (int64_t(1) << 38) && r->head_stride < (int64_t(1) << 38),
-              w + ": strides must be positive multiples of 8 elements");
-  return LNG_OK;
-}
-
-static KvView kv_view(const lng_kv_cache* c, const int32_t* cu, int64_t tokens, int64_t max_new) {
-  KvView v{};
-  v.k = c->k;
-  v.v = c->v;
-  v.k_page = c->k_page_stride;
-  v.k_head = c->k_head_stride;
-  v.k_slot = c->k_slot_stride;
-  v.v_page = c->v_page_stride;
-  v.v_head = c->v_head_stride;
-  v.v_slot = c->v_slot_stride;
-  v.table = c->table;
-  v.table_stride = c->table_stride;
-  v.num_pages = c->num_pages;
-  v.lengths = c->lengths;
-  v.cu = cu;
-  v.batch = c->batch;
-  v.tokens = tokens;
-  v.kv_heads = c->num_kv_heads;
-  v.head_dim = c->head_dim;
-  for (v.page_shift = 0; (1 << v.page_shift) < c->page_size; ++v.page_shift) {
-  }
-  v.capacity = int32_t(c->max_pages * c->page_size);
-  v.max_new = int32_t(max_new);
-  return v;
-}
-
-static KvRows kv_rows(const lng_kv_rows* r) { return r ? KvRows{r->ptr, r->token_stride, r->head_stride} : KvRows{}; }
-
 // The tensor map of the cache's keys (or values): [pages][heads][slots][head_dim], one head's slots of one
 // page a copy, 64 values wide (a head beyond 64 takes two copies; columns behind head_dim fill with zeros).
 static int kv_page_map(CUtensorMap* map, const lng_kv_cache* c, void* base, int64_t page, int64_t head, int64_t slot, int box) {
@@ -1762,24 +1698,6 @@ static int kv_query_map(CUtensorMap* map, const lng_kv_cache* c, const lng_kv_ro
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
   return LNG_OK;
-}
-
-// Into how many key ranges units with up to `tiles` key tiles each are divided: one where the units alone fill the
-// SMs, else the count with the least estimated time, in tiles -- waves of units (one an SM) times (a range's
-// tiles + 8 for a unit's start and its state's way out), plus the join of the states.
-static int kv_splits(int64_t units, int64_t tiles) {
-  const int64_t sms = num_sms();
-  int best = 1;
-  if (units >= sms) return best;
-  double least = 1e300;
-  for (int s = 1; s <= 32 && s <= tiles; ++s) {
-    const double cost = double(ceil_div(units * s, sms)) * (ceil_div(tiles, s) + 8) + (s > 1 ? 4 + s * 0.5 : 0.0);
-    if (cost < least) {
-      least = cost;
-      best = s;
-    }
-  }
-  return best;
 }
 
 // How an attention call is carried out, and what it needs of the workspace.
@@ -1850,23 +1768,6 @@ static int launch_kv_tile(const CUtensorMap& tq, const CUtensorMap& tk, const CU
   q.total = units * p.c.kv_heads * p.splits;
   kern<<<unsigned(std::min<int64_t>(q.total, num_sms())), KT_THREADS, Cfg::SMEM, s>>>(tq, tk, tv, q);
   LNG_LAUNCHED("kv_tile_kernel");
-  return LNG_OK;
-}
-
-// A launch that may start while the kernel before it in the stream still runs (griddepcontrol in both).
-template <typename... Params, typename... Args>
-static int launch_dependent(void (*kern)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, Args... args) {
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = pdl;
-  cfg.numAttrs = 1;
-  LNG_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
   return LNG_OK;
 }
 

@@ -5,6 +5,8 @@ The reference's ``decode_step`` keeps dense keys and values in its ``DecodeState
 
 * ``PagedKVCache`` -- the pages, the page table and the sequences' lengths (device tensors; the lengths count
   a step's new tokens from ``extend`` on).
+* ``PagedKVCache8`` -- the same in 8 bits: e4m3 values under one exponent for each page and head.  Steps are still
+  bf16 or fp16; ``kv_append``, ``kv_attend`` and ``attention_step`` take either cache.
 * ``kv_append`` -- a step's keys and values into their slots, keys and queries rotated by position on the way.
 * ``kv_attend`` -- causal attention of the step's tokens over the cache: grouped heads, an optional sliding
   window with the first ``sinks`` tokens visible beside it; one token a sequence or whole prompts.
@@ -59,6 +61,16 @@ class PagedKVCache:
             _require(t.stride(3) == 1 and all(t.stride(i) > 0 and t.stride(i) % 8 == 0 for i in range(3)),
                      "the head dimension must be contiguous and the other strides positive multiples of 8")
             _require(t.data_ptr() % 16 == 0, "k and v must be 16-byte aligned")
+        self._check_table(table, lengths, size)
+        _require(k.device == v.device == table.device == lengths.device, "the cache's tensors must be on one device")
+        self._k, self._v, self._table, self._lengths = k, v, table, lengths
+        self._desc = self._pages_desc(_lib.dtype_code(k.dtype))
+        self._set_up(k.dtype)
+
+    eight = False  # whether the pages hold 8 bits (PagedKVCache8)
+
+    @staticmethod
+    def _check_table(table: Tensor, lengths: Tensor, size: int) -> None:
         _require(table.dim() == 2 and table.dtype == torch.int32 and (table.shape[1] <= 1 or table.stride(1) == 1),
                  "table must be int32 [B, max_pages] with contiguous rows")
         _require(table.shape[0] <= 1 or table.stride(0) >= table.shape[1], "table: the sequences' rows must not overlap")
@@ -66,19 +78,23 @@ class PagedKVCache:
                  "lengths must be contiguous int32 [B]")
         _require(lengths.shape[0] == table.shape[0], "table and lengths must have one row a sequence")
         _require(table.shape[1] * size < 1 << 30, "max_pages * page_size must be below 2^30")
-        _require(k.device == v.device == table.device == lengths.device, "the cache's tensors must be on one device")
-        self._k, self._v, self._table, self._lengths = k, v, table, lengths
-        self._desc = _lib.KvCache(k=k.data_ptr(), v=v.data_ptr(), dtype=_lib.dtype_code(k.dtype), page_size=size,
-                                  num_pages=pages, num_kv_heads=heads, head_dim=dim, k_page_stride=k.stride(0),
-                                  k_head_stride=k.stride(1), k_slot_stride=k.stride(2), v_page_stride=v.stride(0),
-                                  v_head_stride=v.stride(1), v_slot_stride=v.stride(2), table=table.data_ptr(),
-                                  table_stride=max(table.stride(0), table.shape[1]), max_pages=table.shape[1],
-                                  lengths=lengths.data_ptr(), batch=table.shape[0])
+
+    def _pages_desc(self, dtype: int) -> _lib.KvCache:
+        k, v, table, lengths = self._k, self._v, self._table, self._lengths
+        pages, heads, size, dim = k.shape
+        return _lib.KvCache(k=k.data_ptr(), v=v.data_ptr(), dtype=dtype, page_size=size, num_pages=pages, num_kv_heads=heads,
+                            head_dim=dim, k_page_stride=k.stride(0), k_head_stride=k.stride(1), k_slot_stride=k.stride(2),
+                            v_page_stride=v.stride(0), v_head_stride=v.stride(1), v_slot_stride=v.stride(2),
+                            table=table.data_ptr(), table_stride=max(table.stride(0), table.shape[1]), max_pages=table.shape[1],
+                            lengths=lengths.data_ptr(), batch=table.shape[0])
+
+    def _set_up(self, dtype: torch.dtype) -> None:
+        k, table = self._k, self._table
         self._ref = C.byref(self._desc)
-        self.device, self.dtype, self.index = k.device, k.dtype, k.get_device()
+        self.device, self.dtype, self.index = k.device, dtype, k.get_device()
         self._sizes: dict = {}
-        self.batch, self.page_size, self.num_kv_heads, self.head_dim = table.shape[0], size, heads, dim
-        self.capacity = table.shape[1] * size
+        self.batch, self.page_size, self.num_kv_heads, self.head_dim = table.shape[0], k.shape[2], k.shape[1], k.shape[3]
+        self.capacity = table.shape[1] * self.page_size
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -108,6 +124,69 @@ class PagedKVCache:
             torch.minimum(self._lengths, lengths.to(self._lengths), out=self._lengths)
         else:
             self._lengths.clamp_(max=int(lengths))
+
+
+class PagedKVCache8(PagedKVCache):
+    """A cache in 8 bits.  ``k``, ``v``: float8_e4m3fn pages ``[pages, kv_heads, page_size, head_dim]``; ``k_exp``,
+    ``v_exp``: int8 ``[pages, kv_heads]`` exponents; a slot stands for its value times 2^exponent.  ``dtype``: bf16 or
+    fp16, of the rows that are appended and attended with.
+
+    ``kv_append`` gives a page and head the least exponent under which its new values fit e4m3, at least -40 and at most
+    40 (beyond 448 * 2^40 values saturate; NaN and infinities become NaN); a page that holds earlier keys keeps its
+    exponent where that is larger, else the earlier keys are rounded again to the new one.  A power of two as the scale
+    costs no precision: e4m3 has an exponent of its own.  Pages that several sequences name are for reading
+    (``PagePool`` copies a shared page before it is written to)."""
+
+    eight = True
+
+    def __init__(self, k: Tensor, v: Tensor, k_exp: Tensor, v_exp: Tensor, table: Tensor, lengths: Tensor,
+                 dtype: torch.dtype = torch.bfloat16):
+        _require(dtype in _DTYPES, "dtype must be bfloat16 or float16")
+        _require(k.dim() == 4 and v.shape == k.shape, "k and v must be [pages, kv_heads, page_size, head_dim], alike")
+        _require(k.dtype == torch.float8_e4m3fn and v.dtype == k.dtype, "k and v must be float8_e4m3fn")
+        pages, heads, size, dim = k.shape
+        _require(size >= 8 and size <= 256 and size & (size - 1) == 0, "page_size must be a power of two in [8, 256]")
+        _require(16 <= dim <= 128 and dim % 16 == 0, "head_dim must be a multiple of 16 up to 128")
+        _require(pages >= 1 and heads >= 1, "the cache needs at least one page and one head")
+        for t in (k, v):
+            _require(t.stride(3) == 1 and all(t.stride(i) > 0 and t.stride(i) % 16 == 0 for i in range(3)),
+                     "the head dimension must be contiguous and the other strides positive multiples of 16")
+            _require(t.data_ptr() % 16 == 0, "k and v must be 16-byte aligned")
+        for t in (k_exp, v_exp):
+            _require(t.shape == (pages, heads) and t.dtype == torch.int8 and (heads == 1 or t.stride(1) == 1)
+                     and (pages == 1 or t.stride(0) >= heads), "k_exp and v_exp must be int8 [pages, kv_heads] with contiguous rows")
+        self._check_table(table, lengths, size)
+        _require(k.device == v.device == k_exp.device == v_exp.device == table.device == lengths.device,
+                 "the cache's tensors must be on one device")
+        self._k, self._v, self._k_exp, self._v_exp = k, v, k_exp, v_exp
+        self._table, self._lengths = table, lengths
+        self._desc = _lib.KvCache8(pages=self._pages_desc(_lib.dtype_code(dtype)), k_exp=k_exp.data_ptr(), v_exp=v_exp.data_ptr(),
+                                   k_exp_stride=max(k_exp.stride(0), heads), v_exp_stride=max(v_exp.stride(0), heads))
+        self._set_up(dtype)
+
+    k_exp = property(lambda self: self._k_exp)
+    v_exp = property(lambda self: self._v_exp)
+
+    @classmethod
+    def allocate(cls, batch: int, max_len: int, num_kv_heads: int, head_dim: int, page_size: int = 64,
+                 dtype: torch.dtype = torch.bfloat16, device=None) -> "PagedKVCache8":
+        """An empty cache in which every sequence owns ceil(max_len / page_size) pages."""
+        device = device or torch.device("cuda", torch.cuda.current_device())
+        per = -(-int(max_len) // page_size)
+        shape = (max(1, batch * per), num_kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
+        k_exp, v_exp = (torch.zeros(shape[:2], dtype=torch.int8, device=device) for _ in range(2))
+        return cls(k, v, k_exp, v_exp, torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per),
+                   torch.zeros(batch, dtype=torch.int32, device=device), dtype=dtype)
+
+    def values(self) -> tuple[Tensor, Tensor]:
+        """What the slots of all pages stand for: keys and values, bf16 ``[pages, kv_heads, page_size, head_dim]``
+        (every such value is exact in bf16)."""
+        lib = _library(self)
+        k, v = (torch.empty(self._k.shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        with _lib.on_device(self.device):
+            check(lib.lng_kv8_values(self._ref, ptr(k), ptr(v), stream_ptr()), "values")
+        return k, v
 
 
 def _strides(t: Tensor, what: str, cache: PagedKVCache) -> tuple[int, int]:
@@ -215,8 +294,9 @@ def kv_append(cache: PagedKVCache, k: Tensor, v: Tensor, q: Tensor | None = None
         raise ValueError("positions must be contiguous int64 of the step's leading shape")
     lib = _library(cache)
     with _lib.on_device(cache.device):
-        check(lib.lng_kv_append(cache._ref, ptr(cu), tokens, max_new, C.byref(kr), C.byref(vr), qr, qo, ptr(positions),
-                                ptr(inv_freq) if rotary else None, rotary, 1 if interleaved else 0, stream_ptr()), "kv_append")
+        append = lib.lng_kv8_append if cache.eight else lib.lng_kv_append
+        check(append(cache._ref, ptr(cu), tokens, max_new, C.byref(kr), C.byref(vr), qr, qo, ptr(positions),
+                     ptr(inv_freq) if rotary else None, rotary, 1 if interleaved else 0, stream_ptr()), "kv_append")
     return q_out
 
 
@@ -267,10 +347,12 @@ def kv_attend(cache: PagedKVCache, q: Tensor, *, cu: Tensor | None = None, max_n
     window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
     lib = _library(cache)
     with _lib.on_device(cache.device):
-        ws = _workspace(cache, (tokens, max_new, max_len, heads, window, sinks), lambda: lib.lng_kv_attend_workspace_bytes(
+        attend, need = (lib.lng_kv8_attend, lib.lng_kv8_attend_workspace_bytes) if cache.eight else \
+            (lib.lng_kv_attend, lib.lng_kv_attend_workspace_bytes)
+        ws = _workspace(cache, (tokens, max_new, max_len, heads, window, sinks), lambda: need(
             cache._ref, tokens, max_new, max_len, heads, window, sinks))
-        check(lib.lng_kv_attend(cache._ref, ptr(cu), tokens, max_new, max_len, C.byref(qr), scale, window, sinks,
-                                C.byref(orow), ptr(ws), 0 if ws is None else ws.numel(), stream_ptr()), "kv_attend")
+        check(attend(cache._ref, ptr(cu), tokens, max_new, max_len, C.byref(qr), scale, window, sinks,
+                     C.byref(orow), ptr(ws), 0 if ws is None else ws.numel(), stream_ptr()), "kv_attend")
     return out
 
 
@@ -282,7 +364,9 @@ def kv_prefix_attend(cache: PagedKVCache, q: Tensor, prefix_table: Tensor, prefi
     ``lengths`` hold what each sequence adds to it.  The prefix is read once for the whole batch.  ``kv_append``'s own
     positions count a sequence's own keys only: behind a prefix give it ``positions`` that count the prefix too
     (prefix_len + the key's place).  The prefix itself is appended once, through a cache of one sequence over the same
-    pages whose table is ``prefix_table``.  No gradients."""
+    pages whose table is ``prefix_table``.  Not for a cache in 8 bits (a ``PagePool`` shares its pages).  No gradients."""
+    if cache.eight:
+        raise ValueError("kv_prefix_attend takes a cache in 16 bits")
     tokens, max_new, max_len, qr, heads, scale, out, orow = _attend_args(cache, q, cu, max_new, max_len, scale, out)
     prefix_len = int(prefix_len)
     if not 0 <= prefix_len < 1 << 30:

@@ -12,7 +12,8 @@
   device-side ancestor table (``ancestor_table``).
 
 ``MemoryCache`` holds the memory part of the reference's ``DecodeState`` (``ffnmem/infer.py:65-112``):
-codes [B, max_len, R] and conv inputs [B, max_len, d], indexed by absolute position.
+codes [B, max_len, R] and conv inputs [B, max_len, d], indexed by absolute position; ``MemoryCache.reorder`` is
+beam search's reordering of its rows.
 """
 
 from __future__ import annotations
@@ -22,6 +23,7 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import check, ptr, stream_ptr
+from .beams import beam_reorder
 
 
 class MemoryCache:
@@ -36,6 +38,11 @@ class MemoryCache:
         if not 0 <= length <= self.length:
             raise ValueError(f"cannot truncate to {length} (length {self.length})")
         self.length = length
+
+    def reorder(self, parents: Tensor) -> None:
+        """Beam search's reordering, in place: row g * beams + k takes over the codes and conv inputs of row
+        g * beams + parents[g, k] (int64 ``[groups, beams]``, ``beam_select``'s)."""
+        beam_reorder(parents, self.codes, self.conv_in, length=self.length)
 
 
 _ANCESTORS: dict = {}
