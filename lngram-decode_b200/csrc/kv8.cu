@@ -1,5 +1,6 @@
 // The C ABI's entries of the paged cache in 8 bits (include/lngram_b200.h).
 #include "kv8.cuh"
+#include "kv8_step.cuh"
 #include "kv_host.cuh"
 
 namespace lng {
@@ -23,6 +24,61 @@ static int check_kv8(const lng_kv8_cache* c, const int32_t* cu, int64_t tokens, 
 
 static Kv8View kv8_view(const lng_kv8_cache* c, const int32_t* cu, int64_t tokens, int64_t max_new) {
   return Kv8View{kv_view(&c->pages, cu, tokens, max_new), c->k_exp, c->v_exp, c->k_exp_stride, c->v_exp_stride};
+}
+
+// The tensor map of the pages' bytes: one head's slots of one page a copy, the whole head wide (columns behind head_dim
+// fill with zeros), rows of 64 or 128 bytes.
+static int kv8_page_map(CUtensorMap* map, const lng_kv_cache& c, void* base, int64_t page, int64_t head, int64_t slot, int box) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (driver entry point)");
+  const bool wide = c.head_dim > 64;
+  const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.page_size), cuuint64_t(c.num_kv_heads), cuuint64_t(c.num_pages)};
+  const cuuint64_t strides[3] = {cuuint64_t(slot), cuuint64_t(head), cuuint64_t(page)};
+  const cuuint32_t box4[4] = {wide ? 128u : 64u, cuuint32_t(box), 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box4, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LNG_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+  return LNG_OK;
+}
+static int kv8_page_maps(CUtensorMap* k, CUtensorMap* v, const lng_kv_cache& c, int box) {
+  const int st = kv8_page_map(k, c, c.k, c.k_page_stride, c.k_head_stride, c.k_slot_stride, box);
+  return st ? st : kv8_page_map(v, c, c.v, c.v_page_stride, c.v_head_stride, c.v_slot_stride, box);
+}
+
+// How an attention call is carried out, and what it needs of the workspace.
+struct Kv8Plan {
+  bool step;         // by kv8_step_kernel (few rows a key head)
+  int shares;        // into which its work is cut
+  bool warp_shares;  // a share a warp, not a CTA
+  size_t piece_ml, piece_o, bytes;
+};
+static Kv8Plan kv8_plan(const lng_kv8_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len, int32_t q_heads, int32_t window,
+                        int32_t sinks) {
+  Kv8Plan p{};
+  if (!cache || tokens <= 0 || cache->pages.batch <= 0 || cache->pages.num_kv_heads <= 0 || q_heads < cache->pages.num_kv_heads || max_new <= 0)
+    return p;
+  const lng_kv_cache& c = cache->pages;
+  const int64_t group = q_heads / c.num_kv_heads;
+  p.step = group * max_new <= KS_ROWS;
+  if (!p.step) return p;
+  // (many pairs: a share a warp; few pairs: a share a CTA, which leaves an eighth of the pieces to join: kv_plan's rule)
+  p.warp_shares = c.batch * c.num_kv_heads >= num_sms();
+  p.shares = num_sms() * (p.warp_shares ? K8sCfg<128>::WARPS : 1);
+  const size_t pieces = size_t(2) * p.shares * KS_ROWS;
+  p.piece_o = al256(pieces * 8);
+  p.bytes = p.piece_o + al256(pieces * c.head_dim * 4);
+  return p;
+}
+
+template <typename T, int HDP, bool WS>
+static int launch_kv8_step(const CUtensorMap& tk, const CUtensorMap& tv, const K8sParams& p, cudaStream_t s) {
+  using Cfg = K8sCfg<HDP>;
+  auto kern = kv8_step_kernel<T, HDP, WS>;
+  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  kern<<<unsigned(p.s.shares / (WS ? Cfg::WARPS : 1)), Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
+  LNG_LAUNCHED("kv8_step_kernel");
+  return launch_dependent(kv_step_join_kernel<T, Cfg::BK>, unsigned(p.s.c.batch * p.s.c.kv_heads), 256u, size_t(0), s, p.s);
 }
 
 }  // namespace lng
@@ -119,7 +175,7 @@ extern "C" int lng_kv8_values(const lng_kv8_cache* cache, void* k_out, void* v_o
 
 extern "C" size_t lng_kv8_attend_workspace_bytes(const lng_kv8_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
                                                  int32_t q_heads, int32_t window, int32_t sinks) {
-  return 0;
+  return kv8_plan(cache, tokens, max_new, max_len, q_heads, window, sinks).bytes;
 }
 
 extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,
@@ -139,6 +195,37 @@ extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int
   if ((st = check_kv_rows(out, q->heads, "out"))) return st;
   LNG_REQUIRE(out->ptr != q->ptr, "out must not overlap q");
   LNG_REQUIRE(c.batch * c.num_kv_heads < (int64_t(1) << 31), "batch * num_kv_heads must be below 2^31");
+  const Kv8Plan plan = kv8_plan(cache, tokens, max_new, max_len, q->heads, window, sinks);
+  LNG_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
+              "workspace must be 256-byte aligned");
+  LNG_REQUIRE(workspace_bytes >= plan.bytes, "workspace too small");
+  if (plan.step) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    K8sParams p{};
+    p.s.c = kv_view(&c, cu, tokens, max_new);
+    p.s.q = kv_rows(q), p.s.o = kv_rows(out);
+    p.s.q_heads = q->heads;
+    p.s.group = q->heads / c.num_kv_heads;
+    p.s.scale_log2 = scale_log2;
+    p.s.window = std::min(window, 1 << 30);
+    p.s.sinks = std::min(sinks, 1 << 30);
+    p.s.box = std::min(c.page_size, K8sCfg<64>::BK);
+    p.s.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
+    p.s.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
+    p.s.shares = plan.shares;
+    p.k_exp = cache->k_exp, p.v_exp = cache->v_exp;
+    p.k_exp_page = cache->k_exp_stride, p.v_exp_page = cache->v_exp_stride;
+    CUtensorMap tk, tv;
+    if ((st = kv8_page_maps(&tk, &tv, c, p.s.box))) return st;
+    const bool wide = c.head_dim > 64;
+    auto launch = [&](auto type) {
+      using T = decltype(type);
+      if (plan.warp_shares)
+        return wide ? launch_kv8_step<T, 128, true>(tk, tv, p, S(stream)) : launch_kv8_step<T, 64, true>(tk, tv, p, S(stream));
+      return wide ? launch_kv8_step<T, 128, false>(tk, tv, p, S(stream)) : launch_kv8_step<T, 64, false>(tk, tv, p, S(stream));
+    };
+    return c.dtype == LNG_BF16 ? launch(__nv_bfloat16()) : launch(__half());
+  }
   K8RowParams p{};
   p.v = kv8_view(cache, cu, tokens, max_new);
   p.q = kv_rows(q), p.o = kv_rows(out);
