@@ -1,6 +1,7 @@
 // The C ABI's entries of the paged cache in 8 bits (include/lngram_b200.h).
 #include "kv8.cuh"
 #include "kv8_step.cuh"
+#include "kv8_tile.cuh"
 #include "kv_host.cuh"
 
 namespace lng {
@@ -51,7 +52,9 @@ struct Kv8Plan {
   bool step;         // by kv8_step_kernel (few rows a key head)
   int shares;        // into which its work is cut
   bool warp_shares;  // a share a warp, not a CTA
-  size_t piece_ml, piece_o, bytes;
+  int64_t units;     // else by kv8_tile_kernel: its units per key head and range of keys
+  int splits;        // key ranges, whose states are joined when there are several
+  size_t ml, o, bytes;  // states: of the step kernel's pieces, or of the rows in every range
 };
 static Kv8Plan kv8_plan(const lng_kv8_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len, int32_t q_heads, int32_t window,
                         int32_t sinks) {
@@ -60,14 +63,25 @@ static Kv8Plan kv8_plan(const lng_kv8_cache* cache, int64_t tokens, int64_t max_
     return p;
   const lng_kv_cache& c = cache->pages;
   const int64_t group = q_heads / c.num_kv_heads;
-  p.step = group * max_new <= KS_ROWS;
-  if (!p.step) return p;
-  // (many pairs: a share a warp; few pairs: a share a CTA, which leaves an eighth of the pieces to join: kv_plan's rule)
-  p.warp_shares = c.batch * c.num_kv_heads >= num_sms();
-  p.shares = num_sms() * (p.warp_shares ? K8sCfg<128>::WARPS : 1);
-  const size_t pieces = size_t(2) * p.shares * KS_ROWS;
-  p.piece_o = al256(pieces * 8);
-  p.bytes = p.piece_o + al256(pieces * c.head_dim * 4);
+  size_t states = 0;
+  p.step = group * max_new <= KS_ROWS && (group * max_new <= 4 || c.batch * c.num_kv_heads * 16 >= num_sms());
+  if (p.step) {
+    // (many pairs: a share a warp; few pairs: a share a CTA, which leaves an eighth of the pieces to join: kv_plan's rule)
+    p.warp_shares = c.batch * c.num_kv_heads >= num_sms();
+    p.shares = num_sms() * (p.warp_shares ? K8sCfg<128>::WARPS : 1);
+    states = size_t(2) * p.shares * KS_ROWS;
+  } else {
+    const int64_t span = 2 * std::max<int64_t>(1, KT_BM / group);
+    int64_t keys = c.max_pages * c.page_size;
+    if (max_len > 0) keys = std::min(keys, max_len);
+    if (window > 0) keys = std::min(keys, int64_t(window) + sinks + span + KT_BK);
+    // ragged steps: at most one unit a sequence is not full
+    p.units = std::min(c.batch * ceil_div(max_new, span), tokens / span + std::min(c.batch, tokens));
+    p.splits = kv_splits(p.units * c.num_kv_heads, std::max<int64_t>(1, ceil_div(keys, KT_BK)));
+    if (p.splits > 1) states = size_t(p.splits) * tokens * q_heads;
+  }
+  p.o = al256(states * 8);
+  p.bytes = p.o + al256(states * c.head_dim * 4);
   return p;
 }
 
@@ -79,6 +93,18 @@ static int launch_kv8_step(const CUtensorMap& tk, const CUtensorMap& tv, const K
   kern<<<unsigned(p.s.shares / (WS ? Cfg::WARPS : 1)), Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
   LNG_LAUNCHED("kv8_step_kernel");
   return launch_dependent(kv_step_join_kernel<T, Cfg::BK>, unsigned(p.s.c.batch * p.s.c.kv_heads), 256u, size_t(0), s, p.s);
+}
+
+template <typename T, int HDP>
+static int launch_kv8_tile(const CUtensorMap& tk, const CUtensorMap& tv, const K8tParams& p, cudaStream_t s) {
+  using Cfg = K8tCfg<HDP>;
+  auto kern = kv8_tile_kernel<T, HDP>;
+  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  kern<<<unsigned(std::min<int64_t>(p.t.total, num_sms())), K8T_THREADS, Cfg::SMEM, s>>>(tk, tv, p);
+  LNG_LAUNCHED("kv8_tile_kernel");
+  if (p.t.row_ml == nullptr) return LNG_OK;
+  return launch_dependent(kv_rows_join_kernel<T>, unsigned(ceil_div(p.t.c.tokens * p.t.q_heads, 8)), 256u, size_t(0), s, p.t.c,
+                          p.t.q_heads, static_cast<const float2*>(p.t.row_ml), static_cast<const float*>(p.t.row_o), p.t.splits, p.t.o);
 }
 
 }  // namespace lng
@@ -210,8 +236,8 @@ extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int
     p.s.window = std::min(window, 1 << 30);
     p.s.sinks = std::min(sinks, 1 << 30);
     p.s.box = std::min(c.page_size, K8sCfg<64>::BK);
-    p.s.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
-    p.s.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
+    p.s.piece_ml = reinterpret_cast<float2*>(ws + plan.ml);
+    p.s.piece_o = reinterpret_cast<float*>(ws + plan.o);
     p.s.shares = plan.shares;
     p.k_exp = cache->k_exp, p.v_exp = cache->v_exp;
     p.k_exp_page = cache->k_exp_stride, p.v_exp_page = cache->v_exp_stride;
@@ -226,19 +252,32 @@ extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int
     };
     return c.dtype == LNG_BF16 ? launch(__nv_bfloat16()) : launch(__half());
   }
-  K8RowParams p{};
-  p.v = kv8_view(cache, cu, tokens, max_new);
-  p.q = kv_rows(q), p.o = kv_rows(out);
-  p.q_heads = q->heads;
-  p.group = q->heads / c.num_kv_heads;
-  p.scale_log2 = scale_log2;
-  p.window = std::min(window, 1 << 30);
-  p.sinks = std::min(sinks, 1 << 30);
-  const unsigned grid = unsigned(ceil_div(tokens * q->heads, 8));
-  if (c.dtype == LNG_BF16)
-    kv8_row_kernel<__nv_bfloat16><<<grid, 256, 0, S(stream)>>>(p);
-  else
-    kv8_row_kernel<__half><<<grid, 256, 0, S(stream)>>>(p);
-  LNG_LAUNCHED("kv8_row_kernel");
-  return LNG_OK;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  K8tParams p{};
+  p.t.c = kv_view(&c, cu, tokens, max_new);
+  p.t.o = kv_rows(out);
+  p.q = kv_rows(q);
+  p.t.q_heads = q->heads;
+  p.t.group = q->heads / c.num_kv_heads;
+  p.t.tile_tokens = KT_BM / p.t.group;
+  p.t.scale_log2 = scale_log2;
+  p.t.window = std::min(window, 1 << 30);
+  p.t.sinks = std::min(sinks, 1 << 30);
+  p.t.box = std::min(c.page_size, KT_BK);
+  p.t.splits = plan.splits;
+  p.t.total = plan.units * c.num_kv_heads * plan.splits;
+  if (plan.splits > 1) {
+    p.t.row_ml = reinterpret_cast<float2*>(ws + plan.ml);
+    p.t.row_o = reinterpret_cast<float*>(ws + plan.o);
+  }
+  p.k_exp = cache->k_exp, p.v_exp = cache->v_exp;
+  p.k_exp_page = cache->k_exp_stride, p.v_exp_page = cache->v_exp_stride;
+  CUtensorMap tk, tv;
+  if ((st = kv8_page_maps(&tk, &tv, c, p.t.box))) return st;
+  const bool wide = c.head_dim > 64;
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    return wide ? launch_kv8_tile<T, 128>(tk, tv, p, S(stream)) : launch_kv8_tile<T, 64>(tk, tv, p, S(stream));
+  };
+  return c.dtype == LNG_BF16 ? launch(__nv_bfloat16()) : launch(__half());
 }

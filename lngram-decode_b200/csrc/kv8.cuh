@@ -295,78 +295,4 @@ __global__ void __launch_bounds__(256)
   __stcs(out + 2 * x + 1, make_uint4(r[4], r[5], r[6], r[7]));
 }
 
-// ------------------------------------------------------------------ attention, a warp a row
-struct K8RowParams {
-  Kv8View v;
-  KvRows q, o;
-  int32_t q_heads, group;
-  float scale_log2;
-  int32_t window, sinks;
-};
-
-// The simplest form: a warp takes a (token, head) row, its lanes four columns each, one key after another.
-template <typename T>
-__global__ void __launch_bounds__(256) kv8_row_kernel(const K8RowParams p) {
-  const KvView& c = p.v.c;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 5, token = row / p.q_heads;
-  if (token >= c.tokens) return;
-  const int head = int(row - token * p.q_heads), h = head / p.group, col = lane * 4;
-  const int64_t b = kv_sequence_of(c, token);
-  if (b < 0 || b >= c.batch) return;
-  const SeqSpan s = kv_span(c, b);
-  const int64_t i = token - s.first;
-  if (i < 0 || i >= s.n) return;
-  const int32_t pos = s.len - s.n + int32_t(i);
-  const bool on = col < c.head_dim;
-  float q[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  if (on) {
-    const T* src = static_cast<const T*>(p.q.ptr) + token * p.q.token + head * p.q.head + col;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) q[x] = to_f32<T>(src[x]) * p.scale_log2;
-  }
-  bool bad = false;
-  const KeySpan span = key_span(pos, pos, p.window, p.sinks);
-  for (int32_t j = span.sink_end > 0 ? 0 : span.lo; j < span.hi; j = j + 1 == span.sink_end ? span.lo : j + 1) {
-    const int32_t page = page_of(c.table + b * c.table_stride, j, c.page_shift, c.num_pages);
-    const int32_t slot = j & ((1 << c.page_shift) - 1);
-    float x = 0.f;
-    uint32_t kw = 0, vw = 0;
-    float fk = 0.f, fv = 0.f;
-    if (page >= 0) {
-      fk = exp2_whole(p.v.k_exp[page * p.v.k_exp_page + h]);
-      fv = exp2_whole(p.v.v_exp[page * p.v.v_exp_page + h]);
-      if (on) {
-        kw = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.k) + page * c.k_page + h * c.k_head + slot * c.k_slot + col);
-        vw = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(c.v) + page * c.v_page + h * c.v_head + slot * c.v_slot + col);
-      }
-    } else {
-      kv_range_error();
-    }
-    const float2 k0 = k8_floats(kw & 0xffffu), k1 = k8_floats(kw >> 16), v0 = k8_floats(vw & 0xffffu), v1 = k8_floats(vw >> 16);
-    x = warp_sum(q[0] * k0.x + q[1] * k0.y + q[2] * k1.x + q[3] * k1.y) * fk;
-    if (!(x < INFINITY)) bad = true;  // NaN or +inf
-    if (x == -INFINITY) continue;
-    if (x > m) {
-      const float f = m == -INFINITY ? 0.f : exp2f(m - x);
-      l *= f;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) o[y] *= f;
-      m = x;
-    }
-    const float w = exp2f(x - m), wv = w * fv;
-    l += w;
-    o[0] += wv * v0.x;
-    o[1] += wv * v0.y;
-    o[2] += wv * v1.x;
-    o[3] += wv * v1.y;
-  }
-  const float inv = bad ? NAN : l == 0.f ? 0.f : 1.f / l;
-  if (on) {
-    T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + col;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) dst[x] = from_f32<T>(o[x] * inv);
-  }
-}
-
 }  // namespace lng

@@ -303,7 +303,7 @@ __device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
 // Wait bounded by time (two seconds; the longest wait of a working kernel is a unit's, milliseconds), which also
 // gives up when another role has -- but for the waits (ALONE) with which a role ends: whatever has happened, its own
 // copies and products must not outlive the CTA.  An expired wait records the device error.
-template <int HDP, bool ALONE = false>
+template <typename B, bool ALONE = false>
 __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t parity) {
   if (mbar_try_at(bars + bar, parity)) return true;
   uint64_t start, now;
@@ -311,12 +311,12 @@ __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t pa
   for (uint32_t i = 0;; ++i) {
     if (mbar_try_at(bars + bar, parity)) return true;
     if ((i & 63) != 63) continue;
-    if (!ALONE && lds32(bars + KtBars<HDP>::abort)) return false;
+    if (!ALONE && lds32(bars + B::abort)) return false;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
     if (now - start > 2000000000ull) break;
   }
   atomicCAS(&g_error_word, 0u, (unsigned int)DEV_ERR_WAIT_TIMEOUT);
-  sts32(bars + KtBars<HDP>::abort, 1u);
+  sts32(bars + B::abort, 1u);
   return false;
 }
 
@@ -452,7 +452,7 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
     };
     int32_t next = look_up(0);
     if (kv == 0) {
-      if (units > 0) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1));
+      if (units > 0) ok = __all_sync(0xffffffffu, kt_wait<B>(bars, B::q_empty, (units - 1) & 1));
       if (!ok) break;
       if (elect_lane()) {
         const int32_t tiles_q = w.tokens1 > 0 ? 2 : 1, q0 = int32_t(w.s.first + w.t0);
@@ -473,7 +473,7 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
       if (i + 1 < w.n) next = look_up(i + 1);
       const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, page >= 0))) * uint32_t(box) * 128u * (HDP / 64);
       const uint32_t s = it % NS, bar = bars + B::kv_full + 8 * s, dst = ring + s * Cfg::KV_BYTES;
-      if (it >= NS) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
+      if (it >= NS) ok = __all_sync(0xffffffffu, kt_wait<B>(bars, B::kv_empty + 8 * s, (it / NS - 1) & 1));
       if (!ok) break;
       if (elect_lane()) mbar_expect_at(bar, bytes);
       __syncwarp();
@@ -499,22 +499,20 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
   // the last uses of the ring's slots: behind them no copy and no product is in flight
   const uint32_t k0 = it >= NS ? it - NS : kv;
   bool used = true;
-  for (uint32_t k = k0; k < it; k += 2) used = kt_wait<HDP>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1) && used;
-  if (kv == 0 && units > 0) used = kt_wait<HDP>(bars, B::q_empty, (units - 1) & 1) && used;
+  for (uint32_t k = k0; k < it; k += 2) used = kt_wait<B>(bars, B::kv_empty + 8 * (k % NS), (k / NS) & 1) && used;
+  if (kv == 0 && units > 0) used = kt_wait<B>(bars, B::q_empty, (units - 1) & 1) && used;
   if (__all_sync(0xffffffffu, used)) return;
   // (a role has given up: behind the copies themselves)
-  for (uint32_t k = k0; k < it; k += 2) kt_wait<HDP, true>(bars, B::kv_full + 8 * (k % NS), (k / NS) & 1);
-  if (kv == 0 && units > 0) kt_wait<HDP, true>(bars, B::q_full, (units - 1) & 1);
+  for (uint32_t k = k0; k < it; k += 2) kt_wait<B, true>(bars, B::kv_full + 8 * (k % NS), (k / NS) & 1);
+  if (kv == 0 && units > 0) kt_wait<B, true>(bars, B::q_full, (units - 1) & 1);
 }
 
 // One warp a row tile issues its products: the scores of the next key tile (into the other of two S buffers) ahead
 // of O += P V of this one, so that the softmax finds its scores waiting.  P lies over its tile's scores; a product's
 // operands are only overwritten once an mbarrier has shown it done (the ISA orders products of unlike operands
 // through their completion alone).
-template <typename T, int HDP>
+template <typename T, int HDP, typename Cfg = KtCfg<HDP>, typename B = KtBars<HDP>>
 __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, uint32_t qs, uint32_t ring, int G) {
-  using Cfg = KtCfg<HDP>;
-  using B = KtBars<HDP>;
   constexpr uint32_t NS = Cfg::SLOTS;
   const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
   const uint32_t pv_bar = B::pv_done + 8 * G;
@@ -524,8 +522,8 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
   auto scores = [&](uint32_t ik, uint32_t t) -> bool {
     const uint32_t sk = ik % NS;
     // (the values too: whoever has seen the scores may touch them)
-    const bool good = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sk, (ik / NS) & 1) &&
-                                                  kt_wait<HDP>(bars, B::kv_full + 8 * ((ik + 1) % NS), ((ik + 1) / NS) & 1));
+    const bool good = __all_sync(0xffffffffu, kt_wait<B>(bars, B::kv_full + 8 * sk, (ik / NS) & 1) &&
+                                                  kt_wait<B>(bars, B::kv_full + 8 * ((ik + 1) % NS), ((ik + 1) / NS) & 1));
     tc_fence_after();
     if (good && elect_lane()) {
       const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
@@ -545,12 +543,12 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
   while (ok && kt_next(p, walk, w, there)) {
     if (!there || w.n == 0) continue;
     const int32_t cnt = G ? w.cnt1 : w.cnt0;
-    ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::q_full, units & 1));
+    ok = __all_sync(0xffffffffu, kt_wait<B>(bars, B::q_full, units & 1));
     ++units;
     if (cnt > 0 && ok) ok = scores(base, tile);
 #pragma unroll 1
     for (int32_t i = 0; i < cnt && ok; ++i) {
-      if (tile + i > 0) ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, pv_bar, (tile + i - 1) & 1));
+      if (tile + i > 0) ok = __all_sync(0xffffffffu, kt_wait<B>(bars, pv_bar, (tile + i - 1) & 1));
       if (i + 1 < cnt) {
         ok = ok && scores(base + 2 * (i + 1), tile + i + 1);
       } else if (elect_lane()) {
@@ -558,7 +556,7 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
       }
       __syncwarp();
       const uint32_t iv = base + 2 * i + 1, sv = iv % NS, t = tile + i;
-      ok = __all_sync(0xffffffffu, ok && kt_wait<HDP>(bars, B::p_full + 16 * G + 8 * (t & 1), (t >> 1) & 1));
+      ok = __all_sync(0xffffffffu, ok && kt_wait<B>(bars, B::p_full + 16 * G + 8 * (t & 1), (t >> 1) & 1));
       tc_fence_after();
       if (ok && elect_lane()) {
         const uint32_t idesc = umma_idesc<T>(KT_BM, 64, true);
@@ -581,7 +579,7 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
     // last use by the other row tile may still be going on)
     for (uint32_t k = base + 2 * cnt; k < base + 2 * w.n && ok; ++k) {
       const uint32_t sl = k % NS;
-      ok = __all_sync(0xffffffffu, kt_wait<HDP>(bars, B::kv_full + 8 * sl, (k / NS) & 1));
+      ok = __all_sync(0xffffffffu, kt_wait<B>(bars, B::kv_full + 8 * sl, (k / NS) & 1));
       if (ok && elect_lane()) mbar_arrive_at(bars + B::kv_empty + 8 * sl);
       __syncwarp();
     }
@@ -592,7 +590,7 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
   if (__any_sync(0xffffffffu, !ok || lds32(bars + B::abort) != 0)) {
     if (elect_lane()) umma_commit_at(bars + B::idle + 8 * G);
     __syncwarp();
-    kt_wait<HDP, true>(bars, B::idle + 8 * G, 0);
+    kt_wait<B, true>(bars, B::idle + 8 * G, 0);
   }
 }
 
@@ -697,7 +695,7 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32
     for (int32_t i = 0; i < cnt; ++i) {
       const uint32_t t = tile + i;
       const int32_t key0 = tile_index(w.tiles, w.j0 + i) * KT_BK;
-      ok = ok && kt_wait<HDP>(bars, B::s_full + 16 * G + 8 * (t & 1), (t >> 1) & 1);
+      ok = ok && kt_wait<B>(bars, B::s_full + 16 * G + 8 * (t & 1), (t >> 1) & 1);
       if (!all_needed(w.span, key0, key0 + KT_BK)) {
         // slots that no row sees may hold anything: zero weights must not meet a NaN among the values (both row
         // tiles clear them, each before its own product)
@@ -731,7 +729,7 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32
       if (i > 0 && __any_sync(0xffffffffu, grow)) {
         const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
         l *= f;
-        ok = ok && kt_wait<HDP>(bars, pv_bar, (t - 1) & 1);  // the product before this one is done with O
+        ok = ok && kt_wait<B>(bars, pv_bar, (t - 1) & 1);  // the product before this one is done with O
         __syncwarp();
         tc_fence_after();
 #pragma unroll 1
@@ -763,7 +761,7 @@ __device__ __forceinline__ void kt_rows(const KtParams& p, uint32_t bars, uint32
     const bool any = cnt > 0;
     tile += cnt;
     base += 2 * w.n;
-    if (any) ok = ok && kt_wait<HDP>(bars, B::o_full + 8 * G, results++ & 1);
+    if (any) ok = ok && kt_wait<B>(bars, B::o_full + 8 * G, results++ & 1);
     __syncwarp();
     tc_fence_after();
     kt_result<T, HDP>(p, w, to, stage, G, quad, any, __all_sync(0xffffffffu, ok), m, l);
