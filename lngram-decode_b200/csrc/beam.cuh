@@ -1,6 +1,8 @@
 // Beam search: the best continuations over a group's beams and the vocabulary, and the states' reordering.
 #pragma once
 
+#include <type_traits>
+
 #include "kvcache.cuh"
 
 namespace lng {
@@ -67,13 +69,11 @@ struct BeamList {
 // 16 bytes of values from any address that their type allows: one load, or four or five of a word each (of two-byte
 // values at an odd place the first and the last word reach over the values by one).
 template <typename T>
-__device__ __forceinline__ void beam_vector(const T* src, float (&x)[16 / sizeof(T)]) {
+__device__ __forceinline__ uint4 beam_vector(const T* src) {
   const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(src)) & 15u;
+  if (off == 0) return __ldcs(reinterpret_cast<const uint4*>(src));
   uint32_t w[4];
-  if (off == 0) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(src));
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else if ((off & 3u) == 0) {
+  if ((off & 3u) == 0) {
 #pragma unroll
     for (int y = 0; y < 4; ++y) w[y] = reinterpret_cast<const uint32_t*>(src)[y];
   } else {
@@ -86,17 +86,60 @@ __device__ __forceinline__ void beam_vector(const T* src, float (&x)[16 / sizeof
       lo = hi;
     }
   }
-  const T* e = reinterpret_cast<const T*>(w);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The bits of -inf, and a value among the bits of a vector.
+template <typename T>
+__device__ __forceinline__ uint32_t beam_low();
+template <>
+__device__ __forceinline__ uint32_t beam_low<float>() { return 0xff800000u; }
+template <>
+__device__ __forceinline__ uint32_t beam_low<__nv_bfloat16>() { return 0xff80u; }
+template <>
+__device__ __forceinline__ uint32_t beam_low<__half>() { return 0xfc00u; }
+
+// The lane's value among all 32, in falling order.
+__device__ __forceinline__ float beam_sorted(float x, int lane) {
 #pragma unroll
-  for (int y = 0; y < 16 / int(sizeof(T)); ++y) x[y] = to_f32<T>(e[y]);
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, j);
+      const bool larger = ((lane & j) == 0) == ((lane & k) == 0 || k == 32);
+      x = larger ? fmaxf(x, y) : fminf(x, y);
+    }
+  return x;
+}
+
+// e^d for d <= 0.  (log2(e) in fp32 is off by 2^-26 of itself: a row's log of the sum by 1.4e-8 of the mean |d|, which is a
+// few units, and beams of one group by nearly the same.)
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float beam_exp(float d) { return exp2_approx(d * 1.44269502f); }
+
+// The largest of a vector's values (of two at a time where they have two bytes; a NaN only where all are).
+template <typename T>
+__device__ __forceinline__ float beam_top(uint4 w) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  } else {
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const P m = __hmax2(__hmax2(*reinterpret_cast<const P*>(&w.x), *reinterpret_cast<const P*>(&w.y)),
+                        __hmax2(*reinterpret_cast<const P*>(&w.z), *reinterpret_cast<const P*>(&w.w)));
+    return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
+  }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(BS_THREADS) beam_piece_kernel(const BeamParams p) {
-  constexpr int N = 16 / sizeof(T);
+__global__ void __launch_bounds__(BS_THREADS, 4) beam_piece_kernel(const BeamParams p) {
+  constexpr int N = 16 / sizeof(T), U = 2;  // values a load, loads a round
   __shared__ float2 sums[BS_WARPS];
   __shared__ float lv[BS_WARPS][BS_MOST];
   __shared__ int32_t li[BS_WARPS][BS_MOST];
+  __shared__ float sure[BS_WARPS];  // of each warp's values `share` at least are not below its entry
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, last = p.width - 1;
   const int64_t row = blockIdx.x / p.pieces;
   const int32_t piece = int32_t(blockIdx.x - row * p.pieces);
@@ -104,99 +147,179 @@ __global__ void __launch_bounds__(BS_THREADS) beam_piece_kernel(const BeamParams
   const int64_t v0 = piece * p.piece, v1 = v0 + p.piece < p.vocab ? v0 + p.piece : p.vocab;
   // vectors begin at the piece's first value wherever that lies, so that equal rows have equal sums and tie; those that
   // reach over the piece's end, or whose words might reach over the logits, are taken value by value
-  const int64_t vecs = v1 > v0 ? (v1 - v0 + N - 1) / N : 0;
-  const int64_t safe0 = row > 0 ? 0 : 1, safe1 = row + 1 < p.groups * p.beams ? v1 : (v1 < p.vocab ? v1 : v1 - 1);
-  const bool odd = (reinterpret_cast<uintptr_t>(src) & 3) != 0;
+  const int32_t count = v1 > v0 ? int32_t(v1 - v0) : 0, vecs = (count + N - 1) / N, begin = int32_t(v0);
+  const T* const at0 = src + v0;
+  const bool wide = (reinterpret_cast<uintptr_t>(at0) & 15) == 0, odd = (reinterpret_cast<uintptr_t>(at0) & 3) != 0;
+  const int32_t full = wide ? count / N : 0;  // vectors that one load takes
   BeamList<float> list;
   list.clear();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int share = (p.width + BS_WARPS - 1) / BS_WARPS;
+  // so `width` of the CTA's values at least are not below the smallest entry: nothing below that is among the best
+  auto floor_of = [&]() {
+    float f = const_cast<volatile float*>(sure)[lane & (BS_WARPS - 1)];
+#pragma unroll
+    for (int o = 1; o < BS_WARPS; o <<= 1) f = fminf(f, __shfl_xor_sync(0xffffffffu, f, o));
+    return f;
+  };
   float m = -INFINITY, s = 0.f;
   // (all lanes of a warp stay together: the list is the warp's)
-  for (int64_t k0 = int64_t(warp) * 32; k0 < vecs; k0 += BS_THREADS) {
-    const int64_t k = k0 + lane, at = v0 + k * N;
-    float x[N];
-    if (at + N <= v1 && (!odd || (at >= safe0 && at + N <= safe1))) {
-      beam_vector<T>(src + at, x);
-    } else {
+  bool fresh = true;
+  auto slow = [&](int32_t k) -> uint4 {  // vector k of the piece, -inf behind its end
+    const int32_t at = k * N;
+    if (at + N <= count && (!odd || ((at > 0 || v0 > 0 || row > 0) && (at + N < count || v1 < p.vocab || row + 1 < p.groups * p.beams))))
+      return beam_vector<T>(at0 + at);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int y = 0; y < N; ++y) x[y] = at + y < v1 ? to_f32<T>(src[at + y]) : -INFINITY;
+    for (int y = 0; y < N; ++y) {
+      uint32_t bits = beam_low<T>();
+      if (at + y < count) {
+        if constexpr (sizeof(T) == 4)
+          bits = reinterpret_cast<const uint32_t*>(at0)[at + y];
+        else
+          bits = reinterpret_cast<const uint16_t*>(at0)[at + y];
+      }
+      w[y * int(sizeof(T)) / 4] |= bits << (8 * (y * int(sizeof(T)) & 3));
     }
-    float top = x[0];
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  auto load = [&](int32_t k) -> uint4 { return k < full ? __ldcs(reinterpret_cast<const uint4*>(at0) + k) : slow(k); };
+  uint4 ahead[U];  // the next round's
+  const int32_t first = warp * (32 * U) + lane;
 #pragma unroll
-    for (int y = 1; y < N; ++y) top = fmaxf(top, x[y]);
+  for (int u = 0; u < U; ++u) ahead[u] = load(first + u * 32);
+  for (int32_t k0 = warp * (32 * U); fresh || k0 < vecs; k0 += BS_WARPS * 32 * U) {
+    float x[U][N], top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint4 w = ahead[u];
+      top = fmaxf(top, beam_top<T>(w));
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int y = 0; y < N; ++y) x[u][y] = to_f32<T>(e[y]);
+      if (k0 + BS_WARPS * 32 * U < vecs) ahead[u] = load(k0 + BS_WARPS * 32 * U + u * 32 + lane);
+    }
     if (top > m) {
-      s *= m == -INFINITY ? 0.f : __expf(m - top);
+      s *= m == -INFINITY ? 0.f : beam_exp(m - top);
       m = top;
     }
     const float ref = m == -INFINITY ? 0.f : m;
+    const uint64_t less = f2_pack(-ref, -ref), log2e = f2_pack(1.44269502f, 1.44269502f);
+    uint64_t some[2] = {0, 0};
 #pragma unroll
-    for (int y = 0; y < N; ++y) s += __expf(x[y] - ref);
-    if (__any_sync(0xffffffffu, top >= __shfl_sync(0xffffffffu, list.v, last))) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int y = 0; y < N; ++y) {
-        // (a NaN ranks as -inf; a row that holds one offers nothing in the end)
-        list.offer(at + y < v1, x[y] == x[y] ? x[y] : -INFINITY, int32_t(at + y), last);
+      for (int y = 0; y < N; y += 2) {
+        float a, b;
+        f2_unpack(f2_mul(f2_add(f2_pack(x[u][y], x[u][y + 1]), less), log2e), a, b);
+        some[y >> 1 & 1] = f2_add(some[y >> 1 & 1], f2_pack(exp2_approx(a), exp2_approx(b)));
       }
+    {
+      float a, b, c, d;
+      f2_unpack(some[0], a, b);
+      f2_unpack(some[1], c, d);
+      s += (a + b) + (c + d);
+    }
+    float bar;
+    if (fresh) {  // (every warp once: with none of the lists filled, the lanes' largest values tell what to look for)
+      const float sorted = beam_sorted(top, lane);
+      if (lane == share - 1) sure[warp] = sorted;
+      bar = __shfl_sync(0xffffffffu, sorted, last);
+      fresh = false;
+      __syncthreads();
+    } else {
+      bar = __shfl_sync(0xffffffffu, list.v, last);
+    }
+    bar = fmaxf(bar, floor_of());
+    if (__any_sync(0xffffffffu, top >= bar)) {
+      // which of the lane's values may be among the best (no NaN: a row that holds one offers nothing in the end); they
+      // are few, and are read again, so that the list's code stands here once
+      uint32_t some_of = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int y = 0; y < N; ++y)
+          if (x[u][y] >= bar) some_of |= 1u << (u * N + y);
+      while (__any_sync(0xffffffffu, some_of != 0)) {
+        const int y = some_of ? __ffs(some_of) - 1 : 0;
+        const int32_t at = (k0 + (y / N) * 32 + lane) * N + y % N;
+        const bool on = some_of != 0 && at < count;
+        some_of &= some_of - 1;
+        list.offer(on, on ? to_f32<T>(at0[at]) : 0.f, begin + at, last);
+      }
+      const float now = __shfl_sync(0xffffffffu, list.v, share - 1);
+      if (lane == 0 && now > sure[warp]) const_cast<volatile float*>(sure)[warp] = now;
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
     const float n = fmaxf(m, om), r = n == -INFINITY ? 0.f : n;
-    s = s * __expf(m - r) + os * __expf(om - r);
+    s = s * beam_exp(m - r) + os * beam_exp(om - r);
     m = n;
   }
   if (lane == 0) sums[warp] = make_float2(m, s);
   lv[warp][lane] = list.v;
   li[warp][lane] = list.i;
   __syncthreads();
-  if (warp > 0) return;
-  for (int w = 1; w < BS_WARPS; ++w) list.offer(lane < p.width, lv[w][lane], li[w][lane], last);
-  if (lane < p.width) {
-    p.value[(row * p.pieces + piece) * p.width + lane] = list.v;
-    p.index[(row * p.pieces + piece) * p.width + lane] = list.i;
+  // a thread a candidate of the warps' lists: its rank is how many come before it
+  const int64_t out = (row * p.pieces + piece) * p.width;
+  for (int x = tid; x < BS_WARPS * p.width; x += BS_THREADS) {
+    const int w = x / p.width, k = x - w * p.width;
+    const float v = lv[w][k];
+    const int32_t id = li[w][k];
+    int rank = k;
+    for (int y = 0; y < BS_WARPS; ++y)
+      for (int z = 0; y != w && z < p.width && BeamList<float>::before(lv[y][z], li[y][z], v, id); ++z) ++rank;
+    if (rank < p.width) {
+      p.value[out + rank] = v;
+      p.index[out + rank] = id;
+    }
   }
+  if (warp > 0) return;
   if (lane == 0) {
     float n = -INFINITY, t = 0.f;
     for (int w = 0; w < BS_WARPS; ++w) n = fmaxf(n, sums[w].x);
     const float r = n == -INFINITY ? 0.f : n;
-    for (int w = 0; w < BS_WARPS; ++w) t += sums[w].y * __expf(sums[w].x - r);
+    for (int w = 0; w < BS_WARPS; ++w) t += sums[w].y * beam_exp(sums[w].x - r);
     p.part[row * p.pieces + piece] = make_float2(n, t);
   }
 }
 
 __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const BeamParams p) {
-  __shared__ double cv[BS_MOST][BS_MOST];
-  __shared__ int32_t ci[BS_MOST][BS_MOST];
+  __shared__ double cv[BS_MOST * BS_MOST];
+  __shared__ int32_t ci[BS_MOST * BS_MOST];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, last = p.width - 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, last = p.width - 1, width = p.width;
   const int64_t g = blockIdx.x;
   // a warp a row: log of the sum, the row's best
   for (int k = warp; k < p.beams; k += BS_WARPS) {
-    const int64_t row = g * p.beams + k;
+    const int64_t row = g * p.beams + k, n = int64_t(p.pieces) * width;
     const float2* part = p.part + row * p.pieces;
+    const float* value = p.value + row * n;
+    const int32_t* index = p.index + row * n;
+    const float score1 = p.scores[row];
+    const bool ended = p.done != nullptr && p.done[row] != 0;
     float m = -INFINITY;
     for (int i = lane; i < p.pieces; i += 32) m = fmaxf(m, part[i].x);
     m = warp_max(m);
     double s = 0.0;
     for (int i = lane; i < p.pieces; i += 32)
       if (part[i].y != 0.f) s += double(part[i].y) * exp(double(part[i].x) - double(m));  // (0: nothing but -inf)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const double norm = double(m) + log(s), score = double(p.scores[row]);
-    const bool ended = p.done != nullptr && p.done[row] != 0;
-    const bool empty = !(norm < INFINITY) || norm == -INFINITY;
     BeamList<float> list;
     list.clear();
-    if (!ended && !empty) {
-      const int64_t n = int64_t(p.pieces) * p.width;
-      const float* value = p.value + row * n;
-      const int32_t* index = p.index + row * n;
-      for (int64_t i0 = 0; i0 < n; i0 += 32) {
-        const bool on = i0 + lane < n;
-        list.offer(on, on ? value[i0 + lane] : 0.f, on ? index[i0 + lane] : 0, last);
-      }
+    for (int64_t i0 = 0; i0 < n; i0 += 32) {
+      const bool on = i0 + lane < n;
+      const float v = on ? value[i0 + lane] : -INFINITY;
+      const float bar = __shfl_sync(0xffffffffu, beam_sorted(v, lane), last);  // (as in the pieces)
+      list.offer(on && v >= bar, v, on ? index[i0 + lane] : 0, last);
     }
-    double c = score + (double(list.v) - norm);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    // (the logarithm is kept apart from a maximum beside which it may be nothing)
+    const double log_sum = log(s), score = double(score1);
+    const bool empty = !(log_sum < INFINITY) || log_sum == -INFINITY;
+    double c = score + ((double(list.v) - double(m)) - log_sum);
     int32_t token = list.i;
     if (ended || empty) {  // eos at the beam's score, then the lowest other tokens at -inf; or those alone
       const int32_t eos = int32_t(p.eos);
@@ -204,25 +327,25 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const BeamParams 
       if (token >= p.vocab) token = 0x7fffffff;
       c = ended && lane == 0 ? score : -INFINITY;
     }
-    if (c != c) c = -INFINITY;
-    cv[k][lane] = c;
-    ci[k][lane] = token;
+    if (lane < width) {
+      cv[k * width + lane] = c == c ? c : -INFINITY;
+      ci[k * width + lane] = token;
+    }
   }
   __syncthreads();
-  if (warp > 0) return;
-  BeamList<double> best;
-  best.clear();
-  int32_t beam = 0;  // (a candidate's place: beam << 5 | place in the beam's list, which orders as beam * vocab + token does among equals)
-  for (int k = 0; k < p.beams; ++k) {
-    const bool on = lane < p.width && ci[k][lane] != 0x7fffffff;
-    best.offer(on, cv[k][lane], (k << 5) | lane, last);
-  }
-  if (lane < p.width) {
-    beam = best.i >> 5;
-    const bool there = best.i != 0x7fffffff;
-    p.out_scores[g * p.width + lane] = float(best.v);
-    p.tokens[g * p.width + lane] = there ? ci[beam][best.i & 31] : 0;
-    p.parents[g * p.width + lane] = there ? beam : 0;
+  // a thread a candidate: its rank is how many come before it (a row's places order as its tokens do among equals)
+  const int all = p.beams * width;
+  for (int x = threadIdx.x; x < all; x += BS_THREADS) {
+    const double c = cv[x];
+    if (ci[x] == 0x7fffffff) continue;
+    int rank = 0;
+#pragma unroll 8
+    for (int y = 0; y < all; ++y) rank += ci[y] != 0x7fffffff && (cv[y] > c || (cv[y] == c && y < x));
+    if (rank < width) {
+      p.out_scores[g * width + rank] = float(c);
+      p.tokens[g * width + rank] = ci[x];
+      p.parents[g * width + rank] = x / width;
+    }
   }
 }
 

@@ -138,37 +138,43 @@ extern "C" int lng_kv8_append(const lng_kv8_cache* cache, const int32_t* cu, int
   p.per = int32_t((max_new + 2 * c.page_size - 2) / c.page_size);  // floor((max_new - 1 + page - 1) / page) + 1
   p.units = cu ? tokens / c.page_size + 2 * c.batch : c.batch * p.per;
   LNG_REQUIRE(p.units < (int64_t(1) << 31), "the step touches too many pages");
-  p.head_chunk = int32_t(p.units * ceil_div(c.num_kv_heads, K8A_HEADS) * 2 >= 2 * num_sms() ? K8A_HEADS : K8A_THREADS / 32);
-  if (p.head_chunk > c.num_kv_heads) p.head_chunk = c.num_kv_heads;
-  const dim3 grid(unsigned(p.units), unsigned(2 * ceil_div(c.num_kv_heads, p.head_chunk)));
+  // a page's new tokens in registers: as many warps a head as four items a lane need, or as leave none idle
+  const int64_t most = std::min<int64_t>(c.page_size, max_new);
+  const bool keep = c.page_size <= K8A_CHUNK && (interleaved || rotary_dim % 16 == 0);
+  p.head_warps = 1;
+  while (p.head_warps * 32 * K8A_KEEP < most * p.items || (p.head_warps * c.num_kv_heads < K8A_WARPS && p.head_warps * 32 < most * p.items))
+    p.head_warps *= 2;
+  p.head_warps = std::min(p.head_warps, K8A_WARPS);
+  const int64_t per_cta = keep ? K8A_WARPS / p.head_warps : K8A_WARPS;
+  const dim3 grid{unsigned(p.units), unsigned(2 * ceil_div(c.num_kv_heads, per_cta)), 1u};
   LNG_REQUIRE(grid.y <= 65535, "too many key heads");
-  const size_t smem = size_t(std::min<int64_t>(K8A_CHUNK, std::min<int64_t>(c.page_size, max_new))) * (rotary_dim / 2) * sizeof(float2);
-  if (bf16)
-    kv8_append_kernel<__nv_bfloat16><<<grid, K8A_THREADS, smem, S(stream)>>>(p);
-  else
-    kv8_append_kernel<__half><<<grid, K8A_THREADS, smem, S(stream)>>>(p);
+  const size_t smem = size_t(std::min<int64_t>(K8A_CHUNK, most)) * (rotary_dim / 2) * sizeof(float2);
+  if (q) {  // the queries: kv_append_kernel without a key head; keys and values are launched beside it
+    KaParams a{};
+    a.c = p.v.c;
+    a.c.kv_heads = 0;
+    a.qr = kv_rows(q), a.qo = kv_rows(q_out);
+    a.q_heads = q->heads;
+    a.rotary = rotary_dim;
+    a.interleaved = interleaved;
+    a.positions = positions;
+    a.inv_freq = inv_freq;
+    a.items = (c.head_dim / 8 + 1) / 2;
+    a.items_magic = uint32_t((uint64_t(1) << 32) / uint32_t(a.items) + 1);
+    const int64_t rounds = ceil_div(int64_t(a.q_heads) * a.items, int64_t(32));
+    a.parts = int32_t(std::max<int64_t>(1, std::min<int64_t>(rounds, int64_t(num_sms()) * 8 / tokens)));
+    const unsigned blocks = unsigned(ceil_div(tokens * a.parts, int64_t(KA_WARPS)));
+    if (bf16)
+      kv_append_kernel<__nv_bfloat16><<<blocks, KA_WARPS * 32, 0, S(stream)>>>(a);
+    else
+      kv_append_kernel<__half><<<blocks, KA_WARPS * 32, 0, S(stream)>>>(a);
+    LNG_LAUNCHED("kv_append_kernel");
+  }
+  auto kern = bf16 ? (keep ? kv8_append_kernel<__nv_bfloat16, true> : kv8_append_kernel<__nv_bfloat16, false>)
+                   : (keep ? kv8_append_kernel<__half, true> : kv8_append_kernel<__half, false>);
+  if (q) return launch_dependent(kern, grid, unsigned(K8A_THREADS), smem, S(stream), p);
+  kern<<<grid, K8A_THREADS, smem, S(stream)>>>(p);
   LNG_LAUNCHED("kv8_append_kernel");
-  if (!q) return LNG_OK;
-  // the queries: kv_append_kernel without a key head
-  KaParams a{};
-  a.c = p.v.c;
-  a.c.kv_heads = 0;
-  a.qr = kv_rows(q), a.qo = kv_rows(q_out);
-  a.q_heads = q->heads;
-  a.rotary = rotary_dim;
-  a.interleaved = interleaved;
-  a.positions = positions;
-  a.inv_freq = inv_freq;
-  a.items = (c.head_dim / 8 + 1) / 2;
-  a.items_magic = uint32_t((uint64_t(1) << 32) / uint32_t(a.items) + 1);
-  const int64_t rounds = ceil_div(int64_t(a.q_heads) * a.items, int64_t(32));
-  a.parts = int32_t(std::max<int64_t>(1, std::min<int64_t>(rounds, int64_t(num_sms()) * 8 / tokens)));
-  const unsigned blocks = unsigned(ceil_div(tokens * a.parts, int64_t(KA_WARPS)));
-  if (bf16)
-    kv_append_kernel<__nv_bfloat16><<<blocks, KA_WARPS * 32, 0, S(stream)>>>(a);
-  else
-    kv_append_kernel<__half><<<blocks, KA_WARPS * 32, 0, S(stream)>>>(a);
-  LNG_LAUNCHED("kv_append_kernel");
   return LNG_OK;
 }
 

@@ -43,19 +43,20 @@ __device__ __forceinline__ float2 k8_floats(uint32_t two) {
 
 // ------------------------------------------------------------------ append
 // A page's exponent needs the largest value of all its new tokens before the first of them can be rounded, so a CTA
-// takes one page that a sequence writes to (keys or values of all heads, or of four heads where the step has few
-// pages): pass one forms the values and their maximum a head, pass two forms them again (from L1 or L2: the rows are
-// read from memory once) and rounds them.  A warp takes a head and meets no other; an item is two 16-byte
-// vectors of a row as in kv_append_kernel, and cos and sin of a chunk of tokens are formed once for all heads,
-// with angles in 64 bits as there.
-constexpr int K8A_THREADS = 128, K8A_CHUNK = 64, K8A_HEADS = 32;
+// takes one page that a sequence writes to, keys or values of some of its heads.  An item is two 16-byte vectors of a row
+// as in kv_append_kernel, and cos and sin of a token are formed once for all heads, with angles in 64 bits as there.
+// Where a page holds 64 tokens at most (KEEP) so many warps take a head that every lane can keep its items, four at most, in
+// registers from the search for the maximum to the rounding (rotating them twice, which costs less than room for the
+// rotated values): all loads of a page are in flight at once.  Larger pages, and rotations by halves that are no
+// multiple of 8, go through chunks of 64 tokens twice, the second time from L1 or L2.
+constexpr int K8A_WARPS = 8, K8A_THREADS = 32 * K8A_WARPS, K8A_CHUNK = 64, K8A_KEEP = 4;
 
 struct K8AppendParams {
   Kv8View v;
   KvRows kr, vr;
   int32_t rotary, interleaved;
   int32_t per;         // pages that a sequence touches at most, without cu
-  int32_t head_chunk;  // heads a CTA (at most K8A_HEADS)
+  int32_t head_warps;  // warps a head (KEEP)
   int32_t items;       // of a head: head_dim / 16
   int64_t units;
   const int64_t* positions;
@@ -66,31 +67,11 @@ struct K8AppendParams {
 // ceil((n + 1) / page) + 1 pages, which is what lies between two beginnings at least.
 __device__ __forceinline__ int64_t k8_line(const KvView& c, int64_t b) { return (int64_t(c.cu[b]) >> c.page_shift) + 2 * b; }
 
-// The 16 values of an item, rotated, and the first columns of its two halves of 8.
+// The 16 values of an item's two vectors (columns c0 and c1 on), rotated: in pairs across the two, or side by side.
 template <typename T>
-__device__ __forceinline__ void k8_item(const T* src, int item, int half, bool rot, bool split, bool split_vec, const float2* cs,
-                                        int rotary, float (&x)[16], int& c0, int& c1) {
-  c0 = item * 16;
-  c1 = c0 + 8;
-  if (rot && split && !split_vec) {  // halves that are no multiple of 8: value by value
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int j = c0 + e;
-      if (j < half) {
-        const float2 r = cs[j];
-        x[e] = to_f32<T>(src[j]) * r.x - to_f32<T>(src[j + half]) * r.y;
-      } else if (j < rotary) {
-        const float2 r = cs[j - half];
-        x[e] = to_f32<T>(src[j]) * r.x + to_f32<T>(src[j - half]) * r.y;
-      } else {
-        x[e] = to_f32<T>(src[j]);
-      }
-    }
-    return;
-  }
-  const bool pair = rot && split && item * 8 < half;
-  if (pair) c0 = item * 8, c1 = c0 + half;
-  const uint4 w0 = *reinterpret_cast<const uint4*>(src + c0), w1 = *reinterpret_cast<const uint4*>(src + c1);
+__device__ __forceinline__ void k8_values(uint4 w0, uint4 w1, int c0, int c1, int half, bool rot, bool split, const float2* cs, int rotary,
+                                          float (&x)[16]) {
+  const bool pair = rot && split && c0 < half;  // (items that are not begin behind 2 * half)
   const T *e0 = reinterpret_cast<const T*>(&w0), *e1 = reinterpret_cast<const T*>(&w1);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -121,15 +102,95 @@ __device__ __forceinline__ void k8_item(const T* src, int item, int half, bool r
   }
 }
 
+// The 16 values of an item, rotated, and the first columns of its two halves of 8.
 template <typename T>
-__global__ void __launch_bounds__(K8A_THREADS) kv8_append_kernel(const K8AppendParams p) {
-  extern __shared__ float2 k8_cs[];  // [chunk][rotary / 2]
-  __shared__ float most[K8A_HEADS];
-  __shared__ float down[K8A_HEADS];  // 2^-exponent
+__device__ __forceinline__ void k8_item(const T* src, int item, int half, bool rot, bool split, bool split_vec, const float2* cs,
+                                        int rotary, float (&x)[16], int& c0, int& c1) {
+  c0 = item * 16;
+  c1 = c0 + 8;
+  if (rot && split && !split_vec) {  // halves that are no multiple of 8: value by value
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int j = c0 + e;
+      if (j < half) {
+        const float2 r = cs[j];
+        x[e] = to_f32<T>(src[j]) * r.x - to_f32<T>(src[j + half]) * r.y;
+      } else if (j < rotary) {
+        const float2 r = cs[j - half];
+        x[e] = to_f32<T>(src[j]) * r.x + to_f32<T>(src[j - half]) * r.y;
+      } else {
+        x[e] = to_f32<T>(src[j]);
+      }
+    }
+    return;
+  }
+  if (rot && split && item * 8 < half) c0 = item * 8, c1 = c0 + half;
+  k8_values<T>(*reinterpret_cast<const uint4*>(src + c0), *reinterpret_cast<const uint4*>(src + c1), c0, c1, half, rot, split, cs, rotary, x);
+}
+
+// Cos and sin of the tokens [at0, at0 + here) of a page's new ones.
+__device__ __forceinline__ void k8_angles(const K8AppendParams& p, float2* cs, int half, int64_t token0, int32_t j0, int at0, int here) {
+  for (int x = threadIdx.x; x < here * half; x += K8A_THREADS) {
+    const int t = x / half, f = x - t * half;
+    const double pos = p.positions ? double(p.positions[token0 + at0 + t]) : double(j0 + at0 + t);
+    const double turns = pos * double(p.inv_freq[f]) * 0.15915494309189533577;  // 1 / (2 pi)
+    float sn, cn;
+    sincospif(float(2.0 * (turns - rint(turns))), &sn, &cn);
+    cs[x] = make_float2(cn, sn);
+  }
+}
+
+// The magnitude of a value that counts for the exponent.
+__device__ __forceinline__ float k8_counts(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+
+// 16 values under the exponent whose negative's power of two is `down`, to columns c0 and c1 of a slot.
+__device__ __forceinline__ void k8_store(const float (&x)[16], float down, uint8_t* dst, int c0, int c1) {
+  uint32_t w[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    float r[4];
+    // (x * 0 makes NaN of an infinity, which must not be taken for the largest value)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = fmaf(x[4 * y + e], 0.f, x[4 * y + e] * down);
+    w[y] = k8_pack(r[0], r[1]) | (k8_pack(r[2], r[3]) << 16);
+  }
+  *reinterpret_cast<uint2*>(dst + c0) = make_uint2(w[0], w[1]);
+  *reinterpret_cast<uint2*>(dst + c1) = make_uint2(w[2], w[3]);
+}
+
+// The exponent of a page and head from its new values' largest and, where it holds earlier ones, its old one; the
+// earlier slots again where it grew (the lanes of one warp).
+__device__ __forceinline__ int32_t k8_settle(float most, int32_t old, bool held, uint8_t* slots, int64_t slot_stride, int32_t count, int vecs,
+                                             int lane, bool mine) {
+  const int32_t e = k8_exponent(most);
+  if (!held) return e;
+  if (old >= e) return old;
+  if (mine) {
+    const float f = exp2_whole(old - e);
+    for (int x = lane; x < count * vecs; x += 32) {
+      const int t = x / vecs;
+      uint4* at = reinterpret_cast<uint4*>(slots + t * slot_stride + (x - t * vecs) * 16);
+      uint4 w = *at;
+      uint32_t* words = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float2 a = k8_floats(words[y] & 0xffffu), d = k8_floats(words[y] >> 16);
+        words[y] = k8_pack(a.x * f, a.y * f) | (k8_pack(d.x * f, d.y * f) << 16);
+      }
+      *at = w;
+    }
+  }
+  return e;
+}
+
+template <typename T, bool KEEP>
+__device__ __forceinline__ void kv8_append_page(const K8AppendParams& p, float2* cs) {
+  __shared__ uint32_t most[K8A_WARPS];
   const KvView& c = p.v.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool keys = (blockIdx.y & 1) == 0;
-  const int head0 = int(blockIdx.y >> 1) * p.head_chunk, heads = min(p.head_chunk, c.kv_heads - head0);
+  const int per_cta = KEEP ? K8A_WARPS / p.head_warps : K8A_WARPS;  // heads
+  const int head = int(blockIdx.y >> 1) * per_cta + (KEEP ? warp / p.head_warps : warp), sub = KEEP ? warp % p.head_warps : 0;
   int64_t b, i;
   if (c.cu == nullptr) {
     b = blockIdx.x / p.per;
@@ -165,108 +226,110 @@ __global__ void __launch_bounds__(K8A_THREADS) kv8_append_kernel(const K8AppendP
   }
   const int32_t slot0 = j0 - int32_t(from), count = j1 - j0;
   const int64_t token0 = s.first + (j0 - s.pos);
+  const bool on = head < c.kv_heads;
   const KvRows rows = keys ? p.kr : p.vr;
-  uint8_t* const pages = static_cast<uint8_t*>(keys ? c.k : c.v) + page * (keys ? c.k_page : c.v_page);
-  const int64_t head_stride = keys ? c.k_head : c.v_head, slot_stride = keys ? c.k_slot : c.v_slot;
-  int8_t* const exps = (keys ? p.v.k_exp + page * p.v.k_exp_page : p.v.v_exp + page * p.v.v_exp_page) + head0;
-  const int half = keys ? p.rotary >> 1 : 0;
+  const T* const src = static_cast<const T*>(rows.ptr) + token0 * rows.token + (on ? head : 0) * rows.head;
+  const int64_t slot_stride = keys ? c.k_slot : c.v_slot;
+  uint8_t* const slots = static_cast<uint8_t*>(keys ? c.k : c.v) + page * (keys ? c.k_page : c.v_page) + (on ? head : 0) * (keys ? c.k_head : c.v_head);
+  int8_t* const exp = (keys ? p.v.k_exp + page * p.v.k_exp_page : p.v.v_exp + page * p.v.v_exp_page) + (on ? head : 0);
+  const int half = keys ? p.rotary >> 1 : 0, vecs = c.head_dim >> 4;
   const bool rot = half > 0, split = !p.interleaved, split_vec = (half & 7) == 0;
-  if (threadIdx.x < heads) most[threadIdx.x] = 0.f;
-  const int chunks = (count + K8A_CHUNK - 1) / K8A_CHUNK;
-  auto angles = [&](int ch) {  // cos and sin of a chunk's tokens
+  const int32_t old = slot0 > 0 ? *exp : 0;
+  if constexpr (KEEP) {
+    if (threadIdx.x < K8A_WARPS) most[threadIdx.x] = 0u;
+    uint4 raw[K8A_KEEP][2];
+    const int total = on ? count * p.items : 0;
+    // item y of the lane: which token, and its columns
+    auto place = [&](int y, int& t, int& c0, int& c1) {
+      const int it = (y * p.head_warps + sub) * 32 + lane;
+      t = it / p.items;
+      const int item = it - t * p.items;
+      c0 = item * 16;
+      c1 = c0 + 8;
+      const bool pair = rot && split && item * 8 < half;
+      if (pair) c0 = item * 8, c1 = c0 + half;
+      return it < total;
+    };
+#pragma unroll
+    for (int y = 0; y < K8A_KEEP; ++y) {
+      int t, c0, c1;
+      if (place(y, t, c0, c1)) {
+        raw[y][0] = __ldcs(reinterpret_cast<const uint4*>(src + t * rows.token + c0));
+        raw[y][1] = __ldcs(reinterpret_cast<const uint4*>(src + t * rows.token + c1));
+      }
+    }
+    if (rot) k8_angles(p, cs, half, token0, j0, 0, count);
     __syncthreads();
-    if (rot) {
-      const int here = min(K8A_CHUNK, count - ch * K8A_CHUNK);
-      for (int x = threadIdx.x; x < here * half; x += K8A_THREADS) {
-        const int t = x / half, f = x - t * half, at = ch * K8A_CHUNK + t;
-        const double pos = p.positions ? double(p.positions[token0 + at]) : double(j0 + at);
-        const double turns = pos * double(p.inv_freq[f]) * 0.15915494309189533577;  // 1 / (2 pi)
-        float sn, cn;
-        sincospif(float(2.0 * (turns - rint(turns))), &sn, &cn);
-        k8_cs[x] = make_float2(cn, sn);
-      }
-      __syncthreads();
-    }
-  };
-  // pass one: the largest finite value a head
-#pragma unroll 1
-  for (int ch = 0; ch < chunks; ++ch) {
-    angles(ch);
-    const int here = min(K8A_CHUNK, count - ch * K8A_CHUNK);
-    for (int h = warp; h < heads; h += K8A_THREADS / 32) {
-      float top = 0.f;
-      for (int it = lane; it < here * p.items; it += 32) {
-        const int t = it / p.items, item = it - t * p.items;
-        const T* src = static_cast<const T*>(rows.ptr) + (token0 + ch * K8A_CHUNK + t) * rows.token + (head0 + h) * rows.head;
+    float top = 0.f;
+#pragma unroll
+    for (int y = 0; y < K8A_KEEP; ++y) {
+      int t, c0, c1;
+      if (place(y, t, c0, c1)) {
         float x[16];
-        int c0, c1;
-        k8_item<T>(src, item, half, rot, split, split_vec, k8_cs + t * half, p.rotary, x, c0, c1);
+        k8_values<T>(raw[y][0], raw[y][1], c0, c1, half, rot, split, cs + t * half, p.rotary, x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, k8_counts(x[e]));
       }
-      top = warp_max(top);
-      if (lane == 0) most[h] = fmaxf(most[h], top);
-      __syncwarp();
     }
-  }
-  // exponents; earlier slots again where one grew
-  for (int h = warp; h < heads; h += K8A_THREADS / 32) {
-    int32_t e = k8_exponent(most[h]);
-    if (slot0 > 0) {
-      const int32_t old = exps[h];
-      if (old >= e) {
-        e = old;
-      } else {
-        const float f = exp2_whole(old - e);
-        const int vecs = c.head_dim >> 4;
-        for (int x = lane; x < slot0 * vecs; x += 32) {
-          const int t = x / vecs;
-          uint4* at = reinterpret_cast<uint4*>(pages + (head0 + h) * head_stride + t * slot_stride + (x - t * vecs) * 16);
-          uint4 w = *at;
-          uint32_t* words = reinterpret_cast<uint32_t*>(&w);
+    top = warp_max(top);
+    if (lane == 0) atomicMax(&most[warp / p.head_warps], __float_as_uint(top));  // (not negative: they order as their bits)
+    __syncthreads();
+    if (!on) return;
+    const int32_t e = k8_settle(__uint_as_float(most[warp / p.head_warps]), old, slot0 > 0, slots, slot_stride, slot0, vecs, lane, sub == 0);
+    if (sub == 0 && lane == 0) *exp = int8_t(e);
+    const float down = exp2_whole(-e);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float2 a = k8_floats(words[y] & 0xffffu), d = k8_floats(words[y] >> 16);
-            words[y] = k8_pack(a.x * f, a.y * f) | (k8_pack(d.x * f, d.y * f) << 16);
+    for (int y = 0; y < K8A_KEEP; ++y) {
+      int t, c0, c1;
+      if (place(y, t, c0, c1)) {
+        float x[16];
+        k8_values<T>(raw[y][0], raw[y][1], c0, c1, half, rot, split, cs + t * half, p.rotary, x);
+        k8_store(x, down, slots + (slot0 + t) * slot_stride, c0, c1);
+      }
+    }
+  } else {
+    // a warp a head; passes over the tokens in chunks: the maximum, then the rounding
+    const int chunks = (count + K8A_CHUNK - 1) / K8A_CHUNK;
+    float top = 0.f, down = 1.f;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+      for (int ch = 0; ch < chunks; ++ch) {
+        const int at0 = ch * K8A_CHUNK, here = min(K8A_CHUNK, count - at0);
+        if (rot && (pass == 0 || chunks > 1)) {
+          __syncthreads();
+          k8_angles(p, cs, half, token0, j0, at0, here);
+          __syncthreads();
+        }
+        for (int it = lane; on && it < here * p.items; it += 32) {
+          const int t = it / p.items, item = it - t * p.items;
+          float x[16];
+          int c0, c1;
+          k8_item<T>(src + (at0 + t) * rows.token, item, half, rot, split, split_vec, cs + t * half, p.rotary, x, c0, c1);
+          if (pass == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, k8_counts(x[e]));
+          } else {
+            k8_store(x, down, slots + (slot0 + at0 + t) * slot_stride, c0, c1);
           }
-          *at = w;
         }
       }
-    }
-    __syncwarp();
-    if (lane == 0) {
-      exps[h] = int8_t(e);
-      down[h] = exp2_whole(-e);
-    }
-    __syncwarp();
-  }
-  // pass two
-#pragma unroll 1
-  for (int ch = 0; ch < chunks; ++ch) {
-    if (chunks > 1) angles(ch);
-    const int here = min(K8A_CHUNK, count - ch * K8A_CHUNK);
-    for (int h = warp; h < heads; h += K8A_THREADS / 32) {
-      const float f = down[h];
-      for (int it = lane; it < here * p.items; it += 32) {
-        const int t = it / p.items, item = it - t * p.items, at = ch * K8A_CHUNK + t;
-        const T* src = static_cast<const T*>(rows.ptr) + (token0 + at) * rows.token + (head0 + h) * rows.head;
-        float x[16];
-        int c0, c1;
-        k8_item<T>(src, item, half, rot, split, split_vec, k8_cs + t * half, p.rotary, x, c0, c1);
-        uint32_t w[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          // (x * 0 makes NaN of an infinity, which must not be taken for the largest value)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[4 * y + e] = fmaf(x[4 * y + e], 0.f, x[4 * y + e] * f);
-          w[y] = k8_pack(x[4 * y], x[4 * y + 1]) | (k8_pack(x[4 * y + 2], x[4 * y + 3]) << 16);
-        }
-        uint8_t* dst = pages + (head0 + h) * head_stride + (slot0 + at) * slot_stride;
-        *reinterpret_cast<uint2*>(dst + c0) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(dst + c1) = make_uint2(w[2], w[3]);
+      if (pass == 0 && on) {
+        const int32_t e = k8_settle(warp_max(top), old, slot0 > 0, slots, slot_stride, slot0, vecs, lane, true);
+        __syncwarp();
+        if (lane == 0) *exp = int8_t(e);
+        down = exp2_whole(-e);
       }
     }
   }
+}
+
+template <typename T, bool KEEP>
+__global__ void __launch_bounds__(K8A_THREADS, KEEP ? 2 : 4) kv8_append_kernel(const K8AppendParams p) {
+  extern __shared__ float2 k8_cs[];  // [tokens][rotary / 2]
+  kv8_append_page<T, KEEP>(p, k8_cs);
+  // launched beside the queries' kernel, this one must not be complete before it: what follows waits for this one only
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ reading back

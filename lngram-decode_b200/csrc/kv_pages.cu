@@ -129,12 +129,21 @@ struct BeamPlan {
   int64_t piece;
   size_t part, value, index, bytes;
 };
-// Rows are cut until every SM has four CTAs, but not below 2048 values a piece.
+// Into how many pieces a row is cut, the same for every row (equal rows tie): what takes the least time when an SM's share
+// of the pieces run beside one another, a piece costing its values and as much as 10000 more for its start and end.
 static BeamPlan beam_plan(int64_t groups, int64_t beams, int64_t vocab, int64_t width) {
   BeamPlan b{};
   const int64_t rows = groups * beams;
   if (rows <= 0 || vocab <= 0 || width <= 0) return b;
-  int64_t pieces = std::max<int64_t>(1, std::min(ceil_div(int64_t(num_sms()) * 4, rows), ceil_div(vocab, 2048)));
+  int64_t pieces = 1;
+  double least = 1e300;
+  for (int64_t n = 1; n <= 64 && n <= ceil_div(vocab, 2048); ++n) {
+    const double cost = double(ceil_div(rows * n, num_sms())) * (double(vocab) / double(n) + 10000.0);
+    if (cost < least) {
+      least = cost;
+      pieces = n;
+    }
+  }
   b.piece = ceil_div(ceil_div(vocab, pieces), 8) * 8;
   b.pieces = int32_t(ceil_div(vocab, b.piece));
   b.part = 0;

@@ -320,26 +320,6 @@ __device__ __forceinline__ bool kt_wait(uint32_t bars, uint32_t bar, uint32_t pa
   return false;
 }
 
-// Two fp32 operations an instruction (sm_100).
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 // -inf in the columns of a 32-column piece (from column `base` of the tile) that the row does not see.
 __device__ __forceinline__ void kt_mask(uint32_t (&s)[32], int32_t base, int32_t hi, int32_t lo, int32_t sink) {
 #pragma unroll

@@ -83,6 +83,7 @@ __device__ __forceinline__ void ka_rotate(T& a, T& b, float2 cs) {
 template <typename T>
 __global__ void __launch_bounds__(KA_WARPS * 32, 24) kv_append_kernel(const KaParams p) {
   __shared__ __align__(16) float2 cs_all[KA_WARPS][KA_MAX_HALF];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (an 8-bit cache's keys and values go beside its queries)
   const KvView& c = p.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t w = int64_t(blockIdx.x) * KA_WARPS + warp;

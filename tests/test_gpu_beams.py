@@ -178,3 +178,17 @@ def test_captured_on_two_streams(lngram):
     torch.cuda.synchronize()
     for got, w in zip(outs, want):
         assert all(torch.equal(a, b) for a, b in zip(got, w))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_rows_of_the_lowest_and_largest_values(lngram, dtype):
+    """A mask of the type's lowest value over a whole row leaves equal candidates, one over all but a few leaves those;
+    logits of the largest values do not overflow."""
+    info = torch.finfo(DT[dtype])
+    g = torch.Generator(device="cuda").manual_seed(6)
+    logits = torch.randn(3, 2, 3001, generator=g, device="cuda").to(DT[dtype])
+    logits[0, 0] = info.min
+    logits[1, 0, 7:] = info.min
+    logits[2, 1] = info.max
+    logits[2, 0, 3] = info.max
+    check(lngram, logits, torch.zeros(3, 2, device="cuda"), 5)
