@@ -135,6 +135,7 @@ extern "C" int lng_kv8_append(const lng_kv8_cache* cache, const int32_t* cu, int
   p.positions = positions;
   p.inv_freq = inv_freq;
   p.items = c.head_dim / 16;
+  p.items_magic = uint32_t((uint64_t(1) << 32) / uint32_t(p.items) + 1);
   p.per = int32_t((max_new + 2 * c.page_size - 2) / c.page_size);  // floor((max_new - 1 + page - 1) / page) + 1
   p.units = cu ? tokens / c.page_size + 2 * c.batch : c.batch * p.per;
   LNG_REQUIRE(p.units < (int64_t(1) << 31), "the step touches too many pages");

@@ -46,8 +46,9 @@ __device__ __forceinline__ float2 k8_floats(uint32_t two) {
 // takes one page that a sequence writes to, keys or values of some of its heads.  An item is two 16-byte vectors of a row
 // as in kv_append_kernel, and cos and sin of a token are formed once for all heads, with angles in 64 bits as there.
 // Where a page holds 64 tokens at most (KEEP) so many warps take a head that every lane can keep its items, four at most, in
-// registers from the search for the maximum to the rounding (rotating them twice, which costs less than room for the
-// rotated values): all loads of a page are in flight at once.  Larger pages, and rotations by halves that are no
+// registers from the rotation over the search for the maximum to the rounding: all loads of a page are in flight at once.
+// (Rotating twice instead, which leaves room for three CTAs an SM, took 55 us in place of 43 for 32 prompts of 2048 tokens, 4
+// heads of 64.)  Larger pages, and rotations by halves that are no
 // multiple of 8, go through chunks of 64 tokens twice, the second time from L1 or L2.
 constexpr int K8A_WARPS = 8, K8A_THREADS = 32 * K8A_WARPS, K8A_CHUNK = 64, K8A_KEEP = 4;
 
@@ -58,6 +59,7 @@ struct K8AppendParams {
   int32_t per;         // pages that a sequence touches at most, without cu
   int32_t head_warps;  // warps a head (KEEP)
   int32_t items;       // of a head: head_dim / 16
+  uint32_t items_magic;  // i / items = __umulhi(i, items_magic) where items > 1
   int64_t units;
   const int64_t* positions;
   const float* inv_freq;
@@ -67,9 +69,17 @@ struct K8AppendParams {
 // ceil((n + 1) / page) + 1 pages, which is what lies between two beginnings at least.
 __device__ __forceinline__ int64_t k8_line(const KvView& c, int64_t b) { return (int64_t(c.cu[b]) >> c.page_shift) + 2 * b; }
 
-// The 16 values of an item's two vectors (columns c0 and c1 on), rotated: in pairs across the two, or side by side.
+// Where cos and sin of pair f of the t-th token stand: rows of `half`, in which two neighbours (16 bytes) change places so
+// that eight lanes -- eight items of a token, or four of two -- read eight different banks.
+__device__ __forceinline__ int k8_angle_at(int t, int f, int half) {
+  const int q = f >> 1;
+  return t * half + (((half & 7) ? q : q ^ ((q >> 3) & 3) ^ ((t & 1) << 1)) << 1) + (f & 1);
+}
+
+// The 16 values of an item's two vectors (columns c0 and c1 on) of the t-th token, rotated: in pairs across the two, or side
+// by side.
 template <typename T>
-__device__ __forceinline__ void k8_values(uint4 w0, uint4 w1, int c0, int c1, int half, bool rot, bool split, const float2* cs, int rotary,
+__device__ __forceinline__ void k8_values(uint4 w0, uint4 w1, int c0, int c1, int t, int half, bool rot, bool split, const float2* cs, int rotary,
                                           float (&x)[16]) {
   const bool pair = rot && split && c0 < half;  // (items that are not begin behind 2 * half)
   const T *e0 = reinterpret_cast<const T*>(&w0), *e1 = reinterpret_cast<const T*>(&w1);
@@ -80,11 +90,13 @@ __device__ __forceinline__ void k8_values(uint4 w0, uint4 w1, int c0, int c1, in
   }
   if (pair) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 r = cs[c0 + e];
-      const float a = x[e], b = x[8 + e];
+    for (int e = 0; e < 8; e += 2) {
+      const float4 r = *reinterpret_cast<const float4*>(cs + k8_angle_at(t, c0 + e, half));
+      const float a = x[e], b = x[8 + e], c = x[e + 1], d = x[9 + e];
       x[e] = a * r.x - b * r.y;
       x[8 + e] = b * r.x + a * r.y;
+      x[e + 1] = c * r.z - d * r.w;
+      x[9 + e] = d * r.z + c * r.w;
     }
   } else if (rot && !split) {
 #pragma unroll
@@ -93,7 +105,7 @@ __device__ __forceinline__ void k8_values(uint4 w0, uint4 w1, int c0, int c1, in
       for (int e = 0; e < 8; e += 2) {
         const int j = (h ? c1 : c0) + e;
         if (j < rotary) {
-          const float2 r = cs[j >> 1];
+          const float2 r = cs[k8_angle_at(t, j >> 1, half)];
           const float a = x[8 * h + e], b = x[8 * h + e + 1];
           x[8 * h + e] = a * r.x - b * r.y;
           x[8 * h + e + 1] = b * r.x + a * r.y;
@@ -102,9 +114,9 @@ __device__ __forceinline__ void k8_values(uint4 w0, uint4 w1, int c0, int c1, in
   }
 }
 
-// The 16 values of an item, rotated, and the first columns of its two halves of 8.
+// The 16 values of an item of the t-th token, rotated, and the first columns of its two halves of 8.
 template <typename T>
-__device__ __forceinline__ void k8_item(const T* src, int item, int half, bool rot, bool split, bool split_vec, const float2* cs,
+__device__ __forceinline__ void k8_item(const T* src, int item, int t, int half, bool rot, bool split, bool split_vec, const float2* cs,
                                         int rotary, float (&x)[16], int& c0, int& c1) {
   c0 = item * 16;
   c1 = c0 + 8;
@@ -113,10 +125,10 @@ __device__ __forceinline__ void k8_item(const T* src, int item, int half, bool r
     for (int e = 0; e < 16; ++e) {
       const int j = c0 + e;
       if (j < half) {
-        const float2 r = cs[j];
+        const float2 r = cs[k8_angle_at(t, j, half)];
         x[e] = to_f32<T>(src[j]) * r.x - to_f32<T>(src[j + half]) * r.y;
       } else if (j < rotary) {
-        const float2 r = cs[j - half];
+        const float2 r = cs[k8_angle_at(t, j - half, half)];
         x[e] = to_f32<T>(src[j]) * r.x + to_f32<T>(src[j - half]) * r.y;
       } else {
         x[e] = to_f32<T>(src[j]);
@@ -125,7 +137,7 @@ __device__ __forceinline__ void k8_item(const T* src, int item, int half, bool r
     return;
   }
   if (rot && split && item * 8 < half) c0 = item * 8, c1 = c0 + half;
-  k8_values<T>(*reinterpret_cast<const uint4*>(src + c0), *reinterpret_cast<const uint4*>(src + c1), c0, c1, half, rot, split, cs, rotary, x);
+  k8_values<T>(*reinterpret_cast<const uint4*>(src + c0), *reinterpret_cast<const uint4*>(src + c1), c0, c1, t, half, rot, split, cs, rotary, x);
 }
 
 // Cos and sin of the tokens [at0, at0 + here) of a page's new ones.
@@ -136,23 +148,36 @@ __device__ __forceinline__ void k8_angles(const K8AppendParams& p, float2* cs, i
     const double turns = pos * double(p.inv_freq[f]) * 0.15915494309189533577;  // 1 / (2 pi)
     float sn, cn;
     sincospif(float(2.0 * (turns - rint(turns))), &sn, &cn);
-    cs[x] = make_float2(cn, sn);
+    cs[k8_angle_at(t, f, half)] = make_float2(cn, sn);
   }
 }
 
-// The magnitude of a value that counts for the exponent.
-__device__ __forceinline__ float k8_counts(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+// The largest magnitude of 16 values that counts for the exponent: infinities do not, nor NaN.
+__device__ __forceinline__ float k8_most(const float (&x)[16]) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+  if (top == INFINITY) {
+    top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.f);
+  }
+  return top;
+}
 
 // 16 values under the exponent whose negative's power of two is `down`, to columns c0 and c1 of a slot.
 __device__ __forceinline__ void k8_store(const float (&x)[16], float down, uint8_t* dst, int c0, int c1) {
   uint32_t w[4];
 #pragma unroll
   for (int y = 0; y < 4; ++y) {
-    float r[4];
-    // (x * 0 makes NaN of an infinity, which must not be taken for the largest value)
+    // (an infinity must not be taken for the largest value: its byte is NaN's)
+    const float a = x[4 * y] * down, b = x[4 * y + 1] * down, c = x[4 * y + 2] * down, d = x[4 * y + 3] * down;
+    w[y] = k8_pack(a, b) | (k8_pack(c, d) << 16);
+    if (fmaxf(fmaxf(fabsf(a), fabsf(b)), fmaxf(fabsf(c), fabsf(d))) == INFINITY) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = fmaf(x[4 * y + e], 0.f, x[4 * y + e] * down);
-    w[y] = k8_pack(r[0], r[1]) | (k8_pack(r[2], r[3]) << 16);
+      for (int e = 0; e < 4; ++e)
+        if (fabsf(x[4 * y + e]) == INFINITY) w[y] |= 0x7fu << (8 * e);
+    }
   }
   *reinterpret_cast<uint2*>(dst + c0) = make_uint2(w[0], w[1]);
   *reinterpret_cast<uint2*>(dst + c1) = make_uint2(w[2], w[3]);
@@ -219,37 +244,27 @@ __device__ __forceinline__ void kv8_append_page(const K8AppendParams& p, float2*
   if (from >= hi) return;
   const int32_t j0 = int32_t(from > lo ? from : lo);
   const int32_t j1 = int32_t(hi < from + (1 << c.page_shift) ? hi : from + (1 << c.page_shift));
-  const int32_t page = page_of(c.table + b * c.table_stride, j0, c.page_shift, c.num_pages);
-  if (page < 0) {
-    kv_range_error();
-    return;
-  }
   const int32_t slot0 = j0 - int32_t(from), count = j1 - j0;
   const int64_t token0 = s.first + (j0 - s.pos);
   const bool on = head < c.kv_heads;
   const KvRows rows = keys ? p.kr : p.vr;
   const T* const src = static_cast<const T*>(rows.ptr) + token0 * rows.token + (on ? head : 0) * rows.head;
-  const int64_t slot_stride = keys ? c.k_slot : c.v_slot;
-  uint8_t* const slots = static_cast<uint8_t*>(keys ? c.k : c.v) + page * (keys ? c.k_page : c.v_page) + (on ? head : 0) * (keys ? c.k_head : c.v_head);
-  int8_t* const exp = (keys ? p.v.k_exp + page * p.v.k_exp_page : p.v.v_exp + page * p.v.v_exp_page) + (on ? head : 0);
   const int half = keys ? p.rotary >> 1 : 0, vecs = c.head_dim >> 4;
   const bool rot = half > 0, split = !p.interleaved, split_vec = (half & 7) == 0;
-  const int32_t old = slot0 > 0 ? *exp : 0;
-  if constexpr (KEEP) {
+  uint4 raw[KEEP ? K8A_KEEP : 1][2];
+  const int total = on ? count * p.items : 0;
+  // item y of the lane: which token, and its columns
+  auto place = [&](int y, int& t, int& c0, int& c1) {
+    const int it = (y * p.head_warps + sub) * 32 + lane;
+    t = p.items > 1 ? int(__umulhi(uint32_t(it), p.items_magic)) : it;
+    const int item = it - t * p.items;
+    c0 = item * 16;
+    c1 = c0 + 8;
+    if (rot && split && item * 8 < half) c0 = item * 8, c1 = c0 + half;
+    return it < total;
+  };
+  if constexpr (KEEP) {  // (the rows' way begins before the page is looked up)
     if (threadIdx.x < K8A_WARPS) most[threadIdx.x] = 0u;
-    uint4 raw[K8A_KEEP][2];
-    const int total = on ? count * p.items : 0;
-    // item y of the lane: which token, and its columns
-    auto place = [&](int y, int& t, int& c0, int& c1) {
-      const int it = (y * p.head_warps + sub) * 32 + lane;
-      t = it / p.items;
-      const int item = it - t * p.items;
-      c0 = item * 16;
-      c1 = c0 + 8;
-      const bool pair = rot && split && item * 8 < half;
-      if (pair) c0 = item * 8, c1 = c0 + half;
-      return it < total;
-    };
 #pragma unroll
     for (int y = 0; y < K8A_KEEP; ++y) {
       int t, c0, c1;
@@ -258,17 +273,26 @@ __device__ __forceinline__ void kv8_append_page(const K8AppendParams& p, float2*
         raw[y][1] = __ldcs(reinterpret_cast<const uint4*>(src + t * rows.token + c1));
       }
     }
+  }
+  const int32_t page = page_of(c.table + b * c.table_stride, j0, c.page_shift, c.num_pages);
+  if (page < 0) {
+    kv_range_error();
+    return;
+  }
+  const int64_t slot_stride = keys ? c.k_slot : c.v_slot;
+  uint8_t* const slots = static_cast<uint8_t*>(keys ? c.k : c.v) + page * (keys ? c.k_page : c.v_page) + (on ? head : 0) * (keys ? c.k_head : c.v_head);
+  int8_t* const exp = (keys ? p.v.k_exp + page * p.v.k_exp_page : p.v.v_exp + page * p.v.v_exp_page) + (on ? head : 0);
+  const int32_t old = slot0 > 0 ? *exp : 0;
+  if constexpr (KEEP) {
     if (rot) k8_angles(p, cs, half, token0, j0, 0, count);
     __syncthreads();
-    float top = 0.f;
+    float x[K8A_KEEP][16], top = 0.f;
 #pragma unroll
     for (int y = 0; y < K8A_KEEP; ++y) {
       int t, c0, c1;
       if (place(y, t, c0, c1)) {
-        float x[16];
-        k8_values<T>(raw[y][0], raw[y][1], c0, c1, half, rot, split, cs + t * half, p.rotary, x);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, k8_counts(x[e]));
+        k8_values<T>(raw[y][0], raw[y][1], c0, c1, t, half, rot, split, cs, p.rotary, x[y]);
+        top = fmaxf(top, k8_most(x[y]));
       }
     }
     top = warp_max(top);
@@ -281,11 +305,7 @@ __device__ __forceinline__ void kv8_append_page(const K8AppendParams& p, float2*
 #pragma unroll
     for (int y = 0; y < K8A_KEEP; ++y) {
       int t, c0, c1;
-      if (place(y, t, c0, c1)) {
-        float x[16];
-        k8_values<T>(raw[y][0], raw[y][1], c0, c1, half, rot, split, cs + t * half, p.rotary, x);
-        k8_store(x, down, slots + (slot0 + t) * slot_stride, c0, c1);
-      }
+      if (place(y, t, c0, c1)) k8_store(x[y], down, slots + (slot0 + t) * slot_stride, c0, c1);
     }
   } else {
     // a warp a head; passes over the tokens in chunks: the maximum, then the rounding
@@ -305,13 +325,11 @@ __device__ __forceinline__ void kv8_append_page(const K8AppendParams& p, float2*
           const int t = it / p.items, item = it - t * p.items;
           float x[16];
           int c0, c1;
-          k8_item<T>(src + (at0 + t) * rows.token, item, half, rot, split, split_vec, cs + t * half, p.rotary, x, c0, c1);
-          if (pass == 0) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, k8_counts(x[e]));
-          } else {
+          k8_item<T>(src + (at0 + t) * rows.token, item, t, half, rot, split, split_vec, cs, p.rotary, x, c0, c1);
+          if (pass == 0)
+            top = fmaxf(top, k8_most(x));
+          else
             k8_store(x, down, slots + (slot0 + at0 + t) * slot_stride, c0, c1);
-          }
         }
       }
       if (pass == 0 && on) {
