@@ -570,14 +570,13 @@ int lng_kv8_values(const lng_kv8_cache* cache, void* k_out, void* v_out, lng_str
 
 /* Every sequence grows by its tokens of the step (cu or max_new as for lng_kv_append).  New pages are the lowest
  * free ones, in order of sequence and then of column.  A partly filled last page that other rows hold too is replaced by
- * a page of the sequence's own, and its copy noted.  A sequence that does not fit its table's row, or for which too few
+ * a page of the sequence's own, into which its filled slots are copied in each of the `count` caches (a model's layers,
+ * of one geometry; table and lengths are caches[0]'s).  A sequence that does not fit its table's row, or for which too few
  * pages are free once those before it have theirs, is suspended (served = 0); one that needs no page is served always.
- * slots i64 [tokens]: page * page_size + slot of every new token, -1 where it has none.  copies i32 [batch, 4]:
- * (source page, target page, filled slots, 0), target -1 where nothing is copied. */
-int lng_kv_pages_extend(const lng_kv8_cache* cache, int32_t* refs, const int32_t* cu, int64_t tokens, int64_t max_new,
-                        int64_t* slots, uint8_t* served, int32_t* copies, lng_stream_t stream);
-/* Carries out an extend's copies in one cache (one call a layer, where layers share the table), before its append. */
-int lng_kv_pages_copy(const lng_kv8_cache* cache, const int32_t* copies, lng_stream_t stream);
+ * slots i64 [tokens]: page * page_size + slot of every new token, -1 where it has none.  copies i32 [batch, 4], 16-byte
+ * aligned, is written by the call: (source page, target page, filled slots, 0), target -1 where nothing is copied. */
+int lng_kv_pages_extend(const lng_kv8_cache* caches_host, int32_t count, int32_t* refs, const int32_t* cu, int64_t tokens,
+                        int64_t max_new, int64_t* slots, uint8_t* served, int32_t* copies, lng_stream_t stream);
 /* Sequence b keeps its first min(lengths[b], its length) keys (most for all where lengths is NULL); the pages behind
  * them are given back. */
 int lng_kv_pages_truncate(const lng_kv8_cache* cache, int32_t* refs, const int32_t* lengths, int64_t most, lng_stream_t stream);

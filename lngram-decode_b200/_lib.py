@@ -151,8 +151,7 @@ SIGNATURES = {
     "lng_kv8_attend_workspace_bytes": (sz, [PK8, i64, i64, i64, i32, i32, i32]),
     "lng_kv8_attend": (C.c_int, [PK8, P, i64, i64, i64, PW, f32, i32, i32, PW, P, sz, P]),
     "lng_kv8_values": (C.c_int, [PK8, P, P, P]),
-    "lng_kv_pages_extend": (C.c_int, [PK8, P, P, i64, i64, P, P, P, P]),
-    "lng_kv_pages_copy": (C.c_int, [PK8, P, P]),
+    "lng_kv_pages_extend": (C.c_int, [PK8, i32, P, P, i64, i64, P, P, P, P]),
     "lng_kv_pages_truncate": (C.c_int, [PK8, P, P, i64, P]),
     "lng_kv_pages_reorder": (C.c_int, [PK8, P, P, i64, i64, P]),
     "lng_beam_workspace_bytes": (sz, [i64, i64, i64, i64]),

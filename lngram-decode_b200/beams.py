@@ -20,6 +20,7 @@ from . import _lib
 from ._lib import check, ptr, stream_ptr
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_SIZES: dict = {}  # workspace bytes by a call's shape and device
 
 
 def _no_grad(*tensors: Tensor | None) -> None:
@@ -78,7 +79,11 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, don
     out = torch.empty(groups, width, dtype=torch.float32, device=device)
     tokens, parents = (torch.empty(groups, width, dtype=torch.int64, device=device) for _ in range(2))
     with _lib.on_device(device):
-        need = lib.lng_beam_workspace_bytes(groups, beams, vocab, width)
+        need = _SIZES.get((index, groups, beams, vocab, width))
+        if need is None:
+            if len(_SIZES) > 256:
+                _SIZES.clear()
+            need = _SIZES[index, groups, beams, vocab, width] = lib.lng_beam_workspace_bytes(groups, beams, vocab, width)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         check(lib.lng_beam_select(ptr(logits), _lib.dtype_code(logits.dtype), stride, groups, beams, vocab, ptr(scores), ptr(done),
                                   0 if done is None else int(eos), width, ptr(out), ptr(tokens), ptr(parents), ptr(ws), need,

@@ -49,10 +49,10 @@ static int kv8_page_maps(CUtensorMap* k, CUtensorMap* v, const lng_kv_cache& c, 
 
 // How an attention call is carried out, and what it needs of the workspace.
 struct Kv8Plan {
-  bool step;         // by kv8_step_kernel (few rows a key head)
-  int shares;        // into which its work is cut
+  int groups;        // by kv8_step_kernel (few rows a key head), of so many groups of eight; 0:
+  int shares;        // into which the step kernel's work is cut
   bool warp_shares;  // a share a warp, not a CTA
-  int64_t units;     // else by kv8_tile_kernel: its units per key head and range of keys
+  int64_t units;     // by kv8_tile_kernel: its units per key head and range of keys
   int splits;        // key ranges, whose states are joined when there are several
   size_t ml, o, bytes;  // states: of the step kernel's pieces, or of the rows in every range
 };
@@ -64,17 +64,26 @@ static Kv8Plan kv8_plan(const lng_kv8_cache* cache, int64_t tokens, int64_t max_
   const lng_kv_cache& c = cache->pages;
   const int64_t group = q_heads / c.num_kv_heads;
   size_t states = 0;
-  p.step = group * max_new <= KS_ROWS && (group * max_new <= 4 || c.batch * c.num_kv_heads * 16 >= num_sms());
-  if (p.step) {
-    // (many pairs: a share a warp; few pairs: a share a CTA, which leaves an eighth of the pieces to join: kv_plan's rule)
-    p.warp_shares = c.batch * c.num_kv_heads >= num_sms();
-    p.shares = num_sms() * (p.warp_shares ? K8sCfg<128>::WARPS : 1);
-    states = size_t(2) * p.shares * KS_ROWS;
+  const int64_t rows = group * max_new, pairs = c.batch * c.num_kv_heads, span = 2 * std::max<int64_t>(1, KT_BM / group);
+  int64_t keys = c.max_pages * c.page_size;
+  if (max_len > 0) keys = std::min(keys, max_len);
+  if (window > 0) keys = std::min(keys, int64_t(window) + sinks + span + KT_BK);
+  // Up to four rows the step kernel always, up to 16 unless so few pairs fall into many pieces each (one sequence of 4000
+  // keys, 4 key heads of 64, 16 rows: 31 against 19 us by the tile kernel), up to 32 where there are pairs for all SMs: 64
+  // sequences of 1024 keys, 4 heads of 64: 45 against 51 us, 8 of 128: 92 against 119, of 8000 keys 349 against 572; but 16
+  // sequences of 1024 keys 61 against 33.  (64 rows as two pairs of 32 were no faster than the tile kernel, 51 and 51, 144
+  // and 120 us.)
+  if (rows <= 4 || (rows <= 16 && pairs * 16 >= num_sms()) || (rows <= 32 && pairs >= num_sms()))
+    p.groups = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  if (p.groups) {
+    // (many pairs: a share a warp; few pairs: a share a CTA, which leaves a twelfth or an eighth of the pieces to join)
+    p.warp_shares = pairs >= num_sms() || p.groups > 2;
+    const int warps = p.groups == 1 ? K8sCfg<64, 1>::WARPS : K8sCfg<64, 2>::WARPS;
+    p.shares = num_sms() * (p.warp_shares ? warps : 1);
+    // (no more shares than give every warp of a CTA a block: fewer pieces to join)
+    if (!p.warp_shares) p.shares = int(std::max<int64_t>(1, std::min<int64_t>(p.shares, ceil_div(pairs * (ceil_div(keys, 32) + 1), warps))));
+    states = size_t(2) * p.shares * 8 * p.groups;
   } else {
-    const int64_t span = 2 * std::max<int64_t>(1, KT_BM / group);
-    int64_t keys = c.max_pages * c.page_size;
-    if (max_len > 0) keys = std::min(keys, max_len);
-    if (window > 0) keys = std::min(keys, int64_t(window) + sinks + span + KT_BK);
     // ragged steps: at most one unit a sequence is not full
     p.units = std::min(c.batch * ceil_div(max_new, span), tokens / span + std::min(c.batch, tokens));
     p.splits = kv_splits(p.units * c.num_kv_heads, std::max<int64_t>(1, ceil_div(keys, KT_BK)));
@@ -85,11 +94,12 @@ static Kv8Plan kv8_plan(const lng_kv8_cache* cache, int64_t tokens, int64_t max_
   return p;
 }
 
-template <typename T, int HDP, bool WS>
+template <typename T, int HDP, int NR, bool WS>
 static int launch_kv8_step(const CUtensorMap& tk, const CUtensorMap& tv, const K8sParams& p, cudaStream_t s) {
-  using Cfg = K8sCfg<HDP>;
-  auto kern = kv8_step_kernel<T, HDP, WS>;
-  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  using Cfg = K8sCfg<HDP, NR>;
+  auto kern = kv8_step_kernel<T, HDP, NR, WS>;
+  static std::atomic<uint64_t> known{0};
+  if (const int st = allow_smem(kern, Cfg::SMEM, known)) return st;
   kern<<<unsigned(p.s.shares / (WS ? Cfg::WARPS : 1)), Cfg::THREADS, Cfg::SMEM, s>>>(tk, tv, p);
   LNG_LAUNCHED("kv8_step_kernel");
   return launch_dependent(kv_step_join_kernel<T, Cfg::BK>, unsigned(p.s.c.batch * p.s.c.kv_heads), 256u, size_t(0), s, p.s);
@@ -99,7 +109,8 @@ template <typename T, int HDP>
 static int launch_kv8_tile(const CUtensorMap& tk, const CUtensorMap& tv, const K8tParams& p, cudaStream_t s) {
   using Cfg = K8tCfg<HDP>;
   auto kern = kv8_tile_kernel<T, HDP>;
-  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Cfg::SMEM)));
+  static std::atomic<uint64_t> known{0};
+  if (const int st = allow_smem(kern, Cfg::SMEM, known)) return st;
   kern<<<unsigned(std::min<int64_t>(p.t.total, num_sms())), K8T_THREADS, Cfg::SMEM, s>>>(tk, tv, p);
   LNG_LAUNCHED("kv8_tile_kernel");
   if (p.t.row_ml == nullptr) return LNG_OK;
@@ -188,20 +199,21 @@ extern "C" int lng_kv8_values(const lng_kv8_cache* cache, void* k_out, void* v_o
   if (const int st = check_kv8(&one, nullptr, 1, 1)) return st;
   LNG_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0, "outputs must be 16-byte aligned");
   const lng_kv_cache& c = cache->pages;
-  int shift = 0;
-  while ((1 << shift) < c.page_size) ++shift;
-  const int vecs = c.head_dim / 16;
-  const int64_t total = c.num_pages * c.num_kv_heads * c.page_size * vecs;
-  LNG_REQUIRE(ceil_div(total, 256) < (int64_t(1) << 31), "the cache is too large");
-  const unsigned grid = unsigned(ceil_div(total, 256));
-  if (k_out)
-    kv8_values_kernel<<<grid, 256, 0, S(stream)>>>(static_cast<const uint8_t*>(c.k), c.k_page_stride, c.k_head_stride, c.k_slot_stride,
-                                                  cache->k_exp, cache->k_exp_stride, c.num_kv_heads, shift, vecs, total,
-                                                  static_cast<uint4*>(k_out));
-  if (v_out)
-    kv8_values_kernel<<<grid, 256, 0, S(stream)>>>(static_cast<const uint8_t*>(c.v), c.v_page_stride, c.v_head_stride, c.v_slot_stride,
-                                                  cache->v_exp, cache->v_exp_stride, c.num_kv_heads, shift, vecs, total,
-                                                  static_cast<uint4*>(v_out));
+  K8ValuesParams p{};
+  while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
+  p.pages[0] = static_cast<const uint8_t*>(c.k), p.pages[1] = static_cast<const uint8_t*>(c.v);
+  p.page[0] = c.k_page_stride, p.page[1] = c.v_page_stride;
+  p.head[0] = c.k_head_stride, p.head[1] = c.v_head_stride;
+  p.slot[0] = c.k_slot_stride, p.slot[1] = c.v_slot_stride;
+  p.exps[0] = cache->k_exp, p.exps[1] = cache->v_exp;
+  p.exp_page[0] = cache->k_exp_stride, p.exp_page[1] = cache->v_exp_stride;
+  p.out[0] = static_cast<uint4*>(k_out), p.out[1] = static_cast<uint4*>(v_out);
+  p.heads = c.num_kv_heads;
+  p.vecs = c.head_dim / 16;
+  p.total = c.num_pages * c.num_kv_heads * c.page_size * p.vecs;
+  LNG_REQUIRE(ceil_div(p.total, 256) < (int64_t(1) << 31), "the cache is too large");
+  const dim3 grid{unsigned(ceil_div(p.total, 256)), 2u, 1u};
+  kv8_values_kernel<<<grid, 256, 0, S(stream)>>>(p);
   LNG_LAUNCHED("kv8_values_kernel");
   return LNG_OK;
 }
@@ -232,7 +244,7 @@ extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int
   LNG_REQUIRE(plan.bytes == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
               "workspace must be 256-byte aligned");
   LNG_REQUIRE(workspace_bytes >= plan.bytes, "workspace too small");
-  if (plan.step) {
+  if (plan.groups) {
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     K8sParams p{};
     p.s.c = kv_view(&c, cu, tokens, max_new);
@@ -242,9 +254,10 @@ extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int
     p.s.scale_log2 = scale_log2;
     p.s.window = std::min(window, 1 << 30);
     p.s.sinks = std::min(sinks, 1 << 30);
-    p.s.box = std::min(c.page_size, K8sCfg<64>::BK);
+    p.s.box = std::min(c.page_size, K8sCfg<64, 1>::BK);
     p.s.piece_ml = reinterpret_cast<float2*>(ws + plan.ml);
     p.s.piece_o = reinterpret_cast<float*>(ws + plan.o);
+    p.s.piece_rows = 8 * plan.groups;
     p.s.shares = plan.shares;
     p.k_exp = cache->k_exp, p.v_exp = cache->v_exp;
     p.k_exp_page = cache->k_exp_stride, p.v_exp_page = cache->v_exp_stride;
@@ -253,9 +266,17 @@ extern "C" int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int
     const bool wide = c.head_dim > 64;
     auto launch = [&](auto type) {
       using T = decltype(type);
-      if (plan.warp_shares)
-        return wide ? launch_kv8_step<T, 128, true>(tk, tv, p, S(stream)) : launch_kv8_step<T, 64, true>(tk, tv, p, S(stream));
-      return wide ? launch_kv8_step<T, 128, false>(tk, tv, p, S(stream)) : launch_kv8_step<T, 64, false>(tk, tv, p, S(stream));
+      const bool ws = plan.warp_shares;
+      const cudaStream_t cs = S(stream);
+      switch (plan.groups) {
+        case 1:
+          if (wide) return ws ? launch_kv8_step<T, 128, 1, true>(tk, tv, p, cs) : launch_kv8_step<T, 128, 1, false>(tk, tv, p, cs);
+          return ws ? launch_kv8_step<T, 64, 1, true>(tk, tv, p, cs) : launch_kv8_step<T, 64, 1, false>(tk, tv, p, cs);
+        case 2:
+          if (wide) return ws ? launch_kv8_step<T, 128, 2, true>(tk, tv, p, cs) : launch_kv8_step<T, 128, 2, false>(tk, tv, p, cs);
+          return ws ? launch_kv8_step<T, 64, 2, true>(tk, tv, p, cs) : launch_kv8_step<T, 64, 2, false>(tk, tv, p, cs);
+        default: return wide ? launch_kv8_step<T, 128, 4, true>(tk, tv, p, cs) : launch_kv8_step<T, 64, 4, true>(tk, tv, p, cs);
+      }
     };
     return c.dtype == LNG_BF16 ? launch(__nv_bfloat16()) : launch(__half());
   }

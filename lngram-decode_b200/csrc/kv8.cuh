@@ -351,18 +351,26 @@ __global__ void __launch_bounds__(K8A_THREADS, KEEP ? 2 : 4) kv8_append_kernel(c
 }
 
 // ------------------------------------------------------------------ reading back
-// Memory bound: a byte in, two out.  A thread takes 16 bytes of a slot.
-__global__ void __launch_bounds__(256)
-    kv8_values_kernel(const uint8_t* __restrict__ pages, int64_t page, int64_t head, int64_t slot, const int8_t* __restrict__ exps,
-                      int64_t exp_page, int32_t heads, int32_t page_shift, int32_t vecs, int64_t total, uint4* __restrict__ out) {
+// Memory bound: a byte in, two out.  A thread takes 16 bytes of a slot; keys (blocks with y = 0) and values in one launch.
+struct K8ValuesParams {
+  const uint8_t* pages[2];
+  int64_t page[2], head[2], slot[2], exp_page[2];
+  const int8_t* exps[2];
+  uint4* out[2];
+  int32_t heads, page_shift, vecs;
+  int64_t total;
+};
+__global__ void __launch_bounds__(256) kv8_values_kernel(const __grid_constant__ K8ValuesParams p) {
+  const int which = blockIdx.y;
   const int64_t x = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (x >= total) return;
-  const int64_t row = x / vecs;  // (page, head, slot)
-  const int32_t s = int32_t(row & ((1 << page_shift) - 1));
-  const int64_t ph = row >> page_shift, pg = ph / heads;
-  const int32_t h = int32_t(ph - pg * heads);
-  const uint4 w = __ldcs(reinterpret_cast<const uint4*>(pages + pg * page + h * head + s * slot + (x - row * vecs) * 16));
-  const float f = exp2_whole(exps[pg * exp_page + h]);
+  if (x >= p.total || p.out[which] == nullptr) return;
+  const int64_t row = x / p.vecs;  // (page, head, slot)
+  const int32_t s = int32_t(row & ((1 << p.page_shift) - 1));
+  const int64_t ph = row >> p.page_shift, pg = ph / p.heads;
+  const int32_t h = int32_t(ph - pg * p.heads);
+  const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p.pages[which] + pg * p.page[which] + h * p.head[which] + s * p.slot[which] +
+                                                        (x - row * p.vecs) * 16));
+  const float f = exp2_whole(p.exps[which][pg * p.exp_page[which] + h]);
   const uint32_t words[4] = {w.x, w.y, w.z, w.w};
   uint32_t r[8];
 #pragma unroll
@@ -372,8 +380,8 @@ __global__ void __launch_bounds__(256)
     r[2 * y] = *reinterpret_cast<const uint32_t*>(&u);
     r[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&v);
   }
-  __stcs(out + 2 * x, make_uint4(r[0], r[1], r[2], r[3]));
-  __stcs(out + 2 * x + 1, make_uint4(r[4], r[5], r[6], r[7]));
+  __stcs(p.out[which] + 2 * x, make_uint4(r[0], r[1], r[2], r[3]));
+  __stcs(p.out[which] + 2 * x + 1, make_uint4(r[4], r[5], r[6], r[7]));
 }
 
 }  // namespace lng

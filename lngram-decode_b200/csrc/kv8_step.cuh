@@ -1,20 +1,26 @@
-// Attention of few rows over the 8-bit cache: decoding and the verification of a few drafts, at most 16
-// (token, head) rows a key head.
+// Attention of few rows over the 8-bit cache: decoding and the verification of drafts, up to 32 (token, head) rows a key
+// head.
 //
 // kv_step_kernel's plan (kv_step.cuh): all blocks of 32 visible keys in one line, cut into equal shares; each
 // warp streams its blocks through a ring of its own that an elected lane fills by TMA; cut pairs are joined by
-// kv_step_join_kernel.  What differs is what a block is: half the bytes, and e4m3 under exponents.
+// kv_step_join_kernel.  What differs is what a block is: half the bytes, and e4m3 under exponents, which makes the
+// conversion to the products' type the larger part of the work.
 //
 // Products in fp16 (mma.sync m16n8k16): e4m3 is exact in it, and a row of queries is scaled by a power of two so that its
-// largest value lies in [2^14, 2^15) (fp16 queries are taken as they are).  The contraction may run over columns, and
-// over keys, in any order, so fragments are read where they lie: a lane takes 16 consecutive bytes of a key (its
-// columns of four products), 16 of a value row for each of its four keys (a column of sixteen products).  Keys are put
-// to the products' columns so that eight lanes always meet eight different 16-byte banks (key_of).
+// largest value lies in [2^14, 2^15) (fp16 queries are taken as they are).  Keys and values are the A operands,
+// S^T = K Q^T and O^T = V^T P^T, so that a converted fragment serves all rows, eight a product: NR = 1, 2 or 4 groups of
+// eight.  (With the rows as the A operand, 16 at least, a step of 64 sequences with 4 rows a key head took 208 us; so it
+// takes 195.)  P^T, whose keys stand along the wrong axis of the accumulators, is turned by movmatrix.  The
+// contraction may run over columns, and over keys, in any order, so fragments are read where they lie: a lane takes 16
+// consecutive bytes of a key (its columns of four products), and 16 of a value row for each of its four keys.  Keys are put
+// to the products' rows so that eight lanes always meet eight different 16-byte banks (key_of).
 //
 // Exponents: keys' go into the scores' factor, one a tile of 8 keys (pages hold 8 at least).  Values' go into the
-// exponential: with u = score + exponent in base 2, weights 2^(u - max u) are at most 1 and fit fp16 whatever the
-// pages' exponents, their products with the bare e4m3 values need no scaling, and the sum takes 2^-exponent
-// back: o = sum w v / sum w 2^-exponent.  Weights are rounded to fp16 once, their sum is not.
+// exponential: with u = score + exponent in base 2, weights 2^(u - M) fit fp16 whatever the pages' exponents, their
+// products with the bare e4m3 values need no scaling, and the sum takes 2^-exponent back:
+// o = sum w v / sum w 2^-exponent.  M follows the largest u only when that has grown past it by 8 (weights reach 2^8 at
+// most), which a vote over the lanes' own values tells: the maximum over the lanes is formed only then.  Weights are
+// rounded to fp16 once, their sum is not.
 #pragma once
 
 #include "kv8.cuh"
@@ -22,12 +28,17 @@
 
 namespace lng {
 
-template <int HDP>  // head size padded to 64 or 128
+// HDP: head size padded to 64 or 128; NR: groups of eight rows.
+template <int HDP, int NR>
 struct K8sCfg {
-  static constexpr int BK = 32, WARPS = 8, THREADS = 32 * WARPS, STAGES = HDP == 128 ? 3 : 6;
-  static constexpr uint32_t KV_BYTES = BK * HDP, STAGE_BYTES = 2 * KV_BYTES, RING_BYTES = STAGE_BYTES * STAGES;
-  static constexpr uint32_t MERGE_BYTES = 4 * KS_ROWS * HDP * 4;  // the products of four warps
-  static constexpr size_t SMEM = size_t(WARPS) * RING_BYTES + MERGE_BYTES + WARPS * KS_ROWS * 8 + WARPS * STAGES * 16 + 64 + 1024;
+  static constexpr int BK = 32, ROWS = 8 * NR;
+  static constexpr bool Q_REGS = HDP * NR <= 256;  // query fragments in registers, else in shared memory
+  static constexpr int WARPS = NR == 1 ? 12 : 8, THREADS = 32 * WARPS;
+  static constexpr uint32_t KV_BYTES = BK * HDP, STAGE_BYTES = 2 * KV_BYTES;
+  static constexpr int STAGES = (Q_REGS ? 192 : 128) * 1024 / WARPS / STAGE_BYTES;
+  static constexpr uint32_t RING_BYTES = STAGE_BYTES * STAGES, Q_BYTES = Q_REGS ? 0 : ROWS * HDP * 2;  // one warp's
+  static constexpr uint32_t MERGE_BYTES = NR <= 2 ? 4 * ROWS * HDP * 4 : 0;  // the products of four warps
+  static constexpr size_t SMEM = size_t(WARPS) * (RING_BYTES + Q_BYTES) + MERGE_BYTES + WARPS * ROWS * 8 + WARPS * STAGES * 16 + 64 + 1024;
 };
 
 struct K8sParams {
@@ -69,23 +80,32 @@ __device__ __forceinline__ uint32_t k8_query(uint32_t two, float down) {
   return pack2<__half>(f.x * down, f.y * down);
 }
 
-// WS: a share a warp (many pairs), else a share a CTA (few pairs).
-template <typename T, int HDP, bool WS>
-__global__ void __launch_bounds__(K8sCfg<HDP>::THREADS, 1)
+// The 8 x 8 matrix of 16-bit values of which lane 4 r + c holds row r, columns 2 c and 2 c + 1, turned.
+__device__ __forceinline__ uint32_t k8_turn(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// WS: a share a warp (many pairs), else a share a CTA (few pairs; NR up to 2).
+template <typename T, int HDP, int NR, bool WS>
+__global__ void __launch_bounds__(K8sCfg<HDP, NR>::THREADS, 1)
     kv8_step_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const K8sParams pp) {
-  using Cfg = K8sCfg<HDP>;
-  constexpr int WARPS = Cfg::WARPS, BK = Cfg::BK, STAGES = Cfg::STAGES, KSTEPS = HDP / 16, NT = HDP / 8, ST = BK / 8;
+  using Cfg = K8sCfg<HDP, NR>;
+  constexpr int WARPS = Cfg::WARPS, BK = Cfg::BK, STAGES = Cfg::STAGES, ROWS = Cfg::ROWS, KSTEPS = HDP / 16, MT = HDP / 16, ST = BK / 8;
+  static_assert(WS || NR <= 2, "shares of a CTA: up to 16 rows");
   extern __shared__ uint8_t ks_smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ks_smem_raw) + 1023) & ~uintptr_t(1023));
-  float* merge_o = reinterpret_cast<float*>(base + WARPS * Cfg::RING_BYTES);  // [4][16][HDP]
-  float2* merge_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(merge_o) + Cfg::MERGE_BYTES);  // [WARPS][16]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(merge_ml + WARPS * KS_ROWS);   // [WARPS][STAGES]
-  uint64_t* exps_all = bars + WARPS * STAGES;                                 // likewise: four tiles' (key, value) exponents
+  float* merge_o = reinterpret_cast<float*>(base + WARPS * (Cfg::RING_BYTES + Cfg::Q_BYTES));  // [4][ROWS][HDP]
+  float2* merge_ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(merge_o) + Cfg::MERGE_BYTES);  // [WARPS][ROWS]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(merge_ml + WARPS * ROWS);  // [WARPS][STAGES]
+  uint64_t* exps_all = bars + WARPS * STAGES;                             // likewise: four tiles' (key, value) exponents
   __shared__ int64_t warp_tot[WARPS], found[WS ? WARPS : 1][2];
   const KsParams& p = pp.s;
   const KvView& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = base + warp * Cfg::RING_BYTES;
+  const uint32_t qs = smem_addr(base + WARPS * Cfg::RING_BYTES + warp * Cfg::Q_BYTES);  // [k step][group][lane] fragments
   uint64_t* bar = bars + warp * STAGES;
   uint16_t* exps = reinterpret_cast<uint16_t*>(exps_all + warp * STAGES);
 
@@ -176,60 +196,68 @@ __global__ void __launch_bounds__(K8sCfg<HDP>::THREADS, 1)
   for (int i = 0; i < STAGES; ++i) issue();
 
   const int g = lane >> 2, t4 = lane & 3;
-  const int rows_of_n = p.group;
-  const int key_row = key_of<HDP>(g);                                  // of a tile of 8: the lane's key
-  const int va = key_of<HDP>(2 * t4), vb = key_of<HDP>(2 * t4 + 1);    // and its rows of values
+  const int key_row = key_of<HDP>(g);                                // of a tile of 8: the lane's key
+  const int va = key_of<HDP>(2 * t4), vb = key_of<HDP>(2 * t4 + 1);  // and its rows of values
   bool ok = true;
   for (; !cw.done(); cw.next(c, p.window, p.sinks)) {
-    const int32_t rows = rows_of_n * cw.s.n;  // <= 16
+    const int32_t rows = p.group * cw.s.n;  // <= ROWS; row r = token r / group, head r % group
     const int32_t pos0 = cw.s.len - cw.s.n;
-    // Q fragments (row r = token r / group, head r % group); rows and columns that are not there are zero.  Product kk
-    // contracts columns col(kk) + {0, 1} (first halves) and + {2, 3} of every lane's 16
-    uint32_t qf[KSTEPS][4];
-    float fa = p.scale_log2, fb = p.scale_log2;
-    {
-      float top[2] = {0.f, 0.f};
+    // Q fragments: lane (g, t4) holds row g of every group of eight, columns col + {0, 1}, {2, 3} of its 16 for product k.
+    // Rows and columns that are not there are zero
+    uint32_t qf[Cfg::Q_REGS ? KSTEPS : 1][Cfg::Q_REGS ? NR : 1][2];
+    float scale[NR][2];  // of the scores of rows 8 n + 2 t4 and the next
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = g + 8 * i;
-        const int tok = r / rows_of_n, hd = r - tok * rows_of_n;
-        const T* src = r < rows ? static_cast<const T*>(p.q.ptr) + (cw.s.first + tok) * p.q.token + (cw.h * p.group + hd) * p.q.head : nullptr;
+    for (int n = 0; n < NR; ++n) {
+      const int r = 8 * n + g, tok = r / p.group, hd = r - tok * p.group;
+      const T* src = r < rows ? static_cast<const T*>(p.q.ptr) + (cw.s.first + tok) * p.q.token + (cw.h * p.group + hd) * p.q.head : nullptr;
+      uint32_t w[KSTEPS][2];
 #pragma unroll
-        for (int k = 0; k < KSTEPS; k += 2) {
-          const int col = (k >> 2) * 64 + t4 * 16 + (k & 3) * 4;
-          const uint4 w = src && col < c.head_dim ? *reinterpret_cast<const uint4*>(src + col) : make_uint4(0, 0, 0, 0);
-          qf[k][i] = w.x;
-          qf[k][i + 2] = w.y;
-          qf[k + 1][i] = w.z;
-          qf[k + 1][i + 2] = w.w;
-        }
-        if constexpr (!std::is_same<T, __half>::value) {
+      for (int k = 0; k < KSTEPS; k += 2) {
+        const int col = (k >> 2) * 64 + t4 * 16 + (k & 3) * 4;
+        const uint4 v = src && col < c.head_dim ? *reinterpret_cast<const uint4*>(src + col) : make_uint4(0, 0, 0, 0);
+        w[k][0] = v.x, w[k][1] = v.y, w[k + 1][0] = v.z, w[k + 1][1] = v.w;
+      }
+      float mine = p.scale_log2;
+      if constexpr (!std::is_same<T, __half>::value) {
+        float top = 0.f;
 #pragma unroll
-          for (int k = 0; k < KSTEPS; ++k)
+        for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
-            for (int y = i; y < 4; y += 2) {
-              const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qf[k][y]));
-              top[i] = fmaxf(top[i], fmaxf(fabsf(v.x), fabsf(v.y)));
-            }
-          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-          const int32_t e = k8_query_exponent(top[i]);
-          const float down = exp2_whole(-e);
-          (i ? fb : fa) = p.scale_log2 * exp2_whole(e);
+          for (int y = 0; y < 2; ++y) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[k][y]));
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int32_t e = k8_query_exponent(top);
+        const float down = exp2_whole(-e);
+        mine *= exp2_whole(e);
 #pragma unroll
-          for (int k = 0; k < KSTEPS; ++k)
+        for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
-            for (int y = i; y < 4; y += 2) qf[k][y] = k8_query<T>(qf[k][y], down);
-        }
+          for (int y = 0; y < 2; ++y) w[k][y] = k8_query<T>(w[k][y], down);
+      }
+      scale[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t4);      // (a lane of row 2 t4)
+      scale[n][1] = __shfl_sync(0xffffffffu, mine, 8 * t4 + 4);
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        if constexpr (Cfg::Q_REGS)
+          qf[k][n][0] = w[k][0], qf[k][n][1] = w[k][1];
+        else
+          asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(qs + uint32_t(((k * NR + n) * 32 + lane) * 8)), "r"(w[k][0]), "r"(w[k][1]) : "memory");
       }
     }
-    const int32_t pa = pos0 + g / rows_of_n, pb = pos0 + (g + 8) / rows_of_n;  // the rows' positions
-    float oacc[NT][4];
+    __syncwarp();
+    float oacc[MT][NR][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) oacc[i][j] = 0.f;
-    float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) oacc[i][n][j] = 0.f;
+    float m[NR][2], l[NR][2];  // of rows 8 n + 2 t4 and the next; l: the lane's keys only
+#pragma unroll
+    for (int n = 0; n < NR; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
 
     for (int32_t k = cw.k0 + start; k < cw.k1; k += STRIDE) {
       const uint32_t s = taken % STAGES;
@@ -239,8 +267,7 @@ __global__ void __launch_bounds__(K8sCfg<HDP>::THREADS, 1)
       uint8_t* sk = ring + s * Cfg::STAGE_BYTES;
       uint8_t* sv = sk + Cfg::KV_BYTES;
       const int32_t key0 = tile_index(cw.tiles, k) * BK;
-      const bool whole = all_needed(cw.span, key0, key0 + BK);
-      if (!whole) {
+      if (!all_needed(cw.span, key0, key0 + BK)) {
         // values of keys that no row sees may be anything in memory: zero weights must not meet a NaN
         if (!key_needed(cw.span, key0 + lane)) {
 #pragma unroll
@@ -251,82 +278,104 @@ __global__ void __launch_bounds__(K8sCfg<HDP>::THREADS, 1)
       }
       const uint32_t skb = smem_addr(sk), svb = smem_addr(sv);
       const uint2 packed = k8_lds64(smem_addr(exps + s * ST));
-      // u = scores in base 2 plus the values' exponents: 16 rows x BK keys
-      float sacc[ST][4];
-      float back[ST];  // 2^-(values' exponent)
+      // S^T: tile pair i holds keys key_row of tiles 2 i (values 0, 1: rows 2 t4 and the next) and 2 i + 1 (values 2, 3)
+      float u[2][NR][4];
 #pragma unroll
-      for (int n = 0; n < ST; ++n) {
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sacc[n][j] = 0.f;
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) u[i][n][j] = 0.f;
 #pragma unroll
         for (int hh = 0; hh < HDP / 64; ++hh) {
-          const uint4 w = k8_lds128(skb + k8_at<HDP>(n * 8 + key_row, hh * 4 + t4));
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+          const uint4 wa = k8_lds128(skb + k8_at<HDP>(16 * i + key_row, hh * 4 + t4)), wb = k8_lds128(skb + k8_at<HDP>(16 * i + 8 + key_row, hh * 4 + t4));
+          const uint32_t xa[4] = {wa.x, wa.y, wa.z, wa.w}, xb[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_16816<__half>(sacc[n], qf[hh * 4 + kk], k8_unpack(words[kk] & 0xffffu), k8_unpack(words[kk] >> 16));
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t a[4] = {k8_unpack(xa[kk] & 0xffffu), k8_unpack(xb[kk] & 0xffffu), k8_unpack(xa[kk] >> 16), k8_unpack(xb[kk] >> 16)};
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              if constexpr (Cfg::Q_REGS) {
+                mma_16816<__half>(u[i][n], a, qf[hh * 4 + kk][n][0], qf[hh * 4 + kk][n][1]);
+              } else {
+                const uint2 b = k8_lds64(qs + uint32_t((((hh * 4 + kk) * NR + n) * 32 + lane) * 8));
+                mma_16816<__half>(u[i][n], a, b.x, b.y);
+              }
+            }
+          }
         }
-        const uint32_t e = (n < 2 ? packed.x : packed.y) >> (16 * (n & 1));
+      }
+      float back[4];  // 2^-(values' exponent) of the four tiles
+      float most[NR][2];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t e = (x < 2 ? packed.x : packed.y) >> (16 * (x & 1));
         const float fk = exp2_whole(int32_t(int8_t(e & 0xff)));
         const int32_t ev = int32_t(int8_t((e >> 8) & 0xff));
-        back[n] = exp2_whole(-ev);
-        const float ga = fa * fk, gb = fb * fk, add = float(ev);
-        sacc[n][0] = fmaf(sacc[n][0], ga, add);
-        sacc[n][1] = fmaf(sacc[n][1], ga, add);
-        sacc[n][2] = fmaf(sacc[n][2], gb, add);
-        sacc[n][3] = fmaf(sacc[n][3], gb, add);
+        back[x] = exp2_whole(-ev);
+        const float add = float(ev);
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float& v = u[x >> 1][n][2 * (x & 1) + j];
+            v = fmaf(v, scale[n][j] * fk, add);
+          }
       }
       if (!all_visible(key0, key0 + BK, pos0, cw.s.len - 1, p.window, p.sinks)) {
 #pragma unroll
-        for (int n = 0; n < ST; ++n)
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int32_t key = key0 + n * 8 + ((j & 1) ? vb : va);
-            if (!key_visible(key, j < 2 ? pa : pb, p.window, p.sinks)) sacc[n][j] = -INFINITY;
+          for (int j = 0; j < 2; ++j) {
+            const int32_t pos = pos0 + (8 * n + 2 * t4 + j) / p.group;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (!key_visible(key0 + 8 * x + key_row, pos, p.window, p.sinks)) u[x >> 1][n][2 * (x & 1) + j] = -INFINITY;
           }
       }
-      // running maximum and sum of the two rows
-      float xa = -INFINITY, xb = -INFINITY;
+      bool grow = false;
 #pragma unroll
-      for (int n = 0; n < ST; ++n) {
-        xa = fmaxf(xa, fmaxf(sacc[n][0], sacc[n][1]));
-        xb = fmaxf(xb, fmaxf(sacc[n][2], sacc[n][3]));
-      }
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, o));
-        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o));
-      }
-      const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
-      if (__any_sync(0xffffffffu, na > ma || nb > mb)) {
-        const float da = ma == -INFINITY ? 0.f : exp2_fast(ma - na), db = mb == -INFINITY ? 0.f : exp2_fast(mb - nb);
-        la *= da;
-        lb *= db;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          oacc[i][0] *= da;
-          oacc[i][1] *= da;
-          oacc[i][2] *= db;
-          oacc[i][3] *= db;
+        for (int j = 0; j < 2; ++j) {
+          most[n][j] = fmaxf(fmaxf(u[0][n][j], u[0][n][2 + j]), fmaxf(u[1][n][j], u[1][n][2 + j]));
+          grow = grow || most[n][j] > m[n][j] + 8.f;
         }
-        ma = na;
-        mb = nb;
-      }
-      const float ra = ma == -INFINITY ? 0.f : ma, rb = mb == -INFINITY ? 0.f : mb;
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int n = 0; n < ST; ++n) {
-        sacc[n][0] = exp2_fast(sacc[n][0] - ra);
-        sacc[n][1] = exp2_fast(sacc[n][1] - ra);
-        sacc[n][2] = exp2_fast(sacc[n][2] - rb);
-        sacc[n][3] = exp2_fast(sacc[n][3] - rb);
-        la = fmaf(sacc[n][0] + sacc[n][1], back[n], la);
-        lb = fmaf(sacc[n][2] + sacc[n][3], back[n], lb);
-      }
-      // O += P V
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk) {
-        const uint32_t a[4] = {pack2<__half>(sacc[2 * kk][0], sacc[2 * kk][1]), pack2<__half>(sacc[2 * kk][2], sacc[2 * kk][3]),
-                               pack2<__half>(sacc[2 * kk + 1][0], sacc[2 * kk + 1][1]), pack2<__half>(sacc[2 * kk + 1][2], sacc[2 * kk + 1][3])};
+          for (int j = 0; j < 2; ++j) {
+            float x = most[n][j];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            x = fmaxf(x, m[n][j]);
+            const float d = m[n][j] == -INFINITY ? 0.f : exp2_fast(m[n][j] - x);
+            m[n][j] = x;
+            l[n][j] *= d;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              oacc[i][n][j] *= d;
+              oacc[i][n][2 + j] *= d;
+            }
+          }
+      }
+      // weights, and their turned fragments: keys along the products' contraction, a row a lane
+      uint32_t pf[2][NR][2];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const float ra = m[n][0] == -INFINITY ? 0.f : m[n][0], rb = m[n][1] == -INFINITY ? 0.f : m[n][1];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float wa = exp2_fast(u[x >> 1][n][2 * (x & 1)] - ra), wb = exp2_fast(u[x >> 1][n][2 * (x & 1) + 1] - rb);
+          l[n][0] = fmaf(wa, back[x], l[n][0]);
+          l[n][1] = fmaf(wb, back[x], l[n][1]);
+          pf[x >> 1][n][x & 1] = k8_turn(pack2<__half>(wa, wb));
+        }
+      }
+      // O^T += V^T P^T: product i of the lane's columns 2 i (values 0, 1) and 2 i + 1 (values 2, 3)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
         uint32_t w[4][HDP / 32];  // the lane's columns of its four rows
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
@@ -343,10 +392,13 @@ __global__ void __launch_bounds__(K8sCfg<HDP>::THREADS, 1)
         for (int x = 0; x < HDP / 32; ++x) {
           const uint32_t lo0 = __byte_perm(w[0][x], w[1][x], 0x5140), hi0 = __byte_perm(w[0][x], w[1][x], 0x7362);
           const uint32_t lo1 = __byte_perm(w[2][x], w[3][x], 0x5140), hi1 = __byte_perm(w[2][x], w[3][x], 0x7362);
-          mma_16816<__half>(oacc[4 * x], a, k8_unpack(lo0 & 0xffffu), k8_unpack(lo1 & 0xffffu));
-          mma_16816<__half>(oacc[4 * x + 1], a, k8_unpack(lo0 >> 16), k8_unpack(lo1 >> 16));
-          mma_16816<__half>(oacc[4 * x + 2], a, k8_unpack(hi0 & 0xffffu), k8_unpack(hi1 & 0xffffu));
-          mma_16816<__half>(oacc[4 * x + 3], a, k8_unpack(hi0 >> 16), k8_unpack(hi1 >> 16));
+          const uint32_t a0[4] = {k8_unpack(lo0 & 0xffffu), k8_unpack(lo0 >> 16), k8_unpack(lo1 & 0xffffu), k8_unpack(lo1 >> 16)};
+          const uint32_t a1[4] = {k8_unpack(hi0 & 0xffffu), k8_unpack(hi0 >> 16), k8_unpack(hi1 & 0xffffu), k8_unpack(hi1 >> 16)};
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            mma_16816<__half>(oacc[2 * x][n], a0, pf[kk][n][0], pf[kk][n][1]);
+            mma_16816<__half>(oacc[2 * x + 1][n], a1, pf[kk][n][0], pf[kk][n][1]);
+          }
         }
       }
       ++taken;
@@ -355,124 +407,110 @@ __global__ void __launch_bounds__(K8sCfg<HDP>::THREADS, 1)
     }
 
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      la += __shfl_xor_sync(0xffffffffu, la, o);
-      lb += __shfl_xor_sync(0xffffffffu, lb, o);
-    }
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], o);
     const bool begins = cw.k0 == 0, ends = cw.k1 == cw.blocks, finished = begins && ends;
-    const int64_t piece = 2 * share + (begins ? 1 : 0);
-    // of row g (or g + 8) the lane holds columns t4 * NT * 2 + [0, NT) in oacc[.][0] (or [2]) and the NT behind them in the next
+    const int64_t piece = (2 * share + (begins ? 1 : 0)) * p.piece_rows;
+    // of row 8 n + 2 t4 + j the lane holds columns col + [0, HDP / 8): oacc[i][n][j] and [2 + j] are 2 i and 2 i + 1
+    const int col = g * (HDP / 8);
     if constexpr (WS) {
       if (!ok) continue;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = g + 8 * i;
-        if (r >= rows) continue;
-        const float m = i ? mb : ma, l = i ? lb : la;
-        const int tok = r / rows_of_n, head = cw.h * p.group + (r - tok * rows_of_n);
-        const int64_t token = cw.s.first + tok;
-        if (finished) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          T* dst = static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head;
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2)
+        for (int j = 0; j < 2; ++j) {
+          const int r = 8 * n + 2 * t4 + j;
+          if (r >= rows || col >= c.head_dim) continue;
+          if (finished) {
+            const int tok = r / p.group, head = cw.h * p.group + (r - tok * p.group);
+            const float inv = l[n][j] == 0.f ? 0.f : 1.f / l[n][j];
+            T* dst = static_cast<T*>(p.o.ptr) + (cw.s.first + tok) * p.o.token + head * p.o.head + col;
 #pragma unroll
-            for (int n = 0; n < NT; n += 8) {
-              const int col = t4 * NT * 2 + h2 * NT + n;
-              if (col < c.head_dim) {
-                uint32_t w[4];
+            for (int i = 0; i < MT; i += 4) {
+              uint32_t w[4];
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  w[y] = pack2<T>(oacc[n + 2 * y][2 * i + h2] * inv, oacc[n + 2 * y + 1][2 * i + h2] * inv);
-                *reinterpret_cast<uint4*>(dst + col) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int y = 0; y < 4; ++y) w[y] = pack2<T>(oacc[i + y][n][j] * inv, oacc[i + y][n][2 + j] * inv);
+              *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            // (scores that are all NaN leave the maximum at -inf: their NaN sum must not be taken for an empty state)
+            if (g == 0) p.piece_ml[piece + r] = make_float2(l[n][j] == l[n][j] ? m[n][j] : 0.f, l[n][j]);
+            float* po = p.piece_o + (piece + r) * c.head_dim + col;
+#pragma unroll
+            for (int i = 0; i < MT; i += 2)
+              *reinterpret_cast<float4*>(po + 2 * i) = make_float4(oacc[i][n][j], oacc[i][n][2 + j], oacc[i + 1][n][j], oacc[i + 1][n][2 + j]);
+          }
+        }
+    } else {
+      // the warps' states meet: maxima and sums first, then the products, each scaled to the common maximum, four warps
+      // at a time into four slots
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (g == 0) merge_ml[warp * ROWS + 8 * n + 2 * t4 + j] = make_float2(l[n][j] == l[n][j] ? m[n][j] : 0.f, l[n][j]);
+      __syncthreads();
+      // (16-byte vectors change places by row and by eight, so that a store's lanes lie in different banks)
+      float* slot_o = merge_o + (warp & 3) * ROWS * HDP;
+      auto vec_at = [&](int row, int v) { return row * HDP + ((v ^ (row & 7) ^ ((v >> 3) & 7)) << 2); };
+#pragma unroll 1
+      for (int turn = 0; turn < WARPS / 4; ++turn) {
+        if (warp >> 2 == turn) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int r = 8 * n + 2 * t4 + j;
+              float top = -INFINITY;
+              for (int w = 0; w < WARPS; ++w) top = fmaxf(top, merge_ml[w * ROWS + r].x);
+              const float own = merge_ml[warp * ROWS + r].x, e = own == -INFINITY ? 0.f : exp2_fast(own - top);
+#pragma unroll
+              for (int i = 0; i < MT; i += 2) {
+                float4* at = reinterpret_cast<float4*>(slot_o + vec_at(r, (col >> 2) + (i >> 1)));
+                float4 v = turn > 0 ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                v.x += e * oacc[i][n][j];
+                v.y += e * oacc[i][n][2 + j];
+                v.z += e * oacc[i + 1][n][j];
+                v.w += e * oacc[i + 1][n][2 + j];
+                *at = v;
               }
             }
+        }
+        __syncthreads();
+      }
+      const int vecs = c.head_dim >> 2;
+      for (int it = threadIdx.x; it < rows * vecs; it += Cfg::THREADS) {
+        const int r = it / vecs, v = it - r * vecs;
+        float top = -INFINITY, sum = 0.f;
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, merge_ml[w * ROWS + r].x);
+        for (int w = 0; w < WARPS; ++w) {
+          const float2 ml = merge_ml[w * ROWS + r];
+          sum += (ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top)) * ml.y;
+        }
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(merge_o + w * ROWS * HDP + vec_at(r, v));
+          o.x += x.x;
+          o.y += x.y;
+          o.z += x.z;
+          o.w += x.w;
+        }
+        if (finished) {
+          const int tok = r / p.group, head = cw.h * p.group + (r - tok * p.group);
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.o.ptr) + (cw.s.first + tok) * p.o.token + head * p.o.head + 4 * v) =
+              make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
         } else {
-          if (t4 == 0) p.piece_ml[piece * KS_ROWS + r] = make_float2(l == l ? m : 0.f, l);
-          float* po = p.piece_o + (piece * KS_ROWS + r) * c.head_dim;
-#pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2)
-#pragma unroll
-            for (int n = 0; n < NT; n += 4) {
-              const int col = t4 * NT * 2 + h2 * NT + n;
-              if (col < c.head_dim)
-                *reinterpret_cast<float4*>(po + col) =
-                    make_float4(oacc[n][2 * i + h2], oacc[n + 1][2 * i + h2], oacc[n + 2][2 * i + h2], oacc[n + 3][2 * i + h2]);
-            }
+          if (v == 0) p.piece_ml[piece + r] = make_float2(top, sum);
+          *reinterpret_cast<float4*>(p.piece_o + (piece + r) * c.head_dim + 4 * v) = o;
         }
       }
-      continue;
+      __syncthreads();
     }
-    // the warps' states meet: maximum and sum first, then the products, each scaled to the common maximum
-    if (t4 == 0) {
-      // (scores that are all NaN leave the maximum at -inf: their NaN sum must not be taken for an empty state)
-      merge_ml[warp * KS_ROWS + g] = make_float2(la == la ? ma : 0.f, la);
-      merge_ml[warp * KS_ROWS + g + 8] = make_float2(lb == lb ? mb : 0.f, lb);
-    }
-    // (16-byte vectors swizzled by row and by eight, so that a store's lanes lie in different banks)
-    float* slot_o = merge_o + (warp & 3) * KS_ROWS * HDP;
-    auto vec_at = [&](int row, int v) { return row * HDP + (((v & ~7) | ((v ^ row ^ ((v >> 3) << 1)) & 7)) << 2); };
-    if (warp >= 4) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2)
-#pragma unroll
-          for (int n = 0; n < NT; n += 4)
-            *reinterpret_cast<float4*>(slot_o + vec_at(g + 8 * i, (t4 * NT * 2 + h2 * NT + n) >> 2)) =
-                make_float4(oacc[n][2 * i + h2], oacc[n + 1][2 * i + h2], oacc[n + 2][2 * i + h2], oacc[n + 3][2 * i + h2]);
-    }
-    __syncthreads();
-    if (warp < 4) {  // the upper four warps' states join the lower four's
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 x = merge_ml[(warp + 4) * KS_ROWS + g + 8 * i], y = merge_ml[warp * KS_ROWS + g + 8 * i];
-        const float n2 = fmaxf(x.x, y.x);
-        const float ex = x.x == -INFINITY ? 0.f : exp2_fast(x.x - n2), ey = y.x == -INFINITY ? 0.f : exp2_fast(y.x - n2);
-#pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2)
-#pragma unroll
-          for (int n = 0; n < NT; n += 4) {
-            float4* at = reinterpret_cast<float4*>(slot_o + vec_at(g + 8 * i, (t4 * NT * 2 + h2 * NT + n) >> 2));
-            const float4 v = *at;
-            *at = make_float4(oacc[n][2 * i + h2] * ey + v.x * ex, oacc[n + 1][2 * i + h2] * ey + v.y * ex,
-                              oacc[n + 2][2 * i + h2] * ey + v.z * ex, oacc[n + 3][2 * i + h2] * ey + v.w * ex);
-          }
-        __syncwarp();
-        if (t4 == 0) merge_ml[warp * KS_ROWS + g + 8 * i] = make_float2(n2, y.y * ey + x.y * ex);
-      }
-    }
-    __syncthreads();
-    const int vecs = c.head_dim >> 2;
-    for (int it = threadIdx.x; it < rows * vecs; it += Cfg::THREADS) {
-      const int r = it / vecs, v = it - r * vecs, col = v << 2;
-      float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) m = fmaxf(m, merge_ml[w * KS_ROWS + r].x);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float2 ml = merge_ml[w * KS_ROWS + r];
-        const float e = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
-        const float4 x = *reinterpret_cast<const float4*>(merge_o + w * KS_ROWS * HDP + vec_at(r, v));
-        l += e * ml.y;
-        o.x += e * x.x;
-        o.y += e * x.y;
-        o.z += e * x.z;
-        o.w += e * x.w;
-      }
-      const int tok = r / rows_of_n, head = cw.h * p.group + (r - tok * rows_of_n);
-      const int64_t token = cw.s.first + tok;
-      if (finished) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.o.ptr) + token * p.o.token + head * p.o.head + col) =
-            make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-      } else {
-        if (col == 0) p.piece_ml[piece * KS_ROWS + r] = make_float2(m, l);
-        *reinterpret_cast<float4*>(p.piece_o + (piece * KS_ROWS + r) * c.head_dim + col) = o;
-      }
-    }
-    __syncthreads();
   }
   // a wait has run out: behind this warp's copies in flight, which must not outlive the CTA
   if (!ok)

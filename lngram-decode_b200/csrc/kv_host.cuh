@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "kvcache.cuh"
@@ -91,6 +92,18 @@ static int kv_splits(int64_t units, int64_t tiles) {
     }
   }
   return best;
+}
+
+// Lets a kernel use so much dynamic shared memory, once a device (known: a bit for each).
+template <typename K>
+static int allow_smem(K kern, size_t bytes, std::atomic<uint64_t>& known) {
+  int dev = 0;
+  LNG_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (known.load(std::memory_order_relaxed) & bit) return LNG_OK;
+  LNG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  known.fetch_or(bit, std::memory_order_relaxed);
+  return LNG_OK;
 }
 
 // A launch that may start while the kernel before it in the stream still runs (griddepcontrol in both).

@@ -35,42 +35,16 @@ static PgParams pg_params(const lng_kv8_cache* c, int32_t* refs, const int32_t* 
 
 using namespace lng;
 
-extern "C" int lng_kv_pages_extend(const lng_kv8_cache* cache, int32_t* refs, const int32_t* cu, int64_t tokens, int64_t max_new,
-                                   int64_t* slots, uint8_t* served, int32_t* copies, lng_stream_t stream) {
-  if (const int st = check_pool(cache, refs, cu, tokens, max_new)) return st;
-  if (cache->pages.batch == 0) return LNG_OK;
-  LNG_REQUIRE(served && copies && (slots || tokens == 0), "NULL pointer");
-  LNG_REQUIRE((reinterpret_cast<uintptr_t>(copies) & 15) == 0, "copies must be 16-byte aligned");
-  PgParams p = pg_params(cache, refs, cu, tokens, max_new);
-  p.slots = slots;
-  p.served = served;
-  p.copies = reinterpret_cast<int4*>(copies);
-  const int64_t words = ceil_div(p.c.num_pages, 32 * PG_CTAS);
-  const size_t smem = size_t(3 * p.c.batch + words) * 4;
-  if (smem > 40 * 1024)
-    LNG_CUDA(cudaFuncSetAttribute(kv_pages_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-  // (rows that belong to no sequence)
-  if (cu && tokens > 0) LNG_CUDA(cudaMemsetAsync(slots, 0xff, size_t(tokens) * 8, S(stream)));
-  kv_pages_extend_kernel<<<PG_CTAS, PG_THREADS, smem, S(stream)>>>(p);
-  LNG_LAUNCHED("kv_pages_extend_kernel");
-  return LNG_OK;
-}
-
-extern "C" int lng_kv_pages_copy(const lng_kv8_cache* cache, const int32_t* copies, lng_stream_t stream) {
-  LNG_REQUIRE(cache != nullptr, "cache descriptor is NULL");
-  lng_kv_cache c = cache->pages;
-  if (c.batch == 0) return LNG_OK;
-  if (const int st = check_kv(&c, nullptr, c.batch, 1)) return st;
-  LNG_REQUIRE((cache->k_exp == nullptr) == (cache->v_exp == nullptr), "k_exp and v_exp go together");
-  LNG_REQUIRE(c.batch <= PG_MOST_BATCH, "a pool serves at most 8192 sequences");
-  LNG_REQUIRE(copies != nullptr && (reinterpret_cast<uintptr_t>(copies) & 15) == 0, "copies must be 16-byte aligned");
-  const int64_t size = cache->k_exp ? 1 : 2;  // bytes a value
+// An extend's copies in one cache: a dependent launch, that waits for the whole of the kernel that notes them.
+static int launch_pages_copy(const lng_kv8_cache& cache, const int32_t* copies, cudaStream_t stream) {
+  const lng_kv_cache& c = cache.pages;
+  const int64_t size = cache.k_exp ? 1 : 2;  // bytes a value
   PgCopyParams p{};
   p.k = static_cast<uint8_t*>(c.k), p.v = static_cast<uint8_t*>(c.v);
   p.k_page = c.k_page_stride * size, p.k_head = c.k_head_stride * size, p.k_slot = c.k_slot_stride * size;
   p.v_page = c.v_page_stride * size, p.v_head = c.v_head_stride * size, p.v_slot = c.v_slot_stride * size;
-  p.k_exp = cache->k_exp, p.v_exp = cache->v_exp;
-  p.k_exp_page = cache->k_exp_stride, p.v_exp_page = cache->v_exp_stride;
+  p.k_exp = cache.k_exp, p.v_exp = cache.v_exp;
+  p.k_exp_page = cache.k_exp_stride, p.v_exp_page = cache.v_exp_stride;
   p.num_pages = c.num_pages;
   p.heads = c.num_kv_heads;
   p.page_size = c.page_size;
@@ -78,17 +52,38 @@ extern "C" int lng_kv_pages_copy(const lng_kv8_cache* cache, const int32_t* copi
   // strides are multiples of 8 values: 16 bytes in 16 bits, 8 bytes in 8
   const int vec = size == 2 ? 16 : 8;
   p.vecs = int32_t(c.head_dim * size / vec);
-  const dim3 grid(unsigned(c.batch), unsigned(2 * std::min<int64_t>(8, c.num_kv_heads)));
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(128);
-  cfg.stream = S(stream);
-  cfg.attrs = pdl;
-  cfg.numAttrs = 1;
-  LNG_CUDA(cudaLaunchKernelEx(&cfg, vec == 16 ? kv_pages_copy_kernel<16> : kv_pages_copy_kernel<8>, p));
+  const dim3 grid{unsigned(c.batch), unsigned(2 * std::min<int64_t>(8, c.num_kv_heads)), 1u};
+  return launch_dependent(vec == 16 ? kv_pages_copy_kernel<16> : kv_pages_copy_kernel<8>, grid, 128u, size_t(0), stream, p);
+}
+
+extern "C" int lng_kv_pages_extend(const lng_kv8_cache* caches, int32_t count, int32_t* refs, const int32_t* cu, int64_t tokens,
+                                   int64_t max_new, int64_t* slots, uint8_t* served, int32_t* copies, lng_stream_t stream) {
+  LNG_REQUIRE(count >= 1 && caches != nullptr, "a pool needs at least one cache");
+  for (int32_t i = 0; i < count; ++i) {
+    if (const int st = check_pool(&caches[i], refs, cu, tokens, max_new)) return st;
+    LNG_REQUIRE(caches[i].pages.k && caches[i].pages.v, "NULL pointer in the cache descriptor");
+    LNG_REQUIRE(caches[i].pages.batch == caches[0].pages.batch && caches[i].pages.num_pages == caches[0].pages.num_pages &&
+                    caches[i].pages.page_size == caches[0].pages.page_size,
+                "a pool's caches must be of one geometry");
+  }
+  if (caches->pages.batch == 0) return LNG_OK;
+  LNG_REQUIRE(served && copies && (slots || tokens == 0), "NULL pointer");
+  LNG_REQUIRE((reinterpret_cast<uintptr_t>(copies) & 15) == 0, "copies must be 16-byte aligned");
+  PgParams p = pg_params(caches, refs, cu, tokens, max_new);
+  p.slots = slots;
+  p.served = served;
+  p.copies = reinterpret_cast<int4*>(copies);
+  const int64_t words = ceil_div(p.c.num_pages, 32 * PG_CTAS);
+  const size_t smem = size_t(3 * p.c.batch + words) * 4;
+  static std::atomic<uint64_t> known{0};
+  if (smem > 40 * 1024)
+    if (const int st = allow_smem(kv_pages_extend_kernel, 200 * 1024, known)) return st;
+  // (rows that belong to no sequence)
+  if (cu && tokens > 0) LNG_CUDA(cudaMemsetAsync(slots, 0xff, size_t(tokens) * 8, S(stream)));
+  kv_pages_extend_kernel<<<PG_CTAS, PG_THREADS, smem, S(stream)>>>(p);
+  LNG_LAUNCHED("kv_pages_extend_kernel");
+  for (int32_t i = 0; i < count; ++i)
+    if (const int st = launch_pages_copy(caches[i], copies, S(stream))) return st;
   return LNG_OK;
 }
 
@@ -114,8 +109,9 @@ extern "C" int lng_kv_pages_reorder(const lng_kv8_cache* cache, int32_t* refs, c
   LNG_REQUIRE(parents != nullptr, "parents is NULL");
   const PgParams p = pg_params(cache, refs, nullptr, cache->pages.batch, 1);
   const size_t smem = size_t(3 * beams + std::max<int64_t>(PG_REORDER_CELLS, beams)) * 4;
+  static std::atomic<uint64_t> known{0};
   if (smem > 48 * 1024)
-    LNG_CUDA(cudaFuncSetAttribute(kv_pages_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (const int st = allow_smem(kv_pages_reorder_kernel, 160 * 1024, known)) return st;
   kv_pages_reorder_kernel<<<unsigned(groups), PG_REORDER_THREADS, smem, S(stream)>>>(p, parents, int32_t(beams));
   LNG_LAUNCHED("kv_pages_reorder_kernel");
   return LNG_OK;

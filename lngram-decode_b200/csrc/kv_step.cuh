@@ -56,8 +56,9 @@ struct KsParams {
   int32_t window, sinks;
   int32_t box;       // keys a TMA copy: min(page size, 32)
   // pieces: slot 2 * share (a pair begun before the share) and 2 * share + 1 (one that goes on behind it)
-  float2* piece_ml;  // [2 * shares][16] (maximum, sum), base 2
-  float* piece_o;    // [2 * shares][16][head_dim]
+  float2* piece_ml;  // [2 * shares][piece_rows] (maximum, sum), base 2
+  float* piece_o;    // [2 * shares][piece_rows][head_dim]
+  int32_t piece_rows;  // room for a pair's rows: 16 here
   int32_t shares;    // into which the line is cut
   // a shared prefix: states of `prefix_slots` ranges of it, [slot][row][..] with row = token * q_heads + head;
   // pairs finished by one CTA then go to slot prefix_slots (null: to o)
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(256) kv_step_join_kernel(const KsParams p) {
     const bool live = r < rows;
     const int tok = r / p.group, head = h * p.group + (r - tok * p.group);
     const int64_t token = s.first + tok, row = token * p.q_heads + head;
-    auto piece = [&](int i) { return (2 * (c0 + i) + (i == 0 ? 1 : 0)) * KS_ROWS + r; };
+    auto piece = [&](int i) { return (2 * (c0 + i) + (i == 0 ? 1 : 0)) * p.piece_rows + r; };
     KsRow x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
     if (live)
       x = ks_join_states(

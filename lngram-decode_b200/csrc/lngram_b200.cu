@@ -1874,6 +1874,7 @@ static int kv_attend_run(const lng_kv_cache* cache, const int32_t* prefix_table,
   p.box = std::min(cache->page_size, KsCfg<64>::BK);
   p.piece_ml = reinterpret_cast<float2*>(ws + plan.piece_ml);
   p.piece_o = reinterpret_cast<float*>(ws + plan.piece_o);
+  p.piece_rows = KS_ROWS;
   p.shares = plan.shares;
   p.row_ml = row_ml;
   p.row_o = row_o;

@@ -55,7 +55,10 @@ class PagePool:
         _require(refs.shape == (pages,) and refs.dtype == torch.int32 and refs.is_contiguous(), f"refs must be contiguous int32 [{pages}]")
         _require(refs.device == first.device, "refs must be on the caches' device")
         self.caches, self.cache, self._refs = caches, first, refs
-        self._descs = [c._desc if c.eight else _lib.KvCache8(pages=c._desc) for c in caches]
+        descs = [c._desc if c.eight else _lib.KvCache8(pages=c._desc) for c in caches]
+        self._descs = (_lib.KvCache8 * len(descs))(*descs)
+        self._ref = C.byref(self._descs[0])
+        self._copies = torch.empty(first.batch, 4, dtype=torch.int32, device=first.device)  # an extend's, until its last copy
 
     refs = property(lambda self: self._refs)
 
@@ -111,12 +114,9 @@ class PagePool:
         lib = _library(c)
         slots = torch.empty(shape, dtype=torch.int64, device=c.device)
         served = torch.empty(c.batch, dtype=torch.bool, device=c.device)
-        copies = torch.empty(c.batch, 4, dtype=torch.int32, device=c.device)
         with _lib.on_device(c.device):
-            check(lib.lng_kv_pages_extend(C.byref(self._descs[0]), ptr(self._refs), ptr(cu), tokens, n, ptr(slots), ptr(served),
-                                          ptr(copies), stream_ptr()), "extend")
-            for desc in self._descs:
-                check(lib.lng_kv_pages_copy(C.byref(desc), ptr(copies), stream_ptr()), "extend")
+            check(lib.lng_kv_pages_extend(self._ref, len(self.caches), ptr(self._refs), ptr(cu), tokens, n, ptr(slots), ptr(served),
+                                          ptr(self._copies), stream_ptr()), "extend")
         return slots, served
 
     def truncate(self, lengths) -> None:
@@ -134,7 +134,7 @@ class PagePool:
                 raise ValueError("lengths must not be negative")
         lib = _library(c)
         with _lib.on_device(c.device):
-            check(lib.lng_kv_pages_truncate(C.byref(self._descs[0]), ptr(self._refs), ptr(lengths), most, stream_ptr()), "truncate")
+            check(lib.lng_kv_pages_truncate(self._ref, ptr(self._refs), ptr(lengths), most, stream_ptr()), "truncate")
 
     def reorder(self, parents: Tensor) -> None:
         """Beams: row g * beams + k takes over the pages and the length of row g * beams + ``parents[g, k]`` (int64
@@ -146,5 +146,5 @@ class PagePool:
             raise ValueError(f"parents must be contiguous int64 [groups, beams] of {c.batch} rows on the cache's device")
         lib = _library(c)
         with _lib.on_device(c.device):
-            check(lib.lng_kv_pages_reorder(C.byref(self._descs[0]), ptr(self._refs), ptr(parents), parents.shape[0],
+            check(lib.lng_kv_pages_reorder(self._ref, ptr(self._refs), ptr(parents), parents.shape[0],
                                            parents.shape[1], stream_ptr()), "reorder")

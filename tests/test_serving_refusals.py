@@ -188,13 +188,12 @@ def test_c_entries_refuse_before_any_launch(lngram):
         assert append(cache(), **kw) == bad_arg, kw
     assert lib.lng_kv8_values(cache(), 8, None, None) == bad_arg and lib.lng_kv8_values(cache(k_exp=None), 16, None, None) == bad_arg
 
-    extend = lambda c, refs=64, tokens=6, slots=64, served=64, copies=64: lib.lng_kv_pages_extend(  # noqa: E731
-        c, refs, None, tokens, 3, slots, served, copies, None)
+    extend = lambda c, refs=64, tokens=6, slots=64, served=64, copies=64, count=1: lib.lng_kv_pages_extend(  # noqa: E731
+        c, count, refs, None, tokens, 3, slots, served, copies, None)
     for c in (cache(k_exp=None), cache(dict(batch=8193)), cache(dict(num_pages=(1 << 22) + 1)), cache(dict(max_pages=0))):
         assert extend(c) == bad_arg
-    for kw in (dict(refs=None), dict(slots=None), dict(served=None), dict(copies=None), dict(copies=72), dict(tokens=4)):
+    for kw in (dict(refs=None), dict(slots=None), dict(served=None), dict(copies=None), dict(copies=72), dict(tokens=4), dict(count=0)):
         assert extend(cache(), **kw) == bad_arg, kw
-    assert lib.lng_kv_pages_copy(cache(), None, None) == bad_arg and lib.lng_kv_pages_copy(cache(), 8, None) == bad_arg
     assert lib.lng_kv_pages_truncate(cache(), None, None, 3, None) == bad_arg
     assert lib.lng_kv_pages_truncate(cache(), 64, None, -1, None) == bad_arg
     assert lib.lng_kv_pages_reorder(cache(), 64, 64, 1, 3, None) == bad_arg
