@@ -117,12 +117,16 @@ def beam_reorder(parents: Tensor, *states: Tensor, length: int | None = None) ->
                 raise ValueError("length must be within every state's second dimension")
             inner = (int(length),) + tuple(inner[1:])
         expected = 1
-        for size, stride in zip(reversed(x.shape[1:]), reversed(x.stride()[1:])):
-            if size != 1 and stride != expected:
-                raise ValueError("a state's rows must be contiguous")
-            expected *= size
-        if x.shape[0] > 1 and x.stride(0) < expected:
-            raise ValueError("a state's rows must not overlap")
+        for n in x.shape[1:]:
+            expected *= n
+        if not x.is_contiguous():
+            inside = 1
+            for n, stride in zip(reversed(x.shape[1:]), reversed(x.stride()[1:])):
+                if n != 1 and stride != inside:
+                    raise ValueError("a state's rows must be contiguous")
+                inside *= n
+            if x.shape[0] > 1 and x.stride(0) < expected:
+                raise ValueError("a state's rows must not overlap")
         size = x.element_size()
         count = 1
         for s in inner:

@@ -50,8 +50,9 @@ struct K8tBars {
 };
 static_assert(K8tBars<64>::abort + 4 <= 512 && K8tBars<128>::abort + 4 <= 512, "barriers outgrow their place");
 
-// Two warps, one for keys, one for values: every tile's bytes into the raw ring, page by page, and its exponents, a
-// lane a piece, into those of the tile.  (Exponents of sixteen tiles: a raw slot is given out again when the tile three
+// Two warps, one for keys (and the exponents of both, which the scores' readers need), one for values: every tile's bytes into
+// the raw ring, page by page.  A page and then its exponents are looked up for so many tiles at once as the lanes have pieces for: two
+// look-ups a tile in a row took longer than the tile's products.  (Exponents of sixteen tiles: a raw slot is given out again when the tile three
 // or six before it has been converted, which is behind the products of the tile five or ten before it.)
 template <int HDP>
 __device__ __forceinline__ void k8t_load(const CUtensorMap* map, const K8tParams& pp, uint32_t bars, uint32_t raw, uint32_t exps,
@@ -70,38 +71,42 @@ __device__ __forceinline__ void k8t_load(const CUtensorMap* map, const K8tParams
   while (ok && kt_next(p, walk, w, there)) {
     if (!there || w.n == 0) continue;
     const int32_t* row = c.table + w.b * c.table_stride;
-    int32_t next_exp = 0;
-    auto look_up = [&](int32_t i) -> int32_t {
-      const int32_t key = tile_index(w.tiles, w.j0 + i) * KT_BK + lane * box;
-      next_exp = 0;
-      if (lane >= boxes || !any_needed(w.span, key, key + box)) return -1;
-      const int32_t page = page_of(row, key, c.page_shift, c.num_pages);
+    // the unit's next tiles, as many as give every lane a piece: its page (-1: no token sees a key of it) and exponents
+    int32_t page = -1, exp_k = 0, exp_v = 0;
+    auto look_up = [&](int32_t i) {
+      page = -1;
+      exp_k = exp_v = 0;
+      if (i + lane / boxes >= w.n) return;
+      const int32_t key = tile_index(w.tiles, w.j0 + i + lane / boxes) * KT_BK + (lane % boxes) * box;
+      if (!any_needed(w.span, key, key + box)) return;
+      page = page_of(row, key, c.page_shift, c.num_pages);
       if (page >= 0) {
-        next_exp = kv == 0 ? pp.k_exp[page * pp.k_exp_page + w.hk] : pp.v_exp[page * pp.v_exp_page + w.hk];
-        return page;
+        if (kv == 0) {
+          exp_k = pp.k_exp[page * pp.k_exp_page + w.hk];
+          exp_v = pp.v_exp[page * pp.v_exp_page + w.hk];
+        }
+      } else {
+        kv_range_error();
+        page = int32_t(c.num_pages);  // behind the last page: the copy fills zeros
       }
-      kv_range_error();
-      return int32_t(c.num_pages);  // behind the last page: the copy fills zeros
     };
-    int32_t next = look_up(0);
 #pragma unroll 1
     for (int32_t i = 0; i < w.n; ++i, it += 2) {
-      const int32_t page = next, exp = next_exp;
+      const int lane0 = (i & (32 / boxes - 1)) * boxes;  // of the tile's first piece
+      if (lane0 == 0) look_up(i);
       const int32_t slot0 = uniform((tile_index(w.tiles, w.j0 + i) * KT_BK) & page_mask);
-      if (i + 1 < w.n) next = look_up(i + 1);
-      const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, page >= 0))) * uint32_t(box * HDP);
+      const uint32_t bytes = uint32_t(__popc((__ballot_sync(0xffffffffu, page >= 0) >> lane0) & ((1u << boxes) - 1u))) * uint32_t(box * HDP);
       const uint32_t s = it % NR, bar = bars + B::raw_full + 8 * s, dst = raw + s * Cfg::RAW_BYTES;
       if (it >= NR) ok = __all_sync(0xffffffffu, kt_wait<B>(bars, B::raw_empty + 8 * s, (it / NR - 1) & 1));
       if (!ok) break;
-      // [8] 2^(keys' exponent), [8] values' exponent, [8] 2^-(values' exponent): a number for 8 keys
-      const int32_t e = __shfl_sync(0xffffffffu, exp, ((lane & 7) * 8) / box);
-      const uint32_t at = exps + (it / 2 % K8T_EXPS) * 96 + (lane & 7) * 4;
-      if (lane < 8) {
-        if (kv == 0) {
-          sts32(at, __float_as_uint(exp2_whole(e)));
-        } else {
-          sts32(at + 32, __float_as_uint(float(e)));
-          sts32(at + 64, __float_as_uint(exp2_whole(-e)));
+      if (kv == 0) {  // [8] 2^(keys' exponent), [8] values' exponent, [8] 2^-(values' exponent): a number for 8 keys
+        const int from = lane0 + ((lane & 7) * 8) / box;
+        const int32_t ek = __shfl_sync(0xffffffffu, exp_k, from), ev = __shfl_sync(0xffffffffu, exp_v, from);
+        const uint32_t at = exps + (it / 2 % K8T_EXPS) * 96 + (lane & 7) * 4;
+        if (lane < 8) {
+          sts32(at, __float_as_uint(exp2_whole(ek)));
+          sts32(at + 32, __float_as_uint(float(ev)));
+          sts32(at + 64, __float_as_uint(exp2_whole(-ev)));
         }
       }
       __syncwarp();
@@ -111,7 +116,7 @@ __device__ __forceinline__ void k8t_load(const CUtensorMap* map, const K8tParams
       for (int r = 0; r < boxes; r += 4) {
         int32_t pg[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) pg[x] = __shfl_sync(0xffffffffu, page, (r + x) & 31);
+        for (int x = 0; x < 4; ++x) pg[x] = __shfl_sync(0xffffffffu, page, (lane0 + r + x) & 31);
         if (elect_lane()) {
 #pragma unroll
           for (int x = 0; x < 4; ++x)
@@ -141,52 +146,69 @@ __device__ __forceinline__ void k8t_convert(const K8tParams& pp, uint32_t bars, 
   constexpr uint32_t NS = Cfg::SLOTS, NR = Cfg::RAW_SLOTS;
   constexpr int HALVES = HDP / 64, PIECES = HDP / 16;  // 16-byte pieces of a row as it comes
   const KtParams& p = pp.t;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, group_magic = (65535 + p.group) / p.group;  // r / group = r * magic >> 16 for r < 128
   uint32_t it = 0, units = 0;
   bool ok = true, there;
   KtWalk walk{};
   KtWork w;
   while (ok && kt_next(p, walk, w, there)) {
     if (!there || w.n == 0) continue;
+    for (int G = 0; G < (w.tokens1 > 0 ? 2 : 1); ++G) {  // the queries' way from memory begins
+      const int r = warp * 32 + lane, tok = (r * group_magic) >> 16;
+      const T* src = static_cast<const T*>(pp.q.ptr) + (w.s.first + w.t0 + G * p.tile_tokens + tok) * pp.q.token +
+                     int64_t(w.hk * p.group + r - tok * p.group) * pp.q.head;
+      if (r < (G ? w.tokens1 : w.tokens0) * p.group)
+        for (int x = 0; x < p.c.head_dim; x += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + x));
+    }
     if (units > 0) ok = __all_sync(0xffffffffu, kt_wait<B>(bars, B::q_empty, (units - 1) & 1));
     if (!ok) break;
-    // queries: eight lanes a row, four rows a step
+    // queries: eight lanes a row, four rows a step, the loads of as many steps in flight as 16 registers hold
+    constexpr int STEPS_Q = 4 / HALVES;
     for (int G = 0; G < (w.tokens1 > 0 ? 2 : 1); ++G) {
       const int32_t rows = (G ? w.tokens1 : w.tokens0) * p.group;
       const int64_t token0 = w.s.first + w.t0 + G * p.tile_tokens;
-#pragma unroll 2
-      for (int i = 0; i < 8; ++i) {
-        const int r = warp * 32 + i * 4 + (lane >> 3), chunk = lane & 7;
-        const int32_t tok = r / p.group;
-        const T* src = static_cast<const T*>(pp.q.ptr) + (token0 + tok) * pp.q.token + (w.hk * p.group + (r - tok * p.group)) * pp.q.head;
-        uint4 x[HALVES];
-        float most = 0.f;
+      const T* const q0 = static_cast<const T*>(pp.q.ptr) + token0 * pp.q.token + int64_t(w.hk) * p.group * pp.q.head;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 8; i0 += STEPS_Q) {
+        const int chunk = lane & 7;
+        uint4 x[STEPS_Q][HALVES];
 #pragma unroll
-        for (int hh = 0; hh < HALVES; ++hh) {
-          const int col = hh * 64 + chunk * 8;
-          x[hh] = r < rows && col < p.c.head_dim ? *reinterpret_cast<const uint4*>(src + col) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < STEPS_Q; ++i) {
+          const int r = warp * 32 + (i0 + i) * 4 + (lane >> 3), tok = (r * group_magic) >> 16;
+          const T* src = q0 + tok * pp.q.token + (r - tok * p.group) * pp.q.head + chunk * 8;
+#pragma unroll
+          for (int hh = 0; hh < HALVES; ++hh)
+            x[i][hh] = r < rows && hh * 64 + chunk * 8 < p.c.head_dim ? *reinterpret_cast<const uint4*>(src + hh * 64) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < STEPS_Q; ++i) {
+          const int r = warp * 32 + (i0 + i) * 4 + (lane >> 3);
+          float down = 1.f, up = 1.f;
           if constexpr (!std::is_same<T, __half>::value) {
-            const uint32_t words[4] = {x[hh].x, x[hh].y, x[hh].z, x[hh].w};
+            uint32_t two = 0;  // the largest magnitudes, a pair
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&words[y]));
-              most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
+            for (int hh = 0; hh < HALVES; ++hh) {
+              const uint32_t words[4] = {x[i][hh].x, x[i][hh].y, x[i][hh].z, x[i][hh].w};
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const uint32_t v = words[y] & 0x7fff7fffu;
+                const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&v));
+                two = *reinterpret_cast<const uint32_t*>(&m);
+              }
             }
+            float most = fmaxf(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int32_t e = k8_query_exponent(most);
+            down = exp2_whole(-e);
+            up = exp2_whole(e);
           }
-        }
-        float down = 1.f, up = 1.f;
-        if constexpr (!std::is_same<T, __half>::value) {
+          if (chunk == 0) sts32(scales + ((units & 1) * 256 + G * 128 + r) * 4, __float_as_uint(p.scale_log2 * up));
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const int32_t e = k8_query_exponent(most);
-          down = exp2_whole(-e);
-          up = exp2_whole(e);
+          for (int hh = 0; hh < HALVES; ++hh)
+            sts128(qs + G * Cfg::Q_BYTES + hh * Cfg::Q_HALF + r * 128 + ((chunk ^ (r & 7)) << 4), k8_query<T>(x[i][hh].x, down),
+                   k8_query<T>(x[i][hh].y, down), k8_query<T>(x[i][hh].z, down), k8_query<T>(x[i][hh].w, down));
         }
-        if (chunk == 0) sts32(scales + ((units & 1) * 256 + G * 128 + r) * 4, __float_as_uint(p.scale_log2 * up));
-#pragma unroll
-        for (int hh = 0; hh < HALVES; ++hh)
-          sts128(qs + G * Cfg::Q_BYTES + hh * Cfg::Q_HALF + r * 128 + ((chunk ^ (r & 7)) << 4), k8_query<T>(x[hh].x, down),
-                 k8_query<T>(x[hh].y, down), k8_query<T>(x[hh].z, down), k8_query<T>(x[hh].w, down));
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -431,11 +453,11 @@ __global__ void __launch_bounds__(K8T_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = lds32(bars + B::tmem);
-  // of the launch's 512 x 128 registers a row's thread takes 168, every other 88: 2 x 168 + 2 x 88 = 4 x 128
+  // of the launch's 512 x 128 registers a row's thread takes 160, every other 96: 2 x 160 + 2 x 96 = 4 x 128
   if (warp < 8)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;" ::: "memory");
   else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;" ::: "memory");
   if (warp < 8) {
     k8t_rows<T, HDP>(p, bars, exps, scales, stage + warp * 4096, warp);
   } else if (warp == 8) {
@@ -443,7 +465,7 @@ __global__ void __launch_bounds__(K8T_THREADS, 1)
   } else if (warp == 9) {
     k8t_load<HDP>(&tmv, p, bars, raw, exps, 1);
   } else if (warp < 12) {
-    kt_multiply<__half, HDP, K8tCfg<HDP>, K8tBars<HDP>>(p.t, bars, qs, ring, warp - 10);
+    kt_multiply<__half, HDP, K8tCfg<HDP>, K8tBars<HDP>, true>(p.t, bars, qs, ring, warp - 10);
   } else {
     k8t_convert<T, HDP>(p, bars, qs, ring, raw, scales, warp - 12);
   }

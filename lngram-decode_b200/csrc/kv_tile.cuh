@@ -490,8 +490,9 @@ __device__ __forceinline__ void kt_load(const CUtensorMap* tmq, const CUtensorMa
 // One warp a row tile issues its products: the scores of the next key tile (into the other of two S buffers) ahead
 // of O += P V of this one, so that the softmax finds its scores waiting.  P lies over its tile's scores; a product's
 // operands are only overwritten once an mbarrier has shown it done (the ISA orders products of unlike operands
-// through their completion alone).
-template <typename T, int HDP, typename Cfg = KtCfg<HDP>, typename B = KtBars<HDP>>
+// through their completion alone).  APART: the values are waited for when their product is issued, not with the keys (nobody
+// touches them in between).
+template <typename T, int HDP, typename Cfg = KtCfg<HDP>, typename B = KtBars<HDP>, bool APART = false>
 __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, uint32_t qs, uint32_t ring, int G) {
   constexpr uint32_t NS = Cfg::SLOTS;
   const uint32_t t_s = Cfg::TMEM_S + G * 128, t_o = Cfg::TMEM_O + G * HDP;  // (all of TMEM is this CTA's: its base is 0)
@@ -503,7 +504,7 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
     const uint32_t sk = ik % NS;
     // (the values too: whoever has seen the scores may touch them)
     const bool good = __all_sync(0xffffffffu, kt_wait<B>(bars, B::kv_full + 8 * sk, (ik / NS) & 1) &&
-                                                  kt_wait<B>(bars, B::kv_full + 8 * ((ik + 1) % NS), ((ik + 1) / NS) & 1));
+                                                  (APART || kt_wait<B>(bars, B::kv_full + 8 * ((ik + 1) % NS), ((ik + 1) / NS) & 1)));
     tc_fence_after();
     if (good && elect_lane()) {
       const uint32_t idesc = umma_idesc<T>(KT_BM, KT_BK, false);
@@ -536,6 +537,7 @@ __device__ __forceinline__ void kt_multiply(const KtParams& p, uint32_t bars, ui
       }
       __syncwarp();
       const uint32_t iv = base + 2 * i + 1, sv = iv % NS, t = tile + i;
+      if (APART) ok = ok && kt_wait<B>(bars, B::kv_full + 8 * sv, (iv / NS) & 1);
       ok = __all_sync(0xffffffffu, ok && kt_wait<B>(bars, B::p_full + 16 * G + 8 * (t & 1), (t >> 1) & 1));
       tc_fence_after();
       if (ok && elect_lane()) {

@@ -476,3 +476,31 @@ def test_attention_step_in_a_graph_and_on_another_stream(lngram):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, w) and torch.equal(got, owant)
+
+
+@pytest.mark.parametrize("window, sinks", [(0, 0), (70, 3), (500, 0), (129, 200)])
+@pytest.mark.parametrize("ctx, new, heads, kv, dim, page", [
+    ([1000, 37, 0, 2000], [16, 16, 16, 16], 16, 4, 64, 64),
+    ([1000, 37, 0, 700], [16, 9, 20, 1], 16, 4, 48, 16),
+    ([300], [128], 1, 1, 64, 128),
+    ([77 * i for i in range(20)], [5] * 20, 32, 4, 32, 8),
+    ([64 * i + 60 for i in range(90)], [7] * 90, 8, 2, 64, 32),
+    ([190, 255, 256, 257], [1, 1, 1, 1], 128, 1, 16, 32),
+])
+def test_attend8_of_up_to_a_row_tile(lngram, window, sinks, ctx, new, heads, kv, dim, page):
+    """Rows that fill a row tile at most: between the few rows of a decode step and the many of a prompt."""
+    s = Setup8(lngram, ctx, new, heads, kv, dim, page, "f16", seed=len(ctx)).fill()
+    q = s.normal(*s.lead, heads, dim)
+    for max_len in (None, max(s.lens)):
+        check_attend(lngram.kv_attend(s.cache, q, window=window, sinks=sinks, max_len=max_len, **s.kw()), *s.want(q, window, sinks))
+    assert lngram._lib.device_error() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 16, 17, 31, 32, 33, 64])
+@pytest.mark.parametrize("dim, batch", [(64, 40), (128, 40), (64, 2), (128, 2)])
+def test_attend8_by_rows_a_key_head(lngram, rows, dim, batch):
+    """Every count of rows that is handled in a way of its own, many pairs and few."""
+    heads, new = (rows, 1) if rows < 10 or rows % 2 else (rows // 2, 2)
+    s = Setup8(lngram, [(97 * i) % 611 for i in range(batch)], [new] * batch, heads * 4, 4, dim, 32, "bf16", seed=rows).fill()
+    q = s.normal(*s.lead, heads * 4, dim)
+    check_attend(lngram.kv_attend(s.cache, q), *s.want(q))
