@@ -146,9 +146,13 @@ __device__ __forceinline__ void k8_angles(const K8AppendParams& p, float2* cs, i
     const int t = x / half, f = x - t * half;
     const double pos = p.positions ? double(p.positions[token0 + at0 + t]) : double(j0 + at0 + t);
     const double turns = pos * double(p.inv_freq[f]) * 0.15915494309189533577;  // 1 / (2 pi)
+    // (what the angle's rounding to fp32 leaves turns sine and cosine once more: without it twice as many keys as in
+    // 64-bit angles fall on the other side of a border between two e4m3 values)
+    const double halves = 2.0 * (turns - rint(turns));
+    const float hi = float(halves), lo = float((halves - double(hi)) * 3.14159265358979323846);
     float sn, cn;
-    sincospif(float(2.0 * (turns - rint(turns))), &sn, &cn);
-    cs[k8_angle_at(t, f, half)] = make_float2(cn, sn);
+    sincospif(hi, &sn, &cn);
+    cs[k8_angle_at(t, f, half)] = make_float2(fmaf(-lo, sn, cn), fmaf(lo, cn, sn));
   }
 }
 
