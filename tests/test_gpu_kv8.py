@@ -504,3 +504,65 @@ def test_attend8_by_rows_a_key_head(lngram, rows, dim, batch):
     s = Setup8(lngram, [(97 * i) % 611 for i in range(batch)], [new] * batch, heads * 4, 4, dim, 32, "bf16", seed=rows).fill()
     q = s.normal(*s.lead, heads * 4, dim)
     check_attend(lngram.kv_attend(s.cache, q), *s.want(q))
+
+
+def test_offsets_past_32_bits_and_strided_exponents(lngram):
+    """Pages beyond 4 GB of keys, exponents in columns of a wider tensor: append, attend and values in the last pages."""
+    pages, heads, page, dim = 70000, 8, 64, 128
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    k, v = (torch.zeros(pages, heads, page, dim, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    wide = torch.full((pages, 40), 77, dtype=torch.int8, device="cuda")
+    k_exp, v_exp = wide[:, 3:11], wide[:, 20:28]
+    table = torch.tensor([[pages - 1, pages - 3, 2], [pages - 2, 65540, pages - 5]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([130, 190], dtype=torch.int32, device="cuda")
+    cache = lngram.PagedKVCache8(k, v, k_exp, v_exp, table, lengths)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = [torch.randn(320, heads, dim, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    cu = torch.tensor([0, 130, 320], dtype=torch.int32, device="cuda")
+    lngram.kv_append(cache, *x, cu=cu, max_new=190)
+    for pages_, exps, rows in ((k, k_exp, x[0]), (v, v_exp, x[1])):
+        for b, (at, n) in enumerate(((0, 130), (130, 190))):
+            j = torch.arange(n, device="cuda")
+            p = table[b][j // page].long()
+            got = pages_.view(torch.uint8)[p, :, j % page].view(E4M3).double() * power(exps[p])[..., None]
+            want = rows[at:at + n].double()
+            assert ((got - want).abs() <= torch.maximum(want.abs() / 16, power(exps[p])[..., None] * 2.0 ** -10)).all()
+    assert (wide[:, :3] == 77).all() and (wide[:, 11:20] == 77).all() and (wide[:, 28:] == 77).all()
+    s = Setup8.__new__(Setup8)
+    s.cache, s.table, s.page, s.kv, s.dim, s.heads, s.dtype = cache, table, page, heads, dim, 16, torch.bfloat16
+    for new in ([1, 1], [40, 40]):
+        s.ctx, s.new = [n - m for n, m in zip((130, 190), new)], new
+        q = torch.randn(2, new[0], 16, dim, generator=g, device="cuda").bfloat16()
+        check_attend(lngram.kv_attend(cache, q), *s.want(q))
+    del s
+    values = cache.values()[0]
+    assert torch.equal(values[pages - 1].double(), k[pages - 1].double() * power(k_exp[pages - 1])[:, None, None])
+    assert lngram._lib.device_error() == 0
+
+
+def test_two_caches_appended_to_at_once(lngram):
+    """Steps on two streams: what one writes and returns is what it would alone."""
+    setups = [Setup8(lngram, [100 * i + 7, 3], [70, 70], 8, 2, 64, 16, seed=i).fill([100 * i + 7, 3]) for i in range(2)]
+    rows = [(s.normal(2, 70, 2, 64), s.normal(2, 70, 2, 64), s.normal(2, 70, 8, 64)) for s in setups]
+    freq = torch.rand(32, device="cuda")
+    keep = [(s.cache.k.view(torch.uint8).clone(), s.cache.k_exp.clone()) for s in setups]
+
+    def step(s, r):
+        q = lngram.kv_append(s.cache, *r, inv_freq=freq)
+        return q, lngram.kv_attend(s.cache, q)
+
+    want = [[t.clone() for t in step(s, r)] + [s.cache.k.view(torch.uint8).clone()] for s, r in zip(setups, rows)]
+    streams = [torch.cuda.Stream() for _ in setups]
+    for _ in range(10):
+        for s, (k, e) in zip(setups, keep):
+            s.cache.k.view(torch.uint8).copy_(k)
+            s.cache.k_exp.copy_(e)
+        torch.cuda.synchronize()
+        got = []
+        for s, r, stream in zip(setups, rows, streams):
+            with torch.cuda.stream(stream):
+                got.append(step(s, r))
+        torch.cuda.synchronize()
+        for s, g, w in zip(setups, got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1]) and torch.equal(s.cache.k.view(torch.uint8), w[2])

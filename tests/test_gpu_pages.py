@@ -171,3 +171,43 @@ def test_captured(lngram):
         model.truncate(lens)
         assert slots.tolist() == want and served.tolist() == ok
         same(pool, model)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_pool_without_pages_left(lngram, eight):
+    """Sequences that get no pages are suspended: their tokens go nowhere, their rows are zero, nothing of theirs or of the
+    others' is lost, and they go on when pages are there again."""
+    err = lngram._lib.device_error
+    pool = lngram.PagePool.allocate(3, 64, 5, 2, 32, page_size=8, device="cuda", eight=eight)
+    other = (lngram.PagedKVCache8 if eight else lngram.PagedKVCache).allocate(3, 64, 2, 32, page_size=8, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def rows(n):
+        return [torch.randn(3, n, h, 32, generator=g, device="cuda").bfloat16() for h in (2, 2, 4)]
+
+    err()
+    k, v, q = rows(8)
+    _, served = pool.extend(8)
+    assert served.tolist() == [True] * 3
+    other.extend(8)
+    for c in (pool.cache, other):
+        lngram.kv_append(c, k, v)
+    # eight more for every sequence: pages for two of them are left
+    k, v, q = rows(8)
+    slots, served = pool.extend(8)
+    assert served.tolist() == [True, True, False] and pool.cache.lengths.tolist() == [16, 16, -9] and (slots[2] == -1).all()
+    other.extend(8)
+    for c in (pool.cache, other):
+        lngram.kv_append(c, k, v)
+    assert err() == 4
+    got, want = lngram.kv_attend(pool.cache, q), lngram.kv_attend(other, q)
+    assert err() == 4 and torch.equal(got[:2], want[:2]) and (got[2] == 0).all()
+    # the first one ends, the third is taken up again with its tokens
+    pool.truncate(torch.tensor([0, 16, 16], dtype=torch.int32, device="cuda"))
+    assert pool.cache.lengths.tolist() == [0, 16, 8] and int((pool.refs == 0).sum()) == 2
+    slots, served = pool.extend(cu=torch.tensor([0, 0, 0, 8], dtype=torch.int32, device="cuda"), max_new=8, tokens=8)
+    assert served.tolist() == [True] * 3 and pool.cache.lengths.tolist() == [0, 16, 16]
+    cu = torch.tensor([0, 0, 0, 8], dtype=torch.int32, device="cuda")
+    lngram.kv_append(pool.cache, k[2], v[2], cu=cu, max_new=8)
+    got = lngram.kv_attend(pool.cache, q[2], cu=cu, max_new=8)
+    assert torch.equal(got, want[2]) and err() == 0
