@@ -11,12 +11,12 @@
 // keys' into the factor of their scores (8 columns at a time, a page's least), the values' into the exponential and
 // back out of the sum.  Weights are rounded to fp16 once, their sum is not.
 //
-// Measured: two prompts of 5001 and 8000 tokens, 28 query and 4 key heads of 128, window of 4096 and 4 sinks: 870 to 910 us (by
-// the power that a box allows), 770 to 810 TFLOP/s, as kv_tile_kernel takes in 16 bits; a key tile takes 1900 cycles, of which a
-// row's thread is busy for 1400 and waits for its scores in the others.  The converters want all four warps on one tile and 96
-// registers (two warps for keys and two for values: 930 us; 88 registers: 885).  64 sequences of 16 drafted tokens after 1024
-// keys, 4 key heads of 64: 52 us, two waves of units of which one row tile has rows (both row tiles on the same rows, the key tiles
-// in turn, their states joined: 62 us).
+// Measured: two prompts of 5001 and 8000 tokens, 28 query and 4 key heads of 128, window of 4096 and 4 sinks: 830 us, 850 TFLOP/s,
+// about what kv_tile_kernel takes in 16 bits; a key tile takes some 1800 cycles, of which a row's thread is busy for 1400
+// and waits for its scores in the others.  The converters want all four warps on one tile and 96 registers (two warps for keys
+// and two for values: 5 % more; 88 or 104 registers: 2 %).  64 sequences of 16 drafted tokens after 1024 keys, 4 key heads of
+// 64: 51 us, two waves of units of which one row tile has rows (both row tiles on the same rows, the key tiles in turn, their
+// states joined: 62 us).
 #pragma once
 
 #include "kv8_step.cuh"
@@ -267,7 +267,9 @@ __device__ __forceinline__ void k8t_convert(const K8tParams& pp, uint32_t bars, 
 }
 
 // Weights of a 32-column piece (four runs of 8 columns, whose factors, exponents less the reference, and way back are
-// f, add and back) to TMEM column tp; otherwise as kt_weights.
+// f, add and back) to TMEM column tp.  Otherwise as kt_weights, but with all exponentials on the special-function unit: the
+// converters leave no slots on the other pipes (of eight pairs there none, one, two, three, four: 830, 832, 838, 848, 843 us for the
+// long prompts above).
 __device__ __forceinline__ void k8t_weights(uint32_t (&s)[32], const float (&f)[4], const float (&add)[4], const float (&back)[4],
                                             uint64_t& sum, uint32_t tp) {
   uint64_t v[16];
@@ -275,23 +277,14 @@ __device__ __forceinline__ void k8t_weights(uint32_t (&s)[32], const float (&f)[
   for (int y = 0; y < 16; ++y)
     v[y] = f2_fma(f2_pack(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1])), f2_pack(f[y >> 2], f[y >> 2]),
                   f2_pack(add[y >> 2], add[y >> 2]));
-#pragma unroll
-  for (int y = 0; y < 16; ++y) {
-    float a, b;
-    if (KT_FMA_EXP >> (y & 7) & 1) {
-      exp2_fma(v[y], a, b);
-    } else {
-      f2_unpack(v[y], a, b);
-      a = exp2_fast(a);
-      b = exp2_fast(b);
-    }
-    v[y] = f2_pack(a, b);
-  }
   uint32_t w[16];
 #pragma unroll
   for (int y = 0; y < 16; ++y) {
     float a, b;
     f2_unpack(v[y], a, b);
+    a = exp2_fast(a);
+    b = exp2_fast(b);
+    v[y] = f2_pack(a, b);
     w[y] = pack2<__half>(a, b);
   }
   tmem_store16(tp, w);

@@ -146,6 +146,11 @@ __device__ __forceinline__ int32_t kt_count(const KeyTiles& t, int32_t last, int
   return n > j0 ? n - j0 : 0;
 }
 
+// a / b for a >= 0 and 0 < b < 2^31 (a 64-bit division takes hundreds of cycles more, of which every unit has two or three).
+__device__ __forceinline__ int64_t kt_quotient(int64_t a, int64_t b) {
+  return a < (int64_t(1) << 32) ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
 __device__ __forceinline__ int32_t uniform(int32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // The CTA's units: unit i of round k is k * grid + i, every second round backwards, so that each CTA's sum of units
@@ -163,8 +168,9 @@ __device__ __forceinline__ bool kt_next(const KtParams& p, KtWalk& walk, KtWork&
   there = false;
   if (k * grid >= p.total) return false;
   if (idx >= p.total) return true;
-  const int64_t u = idx / (int64_t(c.kv_heads) * p.splits);
-  const int32_t rest = int32_t(idx - u * c.kv_heads * p.splits);
+  const int32_t inner = c.kv_heads * p.splits;  // (units of the same tokens: at most 65535 * 32)
+  const int64_t u = kt_quotient(idx, inner);
+  const int32_t rest = int32_t(idx - u * inner);
   w.hk = rest / p.splits;
   w.split = rest - w.hk * p.splits;
   w.shared = p.prefix_table != nullptr;
@@ -187,7 +193,7 @@ __device__ __forceinline__ bool kt_next(const KtParams& p, KtWalk& walk, KtWork&
     if (u * span >= w.s.n) return true;
     w.t0 = int32_t(u * span);
   } else if (c.cu == nullptr) {
-    const int64_t per = (c.max_new + span - 1) / span, r = u / c.batch;
+    const int64_t per = (c.max_new + span - 1) / span, r = kt_quotient(u, c.batch);
     if (r >= per) return true;
     w.b = u - r * c.batch;
     w.s = kv_span(c, w.b);
