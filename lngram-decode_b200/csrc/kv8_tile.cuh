@@ -394,7 +394,7 @@ __device__ __forceinline__ void k8t_rows(const K8tParams& pp, uint32_t bars, uin
       float a0, a1;
       f2_unpack(sum, a0, a1);
       l += a0 + a1;
-      // a NaN score, and one of +inf (inf - inf), makes the row NaN whichever pipe its own weight went through
+      // a NaN score, and one of +inf (inf - inf), makes the row NaN, its sum as well as its weights
       if (!(top < INFINITY)) l = NAN;
       tmem_wait_st();
       tc_fence_before();
