@@ -549,7 +549,10 @@ int lng_kv8_append(const lng_kv8_cache* cache, const int32_t* cu, int64_t tokens
                    const float* inv_freq, int32_t rotary_dim, int32_t interleaved, lng_stream_t stream);
 
 /* lng_kv_attend over a cache in 8 bits.  Products in fp16, in which e4m3 is exact (queries are scaled by a power of two
- * a row), exponents, scores, sums and states in fp32; weights are rounded to fp16 for the product with the values. */
+ * a row), exponents, scores, sums and states in fp32; weights are rounded to fp16 for the product with the values.  A
+ * weight is that of score + values' exponent, in base 2: while that lies no more than 21 below the row's largest it keeps
+ * 11 bits, below that it loses one a power of two, and from 32 below on the key's values may not count.  The likeliest
+ * keys lose nothing while the largest values of a sequence's pages are within 2^21 of one another. */
 size_t lng_kv8_attend_workspace_bytes(const lng_kv8_cache* cache, int64_t tokens, int64_t max_new, int64_t max_len,
                                       int32_t q_heads, int32_t window, int32_t sinks);
 int lng_kv8_attend(const lng_kv8_cache* cache, const int32_t* cu, int64_t tokens, int64_t max_new, int64_t max_len,

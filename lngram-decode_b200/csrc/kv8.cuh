@@ -7,6 +7,9 @@
 namespace lng {
 
 constexpr int K8_LEAST = -40, K8_MOST = 40;  // the exponents that a page may have
+// Attention's weights in fp16: 2^K8_ROOM for a row's largest score when its reference is set, 2^K8_TOP at most before it is set
+// again (fp16 ends below 2^16), so that 7 of the 8 powers of two that nothing else needs lie below the smallest weights.
+constexpr float K8_ROOM = 7.f, K8_TOP = 15.f;
 
 // A cache in 8 bits: c's strides count bytes, exponents lie at page * *_exp_page + head.
 struct Kv8View {

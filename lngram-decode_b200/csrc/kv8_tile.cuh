@@ -9,7 +9,8 @@
 //             largest value (fp16 queries are taken as they are).
 // Bytes come through a ring of their own, half as large a tile as the fp16 one.  Exponents go the way of kv8_step.cuh: the
 // keys' into the factor of their scores (8 columns at a time, a page's least), the values' into the exponential and
-// back out of the sum.  Weights are rounded to fp16 once, their sum is not.
+// back out of the sum, and a row's reference lies below its largest score as there.  Weights are rounded to fp16 once, their sum
+// is not.
 //
 // Measured: two prompts of 5001 and 8000 tokens, 28 query and 4 key heads of 128, window of 4096 and 4 sinks: 830 us, 850 TFLOP/s,
 // about what kv_tile_kernel takes in 16 bits; a key tile takes some 1800 cycles, of which a row's thread is busy for 1400
@@ -364,9 +365,9 @@ __device__ __forceinline__ void k8t_rows(const K8tParams& pp, uint32_t bars, uin
       }
       // (NaN when one of the row's scores is: it is never a new reference, and makes the sum NaN below)
       const float top = max_nan(k8t_max(s0, f0, e0), k8t_max(s1, f1, e1));
-      const bool grow = top > m + 8.f || (i == 0 && top > m);
+      const bool grow = top > m + K8_TOP || (i == 0 && top > m);
       if (i > 0 && __any_sync(0xffffffffu, grow)) {
-        const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - top)) : 1.f;
+        const float f = grow ? (m == -INFINITY ? 0.f : exp2_fast(m - (top - K8_ROOM))) : 1.f;
         l *= f;
         ok = ok && kt_wait<B>(bars, pv_bar, (t - 1) & 1);  // the product before this one is done with O
         __syncwarp();
@@ -381,7 +382,7 @@ __device__ __forceinline__ void k8t_rows(const K8tParams& pp, uint32_t bars, uin
           tmem_store32(to + x, o);
         }
       }
-      if (grow) m = top;
+      if (grow) m = top - K8_ROOM;
       const float ref = m == -INFINITY ? 0.f : m;
       uint64_t sum = 0;
       float back[4];

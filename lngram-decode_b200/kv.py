@@ -134,8 +134,11 @@ class PagedKVCache8(PagedKVCache):
     ``kv_append`` gives a page and head the least exponent under which its new values fit e4m3, at least -40 and at most
     40 (beyond 448 * 2^40 values saturate; NaN and infinities become NaN); a page that holds earlier keys keeps its
     exponent where that is larger, else the earlier keys are rounded again to the new one.  A power of two as the scale
-    costs no precision: e4m3 has an exponent of its own.  Pages that several sequences name are for reading
-    (``PagePool`` copies a shared page before it is written to)."""
+    costs no precision: e4m3 has an exponent of its own.  Attention rounds its weights to fp16, the values' exponents in
+    them: a key's weight keeps its 11 bits while its score (in base 2) + exponent lies up to 21 below the row's largest, and
+    from 32 below on its values may count as zero.  The likeliest keys lose nothing while the pages' largest values are
+    within 2^21 of one another.  Pages that several sequences name are for reading (``PagePool`` copies a shared page
+    before it is written to)."""
 
     eight = True
 
