@@ -595,8 +595,10 @@ int lng_kv_pages_reorder(const lng_kv8_cache* cache, int32_t* refs, const int64_
  * group the `width` largest, in falling order, ties to the lowest k * vocab + v.  logits f32, bf16 or f16, rows of
  * `vocab` values row_stride elements apart; scores f32 [groups, beams]; done (u8, may be NULL): a beam that has ended
  * offers token eos at its own score and -inf for every other.  A row that holds a NaN, +inf or nothing but -inf
- * offers -inf throughout.  Outputs [groups, width]: f32, i64, i64.  beams, width <= 32, width <= beams * vocab,
- * vocab < 2^30.  workspace: 256-byte aligned, used by this call alone until it has finished. */
+ * offers -inf throughout, and so does a beam, ended or not, whose score is -inf or NaN; scores must be below +inf.  (Of
+ * one beam's finite candidates unlike logits never tie, whatever the score rounds away.)  Outputs [groups, width]: f32,
+ * i64, i64.  beams, width <= 32, width <= beams * vocab, vocab < 2^30.  workspace: 256-byte aligned, used by this call
+ * alone until it has finished. */
 size_t lng_beam_workspace_bytes(int64_t groups, int64_t beams, int64_t vocab, int64_t width);
 int lng_beam_select(const void* logits, int32_t dtype, int64_t row_stride, int64_t groups, int64_t beams, int64_t vocab,
                     const float* scores, const uint8_t* done, int64_t eos, int64_t width, float* out_scores,

@@ -43,10 +43,12 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, don
     rows at one stride), ``scores`` fp32 ``[groups, beams]``: of a group's candidates scores[k] + log_softmax(logits[k])[v]
     the ``width`` largest (default: as many as beams), in falling order, ties to the lowest beam, then token.  ``done``
     (bool ``[groups, beams]``): a beam that has ended offers only ``eos``, at its own score, and -inf for the rest.  A row
-    that holds a NaN, +inf or nothing but -inf offers -inf throughout.
+    that holds a NaN, +inf or nothing but -inf offers -inf throughout, and so does a beam (ended or not) whose score is -inf
+    or NaN; scores must be below +inf.
 
     Returns ``scores`` fp32, ``tokens`` int64 and ``parents`` int64, ``[groups, width]``.  Sums are fp32, their joins and
-    the ranking 64 bits.  At most 32 beams, and a width of 32.  No gradients."""
+    the ranking 64 bits; finite candidates of one beam rank as their logits do, whatever the score rounds away.  At most 32
+    beams, and a width of 32.  No gradients."""
     _no_grad(logits, scores)
     if logits.dim() != 3 or logits.dtype not in _DTYPES:
         raise ValueError("logits must be [groups, beams, vocab] in float32, bfloat16 or float16")

@@ -12,7 +12,8 @@ namespace lng {
 // largest logits of its piece of a row beside the piece's maximum and sum of exponentials; a dependent launch, a CTA a
 // group, joins the pieces' sums, ranks each row's candidates, and then the rows' against one another by
 // score + (logit - log sum), in 64 bits: scores a few ulp of 32 bits apart must not change places.  Ties go to the lower
-// index at every step.
+// index at every step (of one beam's candidates, equal logits tie: sums that only 64 bits' rounding makes equal, as beside
+// a score of -10^30, rank as their logits do).
 // Measured: 512 rows of 128000 bf16 logits (131 MB): 50 us and 12 more for the join; bound by instructions (one exponential and
 // some ten others a value, the lists' upkeep in most rounds), 2.6 TB/s.  4 rows of 32000 fp32 logits: 14 us, latency.
 constexpr int BS_THREADS = 256, BS_WARPS = 8, BS_MOST = 32;
@@ -320,14 +321,16 @@ __global__ void __launch_bounds__(BS_THREADS) beam_join_kernel(const BeamParams 
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     // (the logarithm is kept apart from a maximum beside which it may be nothing)
     const double log_sum = log(s), score = double(score1);
-    const bool empty = !(log_sum < INFINITY) || log_sum == -INFINITY;
+    // (a dead beam, whose score is -inf or NaN: whatever it offers is worth the same)
+    const bool dead = !(score > -INFINITY), empty = dead || !(log_sum < INFINITY) || log_sum == -INFINITY;
     double c = score + ((double(list.v) - double(m)) - log_sum);
     int32_t token = list.i;
-    if (ended || empty) {  // eos at the beam's score, then the lowest other tokens at -inf; or those alone
+    if (ended || empty) {  // eos at the beam's score, then the lowest other tokens at -inf; or the lowest tokens alone
       const int32_t eos = int32_t(p.eos);
-      token = !ended ? lane : lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
+      const bool ends = ended && !dead;
+      token = !ends ? lane : lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
       if (token >= p.vocab) token = 0x7fffffff;
-      c = ended && lane == 0 ? score : -INFINITY;
+      c = ends && lane == 0 ? score : -INFINITY;
     }
     if (lane < width) {
       cv[k * width + lane] = c == c ? c : -INFINITY;
