@@ -66,9 +66,12 @@ extern "C" int lng_kv_pages_extend(const lng_kv8_cache* caches, int32_t count, i
                     caches[i].pages.page_size == caches[0].pages.page_size,
                 "a pool's caches must be of one geometry");
   }
-  if (caches->pages.batch == 0) return LNG_OK;
-  LNG_REQUIRE(served && copies && (slots || tokens == 0), "NULL pointer");
+  LNG_REQUIRE(caches->pages.batch == 0 || (served && copies), "NULL pointer");
+  LNG_REQUIRE(slots || tokens == 0, "slots is NULL");
   LNG_REQUIRE((reinterpret_cast<uintptr_t>(copies) & 15) == 0, "copies must be 16-byte aligned");
+  // (rows that belong to no sequence, which without sequences is all of them)
+  if (cu && tokens > 0) LNG_CUDA(cudaMemsetAsync(slots, 0xff, size_t(tokens) * 8, S(stream)));
+  if (caches->pages.batch == 0) return LNG_OK;
   PgParams p = pg_params(caches, refs, cu, tokens, max_new);
   p.slots = slots;
   p.served = served;
@@ -78,8 +81,6 @@ extern "C" int lng_kv_pages_extend(const lng_kv8_cache* caches, int32_t count, i
   static std::atomic<uint64_t> known{0};
   if (smem > 40 * 1024)
     if (const int st = allow_smem(kv_pages_extend_kernel, 200 * 1024, known)) return st;
-  // (rows that belong to no sequence)
-  if (cu && tokens > 0) LNG_CUDA(cudaMemsetAsync(slots, 0xff, size_t(tokens) * 8, S(stream)));
   kv_pages_extend_kernel<<<PG_CTAS, PG_THREADS, smem, S(stream)>>>(p);
   LNG_LAUNCHED("kv_pages_extend_kernel");
   for (int32_t i = 0; i < count; ++i)
