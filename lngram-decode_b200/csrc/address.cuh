@@ -8,21 +8,7 @@
 
 namespace lng {
 
-// First device-side error code (0 = none): a word of its own in every translation unit, whose kernels write it.
-static __device__ unsigned int g_error_word;
-
-// This translation unit's word on the current device (-1: it could not be read).
-static inline int error_word_here(int clear) {
-  unsigned int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_error_word, sizeof(v)) != cudaSuccess) return -1;
-  if (clear && v) {
-    const unsigned int z = 0;
-    cudaMemcpyToSymbol(g_error_word, &z, sizeof(z));
-  }
-  return int(v);
-}
-int error_word_kv8(int clear);    // kv8.cu's
-int error_word_pages(int clear);  // kv_pages.cu's
+__device__ unsigned int g_error_word;  // first device-side error code (0 = none)
 
 enum DeviceError : unsigned int {
   DEV_ERR_CODE_RANGE = 1,   // a route code >= 2^bits (treated as an invalid window)

@@ -2,9 +2,9 @@
 
     python lngram-decode_b200/csrc/build.py [--force] [--verbose]
 
-Every ``*.cu`` of this folder is a translation unit, built with ``-gencode
-arch=compute_100a,code=sm_100a -lineinfo -O3`` (side by side) and linked.  A stamp of the source hashes
-skips rebuilding when nothing changed, one a unit compiling it.  The output is git-ignored and travels with the
+The library is one translation unit (``lngram_b200.cu`` includes every kernel header), built
+with ``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3``.  A stamp of the source hashes
+skips rebuilding when nothing changed.  The output is git-ignored and travels with the
 repository snapshot to the GPU box.
 """
 
@@ -13,11 +13,9 @@ from __future__ import annotations
 import argparse
 import hashlib
 import os
-import re
 import shutil
 import subprocess
 import sys
-from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -25,7 +23,6 @@ PKG = CSRC.parent
 REPO = PKG.parent
 LIB = PKG / "liblngram_b200.so"
 STAMP = PKG / ".liblngram_b200.stamp"
-OBJECTS = CSRC / "_build"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -42,39 +39,6 @@ def _digest(flags: list[str]) -> str:
     return h.hexdigest()
 
 
-def _included(unit: Path) -> list[Path]:
-    """A translation unit and the files of this repository that it includes."""
-    found, todo = [], [unit]
-    while todo:
-        p = todo.pop().resolve()
-        if p in found or not p.exists():
-            continue
-        found.append(p)
-        todo += [p.parent / name for name in re.findall(r'^\s*#include "([^"]+)"', p.read_text(), re.M)]
-    return sorted(found)
-
-
-def _compile(unit: Path, flags: list[str], force: bool, verbose: bool) -> tuple[Path, str]:
-    """The unit's object (kept while neither it nor what it includes changes) and what the compiler said."""
-    h = hashlib.sha256(" ".join(flags).encode())
-    for p in _included(unit):
-        h.update(p.name.encode())
-        h.update(p.read_bytes())
-    obj, stamp = OBJECTS / (unit.stem + ".o"), OBJECTS / (unit.stem + ".stamp")
-    if not force and obj.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
-        return obj, ""
-    cmd = [nvcc()] + flags + ["-c", "-o", str(obj), str(unit)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    out = (res.stdout or "") + (res.stderr or "")
-    out = "\n".join(l for l in out.splitlines() if "Warning: The 'compute_" not in l)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}) on {unit.name}:\n{out}")
-    stamp.write_text(h.hexdigest())
-    return obj, out
-
-
 def nvcc() -> str:
     cand = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     if not Path(cand).exists():
@@ -83,24 +47,21 @@ def nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    flags = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-diag-suppress", "177"]
+    flags = ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-diag-suppress", "177"]
     if ptxas_info:
         flags += ["-Xptxas", "-v"]
     digest = _digest(flags)
     if not force and LIB.exists() and STAMP.exists() and STAMP.read_text().strip() == digest:
         return LIB
-    OBJECTS.mkdir(exist_ok=True)
-    units = sorted(CSRC.glob("*.cu"))
-    with ThreadPoolExecutor(len(units)) as pool:
-        done = list(pool.map(lambda u: _compile(u, flags, force, verbose), units))
-    out = "\n".join(text for _, text in done if text)
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc()] + ARCH + ["-Xcompiler", "-fPIC", "-shared", "-o", str(tmp)] + [str(obj) for obj, _ in done]
+    cmd = [nvcc()] + flags + ["-o", str(tmp), str(CSRC / "lngram_b200.cu")]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
+    out = (res.stdout or "") + (res.stderr or "")
+    out = "\n".join(l for l in out.splitlines() if "Warning: The 'compute_" not in l)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}{res.stderr}")
+        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{out}")
     if verbose or ptxas_info:
         print(out)
     os.replace(tmp, LIB)

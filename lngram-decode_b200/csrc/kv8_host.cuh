@@ -1,12 +1,12 @@
 // The C ABI's entries of the paged cache in 8 bits (include/lngram_b200.h).
+#pragma once
+
 #include "kv8.cuh"
 #include "kv8_step.cuh"
 #include "kv8_tile.cuh"
 #include "kv_host.cuh"
 
 namespace lng {
-
-int error_word_kv8(int clear) { return error_word_here(clear); }
 
 static int check_kv8(const lng_kv8_cache* c, const int32_t* cu, int64_t tokens, int64_t max_new) {
   LNG_REQUIRE(c != nullptr, "cache descriptor is NULL");

@@ -1,4 +1,6 @@
 // The C ABI's entries of page pools and beams (include/lngram_b200.h).
+#pragma once
+
 #include <type_traits>
 
 #include "beam.cuh"
@@ -6,8 +8,6 @@
 #include "kv_pages.cuh"
 
 namespace lng {
-
-int error_word_pages(int clear) { return error_word_here(clear); }
 
 // What the page calls need of a cache of either kind.
 static int check_pool(const lng_kv8_cache* c, const int32_t* refs, const int32_t* cu, int64_t tokens, int64_t max_new) {

@@ -1,5 +1,6 @@
-// lngram_b200: the C ABI of include/lngram_b200.h (kv8.cu and kv_pages.cu hold the entries of the 8-bit
-// cache and of page pools and beams).
+// lngram_b200: the C ABI of include/lngram_b200.h (one translation unit, so every kernel shares
+// the device error word and inlines the addressing helpers; kv8_host.cuh and kv_pages_host.cuh hold the entries of the
+// 8-bit cache and of page pools and beams).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -115,14 +116,13 @@ extern "C" int lng_device_ok(void) {
 }
 
 extern "C" int lng_device_error(int clear) {
-  // a word a translation unit: the first one that holds a code is reported, all are cleared
-  int first = 0;
-  for (int (*word)(int) : {error_word_here, error_word_kv8, error_word_pages}) {
-    const int v = word(clear);
-    if (v < 0) return -1;
-    if (first == 0) first = v;
+  unsigned int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_error_word, sizeof(v)) != cudaSuccess) return -1;
+  if (clear && v) {
+    const unsigned int z = 0;
+    cudaMemcpyToSymbol(g_error_word, &z, sizeof(z));
   }
-  return first;
+  return int(v);
 }
 
 // ====================================================================== router
@@ -1955,3 +1955,7 @@ extern "C" int lng_kv_prefix_attend(const lng_kv_cache* cache, const int32_t* pr
   return kv_attend_run(cache, prefix_table, prefix_len, cu, tokens, max_new, max_len, q, scale, 0, 0, out, workspace,
                        workspace_bytes, stream);
 }
+
+// ====================================================================== the 8-bit cache; page pools and beams
+#include "kv8_host.cuh"
+#include "kv_pages_host.cuh"
