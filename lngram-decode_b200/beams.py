@@ -93,11 +93,30 @@ def beam_select(logits: Tensor, scores: Tensor, *, width: int | None = None, don
     return out, tokens, parents
 
 
+def _meet(a: _lib.BeamState, b: _lib.BeamState, rows: int) -> bool:
+    """Whether what moves of two states has bytes in common."""
+    if a.bytes == 0 or b.bytes == 0:
+        return False
+    if b.ptr < a.ptr:
+        a, b = b, a
+    if a.ptr + (rows - 1) * a.stride + a.bytes <= b.ptr:
+        return False
+    if a.stride == b.stride:
+        inside = (b.ptr - a.ptr) % a.stride  # where b's rows begin in a's
+        return inside < a.bytes or a.stride - inside < b.bytes
+    # of each of a's rows: the first of b's that ends behind its beginning
+    for at in range(a.ptr, a.ptr + rows * a.stride, a.stride):
+        j = max(0, (at - b.ptr - b.bytes) // b.stride + 1)
+        if j < rows and b.ptr + j * b.stride < at + a.bytes:
+            return True
+    return False
+
+
 def beam_reorder(parents: Tensor, *states: Tensor, length: int | None = None) -> None:
     """Rows of ``states``, in place: row g * beams + k becomes what row g * beams + ``parents[g, k]`` was (int64 ``[groups,
     beams]``, on the device).  A state is ``[groups * beams, ...]`` of any type, each row contiguous, rows at any stride
-    that keeps them apart; with ``length`` only the first ``length`` entries of its next dimension move.  States must
-    not overlap.  A parent out of range records device error 4 and leaves its row as it is.  At most 32 beams.  No
+    that keeps them apart; with ``length`` only the first ``length`` entries of its next dimension move.  States that
+    overlap in what moves are refused.  A parent out of range records device error 4 and leaves its row as it is.  At most 32 beams.  No
     gradients."""
     _no_grad(*states)
     if parents.dim() != 2 or parents.dtype is not torch.int64 or not parents.is_contiguous():
@@ -133,7 +152,10 @@ def beam_reorder(parents: Tensor, *states: Tensor, length: int | None = None) ->
         count = 1
         for s in inner:
             count *= s
-        descs.append(_lib.BeamState(x.data_ptr(), max(x.stride(0), expected) * size, count * size))
+        desc = _lib.BeamState(x.data_ptr(), max(x.stride(0), expected) * size, count * size)
+        if any(_meet(desc, other, groups * beams) for other in descs):
+            raise ValueError("states must not overlap")
+        descs.append(desc)
     lib = _library(index)
     with _lib.on_device(parents.device):
         for i in range(0, len(descs), 8):
