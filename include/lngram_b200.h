@@ -606,7 +606,7 @@ int lng_beam_select(const void* logits, int32_t dtype, int64_t row_stride, int64
 
 /* Rows of a state, in place: the first `bytes` bytes of row g * beams + k become those of row g * beams +
  * parents[g, k] (i64, device; a parent out of range records device error 4 and leaves its row as it is).  beams <= 32;
- * at most 8 states a call, whose rows are `stride` bytes apart, stride >= bytes. */
+ * at most 8 states a call, whose rows are `stride` bytes apart, stride >= bytes; what moves of them must not overlap. */
 typedef struct {
   void* ptr;
   int64_t stride, bytes;

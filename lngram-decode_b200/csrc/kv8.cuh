@@ -50,11 +50,12 @@ __device__ __forceinline__ float2 k8_floats(uint32_t two) {
 // as in kv_append_kernel, and cos and sin of a token are formed once for all heads, with angles in 64 bits as there.
 // Where a page holds 64 tokens at most (KEEP) so many warps take a head that every lane can keep its items, four at most, in
 // registers from the rotation over the search for the maximum to the rounding: all loads of a page are in flight at once.
-// (Rotating twice instead, which leaves room for three CTAs an SM, took 55 us in place of 43 for 32 prompts of 2048 tokens, 4
-// heads of 64.)  Larger pages, and rotations by halves that are no
-// multiple of 8, go through chunks of 64 tokens twice, the second time from L1 or L2.
-// Measured: 32 prompts of 2048 tokens, 4 key heads of 64 (100 MB): 39 us behind the queries' 50 us (16 heads, 268 MB); bound by
-// the length of a CTA's sequence -- lengths, rows, angles, two meetings, stores -- at sixteen warps an SM.  64 tokens: 4 us.
+// (Rotating twice instead, which leaves room for three CTAs an SM, took a quarter more.)  Larger pages, and rotations by halves
+// that are no multiple of 8, go through chunks of 64 tokens twice, the second time from L1 or L2, a warp a head.
+// Measured, 32 prompts of 2048 tokens in a replayed graph: 4 key heads of 64 (100 MB) 41 us, and 85 us with 16 heads of queries
+// (268 MB), where the cache in 16 bits takes 36 and 67 us; bound by the length of a CTA's sequence -- lengths, rows, angles, two
+// meetings, stores -- at sixteen warps an SM.  One key head: 28 us.  Pages of 256 keys: 81 us, one key head 56 us, since
+// warps without a head are idle.  64 tokens: 4 us.
 constexpr int K8A_WARPS = 8, K8A_THREADS = 32 * K8A_WARPS, K8A_CHUNK = 64, K8A_KEEP = 4;
 
 struct K8AppendParams {
@@ -151,8 +152,8 @@ __device__ __forceinline__ void k8_angles(const K8AppendParams& p, float2* cs, i
     const int t = x / half, f = x - t * half;
     const double pos = p.positions ? double(p.positions[token0 + at0 + t]) : double(j0 + at0 + t);
     const double turns = pos * double(p.inv_freq[f]) * 0.15915494309189533577;  // 1 / (2 pi)
-    // (what the angle's rounding to fp32 leaves turns sine and cosine once more: without it twice as many keys as in
-    // 64-bit angles fall on the other side of a border between two e4m3 values)
+    // (what the angle's rounding to fp32 leaves turns sine and cosine once more: of 10^8 rotated values 130 fall on the other
+    // side of a border between two e4m3 values, with sine and cosine of 64-bit angles rounded to fp32 135, without this 229)
     const double halves = 2.0 * (turns - rint(turns));
     const float hi = float(halves), lo = float((halves - double(hi)) * 3.14159265358979323846);
     float sn, cn;

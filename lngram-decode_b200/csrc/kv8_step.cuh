@@ -26,6 +26,8 @@
 //
 // Measured, one token a sequence: 64 sequences of 500 to 16000 keys, 32 query and 8 key heads of 128 (1.12 GB): 194 us, 5.8 TB/s
 // (0.89 of the measured copy rate), now bound by the loads; one sequence of 4096 keys, 4 key heads of 64: 16.5 us, latency.
+// With 32 rows the registers do not suffice (heads of 128: 132 and 196 bytes of spill stores in fp16 and bf16, heads of 64: 4); the
+// forms for fewer rows keep everything.
 #pragma once
 
 #include "kv8.cuh"

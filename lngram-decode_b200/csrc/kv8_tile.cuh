@@ -12,12 +12,12 @@
 // back out of the sum, and a row's reference lies below its largest score as there.  Weights are rounded to fp16 once, their sum
 // is not.
 //
-// Measured: two prompts of 5001 and 8000 tokens, 28 query and 4 key heads of 128, window of 4096 and 4 sinks: 830 us, 850 TFLOP/s,
-// about what kv_tile_kernel takes in 16 bits; a key tile takes some 1800 cycles, of which a row's thread is busy for 1400
-// and waits for its scores in the others.  The converters want all four warps on one tile and 96 registers (two warps for keys
-// and two for values: 5 % more; 88 or 104 registers: 2 %).  64 sequences of 16 drafted tokens after 1024 keys, 4 key heads of
-// 64: 51 us, two waves of units of which one row tile has rows (both row tiles on the same rows, the key tiles in turn, their
-// states joined: 62 us).
+// Measured: two prompts of 5001 and 8000 tokens, 28 query and 4 key heads of 128, window of 4096 and 4 sinks: 830 to 865 us by the
+// box, 815 to 850 TFLOP/s, about what kv_tile_kernel takes in 16 bits; a key tile takes some 1800 cycles, of which a row's
+// thread is busy for 1400 and waits for its scores in the others.  The converters want all four warps on one tile and 96
+// registers (two warps for keys and two for values: 5 % more; 88 or 104 registers: 2 %).  64 sequences of 16 drafted tokens
+// after 1024 keys, 4 key heads of 64: 50 us (42 us in 16 bits), two waves of units of which one row tile has rows (both row
+// tiles on the same rows, the key tiles in turn, their states joined: 62 us).
 #pragma once
 
 #include "kv8_step.cuh"

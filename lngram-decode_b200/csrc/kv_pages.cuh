@@ -215,6 +215,9 @@ __global__ void __cluster_dims__(PG_CTAS, 1, 1) __launch_bounds__(PG_THREADS, 1)
 
 // ------------------------------------------------------------------ copies
 // Keys (even blocks in y) or values (odd) of the slots that a copied page holds, of a share of the heads.
+// Bound by latency: a launch a cache, which for every sequence looks up whether a page is to be copied.  64 sequences, caches of 4
+// heads of 64: extend and truncate take 7.5 us for one layer, 35 us for 32; with rows forked before, eight to a page, and 64 pages copied
+// 13 us, and for 32 layers 75 us (16 bits) and 86 us (8 bits, where 8-byte vectors make twice as many accesses a byte).
 struct PgCopyParams {
   uint8_t *k, *v;
   int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;  // bytes
